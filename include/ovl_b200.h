@@ -27,7 +27,8 @@ extern "C" {
 /* Element type codes: wire values of the language's DType enum (opveclib/language.proto:16-37). */
 enum OvlDType {
     OVL_FLOAT16 = 1, OVL_FLOAT32 = 2, OVL_FLOAT64 = 3, OVL_INT8 = 4, OVL_INT16 = 5, OVL_INT32 = 6, OVL_INT64 = 7,
-    OVL_UINT8 = 8, OVL_UINT16 = 9, OVL_UINT32 = 10, OVL_UINT64 = 11
+    OVL_UINT8 = 8, OVL_UINT16 = 9, OVL_UINT32 = 10, OVL_UINT64 = 11,
+    OVL_BFLOAT16 = 12 /* not in the language: only the sequence operators below take it */
 };
 
 /* Status codes.  OVL_ERR_ARITY / OVL_ERR_LENGTH correspond to the reference's `*err = 1` on a wrong number of
@@ -222,6 +223,139 @@ int ovl_scan_f32_static(int op, const float* in, float* out, uint64_t lines, uin
                         void* cuda_stream);
 /* Status word of the most recent ovl_scan_f32_static launch on the current device (synchronises the stream). */
 int ovl_scan_f32_static_status(void* cuda_stream, int32_t* out_status);
+
+/* Sequence operators --------------------------------------------------------------------------------------- */
+/* The parts of a state space block between its matrix products (no counterpart in the reference, whose operator
+ * language has neither 16-bit types nor a recurrence whose factor depends on the data; they stand beside the built-in
+ * scans above, its one-dimensional convolution opveclib/examples/conv1D.py and its LSTM cell
+ * opveclib/examples/lstm.py).  All of them:
+ *  - take tensors of one `dtype`: OVL_FLOAT32, OVL_FLOAT16 or OVL_BFLOAT16, computed in fp32 and rounded once;
+ *  - take inputs whose innermost axis is contiguous, the other strides in elements (they may be 0), and write dense
+ *    outputs; 16-byte aligned pointers, strides and sizes select wide loads, anything else works too;
+ *  - run asynchronously on `cuda_stream`, allocate nothing, keep nothing between calls, and give the same bits for the
+ *    same inputs (no atomics);
+ *  - return OVL_OK without a launch when batch (or rows) is 0 - the gradients of the parameters are then not written
+ *    either, except by ovl_rms_norm_backward - and OVL_ERR_NULL / _INVALID / _DTYPE / _SCRATCH /
+ *    _TOO_LARGE for arguments they do not take.
+ * Every field of the argument structures is 8 bytes wide. */
+
+/* Selective scan.  For batch b, channel d of group g = d / (channels / groups), state n, token t:
+ *     dt = softplus(delta + delta_bias)     (delta_softplus = 0: delta + delta_bias)
+ *     h_t[n] = exp(dt * A[d, n]) * h_{t-1}[n] + dt * u_t * B_t[g, n],     h before the first token: initial_state
+ *     out_t = (sum_n C_t[g, n] * h_t[n] + D[d] * u_t) * silu(z_t)
+ * The states are held in fp32.  Tokens t >= lengths[b] are padding: never looked at, their outputs are zeros, the
+ * states pass them unchanged (lengths are clamped to [0, length]).  states: 1 to 128.
+ *   u, delta, z, gout [batch, length, channels], B, C [batch, length, groups, states]: dtype, strided;
+ *   A [channels, states], D, delta_bias [channels], initial_state, final_state [batch, channels, states]: fp32, dense;
+ *   out, gu, gdelta, gz [batch, length, channels], gB, gC [batch, length, groups, states]: dtype, dense;
+ *   z, D, delta_bias, initial_state, lengths, final_state, checkpoints may be NULL.
+ * ovl_selective_scan with `checkpoints` (fp32 [batch, ceil(length / 16), channels, states]) also leaves the states in
+ * front of every 16th token there; ovl_selective_scan_backward takes them, the forward call's inputs and the gradients
+ * of out (gout) and of the final state (gfinal, NULL: zero), and writes the gradients gu, gdelta, gA, gB, gC and - those
+ * that are not NULL - gD, gz, gdelta_bias, ginitial.  `workspace` must hold ovl_selective_scan_workspace_bytes(args, 0)
+ * bytes for the forward call, (args, 1) for the backward call (0: no workspace needed), and be 16-byte aligned. */
+typedef struct OvlSelectiveScan {
+    int64_t dtype, batch, length, channels, states, groups, delta_softplus;
+    const void *u, *delta, *z, *B, *C;
+    const float *A, *D, *delta_bias, *initial_state;
+    const int32_t* lengths;
+    int64_t u_batch, u_token, delta_batch, delta_token, z_batch, z_token;        /* strides in elements */
+    int64_t B_batch, B_token, B_group, C_batch, C_token, C_group;
+    void* out;
+    float *final_state, *checkpoints;
+    void* workspace;
+    uint64_t workspace_bytes;
+    const void* gout;                                                            /* backward only, from here on */
+    int64_t gout_batch, gout_token;
+    const float* gfinal;
+    void *gu, *gdelta, *gz, *gB, *gC;
+    float *gA, *gD, *gdelta_bias, *ginitial;
+} OvlSelectiveScan;
+uint64_t ovl_selective_scan_workspace_bytes(const OvlSelectiveScan* args, int backward);
+int ovl_selective_scan(const OvlSelectiveScan* args, void* cuda_stream);
+int ovl_selective_scan_backward(const OvlSelectiveScan* args, void* cuda_stream);
+
+/* One token for each of `rows` sequences: the same recurrence, `state` [slots, channels, states] (fp32, dense) updated
+ * in place.  Row r keeps its state in slot slot_of_row[r] (NULL: slot r).  A negative slot marks a padding row: nothing
+ * is read or written but its output, zeros.  A slot behind the last one, or one that an earlier row of the call has
+ * already (its state cannot take two tokens at once), is not touched and the row's output is NaN.
+ *   u, delta, z [rows, channels], B, C [rows, groups, states]: dtype, strided; out [rows, channels]: dtype, dense. */
+typedef struct OvlSelectiveScanStep {
+    int64_t dtype, rows, channels, states, groups, delta_softplus, slots;
+    const void *u, *delta, *z, *B, *C;
+    const float *A, *D, *delta_bias;
+    const int32_t* slot_of_row;
+    int64_t u_row, delta_row, z_row, B_row, B_group, C_row, C_group;
+    float* state;
+    void* out;
+} OvlSelectiveScanStep;
+int ovl_selective_scan_step(const OvlSelectiveScanStep* args, void* cuda_stream);
+
+/* Causal convolution along the tokens, every channel by itself:
+ *     out_t[d] = act(bias[d] + sum_k weight[d, k] * x_{t - (taps - 1) + k}[d]),  act: the identity, or silu
+ * with the taps - 1 inputs in front of the first token taken from initial_state (NULL: zeros); final_state receives the
+ * last taps - 1 inputs of each sequence, those of initial_state among them when the sequence is shorter.  Padding (tokens
+ * t >= lengths[b]) is never looked at, its outputs are zeros.  taps: 1 to 8.
+ *   x, gout [batch, length, channels]: dtype, strided; out, gx: dtype, dense; initial_state, final_state, gfinal, ginitial
+ *   [batch, taps - 1, channels]: dtype, dense; weight, gweight [channels, taps], bias, gbias [channels]: dtype, or fp32
+ *   when params_f32 is set, dense; bias, initial_state, lengths, final_state, gfinal, gbias, ginitial may be NULL.
+ * The backward call needs ovl_causal_conv_workspace_bytes(args) bytes of workspace, the forward call none. */
+typedef struct OvlCausalConv {
+    int64_t dtype, batch, length, channels, taps, silu, params_f32;
+    const void *x, *weight, *bias, *initial_state;
+    const int32_t* lengths;
+    int64_t x_batch, x_token;
+    void *out, *final_state;
+    const void* gout;                                                            /* backward only, from here on */
+    int64_t gout_batch, gout_token;
+    const void* gfinal;
+    void *gx, *gweight, *gbias, *ginitial;
+    void* workspace;
+    uint64_t workspace_bytes;
+} OvlCausalConv;
+uint64_t ovl_causal_conv_workspace_bytes(const OvlCausalConv* args);
+int ovl_causal_conv(const OvlCausalConv* args, void* cuda_stream);
+int ovl_causal_conv_backward(const OvlCausalConv* args, void* cuda_stream);
+
+/* One token for each of `rows` sequences; `state` [slots, taps - 1, channels] (dtype, dense), the last taps - 1 inputs
+ * of each sequence, is shifted in place.  Slots as for ovl_selective_scan_step. */
+typedef struct OvlCausalConvStep {
+    int64_t dtype, rows, channels, taps, silu, params_f32, slots;
+    const void *x, *weight, *bias;
+    const int32_t* slot_of_row;
+    int64_t x_row;
+    void *state, *out;
+} OvlCausalConvStep;
+int ovl_causal_conv_step(const OvlCausalConvStep* args, void* cuda_stream);
+
+/* Root-mean-square norm of rows, with the residual's addition in front of it:
+ *     s = x + residual (residual NULL: s = x),  y = s / sqrt(mean(s^2) + eps) * weight
+ * residual_out receives s rounded to dtype (the norm itself uses the unrounded sum).
+ *   x, residual, y, residual_out, gy, gresidual_out, gx [rows, columns]: dtype; inputs with a row stride, outputs dense;
+ *   weight, gweight [columns]: dtype, or fp32 when params_f32 is set.
+ * With group > 0 the output is 8 bits wide instead: y is cut into groups of `group` columns (which divides columns),
+ *     scale = max(max |y| / 448, 2^-126),  q = y / scale rounded to the nearest e4m3 value, ties to even
+ * with q [rows, columns] bytes and scale [rows, columns / group] fp32.
+ * The backward call takes s as residual_out of the forward call holds it (x itself without a residual) in `x`, and the
+ * gradients of y and of residual_out (NULL: zero); gx is the gradient of x and of the residual alike.  Its workspace:
+ * ovl_rms_norm_workspace_bytes(args) bytes; the forward call needs none. */
+typedef struct OvlRmsNorm {
+    int64_t dtype, rows, columns, params_f32, group;
+    double eps;
+    const void *x, *residual, *weight;
+    int64_t x_row, residual_row;
+    void *y, *residual_out;
+    void* q;
+    float* scale;
+    const void *gy, *gresidual_out;                                              /* backward only, from here on */
+    int64_t gy_row, gresidual_out_row;
+    void *gx, *gweight;
+    void* workspace;
+    uint64_t workspace_bytes;
+} OvlRmsNorm;
+uint64_t ovl_rms_norm_workspace_bytes(const OvlRmsNorm* args);
+int ovl_rms_norm(const OvlRmsNorm* args, void* cuda_stream);
+int ovl_rms_norm_backward(const OvlRmsNorm* args, void* cuda_stream);
 
 #ifdef __cplusplus
 }

@@ -19,6 +19,9 @@ from .expr import arange, if_, elif_, else_
 from .opgraph import operator, gradient
 from .runtime import evaluate, profile
 from .torch_bridge import as_torch, as_tensorflow
+# operators on sequences: the parts of a state space block between its matrix products
+from .sequence import selective_scan, selective_scan_step, causal_conv1d, causal_conv1d_step
+from .sequence import rms_norm, rms_norm_quantize
 # local runtime environment
 from .local import version, logger, cuda_enabled, cache_directory, clear_op_cache
 from .local import math_mode, set_math_mode, get_math_mode

@@ -7,6 +7,7 @@ reference's ``~/.opveclib/<version>/f<sha224>_generic_cuda.so`` cache (opveclib/
 sm_100a, FMA contraction is off and fast-math is never used, so that fp32 results match the reference's C++
 operator.
 """
+import concurrent.futures
 import hashlib
 import json
 import os
@@ -20,8 +21,12 @@ _PKG = os.path.dirname(os.path.abspath(__file__))
 TEMPLATE_DIR = os.path.join(_PKG, 'csrc', 'templates')
 LIB_DIR = os.path.join(_PKG, 'lib')
 LIB_PATH = os.path.join(LIB_DIR, 'libovl_b200.so')
-LAUNCHER_SRC = os.path.join(_PKG, 'csrc', 'ovl_launcher.cu')
-NVCC_FLAGS = ['-O3', '--fmad=false', '-std=c++17', '-lineinfo', '-diag-suppress', '177,186,550']
+CSRC_DIR = os.path.join(_PKG, 'csrc')
+LAUNCHER_SRC = os.path.join(CSRC_DIR, 'ovl_launcher.cu')
+#: every source of the library; they are compiled side by side
+LIBRARY_SOURCES = [LAUNCHER_SRC] + [os.path.join(CSRC_DIR, fn) for fn in
+                                    ('ovl_selective_scan.cu', 'ovl_causal_conv.cu', 'ovl_rms_norm.cu')]
+NVCC_FLAGS = ['-O3', '--fmad=false', '-std=c++17', '-lineinfo', '-diag-suppress', '128,177,186,550']
 _lock = threading.Lock()
 
 
@@ -103,12 +108,13 @@ def _launcher_stamp(deps):
 
 
 def build_launcher(force=False):
-    """Compile csrc/ovl_launcher.cu into lib/libovl_b200.so for sm_100a (no GPU needed).  The library is rebuilt
+    """Compile the sources in csrc into lib/libovl_b200.so for sm_100a (no GPU needed).  The library is rebuilt
     when the content of its sources differs from what it was built from (a digest kept beside it - file times do
     not survive a copy of the tree)."""
     with _lock:
         os.makedirs(LIB_DIR, exist_ok=True)
-        deps = [LAUNCHER_SRC, os.path.join(_PKG, '..', 'include', 'ovl_b200.h')] + \
+        deps = LIBRARY_SOURCES + [os.path.join(CSRC_DIR, 'ovl_sequence.cuh'),
+                                  os.path.join(_PKG, '..', 'include', 'ovl_b200.h')] + \
             [os.path.join(TEMPLATE_DIR, fn) for fn in os.listdir(TEMPLATE_DIR)]
         stamp = _launcher_stamp(deps)
         stamp_path = LIB_PATH + '.stamp'
@@ -117,7 +123,16 @@ def build_launcher(force=False):
                 if f.read().strip() == stamp:
                     return LIB_PATH
         tmp = LIB_PATH + '.%d.tmp' % os.getpid()
-        _run([nvcc_path] + gpu_arch_flags + NVCC_FLAGS + ['-shared', '-Xcompiler', '-fPIC', '-o', tmp, LAUNCHER_SRC])
+        objects = ['%s.%d.o' % (os.path.join(LIB_DIR, os.path.basename(src)), os.getpid()) for src in LIBRARY_SOURCES]
+        try:
+            with concurrent.futures.ThreadPoolExecutor(len(objects)) as pool:
+                list(pool.map(_run, [[nvcc_path] + gpu_arch_flags + NVCC_FLAGS + ['-Xcompiler', '-fPIC', '-c', '-o', obj, src]
+                                     for obj, src in zip(objects, LIBRARY_SOURCES)]))
+            _run([nvcc_path] + gpu_arch_flags + ['-shared', '-o', tmp] + objects)
+        finally:
+            for obj in objects:
+                if os.path.exists(obj):
+                    os.remove(obj)
         os.replace(tmp, LIB_PATH)
         with open(stamp_path + '.%d.tmp' % os.getpid(), 'w') as f:
             f.write(stamp)

@@ -870,3 +870,10 @@ extern "C" int ovl_reduce_f32(int op, const float* in, uint64_t n, double* out_t
     if (!scratch || scratch_bytes < need || ((uintptr_t)scratch % 16) != 0) return OVL_ERR_SCRATCH;
     return launch_reduce(op, in, n, out_total, scratch, (cudaStream_t)cuda_stream);
 }
+
+// ---------------------------------------------------------------------------------------------------------
+// What the sequence operators' sources take from here: the thread-local error word and the SM count.
+namespace ovl {
+__attribute__((visibility("hidden"))) int record_cuda_error(cudaError_t e) { return cuda_fail(e); }
+__attribute__((visibility("hidden"))) int sequence_sm_count() { return sm_count_cached(); }
+}  // namespace ovl

@@ -1,0 +1,424 @@
+// Root-mean-square norm of rows with the residual's addition in front of it, with an output in the tensors' type or in
+// 8 bits with scales, and its backward pass.  Interface: include/ovl_b200.h.
+//
+// What bounds it: bytes.  A team of threads (a warp for short rows, a block for long ones) holds its row in registers
+// between the reduction and the outputs, so every element is read once and written once.
+#include "ovl_sequence.cuh"
+
+namespace ovl {
+namespace {
+
+constexpr int64_t kMaxColumns = 32768;
+constexpr float kE4m3Max = 448.0f;
+constexpr float kMinScale = 1.1754943508e-38f;   // 2^-126, the smallest normal number
+
+struct NormParams {
+    OvlRmsNorm a;
+    int32_t vec;
+    int32_t group_lanes;               // 8-bit output: lanes that share a scale (0: through shared memory)
+    float* part;                       // backward: [blocks, columns]
+};
+
+// Teams: TEAM threads work on a row; a block has THREADS / TEAM teams.
+template <int TEAM>
+struct TeamShape {
+    static constexpr int THREADS = TEAM == 32 ? 128 : TEAM;
+    static constexpr int TEAMS = THREADS / TEAM;
+    static constexpr int WARPS = TEAM / 32;
+};
+
+// sums of V values over a team, in a fixed order; every thread gets them
+template <int TEAM, int V>
+__device__ __forceinline__ void team_sum(float (&v)[V], float (*s_sum)[32]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+        for (int s = 16; s >= 1; s >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], s);
+    if constexpr (TEAM > 32) {
+        const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+        __syncthreads();                                                 // the row before has read its sums
+        if (lane == 0) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) s_sum[i][warp] = v[i];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            v[i] = lane < TeamShape<TEAM>::WARPS ? s_sum[i][lane] : 0.0f;
+#pragma unroll
+            for (int s = 16; s >= 1; s >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], s);
+        }
+    }
+}
+
+// two e4m3 values, nearest with ties to even
+__device__ __forceinline__ uint32_t e4m3_pair(float a, float b) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(b), "f"(a));
+    return r;
+}
+
+// the scale of a group whose largest magnitude has these bits (a NaN stays one)
+__device__ __forceinline__ float scale_of(unsigned int bits) {
+    const float scale = __uint_as_float(bits) / kE4m3Max;
+    return scale < kMinScale ? kMinScale : scale;
+}
+
+template <typename T, int TEAM, int K, bool QUANT>
+__global__ void __launch_bounds__(TeamShape<TEAM>::THREADS) norm_forward(const __grid_constant__ NormParams p) {
+    using S = TeamShape<TEAM>;
+    constexpr int N = 8;
+    __shared__ float s_sum[1][32];
+    extern __shared__ unsigned int s_max[];                              // [teams][columns / group]
+    const OvlRmsNorm& a = p.a;
+    const int team = threadIdx.x / TEAM, me = threadIdx.x % TEAM;
+    const int64_t row = (int64_t)blockIdx.x * S::TEAMS + team;
+    const bool live = row < a.rows;                                      // (a warp as a whole; blocks are whole rows)
+    if (TEAM == 32 && !QUANT && !live) return;
+    const T* const x = reinterpret_cast<const T*>(a.x) + row * a.x_row;
+    const T* const res = a.residual ? reinterpret_cast<const T*>(a.residual) + row * a.residual_row : nullptr;
+    const int columns = (int)a.columns;
+
+    Pack<T, N> raw[K], raw_r[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int col = (me + k * TEAM) * N;
+        const int valid = !live || col >= columns ? 0 : columns - col < N ? columns - col : N;
+        raw[k] = load_pack<T, N>(x + col, p.vec && valid == N, valid);
+        if (res) raw_r[k] = load_pack<T, N>(res + col, p.vec && valid == N, valid);
+    }
+    float s[K][N], sum[1] = {0.0f};
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            s[k][i] = to_f32(raw[k].v[i]);
+            if (res) s[k][i] += to_f32(raw_r[k].v[i]);
+            sum[0] = fmaf(s[k][i], s[k][i], sum[0]);
+        }
+    if (a.residual_out && live) {
+        T* const to = reinterpret_cast<T*>(a.residual_out) + row * a.columns;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int col = (me + k * TEAM) * N;
+            const int valid = col >= columns ? 0 : columns - col < N ? columns - col : N;
+            store_pack<T, N>(to + col, s[k], p.vec && valid == N, valid);
+        }
+    }
+    team_sum<TEAM, 1>(sum, s_sum);
+    const float r = rsqrtf(sum[0] / (float)columns + (float)a.eps);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int col = (me + k * TEAM) * N;
+        const int valid = col >= columns ? 0 : columns - col < N ? columns - col : N;
+        Pack<T, N> w;
+        if (!a.params_f32) w = load_pack<T, N>(reinterpret_cast<const T*>(a.weight) + col, p.vec && valid == N, valid);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float wi = a.params_f32 ? (i < valid ? reinterpret_cast<const float*>(a.weight)[col + i] : 0.0f) : to_f32(w.v[i]);
+            s[k][i] *= r * wi;
+        }
+        if (!QUANT && live)
+            store_pack<T, N>(reinterpret_cast<T*>(a.y) + row * a.columns + col, s[k], p.vec && valid == N, valid);
+    }
+    if constexpr (QUANT) {
+        // The largest magnitude of a group, as the largest bit pattern: a NaN stays the largest.
+        const int group = (int)a.group, groups = columns / group;
+        unsigned int* const maxima = s_max + team * groups;
+        unsigned int top[K];
+        if (p.group_lanes || groups == 1) {
+            unsigned int whole = 0;
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                top[k] = 0;
+#pragma unroll
+                for (int i = 0; i < N; ++i) top[k] = max(top[k], __float_as_uint(s[k][i]) & 0x7fffffffu);
+                whole = max(whole, top[k]);
+            }
+            if (groups == 1) {
+                whole = __reduce_max_sync(0xffffffffu, whole);
+                if (me == 0) maxima[0] = 0;
+                __syncthreads();
+                if (me % 32 == 0) atomicMax(maxima, whole);
+                __syncthreads();
+                whole = maxima[0];
+#pragma unroll
+                for (int k = 0; k < K; ++k) top[k] = whole;
+            } else {
+#pragma unroll
+                for (int k = 0; k < K; ++k)
+                    for (int l = 1; l < p.group_lanes; l *= 2) top[k] = max(top[k], __shfl_xor_sync(0xffffffffu, top[k], l));
+            }
+        } else {
+            for (int i = me; i < groups; i += TEAM) maxima[i] = 0;
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const int col = (me + k * TEAM) * N;
+                unsigned int run = 0;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    if (col + i >= columns) continue;
+                    run = max(run, __float_as_uint(s[k][i]) & 0x7fffffffu);
+                    if (i == N - 1 || col + i + 1 >= columns || (col + i + 1) % group == 0) {
+                        atomicMax(maxima + (col + i) / group, run);
+                        run = 0;
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        if (!live) return;
+        uint8_t* const q = reinterpret_cast<uint8_t*>(a.q) + row * a.columns;
+        float* const scales = a.scale + row * groups;
+        const bool one_scale = p.group_lanes || groups == 1;             // for the 8 values of a thread
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int col = (me + k * TEAM) * N;
+            if (col >= columns) continue;
+            float v[N];
+            if (one_scale) {
+                const float scale = scale_of(top[k]), inverse = 1.0f / scale;
+#pragma unroll
+                for (int i = 0; i < N; ++i) v[i] = s[k][i] * inverse;
+                const int g = groups == 1 ? 0 : col / group;
+                if (col == g * group) scales[g] = scale;
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    if (col + i >= columns) continue;
+                    const int g = (col + i) / group;
+                    const float scale = scale_of(maxima[g]);
+                    v[i] = s[k][i] * (1.0f / scale);
+                    if (col + i == g * group) scales[g] = scale;
+                }
+            }
+            // (an infinite value meets an infinite scale: inf * 0 is NaN, as inf / inf)
+            if (p.vec && col + N <= columns) {
+                uint2 bytes;
+                bytes.x = e4m3_pair(v[0], v[1]) | e4m3_pair(v[2], v[3]) << 16;
+                bytes.y = e4m3_pair(v[4], v[5]) | e4m3_pair(v[6], v[7]) << 16;
+                *reinterpret_cast<uint2*>(q + col) = bytes;
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    if (col + i < columns) q[col + i] = (uint8_t)e4m3_pair(v[i], 0.0f);
+            }
+        }
+    }
+}
+
+// With g = gy w and xhat = s r: gx = r (g - xhat mean(g xhat)) + gresidual_out; gweight = sum over the rows of gy xhat.
+// Every team walks over rows with its sums for gweight in registers.
+template <typename T, int TEAM, int K>
+__global__ void __launch_bounds__(TeamShape<TEAM>::THREADS) norm_backward(const __grid_constant__ NormParams p) {
+    using S = TeamShape<TEAM>;
+    constexpr int N = 8;
+    __shared__ float s_sum[2][32];
+    __shared__ float s_w[TEAM == 32 ? S::TEAMS : 1][TEAM == 32 ? TEAM * K * N : 1];
+    const OvlRmsNorm& a = p.a;
+    const int team = threadIdx.x / TEAM, me = threadIdx.x % TEAM;
+    const int columns = (int)a.columns;
+    float w[K][N], gw[K][N];
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int col = (me + k * TEAM) * N + i;
+            w[k][i] = col < columns ? load_param<T>(a.weight, col, a.params_f32) : 0.0f;
+            gw[k][i] = 0.0f;
+        }
+    for (int64_t row = (int64_t)blockIdx.x * S::TEAMS + team; row < a.rows; row += (int64_t)gridDim.x * S::TEAMS) {
+        const T* const x = reinterpret_cast<const T*>(a.x) + row * a.x_row;
+        const T* const gy = reinterpret_cast<const T*>(a.gy) + row * a.gy_row;
+        const T* const gr = a.gresidual_out ? reinterpret_cast<const T*>(a.gresidual_out) + row * a.gresidual_out_row : nullptr;
+        Pack<T, N> rx[K], rg[K], rr[K];
+        float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int col = (me + k * TEAM) * N;
+            const int valid = col >= columns ? 0 : columns - col < N ? columns - col : N;
+            const bool vec = p.vec && valid == N;
+            rx[k] = load_pack<T, N>(x + col, vec, valid);
+            rg[k] = load_pack<T, N>(gy + col, vec, valid);
+            if (gr) rr[k] = load_pack<T, N>(gr + col, vec, valid);
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float s = to_f32(rx[k].v[i]);
+                sum[0] = fmaf(s, s, sum[0]);
+                sum[1] = fmaf(s * w[k][i], to_f32(rg[k].v[i]), sum[1]);
+            }
+        team_sum<TEAM, 2>(sum, s_sum);
+        const float r = rsqrtf(sum[0] / (float)columns + (float)a.eps);
+        const float mean = r * r * (sum[1] / (float)columns);            // mean(g xhat) r, so that xhat r mean = s r mean
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int col = (me + k * TEAM) * N;
+            const int valid = col >= columns ? 0 : columns - col < N ? columns - col : N;
+            float gx[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float s = to_f32(rx[k].v[i]), g = to_f32(rg[k].v[i]);
+                gx[i] = r * fmaf(-s, mean, g * w[k][i]);
+                if (gr) gx[i] += to_f32(rr[k].v[i]);
+                gw[k][i] = fmaf(g, s * r, gw[k][i]);
+            }
+            store_pack<T, N>(reinterpret_cast<T*>(a.gx) + row * a.columns + col, gx, p.vec && valid == N, valid);
+        }
+    }
+    float* const part = p.part + (int64_t)blockIdx.x * columns;
+    if constexpr (TEAM == 32) {
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int i = 0; i < N; ++i) s_w[team][(me + k * TEAM) * N + i] = gw[k][i];
+        __syncthreads();
+        for (int col = threadIdx.x; col < columns; col += S::THREADS) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int t = 0; t < S::TEAMS; ++t) sum += s_w[t][col];
+            part[col] = sum;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int col = (me + k * TEAM) * N + i;
+                if (col < columns) part[col] = gw[k][i];
+            }
+    }
+}
+
+// gweight: the blocks' parts added up in order; a warp's lanes are 32 columns, the 8 warps of a block slices of the parts
+template <typename T>
+__global__ void __launch_bounds__(256) norm_backward_weight(const __grid_constant__ NormParams p, int64_t parts) {
+    __shared__ float s_part[8][32];
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const int64_t col = (int64_t)blockIdx.x * 32 + lane;
+    float sum = 0.0f;
+    if (col < p.a.columns)
+        for (int64_t r = warp; r < parts; r += 8) sum += p.part[r * p.a.columns + col];
+    s_part[warp][lane] = sum;
+    __syncthreads();
+    if (warp == 0 && col < p.a.columns) {
+        sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) sum += s_part[w][lane];
+        if (p.a.params_f32) reinterpret_cast<float*>(p.a.gweight)[col] = sum;
+        else reinterpret_cast<T*>(p.a.gweight)[col] = from_f32<T>(sum);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// host side
+
+int check(const OvlRmsNorm* a) {
+    if (!a) return OVL_ERR_NULL;
+    if (a->dtype != OVL_FLOAT32 && a->dtype != OVL_FLOAT16 && a->dtype != OVL_BFLOAT16) return OVL_ERR_DTYPE;
+    if (a->rows < 0 || a->columns < 1 || a->group < 0) return OVL_ERR_INVALID;
+    if (a->group > 0 && a->columns % a->group != 0) return OVL_ERR_INVALID;
+    if (a->columns > kMaxColumns) return OVL_ERR_TOO_LARGE;
+    return OVL_OK;
+}
+
+int team_of(int64_t columns) { return columns <= 1024 ? 32 : columns <= 8192 ? 256 : 512; }
+int teams_of_block(int team) { return team == 32 ? 4 : 1; }
+
+// blocks of the backward pass: they stay for all rows, so their parts of gweight are few
+int64_t backward_blocks(const OvlRmsNorm* a) {
+    const int team = team_of(a->columns);
+    const int64_t most = (int64_t)sequence_sm_count() * (team == 32 ? 8 : team == 256 ? 4 : 2);
+    const int64_t blocks = ceil_div(a->rows, teams_of_block(team));
+    return blocks < 1 ? 1 : blocks < most ? blocks : most;
+}
+
+template <typename T, int TEAM, int K>
+int launch(const NormParams& p, bool backward, cudaStream_t stream) {
+    using S = TeamShape<TEAM>;
+    if (backward) {
+        norm_backward<T, TEAM, K><<<(uint32_t)backward_blocks(&p.a), S::THREADS, 0, stream>>>(p);
+        return launch_status();
+    }
+    const int64_t blocks = ceil_div(p.a.rows, S::TEAMS);
+    if (blocks > 0x7fffffff) return OVL_ERR_TOO_LARGE;
+    if (p.a.group > 0) {
+        const size_t groups = p.a.columns / p.a.group;
+        const size_t smem = p.group_lanes && groups > 1 ? 0 : S::TEAMS * groups * sizeof(unsigned int);
+        if (smem > 40 * 1024) {
+            const cudaError_t e = cudaFuncSetAttribute(norm_forward<T, TEAM, K, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+            if (e != cudaSuccess) return record_cuda_error(e);
+        }
+        norm_forward<T, TEAM, K, true><<<(uint32_t)blocks, S::THREADS, smem, stream>>>(p);
+    } else {
+        norm_forward<T, TEAM, K, false><<<(uint32_t)blocks, S::THREADS, 0, stream>>>(p);
+    }
+    return launch_status();
+}
+
+template <typename T>
+int dispatch(const NormParams& p, bool backward, cudaStream_t stream) {
+    const int64_t c = p.a.columns;
+    if (c <= 256) return launch<T, 32, 1>(p, backward, stream);
+    if (c <= 512) return launch<T, 32, 2>(p, backward, stream);
+    if (c <= 1024) return launch<T, 32, 4>(p, backward, stream);
+    if (c <= 2048) return launch<T, 256, 1>(p, backward, stream);
+    if (c <= 4096) return launch<T, 256, 2>(p, backward, stream);
+    if (c <= 8192) return launch<T, 256, 4>(p, backward, stream);
+    if (c <= 16384) return launch<T, 512, 4>(p, backward, stream);
+    return launch<T, 512, 8>(p, backward, stream);
+}
+
+int run(NormParams& p, bool backward, cudaStream_t stream) {
+    if (p.a.dtype == OVL_FLOAT32) return dispatch<float>(p, backward, stream);
+    if (p.a.dtype == OVL_FLOAT16) return dispatch<__half>(p, backward, stream);
+    return dispatch<__nv_bfloat16>(p, backward, stream);
+}
+
+}  // namespace
+}  // namespace ovl
+
+extern "C" uint64_t ovl_rms_norm_workspace_bytes(const OvlRmsNorm* a) {
+    if (ovl::check(a) != OVL_OK) return 0;
+    return (uint64_t)ovl::backward_blocks(a) * a->columns * sizeof(float);
+}
+
+extern "C" int ovl_rms_norm(const OvlRmsNorm* a, void* cuda_stream) {
+    const int st = ovl::check(a);
+    if (st != OVL_OK) return st;
+    if (a->rows == 0) return OVL_OK;
+    if (!a->x || !a->weight) return OVL_ERR_NULL;
+    if (a->group > 0 ? (!a->q || !a->scale) : !a->y) return OVL_ERR_NULL;
+    ovl::NormParams p{};
+    p.a = *a;
+    p.vec = a->columns % 8 == 0 && ovl::aligned16(a->x) && a->x_row % 8 == 0 && ovl::aligned16(a->residual) &&
+            (!a->residual || a->residual_row % 8 == 0) && ovl::aligned16(a->residual_out) && ovl::aligned16(a->weight) &&
+            (a->group > 0 ? ovl::aligned16(a->q) : ovl::aligned16(a->y));
+    const int64_t lanes = a->group / 8;
+    if (a->group % 8 == 0 && lanes >= 1 && lanes <= 32 && (lanes & (lanes - 1)) == 0) p.group_lanes = (int32_t)lanes;
+    return ovl::run(p, false, (cudaStream_t)cuda_stream);
+}
+
+extern "C" int ovl_rms_norm_backward(const OvlRmsNorm* a, void* cuda_stream) {
+    const int st = ovl::check(a);
+    if (st != OVL_OK) return st;
+    if (!a->weight || !a->gweight || (a->rows > 0 && (!a->x || !a->gy || !a->gx))) return OVL_ERR_NULL;
+    if (!a->workspace || a->workspace_bytes < ovl_rms_norm_workspace_bytes(a) || !ovl::aligned16(a->workspace)) return OVL_ERR_SCRATCH;
+    ovl::NormParams p{};
+    p.a = *a;
+    p.part = reinterpret_cast<float*>(a->workspace);
+    p.vec = a->columns % 8 == 0 && ovl::aligned16(a->x) && a->x_row % 8 == 0 && ovl::aligned16(a->gy) && a->gy_row % 8 == 0 &&
+            ovl::aligned16(a->gresidual_out) && (!a->gresidual_out || a->gresidual_out_row % 8 == 0) && ovl::aligned16(a->gx);
+    const cudaStream_t stream = (cudaStream_t)cuda_stream;
+    const int s = ovl::run(p, true, stream);
+    if (s != OVL_OK) return s;
+    const uint32_t grid = (uint32_t)ovl::ceil_div(a->columns, 32);
+    const int64_t parts = ovl::backward_blocks(a);
+    if (a->dtype == OVL_FLOAT32) ovl::norm_backward_weight<float><<<grid, 256, 0, stream>>>(p, parts);
+    else if (a->dtype == OVL_FLOAT16) ovl::norm_backward_weight<__half><<<grid, 256, 0, stream>>>(p, parts);
+    else ovl::norm_backward_weight<__nv_bfloat16><<<grid, 256, 0, stream>>>(p, parts);
+    return ovl::launch_status();
+}

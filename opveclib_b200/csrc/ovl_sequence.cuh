@@ -1,0 +1,206 @@
+// What the sequence operators (selective scan, short causal convolution, residual norm) share: element types and
+// their conversions, vectors of elements that may or may not be aligned, packed fp32 arithmetic, reductions over lanes.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/ovl_b200.h"
+
+namespace ovl {
+
+// Host side: records the CUDA error for ovl_last_cuda_error() and returns OVL_ERR_CUDA (ovl_launcher.cu).
+__attribute__((visibility("hidden"))) int record_cuda_error(cudaError_t e);
+
+inline int launch_status() {
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? OVL_OK : record_cuda_error(e);
+}
+
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+inline bool aligned16(const void* p) { return ((uintptr_t)p % 16) == 0; }
+
+// SM count of the current device (148 on a B200), asked once per device.
+__attribute__((visibility("hidden"))) int sequence_sm_count();
+
+// ---------------------------------------------------------------------------------------------------------
+// element types
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+// one rounding to nearest even
+template <typename T> __device__ __forceinline__ T from_f32(float x);
+template <> __device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <> __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// N elements as loaded, before conversion: N * sizeof(T) bytes in registers
+template <typename T, int N>
+struct alignas(sizeof(T) * N > 16 ? 16 : sizeof(T) * N) Pack {
+    T v[N];
+};
+
+// N consecutive elements; `vec`: the address is aligned to the pack and all N exist; otherwise the first `valid`
+// are read one by one and the others are zero.
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> load_pack(const T* __restrict__ p, bool vec, int valid) {
+    Pack<T, N> r;
+    if (vec) {
+        if constexpr (sizeof(T) * N <= 16) {
+            r = *reinterpret_cast<const Pack<T, N>*>(p);
+        } else {
+            constexpr int H = 16 / sizeof(T);
+#pragma unroll
+            for (int i = 0; i < N; i += H)
+                *reinterpret_cast<Pack<T, H>*>(&r.v[i]) = *reinterpret_cast<const Pack<T, H>*>(p + i);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) r.v[i] = i < valid ? p[i] : from_f32<T>(0.0f);
+    }
+    return r;
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void store_pack(T* __restrict__ p, const float (&x)[N], bool vec, int valid) {
+    if (vec) {
+        constexpr int H = sizeof(T) * N <= 16 ? N : 16 / (int)sizeof(T);
+#pragma unroll
+        for (int i = 0; i < N; i += H) {
+            Pack<T, H> r;
+#pragma unroll
+            for (int k = 0; k < H; ++k) r.v[k] = from_f32<T>(x[i + k]);
+            *reinterpret_cast<Pack<T, H>*>(p + i) = r;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (i < valid) p[i] = from_f32<T>(x[i]);
+    }
+}
+
+// a parameter vector that is either in the tensors' type or in fp32
+template <typename T>
+__device__ __forceinline__ float load_param(const void* p, int64_t i, bool f32) {
+    return f32 ? reinterpret_cast<const float*>(p)[i] : to_f32(reinterpret_cast<const T*>(p)[i]);
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// fp32 arithmetic on pairs: one instruction for two values
+
+struct F2 {
+    unsigned long long v;
+};
+__device__ __forceinline__ F2 pack2(float a, float b) {
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpack2(F2 x, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v));
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ float sum2(F2 x) {
+    float a, b;
+    unpack2(x, a, b);
+    return a + b;
+}
+
+// 2^x: one special-function instruction, at most 2^-22.5 off relatively (measured over [-10, 0]: 1.4e-7 at most,
+// 3e-8 on average, 1e-8 of bias), results below 2^-126 flush to zero
+__device__ __forceinline__ float exp2_approx(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ F2 exp2_pair(F2 x) {
+    float a, b;
+    unpack2(x, a, b);
+    return pack2(exp2_approx(a), exp2_approx(b));
+}
+
+__device__ __forceinline__ float rcp_approx(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// 1 / (1 + e^-x): two special-function instructions
+__device__ __forceinline__ float sigmoid(float x) { return rcp_approx(1.0f + exp2_approx(-kLog2e * x)); }
+__device__ __forceinline__ float silu(float x) { return x * sigmoid(x); }
+
+// log(1 + e^x) = max(x, 0) + log1p(e^-|x|), relatively exact to 3e-7 also where it is small (a step size of 0.001 is
+// softplus(-6.9)): e^-|x| with the product by log2 e in two parts, then log1p(e) = e p(e) with p the polynomial of
+// degree 9 that agrees with log1p(e) / e in the Chebyshev points of [0, 1] (5e-9 off).  A NaN stays one.
+__device__ __forceinline__ float softplus(float x) {
+    const float t = fminf(fabsf(x), 100.0f);
+    const float hi = -kLog2e * t;
+    const float lo = fmaf(-kLog2e, t, -hi) - 1.925963033e-8f * t;
+    float e = exp2_approx(hi);
+    e = fmaf(e, kLn2 * lo, e);
+    float p = -3.176057013e-03f;
+    p = fmaf(p, e, 1.954252645e-02f);
+    p = fmaf(p, e, -5.637361109e-02f);
+    p = fmaf(p, e, 1.054362357e-01f);
+    p = fmaf(p, e, -1.526966691e-01f);
+    p = fmaf(p, e, 1.966327429e-01f);
+    p = fmaf(p, e, -2.495161593e-01f);
+    p = fmaf(p, e, 3.332971036e-01f);
+    p = fmaf(p, e, -4.999989271e-01f);
+    p = fmaf(p, e, 1.0f);
+    return fmaf(p, e, x < 0.0f ? 0.0f : x);
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// Sums over lanes.  V values per lane are summed over the R lanes whose numbers differ in R * STRIDE / STRIDE (lane
+// bits STRIDE, 2 STRIDE, ...).  While a lane holds several values every exchange sends half of them and keeps the
+// other half (V - 1 exchanges for V >= R instead of V log2 R); then whole exchanges.  Afterwards lane l (its number
+// among the R) holds max(1, V / R) totals in v[0...]: those of index reduced_index<V, R>(l) and following.
+template <int V, int R, int STRIDE>
+__device__ __forceinline__ void reduce_lanes(float (&v)[V], int lane) {
+    int count = V;
+#pragma unroll
+    for (int s = R / 2; s >= 1; s >>= 1) {
+        if (count > 1) {
+            const int half = count / 2;
+            const bool upper = lane & (s * STRIDE);
+#pragma unroll
+            for (int i = 0; i < (V > 1 ? V / 2 : 1); ++i) {
+                if (i < half) {
+                    const float keep = upper ? v[i + half] : v[i];
+                    const float send = upper ? v[i] : v[i + half];
+                    v[i] = keep + __shfl_xor_sync(0xffffffffu, send, s * STRIDE);
+                }
+            }
+            count = half;
+        } else {
+            v[0] += __shfl_xor_sync(0xffffffffu, v[0], s * STRIDE);
+        }
+    }
+}
+template <int V, int R>
+__device__ __forceinline__ constexpr int reduced_count() { return V >= R ? V / R : 1; }
+template <int V, int R>
+__device__ __forceinline__ int reduced_index(int l) { return V >= R ? l * (V / R) : l / (R / V); }
+// lanes that hold the same totals when there are more lanes than values: only one of them writes
+template <int V, int R>
+__device__ __forceinline__ bool reduced_owner(int l) { return V >= R ? true : (l % (R / V)) == 0; }
+
+}  // namespace ovl

@@ -33,7 +33,10 @@ EXPORTS = ['ovl_version', 'ovl_status_string', 'ovl_last_cuda_error', 'ovl_devic
            'ovl_profile', 'ovl_run_host', 'ovl_read_kernel_status', 'ovl_scan_f32_scratch_bytes', 'ovl_scan_f32',
            'ovl_reduce_f32_scratch_bytes', 'ovl_reduce_f32', 'ovl_scan_f32_static', 'ovl_scan_f32_static_status', 'ovl_scan_f32_begin',
            'ovl_scan_f32_finish', 'ovl_selftest_scan_timeout', 'ovl_peer_buffer_bytes', 'ovl_peer_alloc',
-           'ovl_peer_open', 'ovl_peer_close', 'ovl_peer_free', 'ovl_scan_f32_begin_peer', 'ovl_scan_f32_finish_peer']
+           'ovl_peer_open', 'ovl_peer_close', 'ovl_peer_free', 'ovl_scan_f32_begin_peer', 'ovl_scan_f32_finish_peer',
+           'ovl_selective_scan_workspace_bytes', 'ovl_selective_scan', 'ovl_selective_scan_backward',
+           'ovl_selective_scan_step', 'ovl_causal_conv_workspace_bytes', 'ovl_causal_conv', 'ovl_causal_conv_backward',
+           'ovl_causal_conv_step', 'ovl_rms_norm_workspace_bytes', 'ovl_rms_norm', 'ovl_rms_norm_backward']
 
 _lib = None
 
@@ -97,6 +100,16 @@ def library():
     lib.ovl_scan_f32_finish_peer.argtypes = [ctypes.c_int, vp, vp, u64, vp, u64, pxp, vp]
     lib.ovl_scan_f32_static.argtypes = [ctypes.c_int, vp, vp, u64, u64, vp, vp]
     lib.ovl_scan_f32_static_status.argtypes = [vp, ctypes.POINTER(i32)]
+    # the argument structures of the sequence operators travel as packed bytes (all fields are 8 bytes wide)
+    for name in ('ovl_selective_scan', 'ovl_selective_scan_backward', 'ovl_selective_scan_step', 'ovl_causal_conv',
+                 'ovl_causal_conv_backward', 'ovl_causal_conv_step', 'ovl_rms_norm', 'ovl_rms_norm_backward'):
+        getattr(lib, name).argtypes = [ctypes.c_char_p, vp]
+    lib.ovl_selective_scan_workspace_bytes.restype = u64
+    lib.ovl_selective_scan_workspace_bytes.argtypes = [ctypes.c_char_p, ctypes.c_int]
+    lib.ovl_causal_conv_workspace_bytes.restype = u64
+    lib.ovl_causal_conv_workspace_bytes.argtypes = [ctypes.c_char_p]
+    lib.ovl_rms_norm_workspace_bytes.restype = u64
+    lib.ovl_rms_norm_workspace_bytes.argtypes = [ctypes.c_char_p]
     _lib = lib
     return lib
 
