@@ -9,8 +9,8 @@
 //
 // Layout.  A channel is P lanes of a warp with 4 states each (P = 1 ... 32: up to 128 states); a block is 128 threads
 // (256 for P = 32) = CH channels of one group of one batch.  Tokens come in tiles of STEPS: while a tile is scanned the
-// next one's elements are in flight to registers; they are converted, masked and combined (softplus, dt * u) into
-// shared memory, double-buffered, with one barrier per tile.  The sums over the states of P steps are formed together
+// next one's elements are in flight to shared memory, each to the thread that will convert, mask and combine them
+// (softplus, dt * u) into what all lanes of a channel read; double-buffered, with one barrier per tile.  The sums over the states of P steps are formed together
 // (reduce_lanes: less than one exchange per step), and the same threads that loaded u and z finish the outputs.
 #include "ovl_sequence.cuh"
 
@@ -26,7 +26,7 @@ struct ScanDims {
     int64_t group_channels, tiles;     // channels of a group, channel tiles of a group
     int64_t segments, segment_length;  // the length cut into segments (a multiple of 32) that run side by side
     int32_t softplus, vec;             // vec: wide loads and stores of channel vectors
-    int32_t vec_states;                // wide loads and stores of 4 states
+    int32_t vec_states, vec_bc;        // wide loads and stores of 4 states; of 4 elements of B and C
 };
 
 struct ScanParams {
@@ -94,24 +94,51 @@ __device__ __forceinline__ Place block_place(const ScanDims& d, int ch) {
     return p;
 }
 
+// exp(dt A) = 2^(dt A log2 e).  The special-function unit's results are 1e-8 to 2e-8 too small on average, which adds up
+// over a state's memory of a thousand tokens; the same amount on the exponent takes most of it away and costs nothing
+// (a multiplication becomes a multiply-add).  2^kExpBias rounds to 1, so dt = 0 still leaves a state as it is.
+constexpr float kExpBias = 2e-8f;
+__device__ __forceinline__ F2 decay(F2 A, F2 dt) { return exp2_pair(fma2(A, dt, same2(kExpBias))); }
+
+// Where (dt, dt, dt u, dt u) of channel c of a tile's token t stands, in float4: a gap after every 8 channels keeps the
+// wide stores of threads with 8 (or 4) channels each off one another's banks.
+template <int CH>
+__device__ __forceinline__ constexpr int du_at(int t, int c) { return t * (CH + CH / 8) + c + c / 8; }
+
 // ---------------------------------------------------------------------------------------------------------
 // forward
+
+template <typename T, int P>
+struct ForwardSmem {
+    using S = Shape<P>;
+    static constexpr size_t du = 0;                                                          // float4 [2][du_at]
+    static constexpr size_t b = du + 2 * sizeof(float4) * S::STEPS * (S::CH + S::CH / 8);    // float [2][STEPS][NP]
+    static constexpr size_t c = b + 2 * sizeof(float) * S::STEPS * S::NP;
+    static constexpr size_t y = c + 2 * sizeof(float) * S::STEPS * S::NP;                    // float [2][STEPS][ROW]
+    static constexpr size_t raw = y + 2 * sizeof(float) * S::STEPS * S::ROW;                 // T [2][3][STEPS][CH]: u, delta, z
+    static constexpr size_t raw_bc = raw + 2 * 3 * sizeof(T) * S::STEPS * S::CH;             // T [2][2][STEPS][NP]
+    static constexpr size_t bytes = raw_bc + 2 * 2 * sizeof(T) * S::STEPS * S::NP;
+};
 
 // LOCAL: only what a segment adds to a state that starts at zero, and its sum of dt (the first of two passes when the
 // length is cut into segments); otherwise the whole operator, seeded from the segments before.
 template <typename T, int P, bool LOCAL>
 __global__ void __launch_bounds__(Shape<P>::THREADS) scan_forward(const __grid_constant__ ScanParams p) {
     using S = Shape<P>;
+    using M = ForwardSmem<T, P>;
     constexpr int THREADS = S::THREADS, CH = S::CH, NP = S::NP, STEPS = S::STEPS, ROW = S::ROW;
     constexpr int CHV = CH / 8, ITEMS = STEPS * CHV;                     // 8 channels of one token
-    constexpr int BCN = (STEPS * NP + THREADS - 1) / THREADS;
-    constexpr int V = P < 16 ? P : 16;                                   // steps whose sums are formed together
+    constexpr int QUADS = STEPS * P, QN = (QUADS + THREADS - 1) / THREADS;   // 4 states of one token
+    constexpr int V = STEPS < 16 ? STEPS : 16;                           // steps whose sums are formed together
     static_assert(ITEMS <= THREADS && STEPS % V == 0 && kCheckpoint % V == 0, "tile shape");
-    extern __shared__ __align__(16) float smem[];
-    float2* const s_du = reinterpret_cast<float2*>(smem);                // [2][STEPS][CH] (dt, dt * u)
-    float* const s_b = smem + 2 * STEPS * CH * 2;                        // [2][STEPS][NP]
-    float* const s_c = s_b + 2 * STEPS * NP;                             // [2][STEPS][NP]
-    float* const s_y = s_c + 2 * STEPS * NP;                             // [2][STEPS][ROW]
+    extern __shared__ __align__(16) char smem[];
+    float4* const s_du = reinterpret_cast<float4*>(smem + M::du);
+    float* const s_b = reinterpret_cast<float*>(smem + M::b);
+    float* const s_c = reinterpret_cast<float*>(smem + M::c);
+    float* const s_y = reinterpret_cast<float*>(smem + M::y);
+    T* const raw = reinterpret_cast<T*>(smem + M::raw);
+    T* const raw_bc = reinterpret_cast<T*>(smem + M::raw_bc);
+    constexpr int DU = STEPS * (CH + CH / 8);
 
     const OvlSelectiveScan& a = p.a;
     const ScanDims& d = p.d;
@@ -128,7 +155,7 @@ __global__ void __launch_bounds__(Shape<P>::THREADS) scan_forward(const __grid_c
     // this thread's part of a tile: 8 channels of one token
     const bool has_item = tid < ITEMS;
     const int item_t = tid / CHV, item_c = (tid % CHV) * 8;
-    const int item_valid = has_item ? (int)(at.n_channels - item_c < 8 ? at.n_channels - item_c : 8) : 0;
+    const int item_valid = !has_item || item_c >= at.n_channels ? 0 : at.n_channels - item_c < 8 ? (int)(at.n_channels - item_c) : 8;
     const bool item_vec = d.vec && item_valid == 8;
     const T* const u = reinterpret_cast<const T*>(a.u) + at.batch * a.u_batch + at.channel0 + item_c;
     const T* const delta = reinterpret_cast<const T*>(a.delta) + at.batch * a.delta_batch + at.channel0 + item_c;
@@ -136,6 +163,7 @@ __global__ void __launch_bounds__(Shape<P>::THREADS) scan_forward(const __grid_c
     T* const out = reinterpret_cast<T*>(a.out) + at.batch * d.length * d.channels + at.channel0 + item_c;
     const T* const B = reinterpret_cast<const T*>(a.B) + at.batch * a.B_batch + at.group * a.B_group;
     const T* const C = reinterpret_cast<const T*>(a.C) + at.batch * a.C_batch + at.group * a.C_group;
+    T* const slot = raw + tid * 8;                                       // u; delta and z follow a tile's elements later
     float skip[8], bias[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -143,60 +171,70 @@ __global__ void __launch_bounds__(Shape<P>::THREADS) scan_forward(const __grid_c
         bias[i] = a.delta_bias && i < item_valid ? a.delta_bias[at.channel0 + item_c + i] : 0.0f;
     }
 
-    Pack<T, 8> raw_u, raw_d, raw_z, next_u, next_d, next_z;
-    T raw_b[BCN], raw_c[BCN];
-    auto fetch = [&](int64_t t0) {
+    auto fetch = [&](int64_t t0, int buf) {
         const int64_t t = t0 + item_t;
-        const int valid = t < t_used ? item_valid : 0;
-        const bool vec = item_vec && valid == 8;
-        if (has_item) {
-            next_u = load_pack<T, 8>(u + t * a.u_token, vec, valid);
-            next_d = load_pack<T, 8>(delta + t * a.delta_token, vec, valid);
-            if (!LOCAL && z) next_z = load_pack<T, 8>(z + t * a.z_token, vec, valid);
+        if (item_valid > 0 && t < t_used) {
+            T* const to = slot + buf * 3 * STEPS * CH;
+            fetch_pack<T, 8>(to, u + t * a.u_token, item_vec, item_valid);
+            fetch_pack<T, 8>(to + STEPS * CH, delta + t * a.delta_token, item_vec, item_valid);
+            if (!LOCAL && z) fetch_pack<T, 8>(to + 2 * STEPS * CH, z + t * a.z_token, item_vec, item_valid);
         }
 #pragma unroll
-        for (int k = 0; k < BCN; ++k) {
-            const int e = tid + k * THREADS;
-            const int64_t tt = t0 + e / NP;
-            const int n = e % NP;
-            const bool in = e < STEPS * NP && tt < t_used && n < states;
-            raw_b[k] = in ? B[tt * a.B_token + n] : from_f32<T>(0.0f);
-            if (!LOCAL) raw_c[k] = in ? C[tt * a.C_token + n] : from_f32<T>(0.0f);
+        for (int k = 0; k < QN; ++k) {
+            const int e = tid + k * THREADS, n = e % P * 4;
+            const int64_t tt = t0 + e / P;
+            if (e < QUADS && tt < t_used && n < states) {
+                T* const to = raw_bc + buf * 2 * STEPS * NP + e * 4;
+                const bool vec = d.vec_bc && n + 4 <= states;
+                fetch_pack<T, 4>(to, B + tt * a.B_token + n, vec, states - n);
+                if (!LOCAL) fetch_pack<T, 4>(to + STEPS * NP, C + tt * a.C_token + n, vec, states - n);
+            }
         }
+        copy_commit();
     };
     auto stage = [&](int64_t t0, int buf) {
-        raw_u = next_u;
-        raw_d = next_d;
-        if (!LOCAL && z) raw_z = next_z;
         if (has_item) {
             const bool in = t0 + item_t < t_used;
-            float2 du[8];
+            float x[8], dt[8];
+            read_slot<T, 8>(slot + buf * 3 * STEPS * CH, x);
+            read_slot<T, 8>(slot + (buf * 3 + 1) * STEPS * CH, dt);
+            float4* const to = s_du + buf * DU + du_at<CH>(item_t, item_c);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                float dt = to_f32(raw_d.v[i]) + bias[i];
-                if (d.softplus) dt = softplus(dt);
-                // padding leaves the state as it is: dt = 0 makes the factor 1 and the addend 0
-                du[i] = in ? make_float2(dt, dt * to_f32(raw_u.v[i])) : make_float2(0.0f, 0.0f);
+            for (int i = 0; i < 8; i += 2) {
+                float e0, e1;
+                dt[i] += bias[i];
+                dt[i + 1] += bias[i + 1];
+                if (d.softplus) softplus_pair(dt[i], dt[i + 1], e0, e1);
+#pragma unroll
+                for (int k = i; k < i + 2; ++k) {
+                    // padding leaves the state as it is: dt = 0 makes the factor 1 and the addend 0
+                    const float s = in && k < item_valid ? dt[k] : 0.0f, su = in && k < item_valid ? dt[k] * x[k] : 0.0f;
+                    to[k] = make_float4(s, s, su, su);
+                }
             }
-            float4* const to = reinterpret_cast<float4*>(s_du + (buf * STEPS + item_t) * CH + item_c);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) to[i] = make_float4(du[2 * i].x, du[2 * i].y, du[2 * i + 1].x, du[2 * i + 1].y);
         }
 #pragma unroll
-        for (int k = 0; k < BCN; ++k) {
+        for (int k = 0; k < QN; ++k) {
             const int e = tid + k * THREADS;
-            if (e < STEPS * NP) {
-                s_b[buf * STEPS * NP + e] = to_f32(raw_b[k]);
-                if (!LOCAL) s_c[buf * STEPS * NP + e] = to_f32(raw_c[k]);
+            if (e < QUADS) {
+                const bool in = t0 + e / P < t_used && e % P * 4 < states;
+                float x[4];
+                read_slot<T, 4>(raw_bc + buf * 2 * STEPS * NP + e * 4, x);
+                const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                reinterpret_cast<float4*>(s_b + buf * STEPS * NP)[e] = in ? make_float4(x[0], x[1], x[2], x[3]) : zero;
+                if (!LOCAL) {
+                    read_slot<T, 4>(raw_bc + (buf * 2 + 1) * STEPS * NP + e * 4, x);
+                    reinterpret_cast<float4*>(s_c + buf * STEPS * NP)[e] = in ? make_float4(x[0], x[1], x[2], x[3]) : zero;
+                }
             }
         }
     };
 
-    // exp(dt A) = 2^(dt A log2 e); padded states have A = B = C = 0
+    // padded states have A = B = C = 0
     const float4 A4 = load_states(a.A + channel * states, 4 * j, states, d.vec_states);
     const F2 A01 = pack2(A4.x * kLog2e, A4.y * kLog2e), A23 = pack2(A4.z * kLog2e, A4.w * kLog2e);
-    F2 h01 = pack2(0.0f, 0.0f), h23 = h01;
-    if (t_begin < t_used) fetch(t_begin);
+    F2 h01 = same2(0.0f), h23 = h01;
+    if (t_begin < t_used) fetch(t_begin, 0);
     if (!LOCAL) {
         const int64_t row = (at.batch * d.channels + channel) * states;
         if (a.initial_state) {
@@ -207,25 +245,24 @@ __global__ void __launch_bounds__(Shape<P>::THREADS) scan_forward(const __grid_c
         // the state in front of this segment: h <- exp(A sum dt) h + (what the segment adds), segment by segment
         for (int64_t s = 0; s < at.segment; ++s) {
             const int64_t cell = (at.batch * d.segments + s) * d.channels + channel;
-            const float sum = p.seg_dt[cell];
+            const F2 sum = same2(p.seg_dt[cell]);
             const float4 add = load_states(p.seg_state + cell * states, 4 * j, states, d.vec_states);
-            const F2 s2 = pack2(sum, sum);
-            h01 = fma2(exp2_pair(mul2(A01, s2)), h01, pack2(add.x, add.y));
-            h23 = fma2(exp2_pair(mul2(A23, s2)), h23, pack2(add.z, add.w));
+            h01 = fma2(decay(A01, sum), h01, pack2(add.x, add.y));
+            h23 = fma2(decay(A23, sum), h23, pack2(add.z, add.w));
         }
     }
     float sum_dt = 0.0f;
+    copy_wait();
     if (t_begin < t_used) stage(t_begin, 0);
     __syncthreads();
 
     int buf = 0;
     for (int64_t t0 = t_begin; t0 < t_used; t0 += STEPS, buf ^= 1) {
         const bool more = t0 + STEPS < t_used;
-        Pack<T, 8> done_u, done_z;
-        if (more) fetch(t0 + STEPS);
-        const float2* const du_row = s_du + buf * STEPS * CH + c;
-        const float* const b_row = s_b + buf * STEPS * NP + 4 * j;
-        const float* const c_row = s_c + buf * STEPS * NP + 4 * j;
+        if (more) fetch(t0 + STEPS, buf ^ 1);
+        const float4* const du_row = s_du + buf * DU + du_at<CH>(0, c);
+        const float4* const b_row = reinterpret_cast<const float4*>(s_b + buf * STEPS * NP) + j;
+        const float4* const c_row = reinterpret_cast<const float4*>(s_c + buf * STEPS * NP) + j;
 #pragma unroll 1
         for (int g = 0; g < STEPS / V; ++g) {
             if (!LOCAL && a.checkpoints && (t0 + g * V) % kCheckpoint == 0 && live && t0 + g * V < d.length) {
@@ -240,15 +277,14 @@ __global__ void __launch_bounds__(Shape<P>::THREADS) scan_forward(const __grid_c
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 const int t = g * V + i;
-                const float2 du = du_row[t * CH];
-                const float4 b = *reinterpret_cast<const float4*>(b_row + t * NP);
-                const F2 dt2 = pack2(du.x, du.x), du2 = pack2(du.y, du.y);
-                h01 = fma2(exp2_pair(mul2(A01, dt2)), h01, mul2(du2, pack2(b.x, b.y)));
-                h23 = fma2(exp2_pair(mul2(A23, dt2)), h23, mul2(du2, pack2(b.z, b.w)));
+                const float4 du = du_row[t * (CH + CH / 8)], b = b_row[t * P];
+                const F2 dt2 = pack2(du.x, du.y), du2 = pack2(du.z, du.w);
+                h01 = fma2(decay(A01, dt2), h01, mul2(du2, pack2(b.x, b.y)));
+                h23 = fma2(decay(A23, dt2), h23, mul2(du2, pack2(b.z, b.w)));
                 if (LOCAL) {
                     sum_dt += du.x;
                 } else {
-                    const float4 cc = *reinterpret_cast<const float4*>(c_row + t * NP);
+                    const float4 cc = c_row[t * P];
                     y[i] = sum2(fma2(h23, pack2(cc.z, cc.w), mul2(h01, pack2(cc.x, cc.y))));
                 }
             }
@@ -261,23 +297,21 @@ __global__ void __launch_bounds__(Shape<P>::THREADS) scan_forward(const __grid_c
                 }
             }
         }
-        if (!LOCAL) {
-            done_u = raw_u;
-            if (z) done_z = raw_z;
+        if (more) {
+            copy_wait();
+            stage(t0 + STEPS, buf ^ 1);
         }
-        if (more) stage(t0 + STEPS, buf ^ 1);
         __syncthreads();
-        if (!LOCAL && has_item && t0 + item_t < t_end) {
+        if (!LOCAL && item_valid > 0 && t0 + item_t < t_end) {
             const int64_t t = t0 + item_t;
             const float* const y = s_y + (buf * STEPS + item_t) * ROW + item_c;
-            float o[8];
+            float o[8], x[8], g[8];
+            read_slot<T, 8>(slot + buf * 3 * STEPS * CH, x);
+            if (z) read_slot<T, 8>(slot + (buf * 3 + 2) * STEPS * CH, g);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                o[i] = fmaf(skip[i], to_f32(done_u.v[i]), y[i]);
-                if (z) {
-                    const float g = to_f32(done_z.v[i]);
-                    o[i] *= g * sigmoid(g);
-                }
+                o[i] = fmaf(skip[i], x[i], y[i]);
+                if (z) o[i] *= silu(g[i]);
                 if (t >= t_used) o[i] = 0.0f;
             }
             store_pack<T, 8>(out + t * d.channels, o, item_vec, item_valid);
@@ -296,7 +330,7 @@ __global__ void __launch_bounds__(Shape<P>::THREADS) scan_forward(const __grid_c
     }
     // outputs of padding behind the last tile
     const int64_t covered = t_used > t_begin ? t_begin + (t_used - t_begin + STEPS - 1) / STEPS * STEPS : t_begin;
-    if (has_item) {
+    if (item_valid > 0) {
         const float zero[8] = {};
         for (int64_t t = covered + item_t; t < t_end; t += STEPS)
             store_pack<T, 8>(out + t * d.channels, zero, item_vec, item_valid);
@@ -307,12 +341,6 @@ __global__ void __launch_bounds__(Shape<P>::THREADS) scan_forward(const __grid_c
         unpack2(h23, h.z, h.w);
         store_states(a.final_state + (at.batch * d.channels + channel) * states, h, 4 * j, states, d.vec_states);
     }
-}
-
-template <int P>
-constexpr size_t forward_smem() {
-    using S = Shape<P>;
-    return sizeof(float) * 2 * (size_t)(S::STEPS * S::CH * 2 + 2 * S::STEPS * S::NP + S::STEPS * S::ROW);
 }
 
 // ---------------------------------------------------------------------------------------------------------
@@ -326,7 +354,7 @@ constexpr size_t forward_smem() {
 //                                                   from partial sums (no atomics: the same bits every time)
 //   w_t = a_t gh_t (handed to the token before), q = w_t h_{t-1}: gA = sum q dt, g(dt) = sum_n q A + u sum_n gh B,
 //   gu = dt sum_n gh B + D gy
-template <int P>
+template <typename T, int P>
 struct BackShape {
     using S = Shape<P>;
     static constexpr int STEPS = kCheckpoint;
@@ -334,26 +362,40 @@ struct BackShape {
     static constexpr int CHV = S::CH / 4;                                // 4 channels of one token per item
     static constexpr int ITEMS = STEPS * CHV;
     static constexpr int IPT = (ITEMS + S::THREADS - 1) / S::THREADS;
-    static constexpr int ROW = S::CH + (P >= 8 ? 4 : 32 / P);
-    static constexpr size_t floats = STEPS * S::CH * 3 + 2 * STEPS * S::NP + 3 * STEPS * ROW + WARPS * STEPS * 2 * S::NP;
+    static constexpr int ROW = S::ROW;
+    // shared memory
+    static constexpr size_t du = 0;                                                    // float4 [du_at]
+    static constexpr size_t gy = du + sizeof(float4) * STEPS * (S::CH + S::CH / 8);    // float2 [STEPS][CH] (gy, gy)
+    static constexpr size_t b = gy + sizeof(float2) * STEPS * S::CH;                   // float [STEPS][NP]
+    static constexpr size_t c = b + sizeof(float) * STEPS * S::NP;
+    static constexpr size_t y = c + sizeof(float) * STEPS * S::NP;                     // float [STEPS][ROW]: C . h
+    static constexpr size_t s = y + sizeof(float) * STEPS * ROW;                       // float [2][STEPS][ROW]: gh . B, q . A / ln 2
+    static constexpr size_t r = s + 2 * sizeof(float) * STEPS * ROW;                   // float [WARPS][STEPS][2][NP]: gC, gB
+    static constexpr size_t keep = r + sizeof(float) * WARPS * STEPS * 2 * S::NP;      // float4 [2][STEPS][CH / 4]
+    static constexpr size_t raw = keep + 2 * sizeof(float) * STEPS * S::CH;            // T [2][4][STEPS][CH]: u, delta, z, gout
+    static constexpr size_t raw_bc = raw + 2 * 4 * sizeof(T) * STEPS * S::CH;          // T [2][STEPS][NP]
+    static constexpr size_t bytes = raw_bc + 2 * sizeof(T) * STEPS * S::NP;
 };
 
 template <typename T, int P, bool LOCAL>
 __global__ void __launch_bounds__(Shape<P>::THREADS) scan_backward(const __grid_constant__ ScanParams p) {
     using S = Shape<P>;
-    using Bk = BackShape<P>;
-    constexpr int THREADS = S::THREADS, CH = S::CH, NP = S::NP, STEPS = Bk::STEPS, ROW = Bk::ROW, WARPS = Bk::WARPS;
-    constexpr int CHV = Bk::CHV, ITEMS = Bk::ITEMS, IPT = Bk::IPT;
-    constexpr int BCN = (STEPS * NP + THREADS - 1) / THREADS;
+    using M = BackShape<T, P>;
+    constexpr int THREADS = S::THREADS, CH = S::CH, NP = S::NP, STEPS = M::STEPS, ROW = M::ROW, WARPS = M::WARPS;
+    constexpr int CHV = M::CHV, ITEMS = M::ITEMS, IPT = M::IPT;
+    constexpr int QUADS = STEPS * P, QN = (QUADS + THREADS - 1) / THREADS;
     constexpr int R = 32 / P;                                            // channels of a warp
-    extern __shared__ __align__(16) float smem[];
-    float2* const s_du = reinterpret_cast<float2*>(smem);                // [STEPS][CH] (dt, dt * u)
-    float* const s_gy = smem + STEPS * CH * 2;                           // [STEPS][CH]
-    float* const s_b = s_gy + STEPS * CH;                                // [STEPS][NP]
-    float* const s_c = s_b + STEPS * NP;                                 // [STEPS][NP]
-    float* const s_y = s_c + STEPS * NP;                                 // [STEPS][ROW] C . h
-    float* const s_s = s_y + STEPS * ROW;                                // [2][STEPS][ROW] sum_n gh B, sum_n q A / ln 2
-    float* const s_r = s_s + 2 * STEPS * ROW;                            // [WARPS][STEPS][2][NP] gC, gB of the warps
+    extern __shared__ __align__(16) char smem[];
+    float4* const s_du = reinterpret_cast<float4*>(smem + M::du);
+    float2* const s_gy = reinterpret_cast<float2*>(smem + M::gy);
+    float* const s_b = reinterpret_cast<float*>(smem + M::b);
+    float* const s_c = reinterpret_cast<float*>(smem + M::c);
+    float* const s_y = reinterpret_cast<float*>(smem + M::y);
+    float* const s_s = reinterpret_cast<float*>(smem + M::s);
+    float* const s_r = reinterpret_cast<float*>(smem + M::r);
+    float4* const s_keep = reinterpret_cast<float4*>(smem + M::keep);    // derivative of dt by delta, of out by z / y
+    T* const raw = reinterpret_cast<T*>(smem + M::raw);
+    T* const raw_bc = reinterpret_cast<T*>(smem + M::raw_bc);
 
     const OvlSelectiveScan& a = p.a;
     const ScanDims& d = p.d;
@@ -377,8 +419,6 @@ __global__ void __launch_bounds__(Shape<P>::THREADS) scan_backward(const __grid_
     const T* const B = reinterpret_cast<const T*>(a.B) + at.batch * a.B_batch + at.group * a.B_group;
     const T* const C = reinterpret_cast<const T*>(a.C) + at.batch * a.C_batch + at.group * a.C_group;
 
-    Pack<T, 4> raw_u[IPT], raw_d[IPT], raw_z[IPT], raw_g[IPT];
-    T raw_b[BCN], raw_c[BCN];
     float4 start;                                                        // the saved state in front of the tile
     auto item_of = [&](int k, int& t, int& cc, int& valid) {
         const int e = tid + k * THREADS;
@@ -387,29 +427,33 @@ __global__ void __launch_bounds__(Shape<P>::THREADS) scan_backward(const __grid_
         const int64_t left = at.n_channels - cc;
         valid = e >= ITEMS || left <= 0 ? 0 : left < 4 ? (int)left : 4;
     };
-    auto fetch = [&](int64_t t0) {
+    auto slot_of = [&](int buf, int which, int k) { return raw + ((buf * 4 + which) * ITEMS + tid + k * THREADS) * 4; };
+    auto fetch = [&](int64_t t0, int buf) {
 #pragma unroll
         for (int k = 0; k < IPT; ++k) {
             int it, cc, valid;
             item_of(k, it, cc, valid);
             const int64_t t = t0 + it;
-            if (t >= t_used) valid = 0;
-            const bool vec = d.vec && valid == 4;
-            if (!LOCAL) raw_u[k] = load_pack<T, 4>(u + t * a.u_token + cc, vec, valid);
-            raw_d[k] = load_pack<T, 4>(delta + t * a.delta_token + cc, vec, valid);
-            if (z) raw_z[k] = load_pack<T, 4>(z + t * a.z_token + cc, vec, valid);
-            raw_g[k] = load_pack<T, 4>(gout + t * a.gout_token + cc, vec, valid);
+            if (valid > 0 && t < t_used) {
+                const bool vec = d.vec && valid == 4;
+                if (!LOCAL) fetch_pack<T, 4>(slot_of(buf, 0, k), u + t * a.u_token + cc, vec, valid);
+                fetch_pack<T, 4>(slot_of(buf, 1, k), delta + t * a.delta_token + cc, vec, valid);
+                if (z) fetch_pack<T, 4>(slot_of(buf, 2, k), z + t * a.z_token + cc, vec, valid);
+                fetch_pack<T, 4>(slot_of(buf, 3, k), gout + t * a.gout_token + cc, vec, valid);
+            }
         }
 #pragma unroll
-        for (int k = 0; k < BCN; ++k) {
-            const int e = tid + k * THREADS;
-            const int64_t t = t0 + e / NP;
-            const int n = e % NP;
-            const bool in = e < STEPS * NP && t < t_used && n < states;
-            if (!LOCAL) raw_b[k] = in ? B[t * a.B_token + n] : from_f32<T>(0.0f);
-            raw_c[k] = in ? C[t * a.C_token + n] : from_f32<T>(0.0f);
+        for (int k = 0; k < QN; ++k) {
+            const int e = tid + k * THREADS, n = e % P * 4;
+            const int64_t t = t0 + e / P;
+            if (e < QUADS && t < t_used && n < states) {
+                const bool vec = d.vec_bc && n + 4 <= states;
+                if (!LOCAL) fetch_pack<T, 4>(raw_bc + e * 4, B + t * a.B_token + n, vec, states - n);
+                fetch_pack<T, 4>(raw_bc + STEPS * NP + e * 4, C + t * a.C_token + n, vec, states - n);
+            }
         }
-        if (!LOCAL)
+        copy_commit();
+        if (!LOCAL && live)
             start = load_states(a.checkpoints + ((at.batch * chunks + t0 / kCheckpoint) * d.channels + channel) * states,
                                 4 * j, states, d.vec_states);
     };
@@ -424,43 +468,78 @@ __global__ void __launch_bounds__(Shape<P>::THREADS) scan_backward(const __grid_
             skip[k][i] = a.D && i < valid ? a.D[base_c + cc + i] : 0.0f;
         }
     }
-    auto stage = [&](int64_t t0) {
+    auto stage = [&](int64_t t0, int buf) {
 #pragma unroll
         for (int k = 0; k < IPT; ++k) {
             int it, cc, valid;
             item_of(k, it, cc, valid);
             if (tid + k * THREADS < ITEMS) {
                 const bool in = t0 + it < t_used;
+                float x[4], dt[4], zz[4], g[4], slope[4], gate_slope[4];
+                if (!LOCAL) read_slot<T, 4>(slot_of(buf, 0, k), x);
+                read_slot<T, 4>(slot_of(buf, 1, k), dt);
+                if (z) read_slot<T, 4>(slot_of(buf, 2, k), zz);
+                read_slot<T, 4>(slot_of(buf, 3, k), g);
+#pragma unroll
+                for (int i = 0; i < 4; i += 2) {
+                    dt[i] += bias[k][i];
+                    dt[i + 1] += bias[k][i + 1];
+                    if (d.softplus) {
+                        const float x0 = dt[i], x1 = dt[i + 1];
+                        float e0, e1;
+                        softplus_pair(dt[i], dt[i + 1], e0, e1);
+                        // the derivative 1 / (1 + e^-x) from e = e^-|x|
+                        const float r0 = rcp_approx(1.0f + e0), r1 = rcp_approx(1.0f + e1);
+                        slope[i] = x0 < 0.0f ? e0 * r0 : r0;
+                        slope[i + 1] = x1 < 0.0f ? e1 * r1 : r1;
+                    } else {
+                        slope[i] = slope[i + 1] = 1.0f;
+                    }
+                }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    float dt = to_f32(raw_d[k].v[i]) + bias[k][i];
-                    if (d.softplus) dt = softplus(dt);
-                    float gy = to_f32(raw_g[k].v[i]);
+                    const bool ok = in && i < valid;
+                    gate_slope[i] = 0.0f;
                     if (z) {
-                        const float g = to_f32(raw_z[k].v[i]);
-                        gy *= g * sigmoid(g);
+                        const float sig = sigmoid(zz[i]), gate = zz[i] * sig;
+                        gate_slope[i] = g[i] * fmaf(gate, 1.0f - sig, sig);
+                        g[i] *= gate;
                     }
-                    const float du = LOCAL ? 0.0f : dt * to_f32(raw_u[k].v[i]);
-                    s_du[it * CH + cc + i] = in ? make_float2(dt, du) : make_float2(0.0f, 0.0f);
-                    s_gy[it * CH + cc + i] = in ? gy : 0.0f;
+                    const float s = ok ? dt[i] : 0.0f, su = ok && !LOCAL ? dt[i] * x[i] : 0.0f, gy = ok ? g[i] : 0.0f;
+                    s_du[du_at<CH>(it, cc + i)] = make_float4(s, s, su, su);
+                    s_gy[it * CH + cc + i] = make_float2(gy, gy);
+                }
+                if (!LOCAL) {
+                    s_keep[tid + k * THREADS] = make_float4(slope[0], slope[1], slope[2], slope[3]);
+                    s_keep[ITEMS + tid + k * THREADS] = make_float4(gate_slope[0], gate_slope[1], gate_slope[2], gate_slope[3]);
                 }
             }
         }
 #pragma unroll
-        for (int k = 0; k < BCN; ++k) {
+        for (int k = 0; k < QN; ++k) {
             const int e = tid + k * THREADS;
-            if (e < STEPS * NP) {
-                if (!LOCAL) s_b[e] = to_f32(raw_b[k]);
-                s_c[e] = to_f32(raw_c[k]);
+            if (e < QUADS) {
+                const bool in = t0 + e / P < t_used && e % P * 4 < states;
+                const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                float x[4];
+                if (!LOCAL) {
+                    read_slot<T, 4>(raw_bc + e * 4, x);
+                    reinterpret_cast<float4*>(s_b)[e] = in ? make_float4(x[0], x[1], x[2], x[3]) : zero;
+                }
+                read_slot<T, 4>(raw_bc + STEPS * NP + e * 4, x);
+                reinterpret_cast<float4*>(s_c)[e] = in ? make_float4(x[0], x[1], x[2], x[3]) : zero;
             }
         }
     };
 
-    const float4 A4 = load_states(a.A + channel * states, 4 * j, states, d.vec_states);
+    // lanes without a channel have A = h = gh = 0: their sums over channels are zeros
+    const float4 zero4 = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const float4 A4 = live ? load_states(a.A + channel * states, 4 * j, states, d.vec_states) : zero4;
     const F2 A01 = pack2(A4.x * kLog2e, A4.y * kLog2e), A23 = pack2(A4.z * kLog2e, A4.w * kLog2e);
-    F2 w01 = pack2(0.0f, 0.0f), w23 = w01;                               // a_{t+1} gh_{t+1}
-    if (last >= first) fetch(last);
-    if (!LOCAL) {
+    F2 w01 = same2(0.0f), w23 = w01;                                     // a_{t+1} gh_{t+1}
+    start = zero4;
+    if (last >= first) fetch(last, 0);
+    if (!LOCAL && live) {
         if (a.gfinal) {
             const float4 g = load_states(a.gfinal + (at.batch * d.channels + channel) * states, 4 * j, states, d.vec_states);
             w01 = pack2(g.x, g.y);
@@ -468,96 +547,82 @@ __global__ void __launch_bounds__(Shape<P>::THREADS) scan_backward(const __grid_
         }
         for (int64_t s = d.segments - 1; s > at.segment; --s) {
             const int64_t cell = (at.batch * d.segments + s) * d.channels + channel;
-            const float sum = p.seg_dt[cell];
+            const F2 sum = same2(p.seg_dt[cell]);
             const float4 add = load_states(p.seg_state + cell * states, 4 * j, states, d.vec_states);
-            const F2 s2 = pack2(sum, sum);
-            w01 = fma2(exp2_pair(mul2(A01, s2)), w01, pack2(add.x, add.y));
-            w23 = fma2(exp2_pair(mul2(A23, s2)), w23, pack2(add.z, add.w));
+            w01 = fma2(decay(A01, sum), w01, pack2(add.x, add.y));
+            w23 = fma2(decay(A23, sum), w23, pack2(add.z, add.w));
         }
     }
     double gA[4] = {0.0, 0.0, 0.0, 0.0};
     float gD[IPT][4] = {}, gbias[IPT][4] = {};
     float sum_dt = 0.0f;
+    const float4* const du_row = s_du + du_at<CH>(0, c);
+    const float2* const gy_row = s_gy + c;
+    const float4* const b_row = reinterpret_cast<const float4*>(s_b) + j;
+    const float4* const c_row = reinterpret_cast<const float4*>(s_c) + j;
 
-    for (int64_t t0 = last; t0 >= first; t0 -= STEPS) {
-        stage(t0);
-        F2 h01[STEPS], h23[STEPS], a01[STEPS], a23[STEPS];
-        const F2 s01 = pack2(start.x, start.y), s23 = pack2(start.z, start.w);
-        Pack<T, 4> now_u[IPT], now_d[IPT], now_z[IPT], now_g[IPT];
-#pragma unroll
-        for (int k = 0; k < IPT; ++k) {
-            now_u[k] = raw_u[k];
-            now_d[k] = raw_d[k];
-            now_z[k] = raw_z[k];
-            now_g[k] = raw_g[k];
-        }
+    int buf = 0;
+    for (int64_t t0 = last; t0 >= first; t0 -= STEPS, buf ^= 1) {
+        copy_wait();
+        stage(t0, buf);
+        F2 h01[STEPS + 1], h23[STEPS + 1], a01[STEPS], a23[STEPS];       // h[t] is the state in front of step t
+        h01[0] = pack2(start.x, start.y);
+        h23[0] = pack2(start.z, start.w);
         __syncthreads();
-        if (t0 > first) fetch(t0 - STEPS);
+        if (t0 > first) fetch(t0 - STEPS, buf ^ 1);
 
         // the states again, forwards
-        F2 x01 = s01, x23 = s23;
 #pragma unroll
         for (int t = 0; t < STEPS; ++t) {
-            const float2 du = s_du[t * CH + c];
-            const F2 dt2 = pack2(du.x, du.x);
-            a01[t] = exp2_pair(mul2(A01, dt2));
-            a23[t] = exp2_pair(mul2(A23, dt2));
+            const float4 du = du_row[t * (CH + CH / 8)];
+            const F2 dt2 = pack2(du.x, du.y);
+            a01[t] = decay(A01, dt2);
+            a23[t] = decay(A23, dt2);
             if (LOCAL) {
                 sum_dt += du.x;
             } else {
-                const float4 b = *reinterpret_cast<const float4*>(s_b + t * NP + 4 * j);
-                const F2 du2 = pack2(du.y, du.y);
-                x01 = fma2(a01[t], x01, mul2(du2, pack2(b.x, b.y)));
-                x23 = fma2(a23[t], x23, mul2(du2, pack2(b.z, b.w)));
-                h01[t] = x01;
-                h23[t] = x23;
+                const float4 b = b_row[t * P];
+                const F2 du2 = pack2(du.z, du.w);
+                h01[t + 1] = fma2(a01[t], h01[t], mul2(du2, pack2(b.x, b.y)));
+                h23[t + 1] = fma2(a23[t], h23[t], mul2(du2, pack2(b.z, b.w)));
             }
         }
         if (!LOCAL && z) {
-            constexpr int V = P < 16 ? P : 16;
+            float y[STEPS];
 #pragma unroll
-            for (int g = 0; g < STEPS / V; ++g) {
-                float y[V];
+            for (int t = 0; t < STEPS; ++t) {
+                const float4 cc = c_row[t * P];
+                y[t] = sum2(fma2(h23[t + 1], pack2(cc.z, cc.w), mul2(h01[t + 1], pack2(cc.x, cc.y))));
+            }
+            reduce_lanes<STEPS, P, 1>(y, lane);
+            if (reduced_owner<STEPS, P>(j)) {
+                const int t = reduced_index<STEPS, P>(j);
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float4 cc = *reinterpret_cast<const float4*>(s_c + (g * V + i) * NP + 4 * j);
-                    y[i] = sum2(fma2(h23[g * V + i], pack2(cc.z, cc.w), mul2(h01[g * V + i], pack2(cc.x, cc.y))));
-                }
-                reduce_lanes<V, P, 1>(y, lane);
-                if (reduced_owner<V, P>(j)) {
-                    const int t = g * V + reduced_index<V, P>(j);
-#pragma unroll
-                    for (int i = 0; i < reduced_count<V, P>(); ++i) s_y[(t + i) * ROW + c] = y[i];
-                }
+                for (int i = 0; i < reduced_count<STEPS, P>(); ++i) s_y[(t + i) * ROW + c] = y[i];
             }
         }
         // the gradients, backwards
-        F2 gA01 = pack2(0.0f, 0.0f), gA23 = gA01;
+        F2 gA01 = same2(0.0f), gA23 = gA01;
 #pragma unroll
         for (int g = STEPS / 4 - 1; g >= 0; --g) {
             float s[8];
 #pragma unroll
             for (int i = 3; i >= 0; --i) {
                 const int t = g * 4 + i;
-                const float gy = s_gy[t * CH + c];
-                const F2 gy2 = pack2(gy, gy);
-                const float4 cc = *reinterpret_cast<const float4*>(s_c + t * NP + 4 * j);
+                const float2 gy = gy_row[t * CH];
+                const F2 gy2 = pack2(gy.x, gy.y);
+                const float4 cc = c_row[t * P];
                 const F2 g01 = fma2(gy2, pack2(cc.x, cc.y), w01), g23 = fma2(gy2, pack2(cc.z, cc.w), w23);
                 w01 = mul2(a01[t], g01);
                 w23 = mul2(a23[t], g23);
                 if (!LOCAL) {
-                    const float2 du = s_du[t * CH + c];
-                    const float4 b = *reinterpret_cast<const float4*>(s_b + t * NP + 4 * j);
-                    const F2 du2 = pack2(du.y, du.y), dt2 = pack2(du.x, du.x);
+                    const float4 du = du_row[t * (CH + CH / 8)], b = b_row[t * P];
+                    const F2 dt2 = pack2(du.x, du.y), du2 = pack2(du.z, du.w);
                     float v[8];
-                    unpack2(mul2(gy2, h01[t]), v[0], v[1]);
-                    unpack2(mul2(gy2, h23[t]), v[2], v[3]);
+                    unpack2(mul2(gy2, h01[t + 1]), v[0], v[1]);
+                    unpack2(mul2(gy2, h23[t + 1]), v[2], v[3]);
                     unpack2(mul2(du2, g01), v[4], v[5]);
                     unpack2(mul2(du2, g23), v[6], v[7]);
-                    if (!live) {
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) v[k] = 0.0f;
-                    }
                     reduce_lanes<8, R, P>(v, lane);
                     if (reduced_owner<8, R>(lane / P)) {
                         const int k0 = reduced_index<8, R>(lane / P);
@@ -566,7 +631,7 @@ __global__ void __launch_bounds__(Shape<P>::THREADS) scan_backward(const __grid_
                         for (int k = 0; k < reduced_count<8, R>(); ++k) to[((k0 + k) / 4) * NP + (k0 + k) % 4] = v[k];
                     }
                     s[2 * i] = sum2(fma2(g23, pack2(b.z, b.w), mul2(g01, pack2(b.x, b.y))));
-                    const F2 q01 = mul2(w01, t > 0 ? h01[t > 0 ? t - 1 : 0] : s01), q23 = mul2(w23, t > 0 ? h23[t > 0 ? t - 1 : 0] : s23);
+                    const F2 q01 = mul2(w01, h01[t]), q23 = mul2(w23, h23[t]);
                     s[2 * i + 1] = sum2(fma2(q23, A23, mul2(q01, A01)));
                     gA01 = fma2(q01, dt2, gA01);
                     gA23 = fma2(q23, dt2, gA23);
@@ -600,23 +665,25 @@ __global__ void __launch_bounds__(Shape<P>::THREADS) scan_backward(const __grid_
                 const int64_t t = t0 + it;
                 if (valid > 0 && t < t_end) {
                     const bool in = t < t_used, vec = d.vec && valid == 4;
-                    float gu[4], gd[4], gz[4];
+                    float x[4], gu[4], gd[4], gz[4];
+                    read_slot<T, 4>(slot_of(buf, 0, k), x);
+                    const float4 over4 = *reinterpret_cast<const float4*>(s_s + it * ROW + cc);
+                    const float4 qa4 = *reinterpret_cast<const float4*>(s_s + (STEPS + it) * ROW + cc);
+                    const float4 slope4 = s_keep[tid + k * THREADS], gs4 = s_keep[ITEMS + tid + k * THREADS];
+                    const float over[4] = {over4.x, over4.y, over4.z, over4.w}, qa[4] = {qa4.x, qa4.y, qa4.z, qa4.w};
+                    const float slope[4] = {slope4.x, slope4.y, slope4.z, slope4.w}, gs[4] = {gs4.x, gs4.y, gs4.z, gs4.w};
+                    float y[4] = {};
+                    if (z) {
+                        const float4 y4 = *reinterpret_cast<const float4*>(s_y + it * ROW + cc);
+                        y[0] = y4.x, y[1] = y4.y, y[2] = y4.z, y[3] = y4.w;
+                    }
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const float xu = to_f32(now_u[k].v[i]), go = to_f32(now_g[k].v[i]);
-                        const float raw = to_f32(now_d[k].v[i]) + bias[k][i];
-                        const float dt = s_du[it * CH + cc + i].x, gy = s_gy[it * CH + cc + i];
-                        const float over = s_s[it * ROW + cc + i];
-                        gu[i] = in ? fmaf(dt, over, skip[k][i] * gy) : 0.0f;
-                        float g = fmaf(xu, over, kLn2 * s_s[(STEPS + it) * ROW + cc + i]);
-                        if (d.softplus) g *= sigmoid(raw);
-                        gd[i] = in ? g : 0.0f;
-                        if (z) {
-                            const float zz = to_f32(now_z[k].v[i]), sig = sigmoid(zz);
-                            const float y = fmaf(skip[k][i], xu, s_y[it * ROW + cc + i]);
-                            gz[i] = in ? go * y * sig * (1.0f + zz * (1.0f - sig)) : 0.0f;
-                        }
-                        gD[k][i] += in ? gy * xu : 0.0f;
+                        const float dt = s_du[du_at<CH>(it, cc + i)].x, gy = s_gy[it * CH + cc + i].x;
+                        gu[i] = in ? fmaf(dt, over[i], skip[k][i] * gy) : 0.0f;
+                        gd[i] = in ? slope[i] * fmaf(x[i], over[i], kLn2 * qa[i]) : 0.0f;
+                        gz[i] = in ? gs[i] * fmaf(skip[k][i], x[i], y[i]) : 0.0f;
+                        gD[k][i] += in ? gy * x[i] : 0.0f;
                         gbias[k][i] += gd[i];
                     }
                     const int64_t o = (at.batch * d.length + t) * d.channels + base_c + cc;
@@ -885,7 +952,7 @@ int with_smem(F kernel, size_t bytes) {
 
 template <typename T, int P>
 int run_forward(const ScanParams& p, int64_t blocks, cudaStream_t stream) {
-    constexpr size_t smem = forward_smem<P>();
+    constexpr size_t smem = ForwardSmem<T, P>::bytes;
     int st;
     if (p.d.segments > 1) {
         if ((st = with_smem(scan_forward<T, P, true>, smem)) != OVL_OK) return st;
@@ -904,7 +971,7 @@ uint32_t grid_for(int64_t items) {
 
 template <typename T, int P>
 int run_backward(const ScanParams& p, int64_t blocks, cudaStream_t stream) {
-    constexpr size_t smem = BackShape<P>::floats * sizeof(float);
+    constexpr size_t smem = BackShape<T, P>::bytes;
     int st;
     if (p.d.segments > 1) {
         if ((st = with_smem(scan_backward<T, P, true>, smem)) != OVL_OK) return st;
@@ -966,6 +1033,9 @@ int run(const OvlSelectiveScan* a, bool backward, cudaStream_t stream) {
         vec = vec && aligned16(a->gout) && multiple_of(8, a->gout_batch, a->gout_token) && aligned16(a->gu) &&
               aligned16(a->gdelta) && aligned16(a->gz);
     p.d.vec = vec;
+    // 4 elements of B and C: 8 or 16 bytes
+    p.d.vec_bc = a->states % 4 == 0 && aligned16(a->B) && aligned16(a->C) && multiple_of(4, a->B_batch, a->B_token) &&
+                 multiple_of(4, a->C_batch, a->C_token) && a->B_group % 4 == 0 && a->C_group % 4 == 0;
     p.d.vec_states = a->states % 4 == 0 && aligned16(a->A) && aligned16(a->initial_state) && aligned16(a->final_state) &&
                      aligned16(a->checkpoints) && aligned16(a->gfinal) && aligned16(a->ginitial);
     if (a->dtype == OVL_FLOAT32) return dispatch<float>(p, backward, stream);

@@ -117,6 +117,12 @@ __device__ __forceinline__ F2 mul2(F2 a, F2 b) {
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
     return r;
 }
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+    F2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 same2(float a) { return pack2(a, a); }
 __device__ __forceinline__ float sum2(F2 x) {
     float a, b;
     unpack2(x, a, b);
@@ -147,25 +153,68 @@ __device__ __forceinline__ float sigmoid(float x) { return rcp_approx(1.0f + exp
 __device__ __forceinline__ float silu(float x) { return x * sigmoid(x); }
 
 // log(1 + e^x) = max(x, 0) + log1p(e^-|x|), relatively exact to 3e-7 also where it is small (a step size of 0.001 is
-// softplus(-6.9)): e^-|x| with the product by log2 e in two parts, then log1p(e) = e p(e) with p the polynomial of
-// degree 9 that agrees with log1p(e) / e in the Chebyshev points of [0, 1] (5e-9 off).  A NaN stays one.
+// softplus(-6.9)): e = e^-|x| with the product by log2 e in two parts, then log1p(e) = e p(e) with p the polynomial of
+// degree 9 that agrees with log1p(e) / e in the Chebyshev points of [0, 1] (5e-9 off).  A NaN stays one.  Two at a time,
+// leaving the two e for the derivative.
+__device__ __forceinline__ void softplus_pair(float& x0, float& x1, float& e0, float& e1) {
+    const F2 t = pack2(fminf(fabsf(x0), 100.0f), fminf(fabsf(x1), 100.0f));
+    const F2 hi = mul2(t, same2(-kLog2e));
+    const F2 lo = fma2(t, same2(1.925963033e-8f), fma2(t, same2(kLog2e), hi));
+    unpack2(hi, e0, e1);
+    F2 e = pack2(exp2_approx(e0), exp2_approx(e1));
+    e = fma2(e, mul2(lo, same2(-kLn2)), e);
+    F2 p = same2(-3.176057013e-03f);
+    p = fma2(p, e, same2(1.954252645e-02f));
+    p = fma2(p, e, same2(-5.637361109e-02f));
+    p = fma2(p, e, same2(1.054362357e-01f));
+    p = fma2(p, e, same2(-1.526966691e-01f));
+    p = fma2(p, e, same2(1.966327429e-01f));
+    p = fma2(p, e, same2(-2.495161593e-01f));
+    p = fma2(p, e, same2(3.332971036e-01f));
+    p = fma2(p, e, same2(-4.999989271e-01f));
+    p = fma2(p, e, same2(1.0f));
+    p = fma2(p, e, pack2(x0 < 0.0f ? 0.0f : x0, x1 < 0.0f ? 0.0f : x1));
+    unpack2(e, e0, e1);
+    unpack2(p, x0, x1);
+}
 __device__ __forceinline__ float softplus(float x) {
-    const float t = fminf(fabsf(x), 100.0f);
-    const float hi = -kLog2e * t;
-    const float lo = fmaf(-kLog2e, t, -hi) - 1.925963033e-8f * t;
-    float e = exp2_approx(hi);
-    e = fmaf(e, kLn2 * lo, e);
-    float p = -3.176057013e-03f;
-    p = fmaf(p, e, 1.954252645e-02f);
-    p = fmaf(p, e, -5.637361109e-02f);
-    p = fmaf(p, e, 1.054362357e-01f);
-    p = fmaf(p, e, -1.526966691e-01f);
-    p = fmaf(p, e, 1.966327429e-01f);
-    p = fmaf(p, e, -2.495161593e-01f);
-    p = fmaf(p, e, 3.332971036e-01f);
-    p = fmaf(p, e, -4.999989271e-01f);
-    p = fmaf(p, e, 1.0f);
-    return fmaf(p, e, x < 0.0f ? 0.0f : x);
+    float y = x, e0, e1;
+    softplus_pair(x, y, e0, e1);
+    return x;
+}
+
+// copies of BYTES (4, 8 or 16) bytes from global to shared memory that the thread does not wait for
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* to, const void* from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from), "n"(BYTES)
+                 : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+
+// N elements into a slot of shared memory that only this thread reads: in flight while it goes on (`vec`: aligned and
+// all there), otherwise element by element
+template <typename T, int N>
+__device__ __forceinline__ void fetch_pack(T* slot, const T* __restrict__ p, bool vec, int valid) {
+    if (vec) {
+        constexpr int BYTES = sizeof(T) * N > 16 ? 16 : (int)sizeof(T) * N, H = BYTES / (int)sizeof(T);
+#pragma unroll
+        for (int i = 0; i < N; i += H) copy_async<BYTES>(slot + i, p + i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) slot[i] = i < valid ? p[i] : from_f32<T>(0.0f);
+    }
+}
+// the same slot, converted
+template <typename T, int N>
+__device__ __forceinline__ void read_slot(const T* slot, float (&x)[N]) {
+    constexpr int H = sizeof(T) * N > 16 ? 16 / (int)sizeof(T) : N;
+#pragma unroll
+    for (int i = 0; i < N; i += H) {
+        const Pack<T, H> r = *reinterpret_cast<const Pack<T, H>*>(slot + i);
+#pragma unroll
+        for (int k = 0; k < H; ++k) x[i + k] = to_f32(r.v[k]);
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------------
