@@ -25,7 +25,8 @@ CSRC_DIR = os.path.join(_PKG, 'csrc')
 LAUNCHER_SRC = os.path.join(CSRC_DIR, 'ovl_launcher.cu')
 #: every source of the library; they are compiled side by side
 LIBRARY_SOURCES = [LAUNCHER_SRC] + [os.path.join(CSRC_DIR, fn) for fn in
-                                    ('ovl_selective_scan.cu', 'ovl_causal_conv.cu', 'ovl_rms_norm.cu')]
+                                    ('ovl_selective_scan.cu', 'ovl_selective_scan_f32.cu', 'ovl_selective_scan_f16.cu',
+                                     'ovl_selective_scan_bf16.cu', 'ovl_causal_conv.cu', 'ovl_rms_norm.cu')]
 NVCC_FLAGS = ['-O3', '--fmad=false', '-std=c++17', '-lineinfo', '-diag-suppress', '128,177,186,550']
 _lock = threading.Lock()
 
@@ -114,6 +115,7 @@ def build_launcher(force=False):
     with _lock:
         os.makedirs(LIB_DIR, exist_ok=True)
         deps = LIBRARY_SOURCES + [os.path.join(CSRC_DIR, 'ovl_sequence.cuh'),
+                                  os.path.join(CSRC_DIR, 'ovl_selective_scan.cuh'),
                                   os.path.join(_PKG, '..', 'include', 'ovl_b200.h')] + \
             [os.path.join(TEMPLATE_DIR, fn) for fn in os.listdir(TEMPLATE_DIR)]
         stamp = _launcher_stamp(deps)

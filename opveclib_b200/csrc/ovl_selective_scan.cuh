@@ -1,0 +1,1106 @@
+// Selective scan: h_t = exp(dt_t A) h_{t-1} + dt_t u_t B_t, out_t = (C_t . h_t + D u_t) silu(z_t), for prompts and
+// training (forward and backward) and for single tokens.  Interface: include/ovl_b200.h.
+//
+// What bounds it.  A (token, channel) moves 8 bytes (u, delta, z, out in 16 bits) and needs one exponential per state.
+// The special-function unit delivers 16 per clock and SM: with 16 states one (token, channel) per clock and SM, 2.8e11
+// per second on 148 SMs, while 8 bytes at the measured copy bandwidth allow 8e11.  So the recurrence itself has to stay
+// out of the way of the exponentials: it runs serially over the tokens in registers (no scan over lanes, which would
+// multiply the arithmetic), and everything that is needed once per (token, channel) is computed once, in shared memory.
+//
+// Layout.  A channel is P lanes of a warp with 4 states each (P = 1 ... 32: up to 128 states); a block is 128 threads
+// (256 for P = 32) = CH channels of one group of one batch.  Tokens come in tiles of STEPS: while a tile is scanned the
+// next one's elements are in flight to shared memory, each to the thread that will convert, mask and combine them
+// (softplus, dt * u) into what all lanes of a channel read; double-buffered, with one barrier per tile.  The sums over the states of P steps are formed together
+// (reduce_lanes: less than one exchange per step), and the same threads that loaded u and z finish the outputs.
+#pragma once
+#include "ovl_sequence.cuh"
+
+namespace ovl {
+
+constexpr int kCheckpoint = 16;        // tokens between two saved states of a training step
+constexpr int kMaxStates = 128;
+constexpr int kMaxSegments = 32;
+
+struct ScanDims {
+    int64_t length, channels, states, groups;
+    int64_t group_channels, tiles;     // channels of a group, channel tiles of a group
+    int64_t segments, segment_length;  // the length cut into segments (a multiple of 32) that run side by side
+    int64_t first_segment, launch_segments;   // those of this launch
+    int32_t ahead;                     // the first of two launches, see below
+    int32_t softplus, vec;             // vec: wide loads and stores of channel vectors
+    int32_t vec_states, vec_bc;        // wide loads and stores of 4 states; of 4 elements of B and C
+};
+
+struct ScanParams {
+    ScanDims d;
+    OvlSelectiveScan a;
+    float* seg_state;                  // [batch, segments, channels, states]: what a segment adds to the state
+    float* seg_dt;                     // [batch, segments, channels]: sum of dt over the segment
+    float* part_bc;                    // [batch, groups, tiles, length, 2, 4P]: gC and gB of a channel tile
+    float* part_A;                     // [batch * segments, channels, states]
+    float* part_D;                     // [batch * segments, 2, channels]: gD, gdelta_bias
+};
+
+// Lanes of a channel, and how much a lane does: channels (forward) or pairs of states (backward).
+struct ScanShape {
+    int lanes, extent, padded_states, block_channels;
+};
+
+// One source per element type (they are compiled side by side).
+__attribute__((visibility("hidden"))) int scan_run_f32(const ScanParams&, const ScanShape&, bool backward, cudaStream_t);
+__attribute__((visibility("hidden"))) int scan_run_f16(const ScanParams&, const ScanShape&, bool backward, cudaStream_t);
+__attribute__((visibility("hidden"))) int scan_run_bf16(const ScanParams&, const ScanShape&, bool backward, cudaStream_t);
+__attribute__((visibility("hidden"))) int scan_step_f32(const OvlSelectiveScanStep&, int lanes, cudaStream_t);
+__attribute__((visibility("hidden"))) int scan_step_f16(const OvlSelectiveScanStep&, int lanes, cudaStream_t);
+__attribute__((visibility("hidden"))) int scan_step_bf16(const OvlSelectiveScanStep&, int lanes, cudaStream_t);
+
+namespace {
+
+// P lanes of a channel with K pairs of states each
+template <int P, int K>
+struct Shape {
+    static constexpr int THREADS = P == 32 ? 256 : 128;
+    static constexpr int CH = THREADS / P;                               // channels of a block
+    static constexpr int NP = 2 * K * P;                                 // states, padded
+    static constexpr int ROW = CH + (P >= 8 ? 4 : 32 / P);               // row of per-channel sums in shared memory:
+                                                                         // lanes of different steps hit different banks
+    static_assert(NP % 4 == 0, "B and C are staged 4 states at a time");
+};
+
+// K pairs of states from state n0 on
+template <int K>
+__device__ __forceinline__ void load_states(F2 (&x)[K], const float* p, int n0, int states, bool vec) {
+    if (vec && n0 < states) {
+        if constexpr (K == 2) {
+            const float4 r = *reinterpret_cast<const float4*>(p + n0);
+            x[0] = pack2(r.x, r.y);
+            x[1] = pack2(r.z, r.w);
+        } else {
+            const float2 r = *reinterpret_cast<const float2*>(p + n0);
+            x[0] = pack2(r.x, r.y);
+        }
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int n = n0 + 2 * k;
+        x[k] = pack2(n < states ? p[n] : 0.0f, n + 1 < states ? p[n + 1] : 0.0f);
+    }
+}
+template <int K>
+__device__ __forceinline__ void store_states(float* p, const F2 (&x)[K], int n0, int states, bool vec) {
+    float v[2 * K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) unpack2(x[k], v[2 * k], v[2 * k + 1]);
+    if (vec && n0 < states) {
+        if constexpr (K == 2) *reinterpret_cast<float4*>(p + n0) = make_float4(v[0], v[1], v[2], v[3]);
+        else *reinterpret_cast<float2*>(p + n0) = make_float2(v[0], v[1]);
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < 2 * K; ++k)
+        if (n0 + k < states) p[n0 + k] = v[k];
+}
+// K pairs of one row of B or C in shared memory
+template <int K>
+__device__ __forceinline__ void read_pairs(F2 (&x)[K], const float* p) {
+    if constexpr (K == 2) {
+        const float4 r = *reinterpret_cast<const float4*>(p);
+        x[0] = pack2(r.x, r.y);
+        x[1] = pack2(r.z, r.w);
+    } else {
+        const float2 r = *reinterpret_cast<const float2*>(p);
+        x[0] = pack2(r.x, r.y);
+    }
+}
+// the sum over both states of K pairs of the products x y
+template <int K>
+__device__ __forceinline__ float dot(const F2 (&x)[K], const F2 (&y)[K]) {
+    F2 r = mul2(x[0], y[0]);
+#pragma unroll
+    for (int k = 1; k < K; ++k) r = fma2(x[k], y[k], r);
+    return sum2(r);
+}
+
+__device__ __forceinline__ int64_t used_length(const int32_t* lengths, int64_t batch, int64_t length) {
+    if (!lengths) return length;
+    const int64_t n = lengths[batch];
+    return n < 0 ? 0 : n > length ? length : n;
+}
+
+// which piece of the problem a block works on (a launch covers the segments from first_segment on)
+struct Place {
+    int64_t batch, segment, group, tile, channel0, n_channels;   // channels channel0 ... channel0 + n_channels - 1
+};
+__device__ __forceinline__ Place block_place(const ScanDims& d, int ch) {
+    Place p;
+    int64_t i = blockIdx.x;
+    p.tile = i % d.tiles;
+    i /= d.tiles;
+    p.group = i % d.groups;
+    i /= d.groups;
+    p.segment = d.first_segment + i % d.launch_segments;
+    p.batch = i / d.launch_segments;
+    p.channel0 = p.group * d.group_channels + p.tile * ch;
+    const int64_t left = d.group_channels - p.tile * ch;
+    p.n_channels = left < ch ? left : ch;
+    return p;
+}
+
+// exp(dt A) = 2^(dt A log2 e).  The special-function unit's results are 1e-8 to 2e-8 too small on average, which adds up
+// over a state's memory of a thousand tokens; the same amount on the exponent takes most of it away and costs nothing
+// (a multiplication becomes a multiply-add).  2^kExpBias rounds to 1, so dt = 0 still leaves a state as it is.
+constexpr float kExpBias = 2e-8f;
+__device__ __forceinline__ F2 decay(F2 A, F2 dt) { return exp2_pair(fma2(A, dt, same2(kExpBias))); }
+
+// ---------------------------------------------------------------------------------------------------------
+// forward
+
+// P lanes x 4 states x M channels: a block is 128 scanning threads = 128 / P * M channels, and 128 helping threads.
+template <int P, int M>
+struct ForwardShape {
+    static constexpr int SCAN = 128, HELP = 128, THREADS = SCAN + HELP;
+    static constexpr int CH = SCAN / P * M;                              // channels of a block
+    static constexpr int NP = 4 * P;                                     // states, padded
+    static constexpr int STEPS = CH >= 128 ? 8 : CH >= 64 ? 16 : 32;     // tokens of a tile
+    static constexpr int V = STEPS < 16 / M ? STEPS : 16 / M;            // steps whose sums are formed together
+    static constexpr int ITEMS = STEPS * CH / 8;                         // 8 channels of one token
+    static constexpr int IPT = (ITEMS + HELP - 1) / HELP;
+    static constexpr int QUADS = STEPS * P, QPT = (QUADS + HELP - 1) / HELP;   // 4 states of one token
+    static constexpr int DU = CH + CH / 8 * 2;                           // row of s_du: 16 bytes of gap after 8 channels
+    static constexpr int ROW = CH + (P >= 8 ? 4 : 32 / P);               // row of s_y: lanes of different steps hit different banks
+};
+
+template <typename T, int P, int M>
+struct ForwardSmem {
+    using S = ForwardShape<P, M>;
+    static constexpr size_t du = 0;                                                          // float2 [2][STEPS][DU]
+    static constexpr size_t b = du + 2 * sizeof(float2) * S::STEPS * S::DU;                  // float [2][STEPS][NP]
+    static constexpr size_t c = b + 2 * sizeof(float) * S::STEPS * S::NP;
+    static constexpr size_t y = c + 2 * sizeof(float) * S::STEPS * S::NP;                    // float [2][STEPS][ROW]
+    static constexpr size_t raw = y + 2 * sizeof(float) * S::STEPS * S::ROW;                 // T [3][3][ITEMS][8]: u, delta, z
+    static constexpr size_t raw_bc = raw + 3 * 3 * sizeof(T) * S::STEPS * S::CH;             // T [2][2][QUADS][4]: B, C
+    static constexpr size_t bytes = raw_bc + 2 * 2 * sizeof(T) * S::STEPS * S::NP;
+};
+
+// The scanning threads: nothing but the recurrence and its sums over the states.  A lane reads 16 bytes of dt and dt u
+// (two channels) and 32 bytes of B and C per step and 8 states: shared memory hands out 128 bytes per clock to the SM's
+// lanes whether they share addresses or not, which would make a lane with one channel wait for it (46 clocks per warp
+// and step measured, 32 for the exponentials).
+template <typename T, int P, int M, bool LOCAL>
+__device__ __forceinline__ void scan_forward_scan(const ScanParams& p, const Place& at, char* smem, int64_t t_begin, int64_t t_used) {
+    using S = ForwardShape<P, M>;
+    using Mem = ForwardSmem<T, P, M>;
+    constexpr int NP = S::NP, STEPS = S::STEPS, V = S::V;
+    const OvlSelectiveScan& a = p.a;
+    const ScanDims& d = p.d;
+    const int tid = threadIdx.x, lane = tid % 32, j = lane % P, c0 = tid / P * M, n0 = 4 * j;
+    const int states = (int)d.states;
+    int64_t row[M];                                                      // of this channel's states in [batch, channels, states]
+    bool live[M];
+    F2 A[M][2], h[M][2];
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+        live[m] = c0 + m < at.n_channels;
+        const int64_t channel = at.channel0 + (live[m] ? c0 + m : 0);
+        row[m] = (at.batch * d.channels + channel) * states;
+        load_states(A[m], a.A + channel * states, n0, states, d.vec_states);    // padded states have A = B = C = 0
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            A[m][k] = mul2(A[m][k], same2(kLog2e));
+            h[m][k] = same2(0.0f);
+        }
+        if (LOCAL) continue;
+        // the state in front of this segment: the one behind the first segment, then h <- exp(A sum dt) h + (what the
+        // segment adds) for those between
+        if (at.segment > 0) load_states(h[m], p.seg_state + (at.batch * d.segments * d.channels + channel) * states, n0, states, d.vec_states);
+        else if (a.initial_state) load_states(h[m], a.initial_state + row[m], n0, states, d.vec_states);
+        for (int64_t s = 1; s < at.segment; ++s) {
+            const int64_t cell = (at.batch * d.segments + s) * d.channels + channel;
+            const F2 sum = same2(p.seg_dt[cell]);
+            F2 add[2];
+            load_states(add, p.seg_state + cell * states, n0, states, d.vec_states);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) h[m][k] = fma2(decay(A[m][k], sum), h[m][k], add[k]);
+        }
+    }
+    const float2* const s_du = reinterpret_cast<const float2*>(smem + Mem::du) + c0 + c0 / 8 * 2;
+    const float* const s_b = reinterpret_cast<const float*>(smem + Mem::b) + n0;
+    const float* const s_c = reinterpret_cast<const float*>(smem + Mem::c) + n0;
+    float* const s_y = reinterpret_cast<float*>(smem + Mem::y) + c0;
+    const int64_t chunks = (d.length + kCheckpoint - 1) / kCheckpoint;
+    float sum_dt[M] = {};
+    __syncthreads();
+    int buf = 0;
+    for (int64_t t0 = t_begin; t0 < t_used; t0 += STEPS, buf ^= 1) {
+#pragma unroll 1
+        for (int g = 0; g < STEPS / V; ++g) {
+            if (!LOCAL && a.checkpoints && (t0 + g * V) % kCheckpoint == 0 && t0 + g * V < d.length) {
+                const int64_t skip = (at.batch * (chunks - 1) + (t0 + g * V) / kCheckpoint) * d.channels * states;
+#pragma unroll
+                for (int m = 0; m < M; ++m)
+                    if (live[m]) store_states(a.checkpoints + skip + row[m], h[m], n0, states, d.vec_states);
+            }
+            float y[M][V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const int t = buf * STEPS + g * V + i;
+                float dt[M], du[M];
+                if constexpr (M == 2) {
+                    const float4 v = *reinterpret_cast<const float4*>(s_du + t * S::DU);
+                    dt[0] = v.x, du[0] = v.y, dt[1] = v.z, du[1] = v.w;
+                } else {
+                    const float2 v = s_du[t * S::DU];
+                    dt[0] = v.x, du[0] = v.y;
+                }
+                F2 b[2], cc[2];
+                read_pairs(b, s_b + t * NP);
+                if (!LOCAL) read_pairs(cc, s_c + t * NP);
+#pragma unroll
+                for (int m = 0; m < M; ++m) {
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) h[m][k] = fma2(decay(A[m][k], same2(dt[m])), h[m][k], mul2(same2(du[m]), b[k]));
+                    if (LOCAL) sum_dt[m] += dt[m];
+                    else y[m][i] = dot(h[m], cc);
+                }
+            }
+            if (!LOCAL) {
+#pragma unroll
+                for (int m = 0; m < M; ++m) {
+                    reduce_lanes<V, P, 1>(y[m], lane);
+                    if (reduced_owner<V, P>(j)) {
+                        const int t = buf * STEPS + g * V + reduced_index<V, P>(j);
+#pragma unroll
+                        for (int i = 0; i < reduced_count<V, P>(); ++i) s_y[(t + i) * S::ROW + m] = y[m][i];
+                    }
+                }
+            }
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+        if (!live[m]) continue;
+        const int64_t channel = at.channel0 + c0 + m, cell = (at.batch * d.segments + at.segment) * d.channels + channel;
+        if (d.ahead) store_states(p.seg_state + cell * states, h[m], n0, states, d.vec_states);
+        if (LOCAL && j == 0) p.seg_dt[cell] = sum_dt[m];
+        if (!LOCAL && a.final_state && at.segment == d.segments - 1)
+            store_states(a.final_state + row[m], h[m], n0, states, d.vec_states);
+    }
+}
+
+// The helping threads, one tile ahead of the scan and one behind it: they fetch u, delta, z, B and C (two tiles ahead,
+// each thread what it will need itself), leave dt, dt u, B and C for the scan, and finish the outputs from its sums.
+template <typename T, int P, int M, bool LOCAL>
+__device__ __forceinline__ void scan_forward_help(const ScanParams& p, const Place& at, char* smem, int64_t t_begin, int64_t t_end,
+                                                  int64_t t_used) {
+    using S = ForwardShape<P, M>;
+    using Mem = ForwardSmem<T, P, M>;
+    constexpr int CH = S::CH, NP = S::NP, STEPS = S::STEPS, IPT = S::IPT, QPT = S::QPT;
+    const OvlSelectiveScan& a = p.a;
+    const ScanDims& d = p.d;
+    const int tid = threadIdx.x - S::SCAN;
+    const int states = (int)d.states;
+    float2* const s_du = reinterpret_cast<float2*>(smem + Mem::du);
+    const T* const u = reinterpret_cast<const T*>(a.u) + at.batch * a.u_batch + at.channel0;
+    const T* const delta = reinterpret_cast<const T*>(a.delta) + at.batch * a.delta_batch + at.channel0;
+    const T* const z = a.z ? reinterpret_cast<const T*>(a.z) + at.batch * a.z_batch + at.channel0 : nullptr;
+    T* const out = reinterpret_cast<T*>(a.out) + at.batch * d.length * d.channels + at.channel0;
+    const T* const B = reinterpret_cast<const T*>(a.B) + at.batch * a.B_batch + at.group * a.B_group;
+    const T* const C = reinterpret_cast<const T*>(a.C) + at.batch * a.C_batch + at.group * a.C_group;
+
+    // this thread's parts of a tile: 8 channels of one token; all of them have the same channels
+    static_assert(S::HELP % (CH / 8) == 0, "the parts of a thread have the same channels");
+    const int item_t = tid / (CH / 8), item_c = tid % (CH / 8) * 8;
+    constexpr int ITEM_STEP = S::HELP / (CH / 8);                        // tokens between two parts of a thread
+    const bool has_item = tid < S::ITEMS;
+    const int valid = !has_item || item_c >= at.n_channels ? 0 : at.n_channels - item_c < 8 ? (int)(at.n_channels - item_c) : 8;
+    const bool vec = d.vec && valid == 8;
+    float skip[8], bias[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        skip[i] = !LOCAL && a.D && i < valid ? a.D[at.channel0 + item_c + i] : 0.0f;
+        bias[i] = a.delta_bias && i < valid ? a.delta_bias[at.channel0 + item_c + i] : 0.0f;
+    }
+    auto slot_of = [&](int slot, int which, int k) {
+        return reinterpret_cast<T*>(smem + Mem::raw) + ((slot * 3 + which) * S::ITEMS + tid + k * S::HELP) * 8;
+    };
+    auto quad_of = [&](int buf, int which, int e) {
+        return reinterpret_cast<T*>(smem + Mem::raw_bc) + ((buf * 2 + which) * S::QUADS + e) * 4;
+    };
+    auto fetch = [&](int64_t t0, int slot, int buf) {
+        if (t0 < t_used) {
+#pragma unroll
+            for (int k = 0; k < IPT; ++k) {
+                const int64_t t = t0 + item_t + k * ITEM_STEP;
+                if (valid > 0 && t < t_used) {
+                    fetch_pack<T, 8>(slot_of(slot, 0, k), u + t * a.u_token + item_c, vec, valid);
+                    fetch_pack<T, 8>(slot_of(slot, 1, k), delta + t * a.delta_token + item_c, vec, valid);
+                    if (!LOCAL && z) fetch_pack<T, 8>(slot_of(slot, 2, k), z + t * a.z_token + item_c, vec, valid);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < QPT; ++k) {
+                const int e = tid + k * S::HELP, n = e % P * 4;
+                const int64_t t = t0 + e / P;
+                if (e < S::QUADS && t < t_used && n < states) {
+                    const bool wide = d.vec_bc && n + 4 <= states;
+                    fetch_pack<T, 4>(quad_of(buf, 0, e), B + t * a.B_token + n, wide, states - n);
+                    if (!LOCAL) fetch_pack<T, 4>(quad_of(buf, 1, e), C + t * a.C_token + n, wide, states - n);
+                }
+            }
+        }
+        copy_commit();
+    };
+    auto stage = [&](int64_t t0, int slot, int buf) {
+#pragma unroll
+        for (int k = 0; k < IPT; ++k) {
+            const int it = item_t + k * ITEM_STEP;
+            if (!has_item) continue;
+            float x[8], dt[8];
+            read_slot<T, 8>(slot_of(slot, 0, k), x);
+            read_slot<T, 8>(slot_of(slot, 1, k), dt);
+            float4* const to = reinterpret_cast<float4*>(s_du + (buf * STEPS + it) * S::DU + item_c + item_c / 8 * 2);
+            // padding leaves the state as it is: dt = 0 makes the factor 1 and the addend 0
+            const bool in = t0 + it < t_used, all = in && valid == 8;
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                float e0, e1;
+                dt[i] += bias[i];
+                dt[i + 1] += bias[i + 1];
+                if (d.softplus) softplus_pair(dt[i], dt[i + 1], e0, e1);
+                float4 v = make_float4(dt[i], dt[i] * x[i], dt[i + 1], dt[i + 1] * x[i + 1]);
+                if (!all) {
+                    if (!in || i >= valid) v.x = v.y = 0.0f;
+                    if (!in || i + 1 >= valid) v.z = v.w = 0.0f;
+                }
+                to[i / 2] = v;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < QPT; ++k) {
+            const int e = tid + k * S::HELP;
+            if (e < S::QUADS) {
+                const bool in = t0 + e / P < t_used && e % P * 4 < states;
+                float x[4] = {}, y[4] = {};
+                if (in) {
+                    read_slot<T, 4>(quad_of(buf, 0, e), x);
+                    if (!LOCAL) read_slot<T, 4>(quad_of(buf, 1, e), y);
+                }
+                reinterpret_cast<float4*>(smem + Mem::b)[buf * S::QUADS + e] = make_float4(x[0], x[1], x[2], x[3]);
+                if (!LOCAL) reinterpret_cast<float4*>(smem + Mem::c)[buf * S::QUADS + e] = make_float4(y[0], y[1], y[2], y[3]);
+            }
+        }
+    };
+    auto finish = [&](int64_t t0, int slot, int buf) {
+#pragma unroll
+        for (int k = 0; k < IPT; ++k) {
+            const int it = item_t + k * ITEM_STEP;
+            const int64_t t = t0 + it;
+            if (valid == 0 || t >= t_end) continue;
+            float o[8] = {};
+            if (t < t_used) {
+                const float4* const y = reinterpret_cast<const float4*>(smem + Mem::y) + ((buf * STEPS + it) * S::ROW + item_c) / 4;
+                const float4 y0 = y[0], y1 = y[1];
+                o[0] = y0.x, o[1] = y0.y, o[2] = y0.z, o[3] = y0.w, o[4] = y1.x, o[5] = y1.y, o[6] = y1.z, o[7] = y1.w;
+                float x[8], g[8];
+                read_slot<T, 8>(slot_of(slot, 0, k), x);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[i] = fmaf(skip[i], x[i], o[i]);
+                if (z) {
+                    read_slot<T, 8>(slot_of(slot, 2, k), g);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) o[i] *= silu(g[i]);
+                }
+            }
+            store_pack<T, 8>(out + t * d.channels + item_c, o, vec, valid);
+        }
+    };
+
+    fetch(t_begin, 0, 0);
+    fetch(t_begin + STEPS, 1, 1);
+    copy_wait<1>();
+    if (t_begin < t_used) stage(t_begin, 0, 0);
+    __syncthreads();
+    int buf = 0, slot = 0;                                               // of the tile that is being scanned
+    for (int64_t t0 = t_begin; t0 < t_used; t0 += STEPS, buf ^= 1) {
+        const int next = slot == 2 ? 0 : slot + 1, before = slot == 0 ? 2 : slot - 1;
+        if (!LOCAL && t0 > t_begin) finish(t0 - STEPS, before, buf ^ 1);
+        fetch(t0 + 2 * STEPS, before, buf);                              // (B and C of this tile are staged already)
+        copy_wait<1>();
+        if (t0 + STEPS < t_used) stage(t0 + STEPS, next, buf ^ 1);
+        slot = next;
+        __syncthreads();
+    }
+    if (LOCAL) return;
+    // the last tile, and the outputs of padding behind it
+    int64_t covered = t_begin;
+    if (t_used > t_begin) {
+        covered += (t_used - t_begin + STEPS - 1) / STEPS * STEPS;
+        finish(covered - STEPS, slot == 0 ? 2 : slot - 1, buf ^ 1);
+    }
+    if (valid > 0) {
+        const float zero[8] = {};
+        constexpr int TOKENS = S::ITEMS < S::HELP ? STEPS : ITEM_STEP;   // that the threads cover together
+        for (int64_t t = covered + item_t; t < t_end; t += TOKENS)
+            store_pack<T, 8>(out + t * d.channels + item_c, zero, vec, valid);
+    }
+}
+
+// A length that is cut into segments takes two launches: the first does the first segment and finds out what each of
+// those between the first and the last adds to the state (LOCAL: the end of a state that starts at zero, and the sum of
+// dt); the second does the other segments, seeded from the segments before.
+template <typename T, int P, int M, bool LOCAL>
+__device__ __forceinline__ void scan_forward_block(const ScanParams& p, const Place& at, char* smem) {
+    const ScanDims& d = p.d;
+    const int64_t used = used_length(p.a.lengths, at.batch, d.length);
+    const int64_t t_begin = at.segment * d.segment_length;
+    const int64_t t_end = t_begin + d.segment_length < d.length ? t_begin + d.segment_length : d.length;
+    const int64_t t_used = used < t_end ? used : t_end;                  // tokens of the segment that count
+    if (threadIdx.x < ForwardShape<P, M>::SCAN) scan_forward_scan<T, P, M, LOCAL>(p, at, smem, t_begin, t_used);
+    else scan_forward_help<T, P, M, LOCAL>(p, at, smem, t_begin, t_end, t_used);
+}
+
+template <typename T, int P, int M>
+__global__ void __launch_bounds__(ForwardShape<P, M>::THREADS) scan_forward(const __grid_constant__ ScanParams p) {
+    extern __shared__ __align__(16) char smem[];
+    const Place at = block_place(p.d, ForwardShape<P, M>::CH);
+    if (p.d.ahead && at.segment > 0) scan_forward_block<T, P, M, true>(p, at, smem);
+    else scan_forward_block<T, P, M, false>(p, at, smem);
+}
+
+// Where (dt, dt, dt u, dt u) of channel c of a tile's token t stands, in float4: a gap after every 8 channels keeps the
+// wide stores of threads with 8 (or 4) channels each off one another's banks.
+template <int CH>
+__device__ __forceinline__ constexpr int du_at(int t, int c) { return t * (CH + CH / 8) + c + c / 8; }
+
+// ---------------------------------------------------------------------------------------------------------
+// backward
+//
+// The gradient of the state runs from the last token to the first: gh_t = C_t gy_t + a_{t+1} gh_{t+1} with gy = gout
+// silu(z).  It meets the states h_t, which are computed again, 16 tokens at a time from the saved state in front of
+// them; the 16 states and factors of a lane stay in registers, so every exponential is computed once here too.
+//   gC_t = sum_d gy h_t, gB_t = sum_d gh_t dt u     sums over the channels: over the lanes of a warp with reduce_lanes,
+//                                                   over the warps in shared memory, over the blocks in a second launch
+//                                                   from partial sums (no atomics: the same bits every time)
+//   w_t = a_t gh_t (handed to the token before), q = w_t h_{t-1}: gA = sum q dt, g(dt) = sum_n q A + u sum_n gh B,
+//   gu = dt sum_n gh B + D gy
+template <typename T, int P, int K>
+struct BackShape {
+    using S = Shape<P, K>;
+    static constexpr int STEPS = kCheckpoint;
+    static constexpr int WARPS = S::THREADS / 32;
+    static constexpr int CHV = S::CH / 4;                                // 4 channels of one token per item
+    static constexpr int ITEMS = STEPS * CHV;
+    static constexpr int IPT = (ITEMS + S::THREADS - 1) / S::THREADS;
+    static constexpr int ROW = S::ROW;
+    // shared memory
+    static constexpr size_t du = 0;                                                    // float4 [du_at]
+    static constexpr size_t gy = du + sizeof(float4) * STEPS * (S::CH + S::CH / 8);    // float2 [STEPS][CH] (gy, gy)
+    static constexpr size_t b = gy + sizeof(float2) * STEPS * S::CH;                   // float [STEPS][NP]
+    static constexpr size_t c = b + sizeof(float) * STEPS * S::NP;
+    static constexpr size_t y = c + sizeof(float) * STEPS * S::NP;                     // float [STEPS][ROW]: C . h
+    static constexpr size_t s = y + sizeof(float) * STEPS * ROW;                       // float [2][STEPS][ROW]: gh . B, q . A / ln 2
+    static constexpr size_t r = s + 2 * sizeof(float) * STEPS * ROW;                   // float [WARPS][STEPS][2][NP]: gC, gB
+    static constexpr size_t keep = r + sizeof(float) * WARPS * STEPS * 2 * S::NP;      // float4 [2][STEPS][CH / 4]
+    static constexpr size_t raw = keep + 2 * sizeof(float) * STEPS * S::CH;            // T [2][4][STEPS][CH]: u, delta, z, gout
+    static constexpr size_t raw_bc = raw + 2 * 4 * sizeof(T) * STEPS * S::CH;          // T [2][STEPS][NP]
+    static constexpr size_t bytes = raw_bc + 2 * sizeof(T) * STEPS * S::NP;
+};
+
+template <typename T, int P, int K, bool LOCAL>
+__device__ __forceinline__ void scan_backward_block(const ScanParams& p, const Place& at) {
+    using S = Shape<P, K>;
+    using M = BackShape<T, P, K>;
+    constexpr int THREADS = S::THREADS, CH = S::CH, NP = S::NP, STEPS = M::STEPS, ROW = M::ROW, WARPS = M::WARPS;
+    constexpr int CHV = M::CHV, ITEMS = M::ITEMS, IPT = M::IPT;
+    constexpr int QUADS = STEPS * NP / 4, QN = (QUADS + THREADS - 1) / THREADS;
+    constexpr int R = 32 / P;                                            // channels of a warp
+    extern __shared__ __align__(16) char smem[];
+    float4* const s_du = reinterpret_cast<float4*>(smem + M::du);
+    float2* const s_gy = reinterpret_cast<float2*>(smem + M::gy);
+    float* const s_b = reinterpret_cast<float*>(smem + M::b);
+    float* const s_c = reinterpret_cast<float*>(smem + M::c);
+    float* const s_y = reinterpret_cast<float*>(smem + M::y);
+    float* const s_s = reinterpret_cast<float*>(smem + M::s);
+    float* const s_r = reinterpret_cast<float*>(smem + M::r);
+    float4* const s_keep = reinterpret_cast<float4*>(smem + M::keep);    // derivative of dt by delta, of out by z / y
+    T* const raw = reinterpret_cast<T*>(smem + M::raw);
+    T* const raw_bc = reinterpret_cast<T*>(smem + M::raw_bc);
+
+    const OvlSelectiveScan& a = p.a;
+    const ScanDims& d = p.d;
+    const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, j = lane % P, c = tid / P;
+    const bool live = c < at.n_channels;
+    const int64_t channel = at.channel0 + (live ? c : 0);
+    const int states = (int)d.states;
+    const int64_t used = used_length(a.lengths, at.batch, d.length);
+    const int64_t t_begin = at.segment * d.segment_length;
+    const int64_t t_end = t_begin + d.segment_length < d.length ? t_begin + d.segment_length : d.length;
+    const int64_t t_used = used < t_end ? used : t_end;
+    const int64_t chunks = (d.length + kCheckpoint - 1) / kCheckpoint;
+    const int64_t first = t_begin, last = t_used > t_begin ? t_begin + (t_used - t_begin - 1) / STEPS * STEPS : t_begin - STEPS;
+
+    const int64_t base_c = at.channel0;
+    const T* const u = reinterpret_cast<const T*>(a.u) + at.batch * a.u_batch + base_c;
+    const T* const delta = reinterpret_cast<const T*>(a.delta) + at.batch * a.delta_batch + base_c;
+    const T* const z = a.z ? reinterpret_cast<const T*>(a.z) + at.batch * a.z_batch + base_c : nullptr;
+    const T* const gout = reinterpret_cast<const T*>(a.gout) + at.batch * a.gout_batch + base_c;
+    const T* const B = reinterpret_cast<const T*>(a.B) + at.batch * a.B_batch + at.group * a.B_group;
+    const T* const C = reinterpret_cast<const T*>(a.C) + at.batch * a.C_batch + at.group * a.C_group;
+
+    const int n0 = 2 * K * j;
+    F2 start[K];                                                         // the saved state in front of the tile
+    auto item_of = [&](int k, int& t, int& cc, int& valid) {
+        const int e = tid + k * THREADS;
+        t = e / CHV;
+        cc = (e % CHV) * 4;
+        const int64_t left = at.n_channels - cc;
+        valid = e >= ITEMS || left <= 0 ? 0 : left < 4 ? (int)left : 4;
+    };
+    auto slot_of = [&](int buf, int which, int k) { return raw + ((buf * 4 + which) * ITEMS + tid + k * THREADS) * 4; };
+    auto fetch = [&](int64_t t0, int buf) {
+#pragma unroll
+        for (int k = 0; k < IPT; ++k) {
+            int it, cc, valid;
+            item_of(k, it, cc, valid);
+            const int64_t t = t0 + it;
+            if (valid > 0 && t < t_used) {
+                const bool vec = d.vec && valid == 4;
+                if (!LOCAL) fetch_pack<T, 4>(slot_of(buf, 0, k), u + t * a.u_token + cc, vec, valid);
+                fetch_pack<T, 4>(slot_of(buf, 1, k), delta + t * a.delta_token + cc, vec, valid);
+                if (z) fetch_pack<T, 4>(slot_of(buf, 2, k), z + t * a.z_token + cc, vec, valid);
+                fetch_pack<T, 4>(slot_of(buf, 3, k), gout + t * a.gout_token + cc, vec, valid);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < QN; ++k) {
+            const int e = tid + k * THREADS, n = e % (NP / 4) * 4;
+            const int64_t t = t0 + e / (NP / 4);
+            if (e < QUADS && t < t_used && n < states) {
+                const bool vec = d.vec_bc && n + 4 <= states;
+                if (!LOCAL) fetch_pack<T, 4>(raw_bc + e * 4, B + t * a.B_token + n, vec, states - n);
+                fetch_pack<T, 4>(raw_bc + STEPS * NP + e * 4, C + t * a.C_token + n, vec, states - n);
+            }
+        }
+        copy_commit();
+        if (!LOCAL && live)
+            load_states(start, a.checkpoints + ((at.batch * chunks + t0 / kCheckpoint) * d.channels + channel) * states, n0,
+                        states, d.vec_states);
+    };
+    float bias[IPT][4], skip[IPT][4];
+#pragma unroll
+    for (int k = 0; k < IPT; ++k) {
+        int it, cc, valid;
+        item_of(k, it, cc, valid);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            bias[k][i] = a.delta_bias && i < valid ? a.delta_bias[base_c + cc + i] : 0.0f;
+            skip[k][i] = a.D && i < valid ? a.D[base_c + cc + i] : 0.0f;
+        }
+    }
+    auto stage = [&](int64_t t0, int buf) {
+#pragma unroll
+        for (int k = 0; k < IPT; ++k) {
+            int it, cc, valid;
+            item_of(k, it, cc, valid);
+            if (tid + k * THREADS < ITEMS) {
+                const bool in = t0 + it < t_used;
+                float x[4], dt[4], zz[4], g[4], slope[4], gate_slope[4];
+                if (!LOCAL) read_slot<T, 4>(slot_of(buf, 0, k), x);
+                read_slot<T, 4>(slot_of(buf, 1, k), dt);
+                if (z) read_slot<T, 4>(slot_of(buf, 2, k), zz);
+                read_slot<T, 4>(slot_of(buf, 3, k), g);
+#pragma unroll
+                for (int i = 0; i < 4; i += 2) {
+                    dt[i] += bias[k][i];
+                    dt[i + 1] += bias[k][i + 1];
+                    if (d.softplus) {
+                        const float x0 = dt[i], x1 = dt[i + 1];
+                        float e0, e1;
+                        softplus_pair(dt[i], dt[i + 1], e0, e1);
+                        // the derivative 1 / (1 + e^-x) from e = e^-|x|
+                        const float r0 = rcp_approx(1.0f + e0), r1 = rcp_approx(1.0f + e1);
+                        slope[i] = x0 < 0.0f ? e0 * r0 : r0;
+                        slope[i + 1] = x1 < 0.0f ? e1 * r1 : r1;
+                    } else {
+                        slope[i] = slope[i + 1] = 1.0f;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const bool ok = in && i < valid;
+                    gate_slope[i] = 0.0f;
+                    if (z) {
+                        const float sig = sigmoid(zz[i]), gate = zz[i] * sig;
+                        gate_slope[i] = g[i] * fmaf(gate, 1.0f - sig, sig);
+                        g[i] *= gate;
+                    }
+                    const float s = ok ? dt[i] : 0.0f, su = ok && !LOCAL ? dt[i] * x[i] : 0.0f, gy = ok ? g[i] : 0.0f;
+                    s_du[du_at<CH>(it, cc + i)] = make_float4(s, s, su, su);
+                    s_gy[it * CH + cc + i] = make_float2(gy, gy);
+                }
+                if (!LOCAL) {
+                    s_keep[tid + k * THREADS] = make_float4(slope[0], slope[1], slope[2], slope[3]);
+                    s_keep[ITEMS + tid + k * THREADS] = make_float4(gate_slope[0], gate_slope[1], gate_slope[2], gate_slope[3]);
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < QN; ++k) {
+            const int e = tid + k * THREADS;
+            if (e < QUADS) {
+                const bool in = t0 + e / (NP / 4) < t_used && e % (NP / 4) * 4 < states;
+                const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                float x[4];
+                if (!LOCAL) {
+                    read_slot<T, 4>(raw_bc + e * 4, x);
+                    reinterpret_cast<float4*>(s_b)[e] = in ? make_float4(x[0], x[1], x[2], x[3]) : zero;
+                }
+                read_slot<T, 4>(raw_bc + STEPS * NP + e * 4, x);
+                reinterpret_cast<float4*>(s_c)[e] = in ? make_float4(x[0], x[1], x[2], x[3]) : zero;
+            }
+        }
+    };
+
+    // lanes without a channel have A = h = gh = 0: their sums over channels are zeros
+    F2 A[K], w[K];                                                       // w: a_{t+1} gh_{t+1}
+#pragma unroll
+    for (int k = 0; k < K; ++k) A[k] = w[k] = start[k] = same2(0.0f);
+    if (live) load_states(A, a.A + channel * states, n0, states, d.vec_states);
+#pragma unroll
+    for (int k = 0; k < K; ++k) A[k] = mul2(A[k], same2(kLog2e));
+    if (last >= first) fetch(last, 0);
+    if (!LOCAL && live) {
+        if (at.segment < d.segments - 1)
+            load_states(w, p.seg_state + ((at.batch * d.segments + d.segments - 1) * d.channels + channel) * states, n0, states,
+                        d.vec_states);
+        else if (a.gfinal)
+            load_states(w, a.gfinal + (at.batch * d.channels + channel) * states, n0, states, d.vec_states);
+        for (int64_t s = d.segments - 2; s > at.segment; --s) {
+            const int64_t cell = (at.batch * d.segments + s) * d.channels + channel;
+            const F2 sum = same2(p.seg_dt[cell]);
+            F2 add[K];
+            load_states(add, p.seg_state + cell * states, n0, states, d.vec_states);
+#pragma unroll
+            for (int k = 0; k < K; ++k) w[k] = fma2(decay(A[k], sum), w[k], add[k]);
+        }
+    }
+    double gA[2 * K] = {};
+    float gD[IPT][4] = {}, gbias[IPT][4] = {};
+    float sum_dt = 0.0f;
+    const float4* const du_row = s_du + du_at<CH>(0, c);
+    const float2* const gy_row = s_gy + c;
+    const float* const b_row = s_b + n0;
+    const float* const c_row = s_c + n0;
+
+    int buf = 0;
+    for (int64_t t0 = last; t0 >= first; t0 -= STEPS, buf ^= 1) {
+        copy_wait<0>();
+        stage(t0, buf);
+        F2 h[STEPS + 1][K], f[STEPS][K];                                 // h[t]: the state in front of step t; factors
+#pragma unroll
+        for (int k = 0; k < K; ++k) h[0][k] = start[k];
+        __syncthreads();
+        if (t0 > first) fetch(t0 - STEPS, buf ^ 1);
+
+        // the states again, forwards
+#pragma unroll
+        for (int t = 0; t < STEPS; ++t) {
+            const float4 du = du_row[t * (CH + CH / 8)];
+            const F2 dt2 = pack2(du.x, du.y), du2 = pack2(du.z, du.w);
+#pragma unroll
+            for (int k = 0; k < K; ++k) f[t][k] = decay(A[k], dt2);
+            if (LOCAL) {
+                sum_dt += du.x;
+            } else {
+                F2 bb[K];
+                read_pairs(bb, b_row + t * NP);
+#pragma unroll
+                for (int k = 0; k < K; ++k) h[t + 1][k] = fma2(f[t][k], h[t][k], mul2(du2, bb[k]));
+            }
+        }
+        if (!LOCAL && z) {
+            float y[STEPS];
+#pragma unroll
+            for (int t = 0; t < STEPS; ++t) {
+                F2 cc[K];
+                read_pairs(cc, c_row + t * NP);
+                y[t] = dot(h[t + 1], cc);
+            }
+            reduce_lanes<STEPS, P, 1>(y, lane);
+            if (reduced_owner<STEPS, P>(j)) {
+                const int t = reduced_index<STEPS, P>(j);
+#pragma unroll
+                for (int i = 0; i < reduced_count<STEPS, P>(); ++i) s_y[(t + i) * ROW + c] = y[i];
+            }
+        }
+        // the gradients, backwards
+        F2 gA_tile[K];
+#pragma unroll
+        for (int k = 0; k < K; ++k) gA_tile[k] = same2(0.0f);
+#pragma unroll
+        for (int g = STEPS / 4 - 1; g >= 0; --g) {
+            float s[8];
+#pragma unroll
+            for (int i = 3; i >= 0; --i) {
+                const int t = g * 4 + i;
+                const float2 gy = gy_row[t * CH];
+                const F2 gy2 = pack2(gy.x, gy.y);
+                F2 cc[K], gh[K];
+                read_pairs(cc, c_row + t * NP);
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    gh[k] = fma2(gy2, cc[k], w[k]);
+                    w[k] = mul2(f[t][k], gh[k]);
+                }
+                if (!LOCAL) {
+                    const float4 du = du_row[t * (CH + CH / 8)];
+                    const F2 dt2 = pack2(du.x, du.y), du2 = pack2(du.z, du.w);
+                    F2 bb[K], q[K];
+                    read_pairs(bb, b_row + t * NP);
+                    float v[4 * K];                                      // gC, then gB
+#pragma unroll
+                    for (int k = 0; k < K; ++k) {
+                        unpack2(mul2(gy2, h[t + 1][k]), v[2 * k], v[2 * k + 1]);
+                        unpack2(mul2(du2, gh[k]), v[2 * K + 2 * k], v[2 * K + 2 * k + 1]);
+                    }
+                    reduce_lanes<4 * K, R, P>(v, lane);
+                    if (reduced_owner<4 * K, R>(lane / P)) {
+                        const int i0 = reduced_index<4 * K, R>(lane / P);
+                        float* const to = s_r + (warp * STEPS + t) * 2 * NP + n0;
+#pragma unroll
+                        for (int k = 0; k < reduced_count<4 * K, R>(); ++k) to[((i0 + k) / (2 * K)) * NP + (i0 + k) % (2 * K)] = v[k];
+                    }
+                    s[2 * i] = dot(gh, bb);
+#pragma unroll
+                    for (int k = 0; k < K; ++k) {
+                        q[k] = mul2(w[k], h[t][k]);
+                        gA_tile[k] = fma2(q[k], dt2, gA_tile[k]);
+                    }
+                    s[2 * i + 1] = dot(q, A);
+                }
+            }
+            if (!LOCAL) {
+                reduce_lanes<8, P, 1>(s, lane);
+                if (reduced_owner<8, P>(j)) {
+                    const int k0 = reduced_index<8, P>(j);
+#pragma unroll
+                    for (int k = 0; k < reduced_count<8, P>(); ++k)
+                        s_s[(((k0 + k) % 2) * STEPS + g * 4 + (k0 + k) / 2) * ROW + c] = s[k];
+                }
+            }
+        }
+        if (!LOCAL) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                float x, y;
+                unpack2(gA_tile[k], x, y);
+                gA[2 * k] += x;
+                gA[2 * k + 1] += y;
+            }
+        }
+        __syncthreads();
+        if (!LOCAL) {
+#pragma unroll
+            for (int k = 0; k < IPT; ++k) {
+                int it, cc, valid;
+                item_of(k, it, cc, valid);
+                const int64_t t = t0 + it;
+                if (valid > 0 && t < t_end) {
+                    const bool in = t < t_used, vec = d.vec && valid == 4;
+                    float x[4], gu[4], gd[4], gz[4];
+                    read_slot<T, 4>(slot_of(buf, 0, k), x);
+                    const float4 over4 = *reinterpret_cast<const float4*>(s_s + it * ROW + cc);
+                    const float4 qa4 = *reinterpret_cast<const float4*>(s_s + (STEPS + it) * ROW + cc);
+                    const float4 slope4 = s_keep[tid + k * THREADS], gs4 = s_keep[ITEMS + tid + k * THREADS];
+                    const float over[4] = {over4.x, over4.y, over4.z, over4.w}, qa[4] = {qa4.x, qa4.y, qa4.z, qa4.w};
+                    const float slope[4] = {slope4.x, slope4.y, slope4.z, slope4.w}, gs[4] = {gs4.x, gs4.y, gs4.z, gs4.w};
+                    float y[4] = {};
+                    if (z) {
+                        const float4 y4 = *reinterpret_cast<const float4*>(s_y + it * ROW + cc);
+                        y[0] = y4.x, y[1] = y4.y, y[2] = y4.z, y[3] = y4.w;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float dt = s_du[du_at<CH>(it, cc + i)].x, gy = s_gy[it * CH + cc + i].x;
+                        gu[i] = in ? fmaf(dt, over[i], skip[k][i] * gy) : 0.0f;
+                        gd[i] = in ? slope[i] * fmaf(x[i], over[i], kLn2 * qa[i]) : 0.0f;
+                        gz[i] = in ? gs[i] * fmaf(skip[k][i], x[i], y[i]) : 0.0f;
+                        gD[k][i] += in ? gy * x[i] : 0.0f;
+                        gbias[k][i] += gd[i];
+                    }
+                    const int64_t o = (at.batch * d.length + t) * d.channels + base_c + cc;
+                    store_pack<T, 4>(reinterpret_cast<T*>(a.gu) + o, gu, vec, valid);
+                    store_pack<T, 4>(reinterpret_cast<T*>(a.gdelta) + o, gd, vec, valid);
+                    if (a.gz) store_pack<T, 4>(reinterpret_cast<T*>(a.gz) + o, gz, vec, valid);
+                }
+            }
+            float* const part =
+                p.part_bc + (((at.batch * d.groups + at.group) * d.tiles + at.tile) * d.length + t0) * 2 * NP;
+            for (int e = tid; e < STEPS * 2 * NP; e += THREADS) {
+                float sum = 0.0f;
+#pragma unroll
+                for (int w = 0; w < WARPS; ++w) sum += s_r[w * STEPS * 2 * NP + e];
+                if (t0 + e / (2 * NP) < t_used) part[e] = sum;
+            }
+            // the epilogue reads what the next stage() overwrites
+            __syncthreads();
+        }
+    }
+    if (LOCAL) {
+        if (live) {
+            const int64_t cell = (at.batch * d.segments + at.segment) * d.channels + channel;
+            store_states(p.seg_state + cell * states, w, n0, states, d.vec_states);
+            if (j == 0) p.seg_dt[cell] = sum_dt;
+        }
+        return;
+    }
+    // gradients of padding behind the last tile
+    for (int64_t t0 = last + STEPS; t0 < t_end; t0 += STEPS) {
+        const float zero[4] = {};
+#pragma unroll
+        for (int k = 0; k < IPT; ++k) {
+            int it, cc, valid;
+            item_of(k, it, cc, valid);
+            if (valid > 0 && t0 + it < t_end) {
+                const bool vec = d.vec && valid == 4;
+                const int64_t o = (at.batch * d.length + t0 + it) * d.channels + base_c + cc;
+                store_pack<T, 4>(reinterpret_cast<T*>(a.gu) + o, zero, vec, valid);
+                store_pack<T, 4>(reinterpret_cast<T*>(a.gdelta) + o, zero, vec, valid);
+                if (a.gz) store_pack<T, 4>(reinterpret_cast<T*>(a.gz) + o, zero, vec, valid);
+            }
+        }
+    }
+    const int64_t part_row = at.batch * d.segments + at.segment;
+    if (live) {
+        F2 sums[K];
+#pragma unroll
+        for (int k = 0; k < K; ++k) sums[k] = pack2((float)gA[2 * k], (float)gA[2 * k + 1]);
+        store_states(p.part_A + (part_row * d.channels + channel) * states, sums, n0, states, d.vec_states);
+        if (d.ahead)
+            store_states(p.seg_state + ((at.batch * d.segments + at.segment) * d.channels + channel) * states, w, n0, states,
+                         d.vec_states);
+        if (a.ginitial && at.segment == 0)
+            store_states(a.ginitial + (at.batch * d.channels + channel) * states, w, n0, states, d.vec_states);
+    }
+    // gD and gdelta_bias: every thread has sums over its token of each tile; over the 16 tokens in shared memory
+    for (int which = 0; which < 2; ++which) {
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < IPT; ++k) {
+            int it, cc, valid;
+            item_of(k, it, cc, valid);
+            if (tid + k * THREADS < ITEMS) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s_y[it * ROW + cc + i] = which ? gbias[k][i] : gD[k][i];
+            }
+        }
+        __syncthreads();
+        for (int e = tid; e < at.n_channels; e += THREADS) {
+            float sum = 0.0f;
+            for (int t = 0; t < STEPS; ++t) sum += s_y[t * ROW + e];
+            p.part_D[(part_row * 2 + which) * d.channels + base_c + e] = sum;
+        }
+    }
+}
+
+// the segments from last to first, in two launches like the forward ones
+template <typename T, int P, int K>
+__global__ void __launch_bounds__(Shape<P, K>::THREADS, K == 1 ? 512 / Shape<P, K>::THREADS : 1) scan_backward(const __grid_constant__ ScanParams p) {
+    const Place at = block_place(p.d, Shape<P, K>::CH);
+    if (p.d.ahead && at.segment < p.d.segments - 1) scan_backward_block<T, P, K, true>(p, at);
+    else scan_backward_block<T, P, K, false>(p, at);
+}
+
+// gB and gC: the channel tiles' parts added up in tile order; one thread per (batch, token, group, state)
+template <typename T>
+__global__ void scan_backward_bc(const __grid_constant__ ScanParams p, int np) {
+    const ScanDims& d = p.d;
+    const int64_t per = d.length * d.groups * d.states;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < p.a.batch * per; i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t b = i / per;
+        int64_t k = i % per;
+        const int n = (int)(k % d.states);
+        k /= d.states;
+        const int64_t g = k % d.groups, t = k / d.groups;
+        float c = 0.0f, bb = 0.0f;
+        if (t < used_length(p.a.lengths, b, d.length)) {
+            const float* src = p.part_bc + ((b * d.groups + g) * d.tiles * d.length + t) * 2 * np + n;
+            for (int64_t tile = 0; tile < d.tiles; ++tile) {
+                c += src[tile * d.length * 2 * np];
+                bb += src[tile * d.length * 2 * np + np];
+            }
+        }
+        reinterpret_cast<T*>(p.a.gC)[i] = from_f32<T>(c);
+        reinterpret_cast<T*>(p.a.gB)[i] = from_f32<T>(bb);
+    }
+}
+
+// gA, gD, gdelta_bias: the parts of batches and segments added up in order
+__global__ void scan_backward_params(const __grid_constant__ ScanParams p) {
+    const ScanDims& d = p.d;
+    const int64_t rows = p.a.batch * d.segments, n_A = d.channels * d.states, total = n_A + 2 * d.channels;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+        const bool in_A = i < n_A;
+        const int64_t k = in_A ? i : i - n_A, stride = in_A ? n_A : 2 * d.channels;
+        const float* src = (in_A ? p.part_A : p.part_D) + k;
+        double sum = 0.0;
+        for (int64_t r = 0; r < rows; ++r) sum += src[r * stride];
+        float* const to = in_A ? p.a.gA : k < d.channels ? p.a.gD : p.a.gdelta_bias;
+        if (to) to[in_A || k < d.channels ? k : k - d.channels] = (float)sum;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// one token
+
+// a thread per 4 states of a (row, channel); a block works on one row
+template <typename T, int P>
+__global__ void __launch_bounds__(128) scan_step(const __grid_constant__ OvlSelectiveScanStep a, int64_t blocks_per_row,
+                                                 int vec_states) {
+    const int64_t row = blockIdx.x / blocks_per_row;
+    const int tid = threadIdx.x, lane = tid % 32, j = lane % P;
+    const int64_t channel_at = (blockIdx.x % blocks_per_row) * (128 / P) + tid / P;
+    const bool live = channel_at < a.channels;
+    const int64_t channel = live ? channel_at : a.channels - 1;
+    T* const out = reinterpret_cast<T*>(a.out) + row * a.channels;
+    int64_t slot = row;
+    if (a.slot_of_row) {
+        slot = a.slot_of_row[row];
+        int taken = 0;
+        for (int64_t r = tid; r < row; r += 128) taken |= slot >= 0 && a.slot_of_row[r] == slot;
+        taken = __syncthreads_or(taken);
+        if (slot < 0 || slot >= a.slots || taken) {
+            if (live && j == 0) out[channel] = from_f32<T>(slot < 0 ? 0.0f : __int_as_float(0x7fffffff));
+            return;
+        }
+    }
+    const int states = (int)a.states;
+    const int64_t group = channel / (a.channels / a.groups);
+    float* const state = a.state + (slot * a.channels + channel) * states;
+    F2 h[2], A[2], bb[2], cc[2];
+    load_states(h, state, 4 * j, states, vec_states);
+    load_states(A, a.A + channel * states, 4 * j, states, vec_states);
+    const T* const B = reinterpret_cast<const T*>(a.B) + row * a.B_row + group * a.B_group;
+    const T* const C = reinterpret_cast<const T*>(a.C) + row * a.C_row + group * a.C_group;
+    const float u = to_f32(reinterpret_cast<const T*>(a.u)[row * a.u_row + channel]);
+    float dt = to_f32(reinterpret_cast<const T*>(a.delta)[row * a.delta_row + channel]);
+    const float z = a.z ? to_f32(reinterpret_cast<const T*>(a.z)[row * a.z_row + channel]) : 0.0f;
+    const float skip = a.D ? a.D[channel] : 0.0f;
+    if (a.delta_bias) dt += a.delta_bias[channel];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int n = 4 * j + 2 * k;
+        bb[k] = pack2(n < states ? to_f32(B[n]) : 0.0f, n + 1 < states ? to_f32(B[n + 1]) : 0.0f);
+        cc[k] = pack2(n < states ? to_f32(C[n]) : 0.0f, n + 1 < states ? to_f32(C[n + 1]) : 0.0f);
+    }
+    if (a.delta_softplus) dt = softplus(dt);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) h[k] = fma2(decay(mul2(A[k], same2(kLog2e)), same2(dt)), h[k], mul2(same2(dt * u), bb[k]));
+    float y[1] = {dot(h, cc)};
+    reduce_lanes<1, P, 1>(y, lane);
+    if (!live) return;
+    store_states(state, h, 4 * j, states, vec_states);
+    if (j == 0) {
+        float o = fmaf(skip, u, y[0]);
+        if (a.z) o *= z * sigmoid(z);
+        out[channel] = from_f32<T>(o);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// launches
+
+template <typename F>
+int allow_smem(F kernel, size_t bytes) {
+    if (bytes > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        if (e != cudaSuccess) return record_cuda_error(e);
+    }
+    return OVL_OK;
+}
+
+// One launch, or the two of a length that is cut into segments.
+template <typename F>
+int launch_segments(F kernel, ScanParams p, int threads, size_t smem, bool backward, cudaStream_t stream) {
+    int st = allow_smem(kernel, smem);
+    if (st != OVL_OK) return st;
+    const int64_t n = p.d.segments, blocks = p.a.batch * p.d.groups * p.d.tiles;
+    for (int launch = n > 1 ? 0 : 1; launch < 2; ++launch) {
+        p.d.ahead = launch == 0;
+        p.d.launch_segments = n > 1 ? n - 1 : 1;
+        p.d.first_segment = n > 1 && p.d.ahead == (backward ? 1 : 0) ? 1 : 0;
+        kernel<<<(uint32_t)(blocks * p.d.launch_segments), threads, smem, stream>>>(p);
+        if ((st = launch_status()) != OVL_OK) return st;
+    }
+    return OVL_OK;
+}
+
+template <typename T, int P, int M>
+int run_forward(const ScanParams& p, cudaStream_t stream) {
+    return launch_segments(scan_forward<T, P, M>, p, ForwardShape<P, M>::THREADS, ForwardSmem<T, P, M>::bytes, false, stream);
+}
+
+inline uint32_t grid_for(int64_t items) {
+    const int64_t blocks = ceil_div(items, 256), most = 16 * 8 * (int64_t)sequence_sm_count();
+    return (uint32_t)(blocks < 1 ? 1 : blocks < most ? blocks : most);
+}
+
+template <typename T, int P, int K>
+int run_backward(const ScanParams& p, cudaStream_t stream) {
+    int st = launch_segments(scan_backward<T, P, K>, p, Shape<P, K>::THREADS, BackShape<T, P, K>::bytes, true, stream);
+    if (st != OVL_OK) return st;
+    scan_backward_bc<T><<<grid_for(p.a.batch * p.d.length * p.d.groups * p.d.states), 256, 0, stream>>>(p, Shape<P, K>::NP);
+    if ((st = launch_status()) != OVL_OK) return st;
+    scan_backward_params<<<grid_for(p.d.channels * (p.d.states + 2)), 256, 0, stream>>>(p);
+    return launch_status();
+}
+
+template <typename T>
+int scan_dispatch(const ScanParams& p, const ScanShape& s, bool backward, cudaStream_t stream) {
+#define OVL_SCAN_CASE(RUN, P, X) \
+    if (s.lanes == P && s.extent == X) return RUN<T, P, X>(p, stream);
+    if (backward) {
+        OVL_SCAN_CASE(run_backward, 2, 1)
+        OVL_SCAN_CASE(run_backward, 4, 1)
+        OVL_SCAN_CASE(run_backward, 8, 1)
+        OVL_SCAN_CASE(run_backward, 16, 1)
+        OVL_SCAN_CASE(run_backward, 32, 1)
+        OVL_SCAN_CASE(run_backward, 32, 2)
+    } else {
+        OVL_SCAN_CASE(run_forward, 1, 1)
+        OVL_SCAN_CASE(run_forward, 2, 1)
+        OVL_SCAN_CASE(run_forward, 4, 1)
+        OVL_SCAN_CASE(run_forward, 8, 1)
+        OVL_SCAN_CASE(run_forward, 16, 1)
+        OVL_SCAN_CASE(run_forward, 1, 2)
+        OVL_SCAN_CASE(run_forward, 2, 2)
+        OVL_SCAN_CASE(run_forward, 4, 2)
+        OVL_SCAN_CASE(run_forward, 8, 2)
+        OVL_SCAN_CASE(run_forward, 16, 2)
+        OVL_SCAN_CASE(run_forward, 32, 2)
+    }
+#undef OVL_SCAN_CASE
+    return OVL_ERR_INVALID;
+}
+
+template <typename T>
+int scan_step_dispatch(const OvlSelectiveScanStep& a, int lanes, cudaStream_t stream) {
+    const int64_t per_row = ceil_div(a.channels, 128 / lanes), blocks = per_row * a.rows;
+    if (blocks > 0x7fffffff) return OVL_ERR_TOO_LARGE;
+    const int vec = a.states % 4 == 0 && aligned16(a.A) && aligned16(a.state);
+    const uint32_t grid = (uint32_t)blocks;
+    switch (lanes) {
+        case 1: scan_step<T, 1><<<grid, 128, 0, stream>>>(a, per_row, vec); break;
+        case 2: scan_step<T, 2><<<grid, 128, 0, stream>>>(a, per_row, vec); break;
+        case 4: scan_step<T, 4><<<grid, 128, 0, stream>>>(a, per_row, vec); break;
+        case 8: scan_step<T, 8><<<grid, 128, 0, stream>>>(a, per_row, vec); break;
+        case 16: scan_step<T, 16><<<grid, 128, 0, stream>>>(a, per_row, vec); break;
+        default: scan_step<T, 32><<<grid, 128, 0, stream>>>(a, per_row, vec); break;
+    }
+    return launch_status();
+}
+
+}  // namespace
+}  // namespace ovl

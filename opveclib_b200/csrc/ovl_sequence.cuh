@@ -190,7 +190,9 @@ __device__ __forceinline__ void copy_async(void* to, const void* from) {
                  : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+// until at most LEFT of the thread's groups of copies are in flight
+template <int LEFT>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
 
 // N elements into a slot of shared memory that only this thread reads: in flight while it goes on (`vec`: aligned and
 // all there), otherwise element by element
