@@ -24,22 +24,19 @@ int lanes_for(int64_t states, int per_lane, int least) {
     return p;
 }
 
-ScanShape forward_shape(int64_t states, int channels_of_lane) {
-    ScanShape s;
-    s.lanes = lanes_for(states, 4, 1);
-    s.extent = channels_of_lane;
-    s.padded_states = 4 * s.lanes;
-    s.block_channels = 128 / s.lanes * s.extent;
+// Two channels per lane need less shared memory bandwidth and fewer instructions for each, one channel gives twice the
+// blocks.  bf16, 16 states, 2048 channels: with 256 blocks of 64 channels (8 x 2048 tokens) 238 us against 268 us, with
+// 128 of them (4 x 2048 tokens) 152 against 138 us.
+ScanShape forward_shape(const OvlSelectiveScan* a) {
+    ScanShape s{lanes_for(a->states, 4, 1), 2, 2};
+    const int64_t blocks = a->batch * a->groups * ceil_div(a->channels / a->groups, s.block_channels());
+    if (s.lanes < 32 && 2 * blocks < 3 * (int64_t)sequence_sm_count()) s.channels = 1;
     return s;
 }
 
-ScanShape backward_shape(int64_t states) {
-    ScanShape s;
-    s.extent = states > 64 ? 2 : 1;
-    s.lanes = lanes_for(states, 2 * s.extent, 2);
-    s.padded_states = 2 * s.extent * s.lanes;
-    s.block_channels = (s.lanes == 32 ? 256 : 128) / s.lanes;
-    return s;
+ScanShape backward_shape(const OvlSelectiveScan* a) {
+    if (a->states > 64) return ScanShape{32, 2, 1};
+    return ScanShape{lanes_for(a->states, 2, 4), 1, 2};
 }
 
 void make_dims(const OvlSelectiveScan* a, ScanDims* d, ScanShape* shape, bool backward) {
@@ -49,18 +46,17 @@ void make_dims(const OvlSelectiveScan* a, ScanDims* d, ScanShape* shape, bool ba
     d->groups = a->groups;
     d->group_channels = a->channels / a->groups;
     d->softplus = a->delta_softplus != 0;
-    int tune_k = 0, tune_s = 0;
-    if (const char* e = getenv("OVL_TUNE")) sscanf(e, "%d,%d", &tune_k, &tune_s);
-    *shape = backward ? backward_shape(a->states) : forward_shape(a->states, tune_k == 1 && a->states <= 64 ? 1 : 2);
-    d->tiles = ceil_div(d->group_channels, shape->block_channels);
+    *shape = backward ? backward_shape(a) : forward_shape(a);
+    d->tiles = ceil_div(d->group_channels, shape->block_channels());
+    int tune_s = 0;
+    if (const char* e = getenv("OVL_TUNE")) sscanf(e, "%d", &tune_s);
     const int64_t blocks = a->batch * a->groups * d->tiles;
-    const int64_t fill = sequence_sm_count() * 3;
-    int64_t s = blocks > 0 ? fill / blocks : 1;
+    int64_t s = blocks > 0 ? 1 + 2 * (int64_t)sequence_sm_count() / blocks : 1;
     if (tune_s) s = tune_s;
     const int64_t most = ceil_div(a->length, 64);
     if (s > most) s = most;
     if (s > kMaxSegments) s = kMaxSegments;
-    if (s < 3) s = 1;
+    if (s < 4) s = 1;
     d->segment_length = ceil_div(ceil_div(a->length > 0 ? a->length : 1, s), 32) * 32;
     d->segments = ceil_div(a->length > 0 ? a->length : 1, d->segment_length);
 }
@@ -83,7 +79,7 @@ Workspace layout(const OvlSelectiveScan* a, const ScanDims& d, const ScanShape& 
         w.dt = take((uint64_t)a->batch * d.segments * d.channels);
     }
     if (backward) {
-        w.bc = take((uint64_t)a->batch * d.groups * d.tiles * d.length * 2 * shape.padded_states);
+        w.bc = take((uint64_t)a->batch * d.groups * d.tiles * d.length * 2 * shape.padded_states());
         w.A = take((uint64_t)a->batch * d.segments * d.channels * d.states);
         w.D = take((uint64_t)a->batch * d.segments * 2 * d.channels);
     }

@@ -41,9 +41,11 @@ struct ScanParams {
     float* part_D;                     // [batch * segments, 2, channels]: gD, gdelta_bias
 };
 
-// Lanes of a channel, and how much a lane does: channels (forward) or pairs of states (backward).
+// Lanes of a channel, pairs of states of a lane, channels of a lane.
 struct ScanShape {
-    int lanes, extent, padded_states, block_channels;
+    int lanes, pairs, channels;
+    int padded_states() const { return 2 * pairs * lanes; }
+    int block_channels() const { return 128 / lanes * channels; }
 };
 
 // One source per element type (they are compiled side by side).
@@ -55,17 +57,6 @@ __attribute__((visibility("hidden"))) int scan_step_f16(const OvlSelectiveScanSt
 __attribute__((visibility("hidden"))) int scan_step_bf16(const OvlSelectiveScanStep&, int lanes, cudaStream_t);
 
 namespace {
-
-// P lanes of a channel with K pairs of states each
-template <int P, int K>
-struct Shape {
-    static constexpr int THREADS = P == 32 ? 256 : 128;
-    static constexpr int CH = THREADS / P;                               // channels of a block
-    static constexpr int NP = 2 * K * P;                                 // states, padded
-    static constexpr int ROW = CH + (P >= 8 ? 4 : 32 / P);               // row of per-channel sums in shared memory:
-                                                                         // lanes of different steps hit different banks
-    static_assert(NP % 4 == 0, "B and C are staged 4 states at a time");
-};
 
 // K pairs of states from state n0 on
 template <int K>
@@ -167,6 +158,7 @@ struct ForwardShape {
     static constexpr int ITEMS = STEPS * CH / 8;                         // 8 channels of one token
     static constexpr int IPT = (ITEMS + HELP - 1) / HELP;
     static constexpr int QUADS = STEPS * P, QPT = (QUADS + HELP - 1) / HELP;   // 4 states of one token
+    static constexpr int AHEAD = 2;                                      // tiles that are fetched ahead of the scan
     static constexpr int DU = CH + CH / 8 * 2;                           // row of s_du: 16 bytes of gap after 8 channels
     static constexpr int ROW = CH + (P >= 8 ? 4 : 32 / P);               // row of s_y: lanes of different steps hit different banks
 };
@@ -178,9 +170,9 @@ struct ForwardSmem {
     static constexpr size_t b = du + 2 * sizeof(float2) * S::STEPS * S::DU;                  // float [2][STEPS][NP]
     static constexpr size_t c = b + 2 * sizeof(float) * S::STEPS * S::NP;
     static constexpr size_t y = c + 2 * sizeof(float) * S::STEPS * S::NP;                    // float [2][STEPS][ROW]
-    static constexpr size_t raw = y + 2 * sizeof(float) * S::STEPS * S::ROW;                 // T [3][3][ITEMS][8]: u, delta, z
-    static constexpr size_t raw_bc = raw + 3 * 3 * sizeof(T) * S::STEPS * S::CH;             // T [2][2][QUADS][4]: B, C
-    static constexpr size_t bytes = raw_bc + 2 * 2 * sizeof(T) * S::STEPS * S::NP;
+    static constexpr size_t raw = y + 2 * sizeof(float) * S::STEPS * S::ROW;                 // T [AHEAD + 1][3][ITEMS][8]: u, delta, z
+    static constexpr size_t raw_bc = raw + (S::AHEAD + 1) * 3 * sizeof(T) * S::STEPS * S::CH;             // T [AHEAD][2][QUADS][4]: B, C
+    static constexpr size_t bytes = raw_bc + S::AHEAD * 2 * sizeof(T) * S::STEPS * S::NP;
 };
 
 // The scanning threads: nothing but the recurrence and its sums over the states.  A lane reads 16 bytes of dt and dt u
@@ -233,45 +225,60 @@ __device__ __forceinline__ void scan_forward_scan(const ScanParams& p, const Pla
     __syncthreads();
     int buf = 0;
     for (int64_t t0 = t_begin; t0 < t_used; t0 += STEPS, buf ^= 1) {
-#pragma unroll 1
-        for (int g = 0; g < STEPS / V; ++g) {
-            if (!LOCAL && a.checkpoints && (t0 + g * V) % kCheckpoint == 0 && t0 + g * V < d.length) {
-                const int64_t skip = (at.batch * (chunks - 1) + (t0 + g * V) / kCheckpoint) * d.channels * states;
+        // The factors and addends of two steps are formed while the two before them are walked, so that a warp that is
+        // alone on its scheduler does not wait for its own exponentials at every step (95 clocks per warp, step and two
+        // channels against 108; 57 against 59 with one channel).
+        F2 f[2][M][2], x[2][M][2], cc[2][2];
+        float y[M][V];
+        auto prepare = [&](int step, int i) {
+            const int t = buf * STEPS + step;
+            float dt[M], du[M];
+            if constexpr (M == 2) {
+                const float4 v = *reinterpret_cast<const float4*>(s_du + t * S::DU);
+                dt[0] = v.x, du[0] = v.y, dt[1] = v.z, du[1] = v.w;
+            } else {
+                const float2 v = s_du[t * S::DU];
+                dt[0] = v.x, du[0] = v.y;
+            }
+            F2 b[2];
+            read_pairs(b, s_b + t * NP);
+            if (!LOCAL) read_pairs(cc[i], s_c + t * NP);
+#pragma unroll
+            for (int m = 0; m < M; ++m) {
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    f[i][m][k] = decay(A[m][k], same2(dt[m]));
+                    x[i][m][k] = mul2(same2(du[m]), b[k]);
+                }
+                if (LOCAL) sum_dt[m] += dt[m];
+            }
+        };
+        prepare(0, 0);
+        prepare(1, 1);
+#pragma unroll
+        for (int step = 0; step < STEPS; ++step) {
+            const int i = step % 2;
+            if (step % V == 0 && !LOCAL && a.checkpoints && (t0 + step) % kCheckpoint == 0 && t0 + step < d.length) {
+                const int64_t skip = (at.batch * (chunks - 1) + (t0 + step) / kCheckpoint) * d.channels * states;
 #pragma unroll
                 for (int m = 0; m < M; ++m)
                     if (live[m]) store_states(a.checkpoints + skip + row[m], h[m], n0, states, d.vec_states);
             }
-            float y[M][V];
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const int t = buf * STEPS + g * V + i;
-                float dt[M], du[M];
-                if constexpr (M == 2) {
-                    const float4 v = *reinterpret_cast<const float4*>(s_du + t * S::DU);
-                    dt[0] = v.x, du[0] = v.y, dt[1] = v.z, du[1] = v.w;
-                } else {
-                    const float2 v = s_du[t * S::DU];
-                    dt[0] = v.x, du[0] = v.y;
-                }
-                F2 b[2], cc[2];
-                read_pairs(b, s_b + t * NP);
-                if (!LOCAL) read_pairs(cc, s_c + t * NP);
+            for (int m = 0; m < M; ++m) {
 #pragma unroll
-                for (int m = 0; m < M; ++m) {
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) h[m][k] = fma2(decay(A[m][k], same2(dt[m])), h[m][k], mul2(same2(du[m]), b[k]));
-                    if (LOCAL) sum_dt[m] += dt[m];
-                    else y[m][i] = dot(h[m], cc);
-                }
+                for (int k = 0; k < 2; ++k) h[m][k] = fma2(f[i][m][k], h[m][k], x[i][m][k]);
+                if (!LOCAL) y[m][step % V] = dot(h[m], cc[i]);
             }
-            if (!LOCAL) {
+            if (step + 2 < STEPS) prepare(step + 2, i);
+            if (!LOCAL && step % V == V - 1) {
 #pragma unroll
                 for (int m = 0; m < M; ++m) {
                     reduce_lanes<V, P, 1>(y[m], lane);
                     if (reduced_owner<V, P>(j)) {
-                        const int t = buf * STEPS + g * V + reduced_index<V, P>(j);
+                        const int t = buf * STEPS + step - (V - 1) + reduced_index<V, P>(j);
 #pragma unroll
-                        for (int i = 0; i < reduced_count<V, P>(); ++i) s_y[(t + i) * S::ROW + m] = y[m][i];
+                        for (int e = 0; e < reduced_count<V, P>(); ++e) s_y[(t + e) * S::ROW + m] = y[m][e];
                     }
                 }
             }
@@ -289,7 +296,7 @@ __device__ __forceinline__ void scan_forward_scan(const ScanParams& p, const Pla
     }
 }
 
-// The helping threads, one tile ahead of the scan and one behind it: they fetch u, delta, z, B and C (two tiles ahead,
+// The helping threads, one tile ahead of the scan and one behind it: they fetch u, delta, z, B and C (AHEAD tiles ahead,
 // each thread what it will need itself), leave dt, dt u, B and C for the scan, and finish the outputs from its sums.
 template <typename T, int P, int M, bool LOCAL>
 __device__ __forceinline__ void scan_forward_help(const ScanParams& p, const Place& at, char* smem, int64_t t_begin, int64_t t_end,
@@ -325,10 +332,11 @@ __device__ __forceinline__ void scan_forward_help(const ScanParams& p, const Pla
     auto slot_of = [&](int slot, int which, int k) {
         return reinterpret_cast<T*>(smem + Mem::raw) + ((slot * 3 + which) * S::ITEMS + tid + k * S::HELP) * 8;
     };
-    auto quad_of = [&](int buf, int which, int e) {
-        return reinterpret_cast<T*>(smem + Mem::raw_bc) + ((buf * 2 + which) * S::QUADS + e) * 4;
+    auto quad_of = [&](int slot, int which, int e) {
+        return reinterpret_cast<T*>(smem + Mem::raw_bc) + ((slot * 2 + which) * S::QUADS + e) * 4;
     };
-    auto fetch = [&](int64_t t0, int slot, int buf) {
+    // `slot` of u, delta, z (kept until the outputs are done), `bc_slot` of B and C (until they are staged)
+    auto fetch = [&](int64_t t0, int slot, int bc_slot) {
         if (t0 < t_used) {
 #pragma unroll
             for (int k = 0; k < IPT; ++k) {
@@ -345,14 +353,14 @@ __device__ __forceinline__ void scan_forward_help(const ScanParams& p, const Pla
                 const int64_t t = t0 + e / P;
                 if (e < S::QUADS && t < t_used && n < states) {
                     const bool wide = d.vec_bc && n + 4 <= states;
-                    fetch_pack<T, 4>(quad_of(buf, 0, e), B + t * a.B_token + n, wide, states - n);
-                    if (!LOCAL) fetch_pack<T, 4>(quad_of(buf, 1, e), C + t * a.C_token + n, wide, states - n);
+                    fetch_pack<T, 4>(quad_of(bc_slot, 0, e), B + t * a.B_token + n, wide, states - n);
+                    if (!LOCAL) fetch_pack<T, 4>(quad_of(bc_slot, 1, e), C + t * a.C_token + n, wide, states - n);
                 }
             }
         }
         copy_commit();
     };
-    auto stage = [&](int64_t t0, int slot, int buf) {
+    auto stage = [&](int64_t t0, int slot, int bc_slot, int buf) {
 #pragma unroll
         for (int k = 0; k < IPT; ++k) {
             const int it = item_t + k * ITEM_STEP;
@@ -384,8 +392,8 @@ __device__ __forceinline__ void scan_forward_help(const ScanParams& p, const Pla
                 const bool in = t0 + e / P < t_used && e % P * 4 < states;
                 float x[4] = {}, y[4] = {};
                 if (in) {
-                    read_slot<T, 4>(quad_of(buf, 0, e), x);
-                    if (!LOCAL) read_slot<T, 4>(quad_of(buf, 1, e), y);
+                    read_slot<T, 4>(quad_of(bc_slot, 0, e), x);
+                    if (!LOCAL) read_slot<T, 4>(quad_of(bc_slot, 1, e), y);
                 }
                 reinterpret_cast<float4*>(smem + Mem::b)[buf * S::QUADS + e] = make_float4(x[0], x[1], x[2], x[3]);
                 if (!LOCAL) reinterpret_cast<float4*>(smem + Mem::c)[buf * S::QUADS + e] = make_float4(y[0], y[1], y[2], y[3]);
@@ -417,19 +425,21 @@ __device__ __forceinline__ void scan_forward_help(const ScanParams& p, const Pla
         }
     };
 
-    fetch(t_begin, 0, 0);
-    fetch(t_begin + STEPS, 1, 1);
-    copy_wait<1>();
-    if (t_begin < t_used) stage(t_begin, 0, 0);
+#pragma unroll
+    for (int k = 0; k < S::AHEAD; ++k) fetch(t_begin + k * STEPS, k, k);
+    copy_wait<S::AHEAD - 1>();
+    if (t_begin < t_used) stage(t_begin, 0, 0, 0);
     __syncthreads();
-    int buf = 0, slot = 0;                                               // of the tile that is being scanned
+    int buf = 0, slot = 0, bc_slot = 0;                                  // of the tile that is being scanned
     for (int64_t t0 = t_begin; t0 < t_used; t0 += STEPS, buf ^= 1) {
-        const int next = slot == 2 ? 0 : slot + 1, before = slot == 0 ? 2 : slot - 1;
+        const int next = slot == S::AHEAD ? 0 : slot + 1, before = slot == 0 ? S::AHEAD : slot - 1;
+        const int bc_next = bc_slot == S::AHEAD - 1 ? 0 : bc_slot + 1;
         if (!LOCAL && t0 > t_begin) finish(t0 - STEPS, before, buf ^ 1);
-        fetch(t0 + 2 * STEPS, before, buf);                              // (B and C of this tile are staged already)
-        copy_wait<1>();
-        if (t0 + STEPS < t_used) stage(t0 + STEPS, next, buf ^ 1);
+        fetch(t0 + S::AHEAD * STEPS, before, bc_slot);                   // (B and C of this tile are staged already)
+        copy_wait<S::AHEAD - 1>();
+        if (t0 + STEPS < t_used) stage(t0 + STEPS, next, bc_next, buf ^ 1);
         slot = next;
+        bc_slot = bc_next;
         __syncthreads();
     }
     if (LOCAL) return;
@@ -437,7 +447,7 @@ __device__ __forceinline__ void scan_forward_help(const ScanParams& p, const Pla
     int64_t covered = t_begin;
     if (t_used > t_begin) {
         covered += (t_used - t_begin + STEPS - 1) / STEPS * STEPS;
-        finish(covered - STEPS, slot == 0 ? 2 : slot - 1, buf ^ 1);
+        finish(covered - STEPS, slot == 0 ? S::AHEAD : slot - 1, buf ^ 1);
     }
     if (valid > 0) {
         const float zero[8] = {};
@@ -462,17 +472,12 @@ __device__ __forceinline__ void scan_forward_block(const ScanParams& p, const Pl
 }
 
 template <typename T, int P, int M>
-__global__ void __launch_bounds__(ForwardShape<P, M>::THREADS) scan_forward(const __grid_constant__ ScanParams p) {
+__global__ void __launch_bounds__(ForwardShape<P, M>::THREADS, 2) scan_forward(const __grid_constant__ ScanParams p) {
     extern __shared__ __align__(16) char smem[];
     const Place at = block_place(p.d, ForwardShape<P, M>::CH);
     if (p.d.ahead && at.segment > 0) scan_forward_block<T, P, M, true>(p, at, smem);
     else scan_forward_block<T, P, M, false>(p, at, smem);
 }
-
-// Where (dt, dt, dt u, dt u) of channel c of a tile's token t stands, in float4: a gap after every 8 channels keeps the
-// wide stores of threads with 8 (or 4) channels each off one another's banks.
-template <int CH>
-__device__ __forceinline__ constexpr int du_at(int t, int c) { return t * (CH + CH / 8) + c + c / 8; }
 
 // ---------------------------------------------------------------------------------------------------------
 // backward
@@ -480,67 +485,272 @@ __device__ __forceinline__ constexpr int du_at(int t, int c) { return t * (CH + 
 // The gradient of the state runs from the last token to the first: gh_t = C_t gy_t + a_{t+1} gh_{t+1} with gy = gout
 // silu(z).  It meets the states h_t, which are computed again, 16 tokens at a time from the saved state in front of
 // them; the 16 states and factors of a lane stay in registers, so every exponential is computed once here too.
-//   gC_t = sum_d gy h_t, gB_t = sum_d gh_t dt u     sums over the channels: over the lanes of a warp with reduce_lanes,
-//                                                   over the warps in shared memory, over the blocks in a second launch
-//                                                   from partial sums (no atomics: the same bits every time)
+//   gC_t = sum_d gy h_t, gB_t = sum_d gh_t dt u     sums over the channels: over the channels of a lane in registers, over
+//                                                   the lanes of a warp with reduce_lanes, over the warps in shared
+//                                                   memory, over the blocks in a second launch from partial sums (no
+//                                                   atomics: the same bits every time)
 //   w_t = a_t gh_t (handed to the token before), q = w_t h_{t-1}: gA = sum q dt, g(dt) = sum_n q A + u sum_n gh B,
 //   gu = dt sum_n gh B + D gy
-template <typename T, int P, int K>
+// Scanning and helping threads as in the forward kernel.  The scanning threads need 132 registers for the states and
+// factors alone, the helping ones few: the block starts with 128 each and hands them over.
+
+// P lanes x K pairs of states x M channels
+template <int P, int K, int M>
 struct BackShape {
-    using S = Shape<P, K>;
+    static constexpr int SCAN = 128, HELP = 128, THREADS = SCAN + HELP;
+    static constexpr int WARPS = SCAN / 32;
+    static constexpr int CH = SCAN / P * M;
+    static constexpr int NP = 2 * K * P;
     static constexpr int STEPS = kCheckpoint;
-    static constexpr int WARPS = S::THREADS / 32;
-    static constexpr int CHV = S::CH / 4;                                // 4 channels of one token per item
-    static constexpr int ITEMS = STEPS * CHV;
-    static constexpr int IPT = (ITEMS + S::THREADS - 1) / S::THREADS;
-    static constexpr int ROW = S::ROW;
-    // shared memory
-    static constexpr size_t du = 0;                                                    // float4 [du_at]
-    static constexpr size_t gy = du + sizeof(float4) * STEPS * (S::CH + S::CH / 8);    // float2 [STEPS][CH] (gy, gy)
-    static constexpr size_t b = gy + sizeof(float2) * STEPS * S::CH;                   // float [STEPS][NP]
-    static constexpr size_t c = b + sizeof(float) * STEPS * S::NP;
-    static constexpr size_t y = c + sizeof(float) * STEPS * S::NP;                     // float [STEPS][ROW]: C . h
-    static constexpr size_t s = y + sizeof(float) * STEPS * ROW;                       // float [2][STEPS][ROW]: gh . B, q . A / ln 2
-    static constexpr size_t r = s + 2 * sizeof(float) * STEPS * ROW;                   // float [WARPS][STEPS][2][NP]: gC, gB
-    static constexpr size_t keep = r + sizeof(float) * WARPS * STEPS * 2 * S::NP;      // float4 [2][STEPS][CH / 4]
-    static constexpr size_t raw = keep + 2 * sizeof(float) * STEPS * S::CH;            // T [2][4][STEPS][CH]: u, delta, z, gout
-    static constexpr size_t raw_bc = raw + 2 * 4 * sizeof(T) * STEPS * S::CH;          // T [2][STEPS][NP]
-    static constexpr size_t bytes = raw_bc + 2 * sizeof(T) * STEPS * S::NP;
+    static constexpr int V = 8;                                          // steps whose C . h are summed together
+    static constexpr int CHV = CH / 4;                                   // 4 channels of one token per item
+    static constexpr int ITEMS = STEPS * CHV, IPT = (ITEMS + HELP - 1) / HELP;
+    static constexpr int QUADS = STEPS * NP / 4, QPT = (QUADS + HELP - 1) / HELP;
+    static constexpr int DU = CH + CH / 8 * 2;
+    static constexpr int ROW = CH + (P >= 8 ? 4 : 32 / P);
+    static constexpr int SLOTS = 3;
+    static constexpr int SCAN_REGISTERS = 192, HELP_REGISTERS = 64;      // together 2 x 128
 };
 
-template <typename T, int P, int K, bool LOCAL>
-__device__ __forceinline__ void scan_backward_block(const ScanParams& p, const Place& at) {
-    using S = Shape<P, K>;
-    using M = BackShape<T, P, K>;
-    constexpr int THREADS = S::THREADS, CH = S::CH, NP = S::NP, STEPS = M::STEPS, ROW = M::ROW, WARPS = M::WARPS;
-    constexpr int CHV = M::CHV, ITEMS = M::ITEMS, IPT = M::IPT;
-    constexpr int QUADS = STEPS * NP / 4, QN = (QUADS + THREADS - 1) / THREADS;
-    constexpr int R = 32 / P;                                            // channels of a warp
-    extern __shared__ __align__(16) char smem[];
-    float4* const s_du = reinterpret_cast<float4*>(smem + M::du);
-    float2* const s_gy = reinterpret_cast<float2*>(smem + M::gy);
-    float* const s_b = reinterpret_cast<float*>(smem + M::b);
-    float* const s_c = reinterpret_cast<float*>(smem + M::c);
-    float* const s_y = reinterpret_cast<float*>(smem + M::y);
-    float* const s_s = reinterpret_cast<float*>(smem + M::s);
-    float* const s_r = reinterpret_cast<float*>(smem + M::r);
-    float4* const s_keep = reinterpret_cast<float4*>(smem + M::keep);    // derivative of dt by delta, of out by z / y
-    T* const raw = reinterpret_cast<T*>(smem + M::raw);
-    T* const raw_bc = reinterpret_cast<T*>(smem + M::raw_bc);
+template <typename T, int P, int K, int M>
+struct BackSmem {
+    using S = BackShape<P, K, M>;
+    static constexpr size_t du = 0;                                                          // float2 [2][STEPS][DU]
+    static constexpr size_t gy = du + 2 * sizeof(float2) * S::STEPS * S::DU;                 // float [2][STEPS][CH]
+    static constexpr size_t b = gy + 2 * sizeof(float) * S::STEPS * S::CH;                   // float [2][STEPS][NP]
+    static constexpr size_t c = b + 2 * sizeof(float) * S::STEPS * S::NP;
+    static constexpr size_t y = c + 2 * sizeof(float) * S::STEPS * S::NP;                    // float [2][STEPS][ROW]: C . h
+    static constexpr size_t s = y + 2 * sizeof(float) * S::STEPS * S::ROW;                   // float [2][2][STEPS][ROW]: gh . B, q . A / ln 2
+    static constexpr size_t r = s + 4 * sizeof(float) * S::STEPS * S::ROW;                   // float [2][WARPS][STEPS][2][NP]: gC, gB
+    static constexpr size_t keep = r + 2 * sizeof(float) * S::WARPS * S::STEPS * 2 * S::NP;  // float4 [2][2][ITEMS]
+    static constexpr size_t raw = keep + 4 * sizeof(float4) * S::ITEMS;                      // T [SLOTS][4][ITEMS][4]: u, delta, z, gout
+    static constexpr size_t raw_bc = raw + S::SLOTS * 4 * sizeof(T) * S::ITEMS * 4;          // T [2][2][QUADS][4]
+    static constexpr size_t bytes = raw_bc + 4 * sizeof(T) * S::QUADS * 4;
+};
 
+template <typename T, int P, int K, int M, bool LOCAL>
+__device__ __forceinline__ void scan_backward_scan(const ScanParams& p, const Place& at, char* smem, int64_t t_begin, int64_t t_used) {
+    using S = BackShape<P, K, M>;
+    using Mem = BackSmem<T, P, K, M>;
+    constexpr int NP = S::NP, STEPS = S::STEPS, V = S::V, R = 32 / P;
     const OvlSelectiveScan& a = p.a;
     const ScanDims& d = p.d;
-    const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, j = lane % P, c = tid / P;
-    const bool live = c < at.n_channels;
-    const int64_t channel = at.channel0 + (live ? c : 0);
+    const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, j = lane % P, c0 = tid / P * M, n0 = 2 * K * j;
     const int states = (int)d.states;
-    const int64_t used = used_length(a.lengths, at.batch, d.length);
-    const int64_t t_begin = at.segment * d.segment_length;
-    const int64_t t_end = t_begin + d.segment_length < d.length ? t_begin + d.segment_length : d.length;
-    const int64_t t_used = used < t_end ? used : t_end;
     const int64_t chunks = (d.length + kCheckpoint - 1) / kCheckpoint;
+    // lanes without a channel have A = h = gh = 0: their sums over channels are zeros
+    bool live[M];
+    F2 A[M][K], w[M][K], start[M][K];                                    // w: a_{t+1} gh_{t+1}; start: the state in front of a tile
+    const float* saved[M];
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+        live[m] = c0 + m < at.n_channels;
+        const int64_t channel = at.channel0 + (live[m] ? c0 + m : 0);
+        saved[m] = a.checkpoints + (at.batch * chunks * d.channels + channel) * states;
+#pragma unroll
+        for (int k = 0; k < K; ++k) A[m][k] = w[m][k] = start[m][k] = same2(0.0f);
+        if (!live[m]) continue;
+        load_states(A[m], a.A + channel * states, n0, states, d.vec_states);
+#pragma unroll
+        for (int k = 0; k < K; ++k) A[m][k] = mul2(A[m][k], same2(kLog2e));
+        if (LOCAL) continue;
+        if (at.segment < d.segments - 1)
+            load_states(w[m], p.seg_state + ((at.batch * d.segments + d.segments - 1) * d.channels + channel) * states, n0, states,
+                        d.vec_states);
+        else if (a.gfinal)
+            load_states(w[m], a.gfinal + (at.batch * d.channels + channel) * states, n0, states, d.vec_states);
+        for (int64_t s = d.segments - 2; s > at.segment; --s) {
+            const int64_t cell = (at.batch * d.segments + s) * d.channels + channel;
+            const F2 sum = same2(p.seg_dt[cell]);
+            F2 add[K];
+            load_states(add, p.seg_state + cell * states, n0, states, d.vec_states);
+#pragma unroll
+            for (int k = 0; k < K; ++k) w[m][k] = fma2(decay(A[m][k], sum), w[m][k], add[k]);
+        }
+    }
     const int64_t first = t_begin, last = t_used > t_begin ? t_begin + (t_used - t_begin - 1) / STEPS * STEPS : t_begin - STEPS;
+    auto fetch_start = [&](int64_t t0) {
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+            if (live[m]) load_states(start[m], saved[m] + t0 / kCheckpoint * d.channels * states, n0, states, d.vec_states);
+    };
+    if (!LOCAL && last >= first) fetch_start(last);
+    const float2* const s_du = reinterpret_cast<const float2*>(smem + Mem::du) + c0 + c0 / 8 * 2;
+    const float* const s_gy = reinterpret_cast<const float*>(smem + Mem::gy) + c0;
+    const float* const s_b = reinterpret_cast<const float*>(smem + Mem::b) + n0;
+    const float* const s_c = reinterpret_cast<const float*>(smem + Mem::c) + n0;
+    float* const s_y = reinterpret_cast<float*>(smem + Mem::y) + c0;
+    float* const s_s = reinterpret_cast<float*>(smem + Mem::s) + c0;
+    float* const s_r = reinterpret_cast<float*>(smem + Mem::r) + warp * STEPS * 2 * NP + n0;
+    double gA[M][2 * K] = {};
+    float sum_dt[M] = {};
+    const bool gated = a.z != nullptr;
+    __syncthreads();
+    int buf = 0;
+    for (int64_t t0 = last; t0 >= first; t0 -= STEPS, buf ^= 1) {
+        auto read_du = [&](int t, float (&dt)[M], float (&du)[M]) {
+            if constexpr (M == 2) {
+                const float4 v = *reinterpret_cast<const float4*>(s_du + (buf * STEPS + t) * S::DU);
+                dt[0] = v.x, du[0] = v.y, dt[1] = v.z, du[1] = v.w;
+            } else {
+                const float2 v = s_du[(buf * STEPS + t) * S::DU];
+                dt[0] = v.x, du[0] = v.y;
+            }
+        };
+        F2 h[STEPS + 1][M][K], f[STEPS][M][K];                           // h[t]: the state in front of step t; factors
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+            for (int k = 0; k < K; ++k) h[0][m][k] = start[m][k];
+        if (!LOCAL && t0 > first) fetch_start(t0 - STEPS);
 
+        // the states again, forwards
+        float y[M][V];
+#pragma unroll
+        for (int t = 0; t < STEPS; ++t) {
+            float dt[M], du[M];
+            F2 b[K], cc[K];
+            read_du(t, dt, du);
+            if (!LOCAL) {
+                read_pairs(b, s_b + (buf * STEPS + t) * NP);
+                read_pairs(cc, s_c + (buf * STEPS + t) * NP);
+            }
+#pragma unroll
+            for (int m = 0; m < M; ++m) {
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    f[t][m][k] = decay(A[m][k], same2(dt[m]));
+                    if (!LOCAL) h[t + 1][m][k] = fma2(f[t][m][k], h[t][m][k], mul2(same2(du[m]), b[k]));
+                }
+                if (LOCAL) sum_dt[m] += dt[m];
+                else y[m][t % V] = dot(h[t + 1][m], cc);
+            }
+            if (!LOCAL && gated && t % V == V - 1) {
+#pragma unroll
+                for (int m = 0; m < M; ++m) {
+                    reduce_lanes<V, P, 1>(y[m], lane);
+                    if (reduced_owner<V, P>(j)) {
+                        const int tt = buf * STEPS + t - (V - 1) + reduced_index<V, P>(j);
+#pragma unroll
+                        for (int e = 0; e < reduced_count<V, P>(); ++e) s_y[(tt + e) * S::ROW + m] = y[m][e];
+                    }
+                }
+            }
+        }
+        // the gradients, backwards
+        F2 gA_tile[M][K];
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+            for (int k = 0; k < K; ++k) gA_tile[m][k] = same2(0.0f);
+#pragma unroll
+        for (int g = STEPS / 4 - 1; g >= 0; --g) {
+            float s[M][8];
+#pragma unroll
+            for (int i = 3; i >= 0; --i) {
+                const int t = g * 4 + i;
+                float gy[M], dt[M], du[M];
+                F2 b[K], cc[K], sum_c[K], sum_b[K];
+                if constexpr (M == 2) {
+                    const float2 v = *reinterpret_cast<const float2*>(s_gy + (buf * STEPS + t) * S::CH);
+                    gy[0] = v.x, gy[1] = v.y;
+                } else {
+                    gy[0] = s_gy[(buf * STEPS + t) * S::CH];
+                }
+                read_pairs(cc, s_c + (buf * STEPS + t) * NP);
+                if (!LOCAL) {
+                    read_du(t, dt, du);
+                    read_pairs(b, s_b + (buf * STEPS + t) * NP);
+                }
+#pragma unroll
+                for (int m = 0; m < M; ++m) {
+                    F2 gh[K], q[K];
+#pragma unroll
+                    for (int k = 0; k < K; ++k) {
+                        gh[k] = fma2(same2(gy[m]), cc[k], w[m][k]);
+                        w[m][k] = mul2(f[t][m][k], gh[k]);
+                        if (LOCAL) continue;
+                        sum_c[k] = m == 0 ? mul2(same2(gy[m]), h[t + 1][m][k]) : fma2(same2(gy[m]), h[t + 1][m][k], sum_c[k]);
+                        sum_b[k] = m == 0 ? mul2(same2(du[m]), gh[k]) : fma2(same2(du[m]), gh[k], sum_b[k]);
+                        q[k] = mul2(w[m][k], h[t][m][k]);
+                        gA_tile[m][k] = fma2(q[k], same2(dt[m]), gA_tile[m][k]);
+                    }
+                    if (!LOCAL) {
+                        s[m][2 * i] = dot(gh, b);
+                        s[m][2 * i + 1] = dot(q, A[m]);
+                    }
+                }
+                if (!LOCAL) {
+                    float v[4 * K];                                      // gC, then gB
+#pragma unroll
+                    for (int k = 0; k < K; ++k) {
+                        unpack2(sum_c[k], v[2 * k], v[2 * k + 1]);
+                        unpack2(sum_b[k], v[2 * K + 2 * k], v[2 * K + 2 * k + 1]);
+                    }
+                    reduce_lanes<4 * K, R, P>(v, lane);
+                    if (reduced_owner<4 * K, R>(lane / P)) {
+                        const int i0 = reduced_index<4 * K, R>(lane / P);
+                        float* const to = s_r + (buf * S::WARPS * STEPS + t) * 2 * NP;
+#pragma unroll
+                        for (int k = 0; k < reduced_count<4 * K, R>(); ++k) to[((i0 + k) / (2 * K)) * NP + (i0 + k) % (2 * K)] = v[k];
+                    }
+                }
+            }
+            if (!LOCAL) {
+#pragma unroll
+                for (int m = 0; m < M; ++m) {
+                    reduce_lanes<8, P, 1>(s[m], lane);
+                    if (reduced_owner<8, P>(j)) {
+                        const int k0 = reduced_index<8, P>(j);
+#pragma unroll
+                        for (int k = 0; k < reduced_count<8, P>(); ++k)
+                            s_s[((buf * 2 + (k0 + k) % 2) * STEPS + g * 4 + (k0 + k) / 2) * S::ROW + m] = s[m][k];
+                    }
+                }
+            }
+        }
+        if (!LOCAL) {
+#pragma unroll
+            for (int m = 0; m < M; ++m)
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    float x0, x1;
+                    unpack2(gA_tile[m][k], x0, x1);
+                    gA[m][2 * k] += x0;
+                    gA[m][2 * k + 1] += x1;
+                }
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+        if (!live[m]) continue;
+        const int64_t channel = at.channel0 + c0 + m, cell = (at.batch * d.segments + at.segment) * d.channels + channel;
+        if (d.ahead) store_states(p.seg_state + cell * states, w[m], n0, states, d.vec_states);
+        if (LOCAL) {
+            if (j == 0) p.seg_dt[cell] = sum_dt[m];
+            continue;
+        }
+        F2 sums[K];
+#pragma unroll
+        for (int k = 0; k < K; ++k) sums[k] = pack2((float)gA[m][2 * k], (float)gA[m][2 * k + 1]);
+        store_states(p.part_A + cell * states, sums, n0, states, d.vec_states);
+        if (a.ginitial && at.segment == 0)
+            store_states(a.ginitial + (at.batch * d.channels + channel) * states, w[m], n0, states, d.vec_states);
+    }
+}
+
+template <typename T, int P, int K, int M, bool LOCAL>
+__device__ __forceinline__ void scan_backward_help(const ScanParams& p, const Place& at, char* smem, int64_t t_begin, int64_t t_end,
+                                                   int64_t t_used) {
+    using S = BackShape<P, K, M>;
+    using Mem = BackSmem<T, P, K, M>;
+    constexpr int CH = S::CH, NP = S::NP, STEPS = S::STEPS, IPT = S::IPT, QPT = S::QPT, ITEMS = S::ITEMS;
+    const OvlSelectiveScan& a = p.a;
+    const ScanDims& d = p.d;
+    const int tid = threadIdx.x - S::SCAN;
+    const int states = (int)d.states;
+    const int64_t first = t_begin, last = t_used > t_begin ? t_begin + (t_used - t_begin - 1) / STEPS * STEPS : t_begin - STEPS;
     const int64_t base_c = at.channel0;
     const T* const u = reinterpret_cast<const T*>(a.u) + at.batch * a.u_batch + base_c;
     const T* const delta = reinterpret_cast<const T*>(a.delta) + at.batch * a.delta_batch + base_c;
@@ -548,369 +758,248 @@ __device__ __forceinline__ void scan_backward_block(const ScanParams& p, const P
     const T* const gout = reinterpret_cast<const T*>(a.gout) + at.batch * a.gout_batch + base_c;
     const T* const B = reinterpret_cast<const T*>(a.B) + at.batch * a.B_batch + at.group * a.B_group;
     const T* const C = reinterpret_cast<const T*>(a.C) + at.batch * a.C_batch + at.group * a.C_group;
+    float2* const s_du = reinterpret_cast<float2*>(smem + Mem::du);
+    float* const s_gy = reinterpret_cast<float*>(smem + Mem::gy);
+    float4* const s_keep = reinterpret_cast<float4*>(smem + Mem::keep);  // derivative of dt by delta, of out by z over y
 
-    const int n0 = 2 * K * j;
-    F2 start[K];                                                         // the saved state in front of the tile
-    auto item_of = [&](int k, int& t, int& cc, int& valid) {
-        const int e = tid + k * THREADS;
-        t = e / CHV;
-        cc = (e % CHV) * 4;
-        const int64_t left = at.n_channels - cc;
-        valid = e >= ITEMS || left <= 0 ? 0 : left < 4 ? (int)left : 4;
+    // this thread's parts of a tile: 4 channels of one token; all of them have the same channels
+    static_assert(S::HELP % S::CHV == 0, "the parts of a thread have the same channels");
+    constexpr int ITEM_STEP = S::HELP / S::CHV;
+    const bool has_item = tid < ITEMS;
+    const int item_t = tid / S::CHV, cc = tid % S::CHV * 4;
+    const int valid = !has_item || cc >= at.n_channels ? 0 : at.n_channels - cc < 4 ? (int)(at.n_channels - cc) : 4;
+    const bool vec = d.vec && valid == 4;
+    float bias[4], skip[4], gD[4] = {}, gbias[4] = {};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        bias[i] = a.delta_bias && i < valid ? a.delta_bias[base_c + cc + i] : 0.0f;
+        skip[i] = a.D && i < valid ? a.D[base_c + cc + i] : 0.0f;
+    }
+    auto slot_of = [&](int slot, int which, int k) {
+        return reinterpret_cast<T*>(smem + Mem::raw) + ((slot * 4 + which) * ITEMS + tid + k * S::HELP) * 4;
     };
-    auto slot_of = [&](int buf, int which, int k) { return raw + ((buf * 4 + which) * ITEMS + tid + k * THREADS) * 4; };
-    auto fetch = [&](int64_t t0, int buf) {
+    auto quad_of = [&](int slot, int which, int e) {
+        return reinterpret_cast<T*>(smem + Mem::raw_bc) + ((slot * 2 + which) * S::QUADS + e) * 4;
+    };
+    auto fetch = [&](int64_t t0, int slot, int bc_slot) {
+        if (t0 >= first) {
 #pragma unroll
-        for (int k = 0; k < IPT; ++k) {
-            int it, cc, valid;
-            item_of(k, it, cc, valid);
-            const int64_t t = t0 + it;
-            if (valid > 0 && t < t_used) {
-                const bool vec = d.vec && valid == 4;
-                if (!LOCAL) fetch_pack<T, 4>(slot_of(buf, 0, k), u + t * a.u_token + cc, vec, valid);
-                fetch_pack<T, 4>(slot_of(buf, 1, k), delta + t * a.delta_token + cc, vec, valid);
-                if (z) fetch_pack<T, 4>(slot_of(buf, 2, k), z + t * a.z_token + cc, vec, valid);
-                fetch_pack<T, 4>(slot_of(buf, 3, k), gout + t * a.gout_token + cc, vec, valid);
+            for (int k = 0; k < IPT; ++k) {
+                const int64_t t = t0 + item_t + k * ITEM_STEP;
+                if (valid > 0 && t < t_used) {
+                    if (!LOCAL) fetch_pack<T, 4>(slot_of(slot, 0, k), u + t * a.u_token + cc, vec, valid);
+                    fetch_pack<T, 4>(slot_of(slot, 1, k), delta + t * a.delta_token + cc, vec, valid);
+                    if (z) fetch_pack<T, 4>(slot_of(slot, 2, k), z + t * a.z_token + cc, vec, valid);
+                    fetch_pack<T, 4>(slot_of(slot, 3, k), gout + t * a.gout_token + cc, vec, valid);
+                }
             }
-        }
 #pragma unroll
-        for (int k = 0; k < QN; ++k) {
-            const int e = tid + k * THREADS, n = e % (NP / 4) * 4;
-            const int64_t t = t0 + e / (NP / 4);
-            if (e < QUADS && t < t_used && n < states) {
-                const bool vec = d.vec_bc && n + 4 <= states;
-                if (!LOCAL) fetch_pack<T, 4>(raw_bc + e * 4, B + t * a.B_token + n, vec, states - n);
-                fetch_pack<T, 4>(raw_bc + STEPS * NP + e * 4, C + t * a.C_token + n, vec, states - n);
+            for (int k = 0; k < QPT; ++k) {
+                const int e = tid + k * S::HELP, n = e % (NP / 4) * 4;
+                const int64_t t = t0 + e / (NP / 4);
+                if (e < S::QUADS && t < t_used && n < states) {
+                    const bool wide = d.vec_bc && n + 4 <= states;
+                    if (!LOCAL) fetch_pack<T, 4>(quad_of(bc_slot, 0, e), B + t * a.B_token + n, wide, states - n);
+                    fetch_pack<T, 4>(quad_of(bc_slot, 1, e), C + t * a.C_token + n, wide, states - n);
+                }
             }
         }
         copy_commit();
-        if (!LOCAL && live)
-            load_states(start, a.checkpoints + ((at.batch * chunks + t0 / kCheckpoint) * d.channels + channel) * states, n0,
-                        states, d.vec_states);
     };
-    float bias[IPT][4], skip[IPT][4];
-#pragma unroll
-    for (int k = 0; k < IPT; ++k) {
-        int it, cc, valid;
-        item_of(k, it, cc, valid);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            bias[k][i] = a.delta_bias && i < valid ? a.delta_bias[base_c + cc + i] : 0.0f;
-            skip[k][i] = a.D && i < valid ? a.D[base_c + cc + i] : 0.0f;
-        }
-    }
-    auto stage = [&](int64_t t0, int buf) {
+    auto stage = [&](int64_t t0, int slot, int buf) {
 #pragma unroll
         for (int k = 0; k < IPT; ++k) {
-            int it, cc, valid;
-            item_of(k, it, cc, valid);
-            if (tid + k * THREADS < ITEMS) {
-                const bool in = t0 + it < t_used;
-                float x[4], dt[4], zz[4], g[4], slope[4], gate_slope[4];
-                if (!LOCAL) read_slot<T, 4>(slot_of(buf, 0, k), x);
-                read_slot<T, 4>(slot_of(buf, 1, k), dt);
-                if (z) read_slot<T, 4>(slot_of(buf, 2, k), zz);
-                read_slot<T, 4>(slot_of(buf, 3, k), g);
+            const int it = item_t + k * ITEM_STEP;
+            if (!has_item) continue;
+            const bool in = t0 + it < t_used;
+            float x[4] = {}, dt[4] = {}, zz[4], g[4] = {}, slope[4], gate_slope[4] = {};
+            if (in && valid > 0) {
+                if (!LOCAL) read_slot<T, 4>(slot_of(slot, 0, k), x);
+                read_slot<T, 4>(slot_of(slot, 1, k), dt);
+                read_slot<T, 4>(slot_of(slot, 3, k), g);
+            }
 #pragma unroll
-                for (int i = 0; i < 4; i += 2) {
-                    dt[i] += bias[k][i];
-                    dt[i + 1] += bias[k][i + 1];
-                    if (d.softplus) {
-                        const float x0 = dt[i], x1 = dt[i + 1];
-                        float e0, e1;
-                        softplus_pair(dt[i], dt[i + 1], e0, e1);
-                        // the derivative 1 / (1 + e^-x) from e = e^-|x|
-                        const float r0 = rcp_approx(1.0f + e0), r1 = rcp_approx(1.0f + e1);
-                        slope[i] = x0 < 0.0f ? e0 * r0 : r0;
-                        slope[i + 1] = x1 < 0.0f ? e1 * r1 : r1;
-                    } else {
-                        slope[i] = slope[i + 1] = 1.0f;
-                    }
+            for (int i = 0; i < 4; i += 2) {
+                dt[i] += bias[i];
+                dt[i + 1] += bias[i + 1];
+                slope[i] = slope[i + 1] = 1.0f;
+                if (d.softplus) {
+                    const float x0 = dt[i], x1 = dt[i + 1];
+                    float e0, e1;
+                    softplus_pair(dt[i], dt[i + 1], e0, e1);
+                    // the derivative 1 / (1 + e^-x) from e = e^-|x|
+                    const float r0 = rcp_approx(1.0f + e0), r1 = rcp_approx(1.0f + e1);
+                    slope[i] = x0 < 0.0f ? e0 * r0 : r0;
+                    slope[i + 1] = x1 < 0.0f ? e1 * r1 : r1;
                 }
+            }
+            if (z && in && valid > 0) {
+                read_slot<T, 4>(slot_of(slot, 2, k), zz);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const bool ok = in && i < valid;
-                    gate_slope[i] = 0.0f;
-                    if (z) {
-                        const float sig = sigmoid(zz[i]), gate = zz[i] * sig;
-                        gate_slope[i] = g[i] * fmaf(gate, 1.0f - sig, sig);
-                        g[i] *= gate;
-                    }
-                    const float s = ok ? dt[i] : 0.0f, su = ok && !LOCAL ? dt[i] * x[i] : 0.0f, gy = ok ? g[i] : 0.0f;
-                    s_du[du_at<CH>(it, cc + i)] = make_float4(s, s, su, su);
-                    s_gy[it * CH + cc + i] = make_float2(gy, gy);
+                    const float sig = sigmoid(zz[i]), gate = zz[i] * sig;
+                    gate_slope[i] = g[i] * fmaf(gate, 1.0f - sig, sig);
+                    g[i] *= gate;
                 }
-                if (!LOCAL) {
-                    s_keep[tid + k * THREADS] = make_float4(slope[0], slope[1], slope[2], slope[3]);
-                    s_keep[ITEMS + tid + k * THREADS] = make_float4(gate_slope[0], gate_slope[1], gate_slope[2], gate_slope[3]);
-                }
+            }
+            // padding: dt = 0 hands the gradient on as it is, gy = dt u = 0 adds nothing
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (!in || i >= valid) dt[i] = g[i] = x[i] = 0.0f;
+                x[i] = in && i < valid ? dt[i] * x[i] : 0.0f;
+            }
+            float4* const to = reinterpret_cast<float4*>(s_du + (buf * STEPS + it) * S::DU + cc + cc / 8 * 2);
+            to[0] = make_float4(dt[0], x[0], dt[1], x[1]);
+            to[1] = make_float4(dt[2], x[2], dt[3], x[3]);
+            *reinterpret_cast<float4*>(s_gy + (buf * STEPS + it) * CH + cc) = make_float4(g[0], g[1], g[2], g[3]);
+            if (!LOCAL) {
+                s_keep[(buf * 2) * ITEMS + tid + k * S::HELP] = make_float4(slope[0], slope[1], slope[2], slope[3]);
+                s_keep[(buf * 2 + 1) * ITEMS + tid + k * S::HELP] = make_float4(gate_slope[0], gate_slope[1], gate_slope[2], gate_slope[3]);
             }
         }
 #pragma unroll
-        for (int k = 0; k < QN; ++k) {
-            const int e = tid + k * THREADS;
-            if (e < QUADS) {
-                const bool in = t0 + e / (NP / 4) < t_used && e % (NP / 4) * 4 < states;
-                const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                float x[4];
-                if (!LOCAL) {
-                    read_slot<T, 4>(raw_bc + e * 4, x);
-                    reinterpret_cast<float4*>(s_b)[e] = in ? make_float4(x[0], x[1], x[2], x[3]) : zero;
+        for (int k = 0; k < QPT; ++k) {
+            const int e = tid + k * S::HELP;
+            if (e < S::QUADS) {
+                float x[4] = {}, y[4] = {};
+                if (t0 + e / (NP / 4) < t_used && e % (NP / 4) * 4 < states) {
+                    if (!LOCAL) read_slot<T, 4>(quad_of(buf, 0, e), x);
+                    read_slot<T, 4>(quad_of(buf, 1, e), y);
                 }
-                read_slot<T, 4>(raw_bc + STEPS * NP + e * 4, x);
-                reinterpret_cast<float4*>(s_c)[e] = in ? make_float4(x[0], x[1], x[2], x[3]) : zero;
+                if (!LOCAL) reinterpret_cast<float4*>(smem + Mem::b)[buf * S::QUADS + e] = make_float4(x[0], x[1], x[2], x[3]);
+                reinterpret_cast<float4*>(smem + Mem::c)[buf * S::QUADS + e] = make_float4(y[0], y[1], y[2], y[3]);
             }
         }
     };
-
-    // lanes without a channel have A = h = gh = 0: their sums over channels are zeros
-    F2 A[K], w[K];                                                       // w: a_{t+1} gh_{t+1}
+    auto finish = [&](int64_t t0, int slot, int buf) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) A[k] = w[k] = start[k] = same2(0.0f);
-    if (live) load_states(A, a.A + channel * states, n0, states, d.vec_states);
+        for (int k = 0; k < IPT; ++k) {
+            const int it = item_t + k * ITEM_STEP;
+            const int64_t t = t0 + it;
+            if (valid == 0 || t >= t_end) continue;
+            float gu[4] = {}, gd[4] = {}, gz[4] = {};
+            if (t < t_used) {
+                float x[4], over[4], qa[4], slope[4], gs[4], y[4] = {}, gy[4], dt[4];
+                auto four = [](float (&v)[4], const float* from) {
+                    const float4 r = *reinterpret_cast<const float4*>(from);
+                    v[0] = r.x, v[1] = r.y, v[2] = r.z, v[3] = r.w;
+                };
+                read_slot<T, 4>(slot_of(slot, 0, k), x);
+                four(over, reinterpret_cast<const float*>(smem + Mem::s) + ((buf * 2) * STEPS + it) * S::ROW + cc);
+                four(qa, reinterpret_cast<const float*>(smem + Mem::s) + ((buf * 2 + 1) * STEPS + it) * S::ROW + cc);
+                four(slope, reinterpret_cast<const float*>(s_keep + (buf * 2) * ITEMS + tid + k * S::HELP));
+                four(gs, reinterpret_cast<const float*>(s_keep + (buf * 2 + 1) * ITEMS + tid + k * S::HELP));
+                four(gy, s_gy + (buf * STEPS + it) * CH + cc);
+                if (z) four(y, reinterpret_cast<const float*>(smem + Mem::y) + (buf * STEPS + it) * S::ROW + cc);
+                const float4* const du = reinterpret_cast<const float4*>(s_du + (buf * STEPS + it) * S::DU + cc + cc / 8 * 2);
+                dt[0] = du[0].x, dt[1] = du[0].z, dt[2] = du[1].x, dt[3] = du[1].z;
 #pragma unroll
-    for (int k = 0; k < K; ++k) A[k] = mul2(A[k], same2(kLog2e));
-    if (last >= first) fetch(last, 0);
-    if (!LOCAL && live) {
-        if (at.segment < d.segments - 1)
-            load_states(w, p.seg_state + ((at.batch * d.segments + d.segments - 1) * d.channels + channel) * states, n0, states,
-                        d.vec_states);
-        else if (a.gfinal)
-            load_states(w, a.gfinal + (at.batch * d.channels + channel) * states, n0, states, d.vec_states);
-        for (int64_t s = d.segments - 2; s > at.segment; --s) {
-            const int64_t cell = (at.batch * d.segments + s) * d.channels + channel;
-            const F2 sum = same2(p.seg_dt[cell]);
-            F2 add[K];
-            load_states(add, p.seg_state + cell * states, n0, states, d.vec_states);
-#pragma unroll
-            for (int k = 0; k < K; ++k) w[k] = fma2(decay(A[k], sum), w[k], add[k]);
+                for (int i = 0; i < 4; ++i) {
+                    gu[i] = fmaf(dt[i], over[i], skip[i] * gy[i]);
+                    gd[i] = slope[i] * fmaf(x[i], over[i], kLn2 * qa[i]);
+                    gz[i] = gs[i] * fmaf(skip[i], x[i], y[i]);
+                    gD[i] = fmaf(gy[i], x[i], gD[i]);
+                    gbias[i] += gd[i];
+                }
+            }
+            const int64_t o = (at.batch * d.length + t) * d.channels + base_c + cc;
+            store_pack<T, 4>(reinterpret_cast<T*>(a.gu) + o, gu, vec, valid);
+            store_pack<T, 4>(reinterpret_cast<T*>(a.gdelta) + o, gd, vec, valid);
+            if (a.gz) store_pack<T, 4>(reinterpret_cast<T*>(a.gz) + o, gz, vec, valid);
         }
-    }
-    double gA[2 * K] = {};
-    float gD[IPT][4] = {}, gbias[IPT][4] = {};
-    float sum_dt = 0.0f;
-    const float4* const du_row = s_du + du_at<CH>(0, c);
-    const float2* const gy_row = s_gy + c;
-    const float* const b_row = s_b + n0;
-    const float* const c_row = s_c + n0;
+        float4* const part = reinterpret_cast<float4*>(
+            p.part_bc + (((at.batch * d.groups + at.group) * d.tiles + at.tile) * d.length + t0) * 2 * NP);
+        const float4* const from = reinterpret_cast<const float4*>(smem + Mem::r) + buf * S::WARPS * STEPS * NP / 2;
+#pragma unroll
+        for (int e = tid; e < STEPS * NP / 2; e += S::HELP) {
+            float4 sum = from[e];
+#pragma unroll
+            for (int w = 1; w < S::WARPS; ++w) {
+                const float4 v = from[w * STEPS * NP / 2 + e];
+                sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+            }
+            if (t0 + e / (NP / 2) < t_used) part[e] = sum;
+        }
+    };
 
-    int buf = 0;
+    fetch(last, 0, 0);
+    fetch(last - STEPS, 1, 1);
+    copy_wait<1>();
+    if (last >= first) stage(last, 0, 0);
+    __syncthreads();
+    int buf = 0, slot = 0;
     for (int64_t t0 = last; t0 >= first; t0 -= STEPS, buf ^= 1) {
-        copy_wait<0>();
-        stage(t0, buf);
-        F2 h[STEPS + 1][K], f[STEPS][K];                                 // h[t]: the state in front of step t; factors
-#pragma unroll
-        for (int k = 0; k < K; ++k) h[0][k] = start[k];
+        const int next = slot == 2 ? 0 : slot + 1, before = slot == 0 ? 2 : slot - 1;
+        if (!LOCAL && t0 < last) finish(t0 + STEPS, before, buf ^ 1);
+        fetch(t0 - 2 * STEPS, before, buf);                              // (B and C of this tile are staged already)
+        copy_wait<1>();
+        if (t0 - STEPS >= first) stage(t0 - STEPS, next, buf ^ 1);
+        slot = next;
         __syncthreads();
-        if (t0 > first) fetch(t0 - STEPS, buf ^ 1);
-
-        // the states again, forwards
-#pragma unroll
-        for (int t = 0; t < STEPS; ++t) {
-            const float4 du = du_row[t * (CH + CH / 8)];
-            const F2 dt2 = pack2(du.x, du.y), du2 = pack2(du.z, du.w);
-#pragma unroll
-            for (int k = 0; k < K; ++k) f[t][k] = decay(A[k], dt2);
-            if (LOCAL) {
-                sum_dt += du.x;
-            } else {
-                F2 bb[K];
-                read_pairs(bb, b_row + t * NP);
-#pragma unroll
-                for (int k = 0; k < K; ++k) h[t + 1][k] = fma2(f[t][k], h[t][k], mul2(du2, bb[k]));
-            }
-        }
-        if (!LOCAL && z) {
-            float y[STEPS];
-#pragma unroll
-            for (int t = 0; t < STEPS; ++t) {
-                F2 cc[K];
-                read_pairs(cc, c_row + t * NP);
-                y[t] = dot(h[t + 1], cc);
-            }
-            reduce_lanes<STEPS, P, 1>(y, lane);
-            if (reduced_owner<STEPS, P>(j)) {
-                const int t = reduced_index<STEPS, P>(j);
-#pragma unroll
-                for (int i = 0; i < reduced_count<STEPS, P>(); ++i) s_y[(t + i) * ROW + c] = y[i];
-            }
-        }
-        // the gradients, backwards
-        F2 gA_tile[K];
-#pragma unroll
-        for (int k = 0; k < K; ++k) gA_tile[k] = same2(0.0f);
-#pragma unroll
-        for (int g = STEPS / 4 - 1; g >= 0; --g) {
-            float s[8];
-#pragma unroll
-            for (int i = 3; i >= 0; --i) {
-                const int t = g * 4 + i;
-                const float2 gy = gy_row[t * CH];
-                const F2 gy2 = pack2(gy.x, gy.y);
-                F2 cc[K], gh[K];
-                read_pairs(cc, c_row + t * NP);
-#pragma unroll
-                for (int k = 0; k < K; ++k) {
-                    gh[k] = fma2(gy2, cc[k], w[k]);
-                    w[k] = mul2(f[t][k], gh[k]);
-                }
-                if (!LOCAL) {
-                    const float4 du = du_row[t * (CH + CH / 8)];
-                    const F2 dt2 = pack2(du.x, du.y), du2 = pack2(du.z, du.w);
-                    F2 bb[K], q[K];
-                    read_pairs(bb, b_row + t * NP);
-                    float v[4 * K];                                      // gC, then gB
-#pragma unroll
-                    for (int k = 0; k < K; ++k) {
-                        unpack2(mul2(gy2, h[t + 1][k]), v[2 * k], v[2 * k + 1]);
-                        unpack2(mul2(du2, gh[k]), v[2 * K + 2 * k], v[2 * K + 2 * k + 1]);
-                    }
-                    reduce_lanes<4 * K, R, P>(v, lane);
-                    if (reduced_owner<4 * K, R>(lane / P)) {
-                        const int i0 = reduced_index<4 * K, R>(lane / P);
-                        float* const to = s_r + (warp * STEPS + t) * 2 * NP + n0;
-#pragma unroll
-                        for (int k = 0; k < reduced_count<4 * K, R>(); ++k) to[((i0 + k) / (2 * K)) * NP + (i0 + k) % (2 * K)] = v[k];
-                    }
-                    s[2 * i] = dot(gh, bb);
-#pragma unroll
-                    for (int k = 0; k < K; ++k) {
-                        q[k] = mul2(w[k], h[t][k]);
-                        gA_tile[k] = fma2(q[k], dt2, gA_tile[k]);
-                    }
-                    s[2 * i + 1] = dot(q, A);
-                }
-            }
-            if (!LOCAL) {
-                reduce_lanes<8, P, 1>(s, lane);
-                if (reduced_owner<8, P>(j)) {
-                    const int k0 = reduced_index<8, P>(j);
-#pragma unroll
-                    for (int k = 0; k < reduced_count<8, P>(); ++k)
-                        s_s[(((k0 + k) % 2) * STEPS + g * 4 + (k0 + k) / 2) * ROW + c] = s[k];
-                }
-            }
-        }
-        if (!LOCAL) {
-#pragma unroll
-            for (int k = 0; k < K; ++k) {
-                float x, y;
-                unpack2(gA_tile[k], x, y);
-                gA[2 * k] += x;
-                gA[2 * k + 1] += y;
-            }
-        }
-        __syncthreads();
-        if (!LOCAL) {
-#pragma unroll
-            for (int k = 0; k < IPT; ++k) {
-                int it, cc, valid;
-                item_of(k, it, cc, valid);
-                const int64_t t = t0 + it;
-                if (valid > 0 && t < t_end) {
-                    const bool in = t < t_used, vec = d.vec && valid == 4;
-                    float x[4], gu[4], gd[4], gz[4];
-                    read_slot<T, 4>(slot_of(buf, 0, k), x);
-                    const float4 over4 = *reinterpret_cast<const float4*>(s_s + it * ROW + cc);
-                    const float4 qa4 = *reinterpret_cast<const float4*>(s_s + (STEPS + it) * ROW + cc);
-                    const float4 slope4 = s_keep[tid + k * THREADS], gs4 = s_keep[ITEMS + tid + k * THREADS];
-                    const float over[4] = {over4.x, over4.y, over4.z, over4.w}, qa[4] = {qa4.x, qa4.y, qa4.z, qa4.w};
-                    const float slope[4] = {slope4.x, slope4.y, slope4.z, slope4.w}, gs[4] = {gs4.x, gs4.y, gs4.z, gs4.w};
-                    float y[4] = {};
-                    if (z) {
-                        const float4 y4 = *reinterpret_cast<const float4*>(s_y + it * ROW + cc);
-                        y[0] = y4.x, y[1] = y4.y, y[2] = y4.z, y[3] = y4.w;
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float dt = s_du[du_at<CH>(it, cc + i)].x, gy = s_gy[it * CH + cc + i].x;
-                        gu[i] = in ? fmaf(dt, over[i], skip[k][i] * gy) : 0.0f;
-                        gd[i] = in ? slope[i] * fmaf(x[i], over[i], kLn2 * qa[i]) : 0.0f;
-                        gz[i] = in ? gs[i] * fmaf(skip[k][i], x[i], y[i]) : 0.0f;
-                        gD[k][i] += in ? gy * x[i] : 0.0f;
-                        gbias[k][i] += gd[i];
-                    }
-                    const int64_t o = (at.batch * d.length + t) * d.channels + base_c + cc;
-                    store_pack<T, 4>(reinterpret_cast<T*>(a.gu) + o, gu, vec, valid);
-                    store_pack<T, 4>(reinterpret_cast<T*>(a.gdelta) + o, gd, vec, valid);
-                    if (a.gz) store_pack<T, 4>(reinterpret_cast<T*>(a.gz) + o, gz, vec, valid);
-                }
-            }
-            float* const part =
-                p.part_bc + (((at.batch * d.groups + at.group) * d.tiles + at.tile) * d.length + t0) * 2 * NP;
-            for (int e = tid; e < STEPS * 2 * NP; e += THREADS) {
-                float sum = 0.0f;
-#pragma unroll
-                for (int w = 0; w < WARPS; ++w) sum += s_r[w * STEPS * 2 * NP + e];
-                if (t0 + e / (2 * NP) < t_used) part[e] = sum;
-            }
-            // the epilogue reads what the next stage() overwrites
-            __syncthreads();
-        }
     }
-    if (LOCAL) {
-        if (live) {
-            const int64_t cell = (at.batch * d.segments + at.segment) * d.channels + channel;
-            store_states(p.seg_state + cell * states, w, n0, states, d.vec_states);
-            if (j == 0) p.seg_dt[cell] = sum_dt;
-        }
-        return;
-    }
+    if (LOCAL) return;
+    if (last >= first) finish(first, slot == 0 ? 2 : slot - 1, buf ^ 1);
     // gradients of padding behind the last tile
     for (int64_t t0 = last + STEPS; t0 < t_end; t0 += STEPS) {
         const float zero[4] = {};
 #pragma unroll
         for (int k = 0; k < IPT; ++k) {
-            int it, cc, valid;
-            item_of(k, it, cc, valid);
-            if (valid > 0 && t0 + it < t_end) {
-                const bool vec = d.vec && valid == 4;
-                const int64_t o = (at.batch * d.length + t0 + it) * d.channels + base_c + cc;
+            const int64_t t = t0 + item_t + k * ITEM_STEP;
+            if (valid > 0 && t < t_end) {
+                const int64_t o = (at.batch * d.length + t) * d.channels + base_c + cc;
                 store_pack<T, 4>(reinterpret_cast<T*>(a.gu) + o, zero, vec, valid);
                 store_pack<T, 4>(reinterpret_cast<T*>(a.gdelta) + o, zero, vec, valid);
                 if (a.gz) store_pack<T, 4>(reinterpret_cast<T*>(a.gz) + o, zero, vec, valid);
             }
         }
     }
-    const int64_t part_row = at.batch * d.segments + at.segment;
-    if (live) {
-        F2 sums[K];
+    // gD and gdelta_bias: sums over the thread's tokens; over the threads in shared memory, in thread order.  Only the
+    // helping threads are still here, so they wait for one another alone.
+    float* const sums = reinterpret_cast<float*>(smem + Mem::keep);      // [2][threads of a row][CH]
+    constexpr int ROWS = ITEMS < S::HELP ? STEPS : ITEM_STEP;
+    asm volatile("bar.sync 1, %0;" ::"n"(S::HELP) : "memory");
+    if (has_item) {
 #pragma unroll
-        for (int k = 0; k < K; ++k) sums[k] = pack2((float)gA[2 * k], (float)gA[2 * k + 1]);
-        store_states(p.part_A + (part_row * d.channels + channel) * states, sums, n0, states, d.vec_states);
-        if (d.ahead)
-            store_states(p.seg_state + ((at.batch * d.segments + at.segment) * d.channels + channel) * states, w, n0, states,
-                         d.vec_states);
-        if (a.ginitial && at.segment == 0)
-            store_states(a.ginitial + (at.batch * d.channels + channel) * states, w, n0, states, d.vec_states);
+        for (int i = 0; i < 4; ++i) {
+            sums[item_t * CH + cc + i] = gD[i];
+            sums[(ROWS + item_t) * CH + cc + i] = gbias[i];
+        }
     }
-    // gD and gdelta_bias: every thread has sums over its token of each tile; over the 16 tokens in shared memory
-    for (int which = 0; which < 2; ++which) {
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < IPT; ++k) {
-            int it, cc, valid;
-            item_of(k, it, cc, valid);
-            if (tid + k * THREADS < ITEMS) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s_y[it * ROW + cc + i] = which ? gbias[k][i] : gD[k][i];
-            }
-        }
-        __syncthreads();
-        for (int e = tid; e < at.n_channels; e += THREADS) {
-            float sum = 0.0f;
-            for (int t = 0; t < STEPS; ++t) sum += s_y[t * ROW + e];
-            p.part_D[(part_row * 2 + which) * d.channels + base_c + e] = sum;
-        }
+    asm volatile("bar.sync 1, %0;" ::"n"(S::HELP) : "memory");
+    const int64_t part_row = at.batch * d.segments + at.segment;
+    for (int e = tid; e < 2 * CH; e += S::HELP) {
+        const int which = e / CH, ch = e % CH;
+        if (ch >= at.n_channels) continue;
+        float sum = 0.0f;
+        for (int t = 0; t < ROWS; ++t) sum += sums[(which * ROWS + t) * CH + ch];
+        p.part_D[(part_row * 2 + which) * d.channels + base_c + ch] = sum;
+    }
+}
+
+template <typename T, int P, int K, int M, bool LOCAL>
+__device__ __forceinline__ void scan_backward_block(const ScanParams& p, const Place& at, char* smem) {
+    using S = BackShape<P, K, M>;
+    const ScanDims& d = p.d;
+    const int64_t used = used_length(p.a.lengths, at.batch, d.length);
+    const int64_t t_begin = at.segment * d.segment_length;
+    const int64_t t_end = t_begin + d.segment_length < d.length ? t_begin + d.segment_length : d.length;
+    const int64_t t_used = used < t_end ? used : t_end;
+    if (threadIdx.x < S::SCAN) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::SCAN_REGISTERS));
+        scan_backward_scan<T, P, K, M, LOCAL>(p, at, smem, t_begin, t_used);
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::HELP_REGISTERS));
+        scan_backward_help<T, P, K, M, LOCAL>(p, at, smem, t_begin, t_end, t_used);
     }
 }
 
 // the segments from last to first, in two launches like the forward ones
-template <typename T, int P, int K>
-__global__ void __launch_bounds__(Shape<P, K>::THREADS, K == 1 ? 512 / Shape<P, K>::THREADS : 1) scan_backward(const __grid_constant__ ScanParams p) {
-    const Place at = block_place(p.d, Shape<P, K>::CH);
-    if (p.d.ahead && at.segment < p.d.segments - 1) scan_backward_block<T, P, K, true>(p, at);
-    else scan_backward_block<T, P, K, false>(p, at);
+template <typename T, int P, int K, int M>
+__global__ void __launch_bounds__(BackShape<P, K, M>::THREADS, 2) scan_backward(const __grid_constant__ ScanParams p) {
+    extern __shared__ __align__(16) char smem[];
+    const Place at = block_place(p.d, BackShape<P, K, M>::CH);
+    if (p.d.ahead && at.segment < p.d.segments - 1) scan_backward_block<T, P, K, M, true>(p, at, smem);
+    else scan_backward_block<T, P, K, M, false>(p, at, smem);
 }
 
 // gB and gC: the channel tiles' parts added up in tile order; one thread per (batch, token, group, state)
@@ -1047,11 +1136,17 @@ inline uint32_t grid_for(int64_t items) {
     return (uint32_t)(blocks < 1 ? 1 : blocks < most ? blocks : most);
 }
 
-template <typename T, int P, int K>
+template <typename T, int P, int K, int M>
 int run_backward(const ScanParams& p, cudaStream_t stream) {
-    int st = launch_segments(scan_backward<T, P, K>, p, Shape<P, K>::THREADS, BackShape<T, P, K>::bytes, true, stream);
+    using S = BackShape<P, K, M>;
+    // the scanning threads' registers come out of those that the block starts with
+    cudaFuncAttributes attributes;
+    const cudaError_t e = cudaFuncGetAttributes(&attributes, scan_backward<T, P, K, M>);
+    if (e != cudaSuccess) return record_cuda_error(e);
+    if (attributes.numRegs * S::THREADS < S::SCAN * S::SCAN_REGISTERS + S::HELP * S::HELP_REGISTERS) return OVL_ERR_INVALID;
+    int st = launch_segments(scan_backward<T, P, K, M>, p, S::THREADS, BackSmem<T, P, K, M>::bytes, true, stream);
     if (st != OVL_OK) return st;
-    scan_backward_bc<T><<<grid_for(p.a.batch * p.d.length * p.d.groups * p.d.states), 256, 0, stream>>>(p, Shape<P, K>::NP);
+    scan_backward_bc<T><<<grid_for(p.a.batch * p.d.length * p.d.groups * p.d.states), 256, 0, stream>>>(p, S::NP);
     if ((st = launch_status()) != OVL_OK) return st;
     scan_backward_params<<<grid_for(p.d.channels * (p.d.states + 2)), 256, 0, stream>>>(p);
     return launch_status();
@@ -1059,28 +1154,30 @@ int run_backward(const ScanParams& p, cudaStream_t stream) {
 
 template <typename T>
 int scan_dispatch(const ScanParams& p, const ScanShape& s, bool backward, cudaStream_t stream) {
-#define OVL_SCAN_CASE(RUN, P, X) \
-    if (s.lanes == P && s.extent == X) return RUN<T, P, X>(p, stream);
     if (backward) {
-        OVL_SCAN_CASE(run_backward, 2, 1)
-        OVL_SCAN_CASE(run_backward, 4, 1)
-        OVL_SCAN_CASE(run_backward, 8, 1)
-        OVL_SCAN_CASE(run_backward, 16, 1)
-        OVL_SCAN_CASE(run_backward, 32, 1)
-        OVL_SCAN_CASE(run_backward, 32, 2)
-    } else {
-        OVL_SCAN_CASE(run_forward, 1, 1)
-        OVL_SCAN_CASE(run_forward, 2, 1)
-        OVL_SCAN_CASE(run_forward, 4, 1)
-        OVL_SCAN_CASE(run_forward, 8, 1)
-        OVL_SCAN_CASE(run_forward, 16, 1)
-        OVL_SCAN_CASE(run_forward, 1, 2)
-        OVL_SCAN_CASE(run_forward, 2, 2)
-        OVL_SCAN_CASE(run_forward, 4, 2)
-        OVL_SCAN_CASE(run_forward, 8, 2)
-        OVL_SCAN_CASE(run_forward, 16, 2)
-        OVL_SCAN_CASE(run_forward, 32, 2)
+#define OVL_SCAN_CASE(P, K, M) \
+    if (s.lanes == P && s.pairs == K) return run_backward<T, P, K, M>(p, stream);
+        OVL_SCAN_CASE(4, 1, 2)
+        OVL_SCAN_CASE(8, 1, 2)
+        OVL_SCAN_CASE(16, 1, 2)
+        OVL_SCAN_CASE(32, 1, 2)
+        OVL_SCAN_CASE(32, 2, 1)
+#undef OVL_SCAN_CASE
+        return OVL_ERR_INVALID;
     }
+#define OVL_SCAN_CASE(P, M) \
+    if (s.lanes == P && s.channels == M) return run_forward<T, P, M>(p, stream);
+    OVL_SCAN_CASE(1, 1)
+    OVL_SCAN_CASE(2, 1)
+    OVL_SCAN_CASE(4, 1)
+    OVL_SCAN_CASE(8, 1)
+    OVL_SCAN_CASE(16, 1)
+    OVL_SCAN_CASE(1, 2)
+    OVL_SCAN_CASE(2, 2)
+    OVL_SCAN_CASE(4, 2)
+    OVL_SCAN_CASE(8, 2)
+    OVL_SCAN_CASE(16, 2)
+    OVL_SCAN_CASE(32, 2)
 #undef OVL_SCAN_CASE
     return OVL_ERR_INVALID;
 }
