@@ -10,13 +10,14 @@ namespace ovl {
 namespace {
 
 constexpr int kMaxTaps = 8;
-constexpr int kStrip = 32;             // tokens of a thread, forward
-constexpr int kBackStrip = 64;         // tokens of a thread, backward
+constexpr int kMaxStrip = 64;          // tokens of a thread, if that leaves enough blocks
+constexpr int kMinStrip = 8;
 constexpr int kWarps = 4;              // warps of a block: strips that follow each other
 
 struct ConvParams {
     OvlCausalConv a;
     int64_t column_tiles, strips;      // tiles of 32 x (channels of a thread) channels, blocks of kWarps strips
+    int64_t strip;                     // tokens of a thread
     int32_t vec;
     float* part;                       // backward: [batch * strips, taps + 1, channels]
 };
@@ -40,10 +41,71 @@ __device__ __forceinline__ Pack<T, N> load_token(const OvlCausalConv& a, int64_t
     return load_pack<T, N>(x, vec && in, in ? valid : 0);
 }
 
+// The weights of a thread's N channels as pairs of channels, the oldest tap first; with TAPS = 8 the unused ones in front
+// are zeros, which the sums leave out.
+template <typename T, int TAPS, int N>
+__device__ __forceinline__ void load_weights(F2 (&w)[TAPS][N / 2], F2 (&bias)[N / 2], const OvlCausalConv& a, int taps, int64_t channel,
+                                             int valid) {
+    float v[TAPS][N], b[N];
+    if (TAPS != kMaxTaps && !a.params_f32 && valid == N && aligned16(a.weight) && (N * TAPS * sizeof(T)) % 16 == 0 && channel % N == 0) {
+        const Pack<T, N * TAPS> raw = load_pack<T, N * TAPS>(reinterpret_cast<const T*>(a.weight) + channel * TAPS, true, 0);
+#pragma unroll
+        for (int c = 0; c < N; ++c)
+#pragma unroll
+            for (int k = 0; k < TAPS; ++k) v[k][c] = to_f32(raw.v[c * TAPS + k]);
+    } else {
+#pragma unroll
+        for (int c = 0; c < N; ++c)
+#pragma unroll
+            for (int k = 0; k < TAPS; ++k) {
+                const int kk = k - (TAPS - taps);
+                v[k][c] = kk >= 0 && c < valid ? load_param<T>(a.weight, (channel + c) * taps + kk, a.params_f32) : 0.0f;
+            }
+    }
+#pragma unroll
+    for (int c = 0; c < N; ++c) b[c] = a.bias && c < valid ? load_param<T>(a.bias, channel + c, a.params_f32) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+        bias[i] = pack2(b[2 * i], b[2 * i + 1]);
+#pragma unroll
+        for (int k = 0; k < TAPS; ++k) w[k][i] = pack2(v[k][2 * i], v[k][2 * i + 1]);
+    }
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void widen(F2 (&x)[N / 2], const Pack<T, N>& raw) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) x[i] = pack2(to_f32(raw.v[2 * i]), to_f32(raw.v[2 * i + 1]));
+}
+
+// Tokens on their way while earlier ones are worked on: every thread copies what it will need itself into slots of its
+// own, so nothing waits but the thread that needs a token (a register that a load may or may not fill is waited for at
+// once: 197 us for the forward pass of bf16 4 x 4096 x 4096 with the next tokens in registers).
+constexpr int kChunk = 4;              // tokens that are copied and worked on together
+constexpr int kAhead = 3;              // chunks on their way
+constexpr int kRing = kAhead + 1;
+
+template <typename T, int N>
+struct Ring {
+    T* base;                           // [kRing][kChunk][threads][N]
+    __device__ __forceinline__ explicit Ring(void* smem) : base(reinterpret_cast<T*>(smem) + threadIdx.x * N) {}
+    __device__ __forceinline__ T* slot(int chunk, int s) const { return base + (chunk * kChunk + s) * (32 * kWarps * N); }
+    static constexpr size_t bytes = sizeof(T) * kRing * kChunk * 32 * kWarps * N;
+};
+
+template <typename T, int N>
+__device__ __forceinline__ void widen_slot(F2 (&x)[N / 2], const T* slot) {
+    float v[N];
+    read_slot<T, N>(slot, v);
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) x[i] = pack2(v[2 * i], v[2 * i + 1]);
+}
+
 // TAPS: the number of taps, or 8 for any number up to 8 (`taps` says which)
 template <typename T, int TAPS>
-__global__ void __launch_bounds__(32 * kWarps) conv_forward(const __grid_constant__ ConvParams p) {
-    constexpr int N = 8, CHUNK = 8;
+__global__ void __launch_bounds__(32 * kWarps, TAPS == kMaxTaps ? 1 : 4) conv_forward(const __grid_constant__ ConvParams p) {
+    constexpr int N = 8, CHUNK = kChunk;
+    extern __shared__ __align__(16) char smem[];
     const OvlCausalConv& a = p.a;
     const int taps = TAPS == kMaxTaps ? (int)a.taps : TAPS;
     int64_t i = blockIdx.x;
@@ -55,7 +117,8 @@ __global__ void __launch_bounds__(32 * kWarps) conv_forward(const __grid_constan
     const int valid = a.channels - channel < N ? (int)(a.channels - channel) : N;
     const bool vec = p.vec && valid == N;
     const int64_t used = used_length(a.lengths, batch, a.length);
-    const int64_t t_begin = strip * kStrip, t_end = t_begin + kStrip < a.length ? t_begin + kStrip : a.length;
+    const int64_t t_begin = strip * p.strip, t_end = t_begin + p.strip < a.length ? t_begin + p.strip : a.length;
+    const int64_t t_used = used < t_end ? used : t_end;
 
     // the state after the sequence, by the thread that has the first strip
     if (strip == 0 && a.final_state) {
@@ -70,56 +133,66 @@ __global__ void __launch_bounds__(32 * kWarps) conv_forward(const __grid_constan
     }
     if (t_begin >= t_end) return;
 
-    // weights of the taps, the oldest first; with TAPS = 8 the unused ones in front stay out of the sum
-    float w[TAPS][N], bias[N], win[TAPS][N];
-#pragma unroll
-    for (int c = 0; c < N; ++c) {
-        bias[c] = a.bias && c < valid ? load_param<T>(a.bias, channel + c, a.params_f32) : 0.0f;
-#pragma unroll
-        for (int k = 0; k < TAPS; ++k) {
-            const int kk = k - (TAPS - taps);
-            w[k][c] = kk >= 0 && c < valid ? load_param<T>(a.weight, (channel + c) * taps + kk, a.params_f32) : 0.0f;
-        }
-    }
-#pragma unroll
-    for (int k = 0; k < TAPS - 1; ++k) {
-        const Pack<T, N> raw = load_token<T, N>(a, batch, t_begin - (TAPS - 1) + k, used, channel, vec, valid);
-#pragma unroll
-        for (int c = 0; c < N; ++c) win[k][c] = to_f32(raw.v[c]);
-    }
+    const T* const x = reinterpret_cast<const T*>(a.x) + batch * a.x_batch + channel;
     T* const out = reinterpret_cast<T*>(a.out) + batch * a.length * a.channels + channel;
-    for (int64_t t0 = t_begin; t0 < t_end; t0 += CHUNK) {
-        Pack<T, N> raw[CHUNK];
+    const Ring<T, N> ring(smem);
+    auto fetch = [&](int64_t t0, int chunk) {
 #pragma unroll
-        for (int s = 0; s < CHUNK; ++s) raw[s] = load_token<T, N>(a, batch, t0 + s, used < t_end ? used : t_end, channel, vec, valid);
+        for (int s = 0; s < CHUNK; ++s)
+            if (t0 + s < t_used) fetch_pack<T, N>(ring.slot(chunk, s), x + (t0 + s) * a.x_token, vec, valid);
+        copy_commit();
+    };
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) fetch(t_begin + k * CHUNK, k);
+    F2 w[TAPS][N / 2], bias[N / 2], win[TAPS][N / 2];
+    load_weights<T, TAPS, N>(w, bias, a, taps, channel, valid);
+#pragma unroll
+    for (int k = 0; k < TAPS - 1; ++k)
+        widen<T, N>(win[k], load_token<T, N>(a, batch, t_begin - (TAPS - 1) + k, used, channel, vec, valid));
+    const bool gated = a.silu;
+    int chunk = 0;
+    for (int64_t t0 = t_begin; t0 < t_end; t0 += CHUNK) {
+        copy_wait<kAhead - 1>();
+        fetch(t0 + kAhead * CHUNK, chunk == 0 ? kAhead : chunk - 1);
 #pragma unroll
         for (int s = 0; s < CHUNK; ++s) {
+            widen_slot<T, N>(win[TAPS - 1], ring.slot(chunk, s));        // (behind the sequence: anything, and not used)
             float y[N];
 #pragma unroll
-            for (int c = 0; c < N; ++c) {
-                win[TAPS - 1][c] = to_f32(raw[s].v[c]);
-                y[c] = bias[c];
+            for (int c = 0; c < N / 2; ++c) {
+                F2 sum = bias[c];
 #pragma unroll
                 for (int k = 0; k < TAPS; ++k)
-                    if (TAPS != kMaxTaps || k >= TAPS - taps) y[c] = fmaf(w[k][c], win[k][c], y[c]);
-                if (a.silu) y[c] = silu(y[c]);
-                if (t0 + s >= used) y[c] = 0.0f;
+                    if (TAPS != kMaxTaps || k >= TAPS - taps) sum = fma2(w[k][c], win[k][c], sum);
+                unpack2(sum, y[2 * c], y[2 * c + 1]);
             }
-            if (t0 + s < t_end) store_pack<T, N>(out + (t0 + s) * a.channels, y, vec, valid);
+            if (gated) {
+#pragma unroll
+                for (int c = 0; c < N; ++c) y[c] = silu(y[c]);
+            }
+            if (t0 + s < t_end) {
+                if (t0 + s >= used) {
+#pragma unroll
+                    for (int c = 0; c < N; ++c) y[c] = 0.0f;
+                }
+                store_pack<T, N>(out + (t0 + s) * a.channels, y, vec, valid);
+            }
 #pragma unroll
             for (int k = 0; k < TAPS - 1; ++k)
 #pragma unroll
-                for (int c = 0; c < N; ++c) win[k][c] = win[k + 1][c];
+                for (int c = 0; c < N / 2; ++c) win[k][c] = win[k + 1][c];
         }
+        chunk = chunk == kAhead ? 0 : chunk + 1;
     }
 }
 
 // gx_t = sum_k w[k] gpre_{t + (taps - 1) - k} with gpre = gout act'(pre): the walk runs taps - 1 tokens past the strip
-// (gx of the strip needs them) and starts taps - 1 tokens in front of it.  The first strip walks from token 0 and also
-// has the gradient of the initial state, gx of the tokens -(taps - 1) ... -1.
+// (gx of the strip needs them).  The first strip also has the gradient of the initial state, gx of the tokens
+// -(taps - 1) ... -1.
 template <typename T, int TAPS>
-__global__ void __launch_bounds__(32 * kWarps) conv_backward(const __grid_constant__ ConvParams p) {
-    constexpr int N = 4, CHUNK = 4;
+__global__ void __launch_bounds__(32 * kWarps, TAPS == kMaxTaps ? 1 : 4) conv_backward(const __grid_constant__ ConvParams p) {
+    constexpr int N = 4, CHUNK = kChunk;
+    extern __shared__ __align__(16) char smem[];
     const OvlCausalConv& a = p.a;
     const int taps = TAPS == kMaxTaps ? (int)a.taps : TAPS;
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
@@ -132,80 +205,108 @@ __global__ void __launch_bounds__(32 * kWarps) conv_backward(const __grid_consta
     const int valid = !live ? 0 : a.channels - channel < N ? (int)(a.channels - channel) : N;
     const bool vec = p.vec && valid == N;
     const int64_t used = used_length(a.lengths, batch, a.length);
-    const int64_t t_begin = strip * kBackStrip, t_end = t_begin + kBackStrip < a.length ? t_begin + kBackStrip : a.length;
+    const int64_t t_begin = strip * p.strip, t_end = t_begin + p.strip < a.length ? t_begin + p.strip : a.length;
 
-    float w[TAPS][N], bias[N], win[TAPS][N], gp[TAPS][N], gw[TAPS][N], gb[N];
+    F2 w[TAPS][N / 2], bias[N / 2], win[TAPS][N / 2], gp[TAPS][N / 2], gw[TAPS][N / 2], gb[N / 2];
 #pragma unroll
-    for (int c = 0; c < N; ++c) {
-        bias[c] = a.bias && c < valid ? load_param<T>(a.bias, channel + c, a.params_f32) : 0.0f;
-        gb[c] = 0.0f;
+    for (int c = 0; c < N / 2; ++c) {
+        gb[c] = same2(0.0f);
 #pragma unroll
-        for (int k = 0; k < TAPS; ++k) {
-            const int kk = k - (TAPS - taps);
-            w[k][c] = kk >= 0 && c < valid ? load_param<T>(a.weight, (channel + c) * taps + kk, a.params_f32) : 0.0f;
-            gw[k][c] = gp[k][c] = 0.0f;
-        }
+        for (int k = 0; k < TAPS; ++k) gw[k][c] = gp[k][c] = same2(0.0f);
     }
-    // A zero-length batch still has its state's gradient to hand on, so the first strip always walks.
+    // A sequence without tokens still has its state's gradient to hand on, so the first strip always walks.
     if (valid > 0 && (t_begin < t_end || strip == 0)) {
-#pragma unroll
-        for (int k = 0; k < TAPS - 1; ++k) {
-            const Pack<T, N> raw = load_token<T, N>(a, batch, t_begin - (TAPS - 1) + k, used, channel, vec, valid);
-#pragma unroll
-            for (int c = 0; c < N; ++c) win[k][c] = to_f32(raw.v[c]);
-        }
-        const T* const gout = reinterpret_cast<const T*>(a.gout) + batch * a.gout_batch + channel;
         const int64_t walk_end = t_end + (taps - 1);                     // gx of token t is complete at t + taps - 1
-        for (int64_t t0 = t_begin; t0 < walk_end; t0 += CHUNK) {
-            Pack<T, N> raw[CHUNK], rawg[CHUNK];
+        const int64_t walk_used = used < walk_end ? used : walk_end;
+        const T* const x = reinterpret_cast<const T*>(a.x) + batch * a.x_batch + channel;
+        const T* const gout = reinterpret_cast<const T*>(a.gout) + batch * a.gout_batch + channel;
+        const Ring<T, N> ring_x(smem), ring_g(smem + Ring<T, N>::bytes);
+        auto fetch = [&](int64_t t0, int chunk) {
 #pragma unroll
             for (int s = 0; s < CHUNK; ++s) {
                 const int64_t t = t0 + s;
-                const bool in = t < walk_end && t < used;
-                raw[s] = load_token<T, N>(a, batch, t, in ? used : 0, channel, vec, valid);
-                rawg[s] = load_pack<T, N>(gout + t * a.gout_token, vec && in, in ? valid : 0);
-            }
-#pragma unroll
-            for (int s = 0; s < CHUNK; ++s) {
-                const int64_t t = t0 + s;
-                float gx[N];
-#pragma unroll
-                for (int c = 0; c < N; ++c) {
-                    win[TAPS - 1][c] = to_f32(raw[s].v[c]);
-                    float g = to_f32(rawg[s].v[c]);
-                    if (a.silu) {
-                        float pre = bias[c];
-#pragma unroll
-                        for (int k = 0; k < TAPS; ++k)
-                            if (TAPS != kMaxTaps || k >= TAPS - taps) pre = fmaf(w[k][c], win[k][c], pre);
-                        const float sig = sigmoid(pre);
-                        g *= sig * fmaf(pre, 1.0f - sig, 1.0f);
-                    }
-                    // outside the sequence nothing comes from above, whatever the input there
-                    g = t < used ? g : 0.0f;
-                    gp[TAPS - 1][c] = g;
-                    if (t < t_end) {
-                        gb[c] += g;
-#pragma unroll
-                        for (int k = 0; k < TAPS; ++k)
-                            if (TAPS != kMaxTaps || k >= TAPS - taps) gw[k][c] = fmaf(g, t < used ? win[k][c] : 0.0f, gw[k][c]);
-                    }
-                    // gp[TAPS - 1 - k] is gpre of token t - k: gx of token t - (taps - 1)
-                    gx[c] = 0.0f;
-#pragma unroll
-                    for (int k = 0; k < TAPS; ++k)
-                        if (TAPS != kMaxTaps || k >= TAPS - taps) gx[c] = fmaf(w[k][c], gp[TAPS - 1 - (k - (TAPS - taps))][c], gx[c]);
+                if (t < walk_used) {
+                    fetch_pack<T, N>(ring_x.slot(chunk, s), x + t * a.x_token, vec, valid);
+                    fetch_pack<T, N>(ring_g.slot(chunk, s), gout + t * a.gout_token, vec, valid);
                 }
+            }
+            copy_commit();
+        };
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) fetch(t_begin + k * CHUNK, k);
+        load_weights<T, TAPS, N>(w, bias, a, taps, channel, valid);
+#pragma unroll
+        for (int k = 0; k < TAPS - 1; ++k)
+            widen<T, N>(win[k], load_token<T, N>(a, batch, t_begin - (TAPS - 1) + k, used, channel, vec, valid));
+        const bool gated = a.silu;
+        int chunk = 0;
+        for (int64_t t0 = t_begin; t0 < walk_end; t0 += CHUNK) {
+            copy_wait<kAhead - 1>();
+            fetch(t0 + kAhead * CHUNK, chunk == 0 ? kAhead : chunk - 1);
+#pragma unroll
+            for (int s = 0; s < CHUNK; ++s) {
+                const int64_t t = t0 + s;
+                float g[N];
+                widen_slot<T, N>(win[TAPS - 1], ring_x.slot(chunk, s));
+                read_slot<T, N>(ring_g.slot(chunk, s), g);
+                if (gated) {
+#pragma unroll
+                    for (int c = 0; c < N / 2; ++c) {
+                        F2 sum = bias[c];
+#pragma unroll
+                        for (int k = 0; k < TAPS; ++k)
+                            if (TAPS != kMaxTaps || k >= TAPS - taps) sum = fma2(w[k][c], win[k][c], sum);
+                        float pre[2];
+                        unpack2(sum, pre[0], pre[1]);
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float sig = sigmoid(pre[e]);
+                            g[2 * c + e] *= sig * fmaf(pre[e], 1.0f - sig, 1.0f);
+                        }
+                    }
+                }
+                // outside the sequence nothing comes from above, whatever the inputs there
+                const bool in = t < used;
+#pragma unroll
+                for (int c = 0; c < N / 2; ++c) gp[TAPS - 1][c] = in ? pack2(g[2 * c], g[2 * c + 1]) : same2(0.0f);
+                if (in && t < t_end) {
+#pragma unroll
+                    for (int c = 0; c < N / 2; ++c) {
+                        gb[c] = add2(gb[c], gp[TAPS - 1][c]);
+#pragma unroll
+                        for (int k = 0; k < TAPS; ++k)
+                            if (TAPS != kMaxTaps || k >= TAPS - taps) gw[k][c] = fma2(gp[TAPS - 1][c], win[k][c], gw[k][c]);
+                    }
+                }
+                // gp[TAPS - 1 - k] is gpre of token t - k: gx of token t - (taps - 1)
                 const int64_t to = t - (taps - 1);
                 const bool state = to < 0;
                 if (t < walk_end && (state ? strip == 0 && a.ginitial != nullptr : to >= t_begin)) {
+                    float gx[N];
+#pragma unroll
+                    for (int c = 0; c < N / 2; ++c) {
+                        F2 sum = same2(0.0f);
+#pragma unroll
+                        for (int k = 0; k < TAPS; ++k)
+                            if (TAPS != kMaxTaps || k >= TAPS - taps) {
+                                if constexpr (TAPS != kMaxTaps) {
+                                    sum = fma2(w[k][c], gp[TAPS - 1 - k][c], sum);
+                                } else {
+                                    // tap k - (8 - taps): gp is indexed by registers, so every possible one is compared
+#pragma unroll
+                                    for (int m = 0; m < TAPS; ++m)
+                                        if (m == k - (TAPS - taps)) sum = fma2(w[k][c], gp[TAPS - 1 - m][c], sum);
+                                }
+                            }
+                        unpack2(sum, gx[2 * c], gx[2 * c + 1]);
+                    }
                     // the state after the sequence holds the inputs used - (taps - 1) ... used - 1
                     const int64_t k = to - (used - (taps - 1));
                     if (a.gfinal && k >= 0 && k < taps - 1) {
-                        const Pack<T, N> g = load_pack<T, N>(
+                        const Pack<T, N> gf = load_pack<T, N>(
                             reinterpret_cast<const T*>(a.gfinal) + (batch * (taps - 1) + k) * a.channels + channel, vec, valid);
 #pragma unroll
-                        for (int c = 0; c < N; ++c) gx[c] += to_f32(g.v[c]);
+                        for (int c = 0; c < N; ++c) gx[c] += to_f32(gf.v[c]);
                     }
                     T* const dst = state ? reinterpret_cast<T*>(a.ginitial) + (batch * (taps - 1) + (taps - 1) + to) * a.channels
                                          : reinterpret_cast<T*>(a.gx) + (batch * a.length + to) * a.channels;
@@ -214,20 +315,28 @@ __global__ void __launch_bounds__(32 * kWarps) conv_backward(const __grid_consta
 #pragma unroll
                 for (int k = 0; k < TAPS - 1; ++k)
 #pragma unroll
-                    for (int c = 0; c < N; ++c) {
+                    for (int c = 0; c < N / 2; ++c) {
                         win[k][c] = win[k + 1][c];
                         gp[k][c] = gp[k + 1][c];
                     }
             }
+            chunk = chunk == kAhead ? 0 : chunk + 1;
         }
     }
     // the warps' sums for the weights and the bias, added up in warp order
     __shared__ float s_part[kWarps][(TAPS + 1) * N][32];
 #pragma unroll
-    for (int c = 0; c < N; ++c) {
+    for (int c = 0; c < N / 2; ++c) {
+        float x0, x1;
 #pragma unroll
-        for (int k = 0; k < TAPS; ++k) s_part[warp][k * N + c][lane] = gw[k][c];
-        s_part[warp][TAPS * N + c][lane] = gb[c];
+        for (int k = 0; k < TAPS; ++k) {
+            unpack2(gw[k][c], x0, x1);
+            s_part[warp][k * N + 2 * c][lane] = x0;
+            s_part[warp][k * N + 2 * c + 1][lane] = x1;
+        }
+        unpack2(gb[c], x0, x1);
+        s_part[warp][TAPS * N + 2 * c][lane] = x0;
+        s_part[warp][TAPS * N + 2 * c + 1][lane] = x1;
     }
     __syncthreads();
     const int64_t row = batch * p.strips + strip_block;
@@ -242,21 +351,30 @@ __global__ void __launch_bounds__(32 * kWarps) conv_backward(const __grid_consta
     }
 }
 
-// the strips' parts added up in order
+// the strips' parts added up in order: the lanes of a warp are 32 sums, the 8 warps of a block slices of the parts
 template <typename T>
-__global__ void conv_backward_params(const __grid_constant__ ConvParams p) {
+__global__ void __launch_bounds__(256) conv_backward_params(const __grid_constant__ ConvParams p) {
+    __shared__ float s_part[8][32];
     const OvlCausalConv& a = p.a;
-    const int64_t total = (a.taps + 1) * a.channels, rows = a.batch * p.strips;
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t k = i / a.channels, ch = i % a.channels;
-        float sum = 0.0f;
-        for (int64_t r = 0; r < rows; ++r) sum += p.part[r * total + i];
-        void* const to = k < a.taps ? a.gweight : a.gbias;
-        const int64_t at = k < a.taps ? ch * a.taps + k : ch;
-        if (!to) continue;
-        if (a.params_f32) reinterpret_cast<float*>(to)[at] = sum;
-        else reinterpret_cast<T*>(to)[at] = from_f32<T>(sum);
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const int64_t total = (a.taps + 1) * a.channels, rows = a.batch * p.strips, i = (int64_t)blockIdx.x * 32 + lane;
+    float sum = 0.0f;
+    if (i < total) {
+#pragma unroll 4
+        for (int64_t r = warp; r < rows; r += 8) sum += p.part[r * total + i];
     }
+    s_part[warp][lane] = sum;
+    __syncthreads();
+    if (warp != 0 || i >= total) return;
+    sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) sum += s_part[w][lane];
+    const int64_t k = i / a.channels, ch = i % a.channels;
+    void* const to = k < a.taps ? a.gweight : a.gbias;
+    const int64_t at = k < a.taps ? ch * a.taps + k : ch;
+    if (!to) return;
+    if (a.params_f32) reinterpret_cast<float*>(to)[at] = sum;
+    else reinterpret_cast<T*>(to)[at] = from_f32<T>(sum);
 }
 
 template <typename T, int TAPS>
@@ -322,9 +440,14 @@ int check(const OvlCausalConv* a) {
     return OVL_OK;
 }
 
-int64_t strip_blocks(const OvlCausalConv* a, int strip) {
-    const int64_t n = ceil_div(a->length, (int64_t)strip * kWarps);
-    return n > 0 ? n : 1;                                                // states without tokens are passed on too
+// Strips of 64 tokens, shorter ones where there would be fewer than four blocks for every SM.
+void cut(const OvlCausalConv* a, int channels_of_thread, ConvParams* p) {
+    p->column_tiles = ceil_div(a->channels, 32 * channels_of_thread);
+    p->strip = kMaxStrip;
+    while (p->strip > kMinStrip && a->batch * p->column_tiles * ceil_div(a->length, p->strip * kWarps) < 4 * (int64_t)sequence_sm_count())
+        p->strip /= 2;
+    p->strips = ceil_div(a->length, p->strip * kWarps);
+    if (p->strips < 1) p->strips = 1;                                    // states without tokens are passed on too
 }
 
 bool wide(const OvlCausalConv* a, int n, bool backward) {
@@ -334,41 +457,46 @@ bool wide(const OvlCausalConv* a, int n, bool backward) {
            aligned16(a->gx) && aligned16(a->ginitial);
 }
 
-template <typename T>
-int run_forward(ConvParams p, cudaStream_t stream) {
-    p.column_tiles = ceil_div(p.a.channels, 32 * 8);
-    p.strips = strip_blocks(&p.a, kStrip);
-    p.vec = wide(&p.a, 8, false);
+template <typename F>
+int launch(F kernel, const ConvParams& p, size_t smem, cudaStream_t stream) {
     const int64_t blocks = p.column_tiles * p.strips * p.a.batch;
     if (blocks > 0x7fffffff) return OVL_ERR_TOO_LARGE;
-    const uint32_t grid = (uint32_t)blocks;
-    switch (p.a.taps) {
-        case 2: conv_forward<T, 2><<<grid, 32 * kWarps, 0, stream>>>(p); break;
-        case 3: conv_forward<T, 3><<<grid, 32 * kWarps, 0, stream>>>(p); break;
-        case 4: conv_forward<T, 4><<<grid, 32 * kWarps, 0, stream>>>(p); break;
-        default: conv_forward<T, kMaxTaps><<<grid, 32 * kWarps, 0, stream>>>(p); break;
+    if (smem > 32 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return record_cuda_error(e);
     }
+    kernel<<<(uint32_t)blocks, 32 * kWarps, smem, stream>>>(p);
     return launch_status();
 }
 
 template <typename T>
+int run_forward(ConvParams p, cudaStream_t stream) {
+    cut(&p.a, 8, &p);
+    p.vec = wide(&p.a, 8, false);
+    constexpr size_t smem = Ring<T, 8>::bytes;
+    switch (p.a.taps) {
+        case 2: return launch(conv_forward<T, 2>, p, smem, stream);
+        case 3: return launch(conv_forward<T, 3>, p, smem, stream);
+        case 4: return launch(conv_forward<T, 4>, p, smem, stream);
+        default: return launch(conv_forward<T, kMaxTaps>, p, smem, stream);
+    }
+}
+
+template <typename T>
 int run_backward(ConvParams p, cudaStream_t stream) {
-    p.column_tiles = ceil_div(p.a.channels, 32 * 4);
-    p.strips = strip_blocks(&p.a, kBackStrip);
+    cut(&p.a, 4, &p);
     p.vec = wide(&p.a, 4, true);
     p.part = reinterpret_cast<float*>(p.a.workspace);
-    const int64_t blocks = p.column_tiles * p.strips * p.a.batch;
-    if (blocks > 0x7fffffff) return OVL_ERR_TOO_LARGE;
-    const uint32_t grid = (uint32_t)blocks;
+    constexpr size_t smem = 2 * Ring<T, 4>::bytes;
+    int st;
     switch (p.a.taps) {
-        case 2: conv_backward<T, 2><<<grid, 32 * kWarps, 0, stream>>>(p); break;
-        case 3: conv_backward<T, 3><<<grid, 32 * kWarps, 0, stream>>>(p); break;
-        case 4: conv_backward<T, 4><<<grid, 32 * kWarps, 0, stream>>>(p); break;
-        default: conv_backward<T, kMaxTaps><<<grid, 32 * kWarps, 0, stream>>>(p); break;
+        case 2: st = launch(conv_backward<T, 2>, p, smem, stream); break;
+        case 3: st = launch(conv_backward<T, 3>, p, smem, stream); break;
+        case 4: st = launch(conv_backward<T, 4>, p, smem, stream); break;
+        default: st = launch(conv_backward<T, kMaxTaps>, p, smem, stream); break;
     }
-    const int st = launch_status();
     if (st != OVL_OK) return st;
-    conv_backward_params<T><<<(uint32_t)ceil_div((p.a.taps + 1) * p.a.channels, 128), 128, 0, stream>>>(p);
+    conv_backward_params<T><<<(uint32_t)ceil_div((p.a.taps + 1) * p.a.channels, 32), 256, 0, stream>>>(p);
     return launch_status();
 }
 
@@ -392,7 +520,9 @@ int run_step(const OvlCausalConvStep& a, cudaStream_t stream) {
 
 extern "C" uint64_t ovl_causal_conv_workspace_bytes(const OvlCausalConv* a) {
     if (ovl::check(a) != OVL_OK) return 0;
-    return (uint64_t)a->batch * ovl::strip_blocks(a, ovl::kBackStrip) * (a->taps + 1) * a->channels * sizeof(float);
+    ovl::ConvParams p{};
+    ovl::cut(a, 4, &p);
+    return (uint64_t)a->batch * p.strips * (a->taps + 1) * a->channels * sizeof(float);
 }
 
 extern "C" int ovl_causal_conv(const OvlCausalConv* a, void* cuda_stream) {

@@ -15,7 +15,7 @@ constexpr float kMinScale = 1.1754943508e-38f;   // 2^-126, the smallest normal 
 struct NormParams {
     OvlRmsNorm a;
     int32_t vec;
-    int32_t group_lanes;               // 8-bit output: lanes that share a scale (0: through shared memory)
+    int32_t group_lanes, group_shift;  // 8-bit output: lanes that share a scale (a power of two; 0: through shared memory)
     float* part;                       // backward: [blocks, columns]
 };
 
@@ -64,7 +64,39 @@ __device__ __forceinline__ float scale_of(unsigned int bits) {
     return scale < kMinScale ? kMinScale : scale;
 }
 
-template <typename T, int TEAM, int K, bool QUANT>
+// How a thread meets its packs of 8 columns, pack k starting at column (me + k * TEAM) * 8.  VEC: columns come in whole
+// packs on 16-byte boundaries; a pack behind the last column reads the last one (no load waits for a condition) and counts
+// as zeros.  Otherwise element by element.
+template <typename T, int TEAM, bool VEC>
+struct Columns {
+    int columns, me;
+    __device__ __forceinline__ int at(int k) const { return (me + k * TEAM) * 8; }
+    __device__ __forceinline__ bool in(int k) const { return at(k) < columns; }
+    __device__ __forceinline__ int valid(int k) const {
+        const int left = columns - at(k);
+        return VEC || left >= 8 ? 8 : left;
+    }
+    __device__ __forceinline__ Pack<T, 8> load(const T* row, int k) const {
+        if (VEC) return load_pack<T, 8>(row + (in(k) ? at(k) : columns - 8), true, 8);
+        return load_pack<T, 8>(row + at(k), false, in(k) ? valid(k) : 0);
+    }
+    __device__ __forceinline__ void store(T* row, int k, const float (&x)[8]) const {
+        if (in(k)) store_pack<T, 8>(row + at(k), x, VEC, valid(k));
+    }
+    // the weights, zeros behind the last column
+    __device__ __forceinline__ void weights(float (&w)[8], const void* weight, bool f32, int k) const {
+        if (f32) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = in(k) && i < valid(k) ? reinterpret_cast<const float*>(weight)[at(k) + i] : 0.0f;
+        } else {
+            const Pack<T, 8> raw = load(reinterpret_cast<const T*>(weight), k);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = in(k) ? to_f32(raw.v[i]) : 0.0f;
+        }
+    }
+};
+
+template <typename T, int TEAM, int K, bool QUANT, bool VEC>
 __global__ void __launch_bounds__(TeamShape<TEAM>::THREADS) norm_forward(const __grid_constant__ NormParams p) {
     using S = TeamShape<TEAM>;
     constexpr int N = 8;
@@ -75,58 +107,62 @@ __global__ void __launch_bounds__(TeamShape<TEAM>::THREADS) norm_forward(const _
     const int64_t row = (int64_t)blockIdx.x * S::TEAMS + team;
     const bool live = row < a.rows;                                      // (a warp as a whole; blocks are whole rows)
     if (TEAM == 32 && !QUANT && !live) return;
-    const T* const x = reinterpret_cast<const T*>(a.x) + row * a.x_row;
-    const T* const res = a.residual ? reinterpret_cast<const T*>(a.residual) + row * a.residual_row : nullptr;
     const int columns = (int)a.columns;
+    const Columns<T, TEAM, VEC> cols{columns, me};
+    const int64_t from = live ? row : a.rows - 1;
+    const T* const x = reinterpret_cast<const T*>(a.x) + from * a.x_row;
+    const T* const res = a.residual ? reinterpret_cast<const T*>(a.residual) + from * a.residual_row : nullptr;
 
     Pack<T, N> raw[K], raw_r[K];
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        const int col = (me + k * TEAM) * N;
-        const int valid = !live || col >= columns ? 0 : columns - col < N ? columns - col : N;
-        raw[k] = load_pack<T, N>(x + col, p.vec && valid == N, valid);
-        if (res) raw_r[k] = load_pack<T, N>(res + col, p.vec && valid == N, valid);
+    for (int k = 0; k < K; ++k) raw[k] = cols.load(x, k);
+    if (res) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) raw_r[k] = cols.load(res, k);
     }
     float s[K][N], sum[1] = {0.0f};
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            s[k][i] = to_f32(raw[k].v[i]);
-            if (res) s[k][i] += to_f32(raw_r[k].v[i]);
-            sum[0] = fmaf(s[k][i], s[k][i], sum[0]);
-        }
+        for (int i = 0; i < N; ++i) s[k][i] = to_f32(raw[k].v[i]);
+    if (res) {
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int i = 0; i < N; ++i) s[k][i] += to_f32(raw_r[k].v[i]);
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        if (VEC && !cols.in(k)) continue;                                // (element by element the rest is zeros already)
+#pragma unroll
+        for (int i = 0; i < N; ++i) sum[0] = fmaf(s[k][i], s[k][i], sum[0]);
+    }
     if (a.residual_out && live) {
         T* const to = reinterpret_cast<T*>(a.residual_out) + row * a.columns;
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const int col = (me + k * TEAM) * N;
-            const int valid = col >= columns ? 0 : columns - col < N ? columns - col : N;
-            store_pack<T, N>(to + col, s[k], p.vec && valid == N, valid);
-        }
+        for (int k = 0; k < K; ++k) cols.store(to, k, s[k]);
     }
     team_sum<TEAM, 1>(sum, s_sum);
     const float r = rsqrtf(sum[0] / (float)columns + (float)a.eps);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        const int col = (me + k * TEAM) * N;
-        const int valid = col >= columns ? 0 : columns - col < N ? columns - col : N;
-        Pack<T, N> w;
-        if (!a.params_f32) w = load_pack<T, N>(reinterpret_cast<const T*>(a.weight) + col, p.vec && valid == N, valid);
+        float w[N];
+        cols.weights(w, a.weight, a.params_f32, k);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float wi = a.params_f32 ? (i < valid ? reinterpret_cast<const float*>(a.weight)[col + i] : 0.0f) : to_f32(w.v[i]);
-            s[k][i] *= r * wi;
+        for (int i = 0; i < N; ++i) s[k][i] *= r * w[i];
+        if (VEC && !cols.in(k)) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) s[k][i] = 0.0f;
         }
-        if (!QUANT && live)
-            store_pack<T, N>(reinterpret_cast<T*>(a.y) + row * a.columns + col, s[k], p.vec && valid == N, valid);
+        if (!QUANT && live) cols.store(reinterpret_cast<T*>(a.y) + row * a.columns, k, s[k]);
     }
     if constexpr (QUANT) {
         // The largest magnitude of a group, as the largest bit pattern: a NaN stays the largest.
         const int group = (int)a.group, groups = columns / group;
         unsigned int* const maxima = s_max + team * groups;
+        const bool one_scale = p.group_lanes || groups == 1;             // for the 8 values of a pack
         unsigned int top[K];
-        if (p.group_lanes || groups == 1) {
+        if (one_scale) {
             unsigned int whole = 0;
 #pragma unroll
             for (int k = 0; k < K; ++k) {
@@ -154,7 +190,7 @@ __global__ void __launch_bounds__(TeamShape<TEAM>::THREADS) norm_forward(const _
             __syncthreads();
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                const int col = (me + k * TEAM) * N;
+                const int col = cols.at(k);
                 unsigned int run = 0;
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
@@ -171,18 +207,17 @@ __global__ void __launch_bounds__(TeamShape<TEAM>::THREADS) norm_forward(const _
         if (!live) return;
         uint8_t* const q = reinterpret_cast<uint8_t*>(a.q) + row * a.columns;
         float* const scales = a.scale + row * groups;
-        const bool one_scale = p.group_lanes || groups == 1;             // for the 8 values of a thread
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            const int col = (me + k * TEAM) * N;
+            const int col = cols.at(k);
             if (col >= columns) continue;
             float v[N];
             if (one_scale) {
                 const float scale = scale_of(top[k]), inverse = 1.0f / scale;
 #pragma unroll
                 for (int i = 0; i < N; ++i) v[i] = s[k][i] * inverse;
-                const int g = groups == 1 ? 0 : col / group;
-                if (col == g * group) scales[g] = scale;
+                const int pack = me + k * TEAM;                          // a group is group_lanes (a power of two) packs
+                if (groups == 1 ? pack == 0 : (pack & (p.group_lanes - 1)) == 0) scales[groups == 1 ? 0 : pack >> p.group_shift] = scale;
             } else {
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
@@ -194,7 +229,7 @@ __global__ void __launch_bounds__(TeamShape<TEAM>::THREADS) norm_forward(const _
                 }
             }
             // (an infinite value meets an infinite scale: inf * 0 is NaN, as inf / inf)
-            if (p.vec && col + N <= columns) {
+            if (VEC) {
                 uint2 bytes;
                 bytes.x = e4m3_pair(v[0], v[1]) | e4m3_pair(v[2], v[3]) << 16;
                 bytes.y = e4m3_pair(v[4], v[5]) | e4m3_pair(v[6], v[7]) << 16;
@@ -209,64 +244,82 @@ __global__ void __launch_bounds__(TeamShape<TEAM>::THREADS) norm_forward(const _
 }
 
 // With g = gy w and xhat = s r: gx = r (g - xhat mean(g xhat)) + gresidual_out; gweight = sum over the rows of gy xhat.
-// Every team walks over rows with its sums for gweight in registers.
-template <typename T, int TEAM, int K>
+// Every team walks over rows with its sums for gweight in registers, the next row's elements on their way.
+template <typename T, int TEAM, int K, bool VEC>
 __global__ void __launch_bounds__(TeamShape<TEAM>::THREADS) norm_backward(const __grid_constant__ NormParams p) {
     using S = TeamShape<TEAM>;
     constexpr int N = 8;
+    constexpr bool AHEAD = K * sizeof(T) <= 8;                           // as long as the registers last
     __shared__ float s_sum[2][32];
     __shared__ float s_w[TEAM == 32 ? S::TEAMS : 1][TEAM == 32 ? TEAM * K * N : 1];
     const OvlRmsNorm& a = p.a;
     const int team = threadIdx.x / TEAM, me = threadIdx.x % TEAM;
     const int columns = (int)a.columns;
+    const Columns<T, TEAM, VEC> cols{columns, me};
     float w[K][N], gw[K][N];
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+    for (int k = 0; k < K; ++k) {
+        cols.weights(w[k], a.weight, a.params_f32, k);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int col = (me + k * TEAM) * N + i;
-            w[k][i] = col < columns ? load_param<T>(a.weight, col, a.params_f32) : 0.0f;
-            gw[k][i] = 0.0f;
-        }
-    for (int64_t row = (int64_t)blockIdx.x * S::TEAMS + team; row < a.rows; row += (int64_t)gridDim.x * S::TEAMS) {
+        for (int i = 0; i < N; ++i) gw[k][i] = 0.0f;
+    }
+    const int64_t first = (int64_t)blockIdx.x * S::TEAMS + team, step = (int64_t)gridDim.x * S::TEAMS;
+    const bool more = a.gresidual_out != nullptr;
+    Pack<T, N> next_x[K], next_g[K], next_r[K];
+    auto fetch = [&](int64_t row) {
         const T* const x = reinterpret_cast<const T*>(a.x) + row * a.x_row;
         const T* const gy = reinterpret_cast<const T*>(a.gy) + row * a.gy_row;
-        const T* const gr = a.gresidual_out ? reinterpret_cast<const T*>(a.gresidual_out) + row * a.gresidual_out_row : nullptr;
+        const T* const gr = reinterpret_cast<const T*>(a.gresidual_out) + row * a.gresidual_out_row;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            next_x[k] = cols.load(x, k);
+            next_g[k] = cols.load(gy, k);
+        }
+        if (more) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) next_r[k] = cols.load(gr, k);
+        }
+    };
+    if (AHEAD && first < a.rows) fetch(first);
+    for (int64_t row = first; row < a.rows; row += step) {
+        if (!AHEAD) fetch(row);
         Pack<T, N> rx[K], rg[K], rr[K];
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            rx[k] = next_x[k];
+            rg[k] = next_g[k];
+            if (more) rr[k] = next_r[k];
+        }
+        // (behind the last row the last one is read again, so that no load waits for a condition)
+        if (AHEAD) fetch(row + step < a.rows ? row + step : a.rows - 1);
         float sum[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            const int col = (me + k * TEAM) * N;
-            const int valid = col >= columns ? 0 : columns - col < N ? columns - col : N;
-            const bool vec = p.vec && valid == N;
-            rx[k] = load_pack<T, N>(x + col, vec, valid);
-            rg[k] = load_pack<T, N>(gy + col, vec, valid);
-            if (gr) rr[k] = load_pack<T, N>(gr + col, vec, valid);
-        }
-#pragma unroll
-        for (int k = 0; k < K; ++k)
+            if (VEC && !cols.in(k)) continue;
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const float s = to_f32(rx[k].v[i]);
                 sum[0] = fmaf(s, s, sum[0]);
                 sum[1] = fmaf(s * w[k][i], to_f32(rg[k].v[i]), sum[1]);
             }
+        }
         team_sum<TEAM, 2>(sum, s_sum);
         const float r = rsqrtf(sum[0] / (float)columns + (float)a.eps);
-        const float mean = r * r * (sum[1] / (float)columns);            // mean(g xhat) r, so that xhat r mean = s r mean
+        const float mean = r * r * (sum[1] / (float)columns);            // xhat mean(g xhat) = s mean, apart from a factor r
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            const int col = (me + k * TEAM) * N;
-            const int valid = col >= columns ? 0 : columns - col < N ? columns - col : N;
             float gx[N];
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const float s = to_f32(rx[k].v[i]), g = to_f32(rg[k].v[i]);
                 gx[i] = r * fmaf(-s, mean, g * w[k][i]);
-                if (gr) gx[i] += to_f32(rr[k].v[i]);
                 gw[k][i] = fmaf(g, s * r, gw[k][i]);
             }
-            store_pack<T, N>(reinterpret_cast<T*>(a.gx) + row * a.columns + col, gx, p.vec && valid == N, valid);
+            if (more) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) gx[i] += to_f32(rr[k].v[i]);
+            }
+            cols.store(reinterpret_cast<T*>(a.gx) + row * a.columns, k, gx);
         }
     }
     float* const part = p.part + (int64_t)blockIdx.x * columns;
@@ -286,10 +339,8 @@ __global__ void __launch_bounds__(TeamShape<TEAM>::THREADS) norm_backward(const 
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const int col = (me + k * TEAM) * N + i;
-                if (col < columns) part[col] = gw[k][i];
-            }
+            for (int i = 0; i < N; ++i)
+                if (cols.at(k) + i < columns) part[cols.at(k) + i] = gw[k][i];
     }
 }
 
@@ -300,8 +351,10 @@ __global__ void __launch_bounds__(256) norm_backward_weight(const __grid_constan
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     const int64_t col = (int64_t)blockIdx.x * 32 + lane;
     float sum = 0.0f;
-    if (col < p.a.columns)
+    if (col < p.a.columns) {
+#pragma unroll 4
         for (int64_t r = warp; r < parts; r += 8) sum += p.part[r * p.a.columns + col];
+    }
     s_part[warp][lane] = sum;
     __syncthreads();
     if (warp == 0 && col < p.a.columns) {
@@ -336,11 +389,11 @@ int64_t backward_blocks(const OvlRmsNorm* a) {
     return blocks < 1 ? 1 : blocks < most ? blocks : most;
 }
 
-template <typename T, int TEAM, int K>
-int launch(const NormParams& p, bool backward, cudaStream_t stream) {
+template <typename T, int TEAM, int K, bool VEC>
+int launch_as(const NormParams& p, bool backward, cudaStream_t stream) {
     using S = TeamShape<TEAM>;
     if (backward) {
-        norm_backward<T, TEAM, K><<<(uint32_t)backward_blocks(&p.a), S::THREADS, 0, stream>>>(p);
+        norm_backward<T, TEAM, K, VEC><<<(uint32_t)backward_blocks(&p.a), S::THREADS, 0, stream>>>(p);
         return launch_status();
     }
     const int64_t blocks = ceil_div(p.a.rows, S::TEAMS);
@@ -349,14 +402,20 @@ int launch(const NormParams& p, bool backward, cudaStream_t stream) {
         const size_t groups = p.a.columns / p.a.group;
         const size_t smem = p.group_lanes && groups > 1 ? 0 : S::TEAMS * groups * sizeof(unsigned int);
         if (smem > 40 * 1024) {
-            const cudaError_t e = cudaFuncSetAttribute(norm_forward<T, TEAM, K, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+            const cudaError_t e =
+                cudaFuncSetAttribute(norm_forward<T, TEAM, K, true, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
             if (e != cudaSuccess) return record_cuda_error(e);
         }
-        norm_forward<T, TEAM, K, true><<<(uint32_t)blocks, S::THREADS, smem, stream>>>(p);
+        norm_forward<T, TEAM, K, true, VEC><<<(uint32_t)blocks, S::THREADS, smem, stream>>>(p);
     } else {
-        norm_forward<T, TEAM, K, false><<<(uint32_t)blocks, S::THREADS, 0, stream>>>(p);
+        norm_forward<T, TEAM, K, false, VEC><<<(uint32_t)blocks, S::THREADS, 0, stream>>>(p);
     }
     return launch_status();
+}
+
+template <typename T, int TEAM, int K>
+int launch(const NormParams& p, bool backward, cudaStream_t stream) {
+    return p.vec ? launch_as<T, TEAM, K, true>(p, backward, stream) : launch_as<T, TEAM, K, false>(p, backward, stream);
 }
 
 template <typename T>
@@ -398,7 +457,10 @@ extern "C" int ovl_rms_norm(const OvlRmsNorm* a, void* cuda_stream) {
             (!a->residual || a->residual_row % 8 == 0) && ovl::aligned16(a->residual_out) && ovl::aligned16(a->weight) &&
             (a->group > 0 ? ovl::aligned16(a->q) : ovl::aligned16(a->y));
     const int64_t lanes = a->group / 8;
-    if (a->group % 8 == 0 && lanes >= 1 && lanes <= 32 && (lanes & (lanes - 1)) == 0) p.group_lanes = (int32_t)lanes;
+    if (a->group % 8 == 0 && lanes >= 1 && lanes <= 32 && (lanes & (lanes - 1)) == 0) {
+        p.group_lanes = (int32_t)lanes;
+        while ((1 << p.group_shift) < p.group_lanes) ++p.group_shift;
+    }
     return ovl::run(p, false, (cudaStream_t)cuda_stream);
 }
 
@@ -411,7 +473,8 @@ extern "C" int ovl_rms_norm_backward(const OvlRmsNorm* a, void* cuda_stream) {
     p.a = *a;
     p.part = reinterpret_cast<float*>(a->workspace);
     p.vec = a->columns % 8 == 0 && ovl::aligned16(a->x) && a->x_row % 8 == 0 && ovl::aligned16(a->gy) && a->gy_row % 8 == 0 &&
-            ovl::aligned16(a->gresidual_out) && (!a->gresidual_out || a->gresidual_out_row % 8 == 0) && ovl::aligned16(a->gx);
+            ovl::aligned16(a->gresidual_out) && (!a->gresidual_out || a->gresidual_out_row % 8 == 0) && ovl::aligned16(a->gx) &&
+            ovl::aligned16(a->weight);
     const cudaStream_t stream = (cudaStream_t)cuda_stream;
     const int s = ovl::run(p, true, stream);
     if (s != OVL_OK) return s;

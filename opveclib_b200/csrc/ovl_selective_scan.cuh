@@ -1044,57 +1044,70 @@ __global__ void scan_backward_params(const __grid_constant__ ScanParams p) {
 // ---------------------------------------------------------------------------------------------------------
 // one token
 
-// a thread per 4 states of a (row, channel); a block works on one row
+// A thread has 4 states of a channel and walks over ROWS rows; what belongs
+// to the channel (A, D, the bias) is loaded once.  What bounds it: bytes, the states in and out.
+constexpr int kStepRows = 4;           // rows of a block, if that leaves enough blocks
+
+// The slot of a row: -1 for padding, -2 for one that does not exist or that an earlier row has.  All threads of the block
+// call it.
+__device__ __forceinline__ int64_t slot_of(const int32_t* slot_of_row, int64_t slots, int64_t row) {
+    if (!slot_of_row) return row;
+    const int slot = slot_of_row[row];
+    int taken = 0;
+    for (int r = threadIdx.x; r < row; r += blockDim.x) taken |= slot >= 0 && slot_of_row[r] == slot;
+    taken = __syncthreads_or(taken);
+    return slot < 0 ? -1 : slot >= slots || taken ? -2 : slot;
+}
+
 template <typename T, int P>
-__global__ void __launch_bounds__(128) scan_step(const __grid_constant__ OvlSelectiveScanStep a, int64_t blocks_per_row,
+__global__ void __launch_bounds__(128) scan_step(const __grid_constant__ OvlSelectiveScanStep a, int tiles, int rows_of_block,
                                                  int vec_states) {
-    const int64_t row = blockIdx.x / blocks_per_row;
-    const int tid = threadIdx.x, lane = tid % 32, j = lane % P;
-    const int64_t channel_at = (blockIdx.x % blocks_per_row) * (128 / P) + tid / P;
-    const bool live = channel_at < a.channels;
-    const int64_t channel = live ? channel_at : a.channels - 1;
-    T* const out = reinterpret_cast<T*>(a.out) + row * a.channels;
-    int64_t slot = row;
-    if (a.slot_of_row) {
-        slot = a.slot_of_row[row];
-        int taken = 0;
-        for (int64_t r = tid; r < row; r += 128) taken |= slot >= 0 && a.slot_of_row[r] == slot;
-        taken = __syncthreads_or(taken);
-        if (slot < 0 || slot >= a.slots || taken) {
-            if (live && j == 0) out[channel] = from_f32<T>(slot < 0 ? 0.0f : __int_as_float(0x7fffffff));
-            return;
+    const int tile = blockIdx.x % tiles, tid = threadIdx.x, lane = tid % 32, j = lane % P, n0 = 4 * j;
+    const int64_t row0 = (int64_t)(blockIdx.x / tiles) * rows_of_block;
+    const int channel_at = tile * (128 / P) + tid / P, channels = (int)a.channels, states = (int)a.states;
+    const bool live = channel_at < channels;
+    const int channel = live ? channel_at : channels - 1;
+    const int group = channel / (channels / (int)a.groups);
+    F2 A[2];
+    load_states(A, a.A + (int64_t)channel * states, n0, states, vec_states);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) A[k] = mul2(A[k], same2(kLog2e));
+    const float skip = a.D ? a.D[channel] : 0.0f, bias = a.delta_bias ? a.delta_bias[channel] : 0.0f;
+    const T* const B = reinterpret_cast<const T*>(a.B) + group * a.B_group + n0;
+    const T* const C = reinterpret_cast<const T*>(a.C) + group * a.C_group + n0;
+    const int left = states - n0;                                        // states of this thread (and behind it)
+    for (int64_t row = row0; row < row0 + rows_of_block && row < a.rows; ++row) {
+        T* const out = reinterpret_cast<T*>(a.out) + row * channels + channel;
+        const int64_t slot = slot_of(a.slot_of_row, a.slots, row);
+        if (slot < 0) {
+            if (live && j == 0) *out = from_f32<T>(slot == -1 ? 0.0f : __int_as_float(0x7fffffff));
+            continue;
         }
-    }
-    const int states = (int)a.states;
-    const int64_t group = channel / (a.channels / a.groups);
-    float* const state = a.state + (slot * a.channels + channel) * states;
-    F2 h[2], A[2], bb[2], cc[2];
-    load_states(h, state, 4 * j, states, vec_states);
-    load_states(A, a.A + channel * states, 4 * j, states, vec_states);
-    const T* const B = reinterpret_cast<const T*>(a.B) + row * a.B_row + group * a.B_group;
-    const T* const C = reinterpret_cast<const T*>(a.C) + row * a.C_row + group * a.C_group;
-    const float u = to_f32(reinterpret_cast<const T*>(a.u)[row * a.u_row + channel]);
-    float dt = to_f32(reinterpret_cast<const T*>(a.delta)[row * a.delta_row + channel]);
-    const float z = a.z ? to_f32(reinterpret_cast<const T*>(a.z)[row * a.z_row + channel]) : 0.0f;
-    const float skip = a.D ? a.D[channel] : 0.0f;
-    if (a.delta_bias) dt += a.delta_bias[channel];
+        float* const state = a.state + (slot * channels + channel) * states;
+        F2 h[2], b[2], c[2];
+        load_states(h, state, n0, states, vec_states);
+        const float u = to_f32(reinterpret_cast<const T*>(a.u)[row * a.u_row + channel]);
+        float dt = to_f32(reinterpret_cast<const T*>(a.delta)[row * a.delta_row + channel]) + bias;
+        const float z = a.z ? to_f32(reinterpret_cast<const T*>(a.z)[row * a.z_row + channel]) : 0.0f;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        const int n = 4 * j + 2 * k;
-        bb[k] = pack2(n < states ? to_f32(B[n]) : 0.0f, n + 1 < states ? to_f32(B[n + 1]) : 0.0f);
-        cc[k] = pack2(n < states ? to_f32(C[n]) : 0.0f, n + 1 < states ? to_f32(C[n + 1]) : 0.0f);
-    }
-    if (a.delta_softplus) dt = softplus(dt);
+        for (int k = 0; k < 2; ++k) {
+            const T* const bk = B + row * a.B_row + 2 * k;
+            const T* const ck = C + row * a.C_row + 2 * k;
+            b[k] = pack2(2 * k < left ? to_f32(bk[0]) : 0.0f, 2 * k + 1 < left ? to_f32(bk[1]) : 0.0f);
+            c[k] = pack2(2 * k < left ? to_f32(ck[0]) : 0.0f, 2 * k + 1 < left ? to_f32(ck[1]) : 0.0f);
+        }
+        if (a.delta_softplus) dt = softplus(dt);
 #pragma unroll
-    for (int k = 0; k < 2; ++k) h[k] = fma2(decay(mul2(A[k], same2(kLog2e)), same2(dt)), h[k], mul2(same2(dt * u), bb[k]));
-    float y[1] = {dot(h, cc)};
-    reduce_lanes<1, P, 1>(y, lane);
-    if (!live) return;
-    store_states(state, h, 4 * j, states, vec_states);
-    if (j == 0) {
-        float o = fmaf(skip, u, y[0]);
-        if (a.z) o *= z * sigmoid(z);
-        out[channel] = from_f32<T>(o);
+        for (int k = 0; k < 2; ++k) h[k] = fma2(decay(A[k], same2(dt)), h[k], mul2(same2(dt * u), b[k]));
+        float y[1] = {dot(h, c)};
+        reduce_lanes<1, P, 1>(y, lane);
+        if (!live) continue;
+        store_states(state, h, n0, states, vec_states);
+        if (j == 0) {
+            float o = fmaf(skip, u, y[0]);
+            if (a.z) o *= silu(z);
+            *out = from_f32<T>(o);
+        }
     }
 }
 
@@ -1184,17 +1197,20 @@ int scan_dispatch(const ScanParams& p, const ScanShape& s, bool backward, cudaSt
 
 template <typename T>
 int scan_step_dispatch(const OvlSelectiveScanStep& a, int lanes, cudaStream_t stream) {
-    const int64_t per_row = ceil_div(a.channels, 128 / lanes), blocks = per_row * a.rows;
-    if (blocks > 0x7fffffff) return OVL_ERR_TOO_LARGE;
+    const int64_t tiles = ceil_div(a.channels, 128 / lanes);
+    const int rows = tiles * ceil_div(a.rows, kStepRows) >= 8 * (int64_t)sequence_sm_count() ? kStepRows : 1;
+    const int64_t blocks = tiles * ceil_div(a.rows, rows);
+    if (blocks > 0x7fffffff || a.channels > 0x7fffffff) return OVL_ERR_TOO_LARGE;
     const int vec = a.states % 4 == 0 && aligned16(a.A) && aligned16(a.state);
     const uint32_t grid = (uint32_t)blocks;
+    const int t = (int)tiles;
     switch (lanes) {
-        case 1: scan_step<T, 1><<<grid, 128, 0, stream>>>(a, per_row, vec); break;
-        case 2: scan_step<T, 2><<<grid, 128, 0, stream>>>(a, per_row, vec); break;
-        case 4: scan_step<T, 4><<<grid, 128, 0, stream>>>(a, per_row, vec); break;
-        case 8: scan_step<T, 8><<<grid, 128, 0, stream>>>(a, per_row, vec); break;
-        case 16: scan_step<T, 16><<<grid, 128, 0, stream>>>(a, per_row, vec); break;
-        default: scan_step<T, 32><<<grid, 128, 0, stream>>>(a, per_row, vec); break;
+        case 1: scan_step<T, 1><<<grid, 128, 0, stream>>>(a, t, rows, vec); break;
+        case 2: scan_step<T, 2><<<grid, 128, 0, stream>>>(a, t, rows, vec); break;
+        case 4: scan_step<T, 4><<<grid, 128, 0, stream>>>(a, t, rows, vec); break;
+        case 8: scan_step<T, 8><<<grid, 128, 0, stream>>>(a, t, rows, vec); break;
+        case 16: scan_step<T, 16><<<grid, 128, 0, stream>>>(a, t, rows, vec); break;
+        default: scan_step<T, 32><<<grid, 128, 0, stream>>>(a, t, rows, vec); break;
     }
     return launch_status();
 }

@@ -24,7 +24,7 @@ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-inline bool aligned16(const void* p) { return ((uintptr_t)p % 16) == 0; }
+__host__ __device__ inline bool aligned16(const void* p) { return ((uintptr_t)p % 16) == 0; }
 
 // SM count of the current device (148 on a B200), asked once per device.
 __attribute__((visibility("hidden"))) int sequence_sm_count();
