@@ -85,6 +85,13 @@ constexpr int kChunk = 4;              // tokens that are copied and worked on t
 constexpr int kAhead = 3;              // chunks on their way
 constexpr int kRing = kAhead + 1;
 
+struct True {
+    static constexpr bool value = true;
+};
+struct False {
+    static constexpr bool value = false;
+};
+
 template <typename T, int N>
 struct Ring {
     T* base;                           // [kRing][kChunk][threads][N]
@@ -151,36 +158,42 @@ __global__ void __launch_bounds__(32 * kWarps, TAPS == kMaxTaps ? 1 : 4) conv_fo
         widen<T, N>(win[k], load_token<T, N>(a, batch, t_begin - (TAPS - 1) + k, used, channel, vec, valid));
     const bool gated = a.silu;
     int chunk = 0;
+    // one token; INSIDE: it belongs to the strip and the sequence
+    auto token = [&](int64_t t, const T* slot, auto inside) {
+        constexpr bool INSIDE = decltype(inside)::value;
+        widen_slot<T, N>(win[TAPS - 1], slot);                           // (behind the sequence: anything, and not used)
+        float y[N];
+#pragma unroll
+        for (int c = 0; c < N / 2; ++c) {
+            F2 sum = bias[c];
+#pragma unroll
+            for (int k = 0; k < TAPS; ++k)
+                if (TAPS != kMaxTaps || k >= TAPS - taps) sum = fma2(w[k][c], win[k][c], sum);
+            unpack2(sum, y[2 * c], y[2 * c + 1]);
+        }
+        if (gated) {
+#pragma unroll
+            for (int c = 0; c < N; ++c) y[c] = silu(y[c]);
+        }
+        if (!INSIDE && t >= used) {
+#pragma unroll
+            for (int c = 0; c < N; ++c) y[c] = 0.0f;
+        }
+        if (INSIDE || t < t_end) store_pack<T, N>(out + t * a.channels, y, vec, valid);
+#pragma unroll
+        for (int k = 0; k < TAPS - 1; ++k)
+#pragma unroll
+            for (int c = 0; c < N / 2; ++c) win[k][c] = win[k + 1][c];
+    };
     for (int64_t t0 = t_begin; t0 < t_end; t0 += CHUNK) {
         copy_wait<kAhead - 1>();
         fetch(t0 + kAhead * CHUNK, chunk == 0 ? kAhead : chunk - 1);
+        if (t0 + CHUNK <= t_used) {
 #pragma unroll
-        for (int s = 0; s < CHUNK; ++s) {
-            widen_slot<T, N>(win[TAPS - 1], ring.slot(chunk, s));        // (behind the sequence: anything, and not used)
-            float y[N];
+            for (int s = 0; s < CHUNK; ++s) token(t0 + s, ring.slot(chunk, s), True{});
+        } else {
 #pragma unroll
-            for (int c = 0; c < N / 2; ++c) {
-                F2 sum = bias[c];
-#pragma unroll
-                for (int k = 0; k < TAPS; ++k)
-                    if (TAPS != kMaxTaps || k >= TAPS - taps) sum = fma2(w[k][c], win[k][c], sum);
-                unpack2(sum, y[2 * c], y[2 * c + 1]);
-            }
-            if (gated) {
-#pragma unroll
-                for (int c = 0; c < N; ++c) y[c] = silu(y[c]);
-            }
-            if (t0 + s < t_end) {
-                if (t0 + s >= used) {
-#pragma unroll
-                    for (int c = 0; c < N; ++c) y[c] = 0.0f;
-                }
-                store_pack<T, N>(out + (t0 + s) * a.channels, y, vec, valid);
-            }
-#pragma unroll
-            for (int k = 0; k < TAPS - 1; ++k)
-#pragma unroll
-                for (int c = 0; c < N / 2; ++c) win[k][c] = win[k + 1][c];
+            for (int s = 0; s < CHUNK; ++s) token(t0 + s, ring.slot(chunk, s), False{});
         }
         chunk = chunk == kAhead ? 0 : chunk + 1;
     }
@@ -240,85 +253,95 @@ __global__ void __launch_bounds__(32 * kWarps, TAPS == kMaxTaps ? 1 : 4) conv_ba
             widen<T, N>(win[k], load_token<T, N>(a, batch, t_begin - (TAPS - 1) + k, used, channel, vec, valid));
         const bool gated = a.silu;
         int chunk = 0;
-        for (int64_t t0 = t_begin; t0 < walk_end; t0 += CHUNK) {
-            copy_wait<kAhead - 1>();
-            fetch(t0 + kAhead * CHUNK, chunk == 0 ? kAhead : chunk - 1);
+        // one token; INSIDE: it belongs to the strip and the sequence, and so does the one whose gx it completes
+        auto token = [&](int64_t t, const T* slot_x, const T* slot_g, auto inside) {
+            constexpr bool INSIDE = decltype(inside)::value;
+            float g[N];
+            widen_slot<T, N>(win[TAPS - 1], slot_x);
+            read_slot<T, N>(slot_g, g);
+            if (gated) {
 #pragma unroll
-            for (int s = 0; s < CHUNK; ++s) {
-                const int64_t t = t0 + s;
-                float g[N];
-                widen_slot<T, N>(win[TAPS - 1], ring_x.slot(chunk, s));
-                read_slot<T, N>(ring_g.slot(chunk, s), g);
-                if (gated) {
+                for (int c = 0; c < N / 2; ++c) {
+                    F2 sum = bias[c];
 #pragma unroll
-                    for (int c = 0; c < N / 2; ++c) {
-                        F2 sum = bias[c];
+                    for (int k = 0; k < TAPS; ++k)
+                        if (TAPS != kMaxTaps || k >= TAPS - taps) sum = fma2(w[k][c], win[k][c], sum);
+                    float pre[2];
+                    unpack2(sum, pre[0], pre[1]);
 #pragma unroll
-                        for (int k = 0; k < TAPS; ++k)
-                            if (TAPS != kMaxTaps || k >= TAPS - taps) sum = fma2(w[k][c], win[k][c], sum);
-                        float pre[2];
-                        unpack2(sum, pre[0], pre[1]);
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const float sig = sigmoid(pre[e]);
-                            g[2 * c + e] *= sig * fmaf(pre[e], 1.0f - sig, 1.0f);
-                        }
+                    for (int e = 0; e < 2; ++e) {
+                        const float sig = sigmoid(pre[e]);
+                        g[2 * c + e] *= sig * fmaf(pre[e], 1.0f - sig, 1.0f);
                     }
                 }
-                // outside the sequence nothing comes from above, whatever the inputs there
-                const bool in = t < used;
+            }
+            // outside the sequence nothing comes from above, whatever the inputs there
+            const bool in = INSIDE || t < used;
 #pragma unroll
-                for (int c = 0; c < N / 2; ++c) gp[TAPS - 1][c] = in ? pack2(g[2 * c], g[2 * c + 1]) : same2(0.0f);
-                if (in && t < t_end) {
+            for (int c = 0; c < N / 2; ++c) gp[TAPS - 1][c] = in ? pack2(g[2 * c], g[2 * c + 1]) : same2(0.0f);
+            if (INSIDE || (in && t < t_end)) {
 #pragma unroll
-                    for (int c = 0; c < N / 2; ++c) {
-                        gb[c] = add2(gb[c], gp[TAPS - 1][c]);
+                for (int c = 0; c < N / 2; ++c) {
+                    gb[c] = add2(gb[c], gp[TAPS - 1][c]);
 #pragma unroll
-                        for (int k = 0; k < TAPS; ++k)
-                            if (TAPS != kMaxTaps || k >= TAPS - taps) gw[k][c] = fma2(gp[TAPS - 1][c], win[k][c], gw[k][c]);
-                    }
+                    for (int k = 0; k < TAPS; ++k)
+                        if (TAPS != kMaxTaps || k >= TAPS - taps) gw[k][c] = fma2(gp[TAPS - 1][c], win[k][c], gw[k][c]);
                 }
-                // gp[TAPS - 1 - k] is gpre of token t - k: gx of token t - (taps - 1)
-                const int64_t to = t - (taps - 1);
-                const bool state = to < 0;
-                if (t < walk_end && (state ? strip == 0 && a.ginitial != nullptr : to >= t_begin)) {
-                    float gx[N];
+            }
+            // gp[TAPS - 1 - k] is gpre of token t - k: gx of token t - (taps - 1)
+            const int64_t to = t - (taps - 1);
+            const bool state = !INSIDE && to < 0;
+            if (INSIDE || (t < walk_end && (state ? strip == 0 && a.ginitial != nullptr : to >= t_begin))) {
+                float gx[N];
 #pragma unroll
-                    for (int c = 0; c < N / 2; ++c) {
-                        F2 sum = same2(0.0f);
+                for (int c = 0; c < N / 2; ++c) {
+                    F2 sum = same2(0.0f);
 #pragma unroll
-                        for (int k = 0; k < TAPS; ++k)
-                            if (TAPS != kMaxTaps || k >= TAPS - taps) {
-                                if constexpr (TAPS != kMaxTaps) {
-                                    sum = fma2(w[k][c], gp[TAPS - 1 - k][c], sum);
-                                } else {
-                                    // tap k - (8 - taps): gp is indexed by registers, so every possible one is compared
+                    for (int k = 0; k < TAPS; ++k)
+                        if (TAPS != kMaxTaps || k >= TAPS - taps) {
+                            if constexpr (TAPS != kMaxTaps) {
+                                sum = fma2(w[k][c], gp[TAPS - 1 - k][c], sum);
+                            } else {
+                                // tap k - (8 - taps): gp is indexed by registers, so every possible one is compared
 #pragma unroll
-                                    for (int m = 0; m < TAPS; ++m)
-                                        if (m == k - (TAPS - taps)) sum = fma2(w[k][c], gp[TAPS - 1 - m][c], sum);
-                                }
+                                for (int m = 0; m < TAPS; ++m)
+                                    if (m == k - (TAPS - taps)) sum = fma2(w[k][c], gp[TAPS - 1 - m][c], sum);
                             }
-                        unpack2(sum, gx[2 * c], gx[2 * c + 1]);
-                    }
+                        }
+                    unpack2(sum, gx[2 * c], gx[2 * c + 1]);
+                }
+                if (!INSIDE && a.gfinal) {
                     // the state after the sequence holds the inputs used - (taps - 1) ... used - 1
                     const int64_t k = to - (used - (taps - 1));
-                    if (a.gfinal && k >= 0 && k < taps - 1) {
+                    if (k >= 0 && k < taps - 1) {
                         const Pack<T, N> gf = load_pack<T, N>(
                             reinterpret_cast<const T*>(a.gfinal) + (batch * (taps - 1) + k) * a.channels + channel, vec, valid);
 #pragma unroll
                         for (int c = 0; c < N; ++c) gx[c] += to_f32(gf.v[c]);
                     }
-                    T* const dst = state ? reinterpret_cast<T*>(a.ginitial) + (batch * (taps - 1) + (taps - 1) + to) * a.channels
-                                         : reinterpret_cast<T*>(a.gx) + (batch * a.length + to) * a.channels;
-                    store_pack<T, N>(dst + channel, gx, vec, valid);
                 }
+                T* const dst = state ? reinterpret_cast<T*>(a.ginitial) + (batch * (taps - 1) + (taps - 1) + to) * a.channels
+                                     : reinterpret_cast<T*>(a.gx) + (batch * a.length + to) * a.channels;
+                store_pack<T, N>(dst + channel, gx, vec, valid);
+            }
 #pragma unroll
-                for (int k = 0; k < TAPS - 1; ++k)
+            for (int k = 0; k < TAPS - 1; ++k)
 #pragma unroll
-                    for (int c = 0; c < N / 2; ++c) {
-                        win[k][c] = win[k + 1][c];
-                        gp[k][c] = gp[k + 1][c];
-                    }
+                for (int c = 0; c < N / 2; ++c) {
+                    win[k][c] = win[k + 1][c];
+                    gp[k][c] = gp[k + 1][c];
+                }
+        };
+        for (int64_t t0 = t_begin; t0 < walk_end; t0 += CHUNK) {
+            copy_wait<kAhead - 1>();
+            fetch(t0 + kAhead * CHUNK, chunk == 0 ? kAhead : chunk - 1);
+            // (gfinal belongs to tokens that the walk completes at t >= used)
+            if (t0 >= t_begin + (taps - 1) && t0 + CHUNK <= t_end && t0 + CHUNK <= used) {
+#pragma unroll
+                for (int s = 0; s < CHUNK; ++s) token(t0 + s, ring_x.slot(chunk, s), ring_g.slot(chunk, s), True{});
+            } else {
+#pragma unroll 1
+                for (int s = 0; s < CHUNK; ++s) token(t0 + s, ring_x.slot(chunk, s), ring_g.slot(chunk, s), False{});
             }
             chunk = chunk == kAhead ? 0 : chunk + 1;
         }

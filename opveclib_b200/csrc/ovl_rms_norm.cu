@@ -344,23 +344,24 @@ __global__ void __launch_bounds__(TeamShape<TEAM>::THREADS) norm_backward(const 
     }
 }
 
-// gweight: the blocks' parts added up in order; a warp's lanes are 32 columns, the 8 warps of a block slices of the parts
+// gweight: the blocks' parts added up in order; a warp's lanes are 32 columns, the 32 warps of a block slices of the parts
+constexpr int kPartWarps = 32;
 template <typename T>
-__global__ void __launch_bounds__(256) norm_backward_weight(const __grid_constant__ NormParams p, int64_t parts) {
-    __shared__ float s_part[8][32];
+__global__ void __launch_bounds__(32 * kPartWarps) norm_backward_weight(const __grid_constant__ NormParams p, int64_t parts) {
+    __shared__ float s_part[kPartWarps][32];
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     const int64_t col = (int64_t)blockIdx.x * 32 + lane;
     float sum = 0.0f;
     if (col < p.a.columns) {
-#pragma unroll 4
-        for (int64_t r = warp; r < parts; r += 8) sum += p.part[r * p.a.columns + col];
+#pragma unroll 8
+        for (int64_t r = warp; r < parts; r += kPartWarps) sum += p.part[r * p.a.columns + col];
     }
     s_part[warp][lane] = sum;
     __syncthreads();
     if (warp == 0 && col < p.a.columns) {
         sum = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 8; ++w) sum += s_part[w][lane];
+        for (int w = 0; w < kPartWarps; ++w) sum += s_part[w][lane];
         if (p.a.params_f32) reinterpret_cast<float*>(p.a.gweight)[col] = sum;
         else reinterpret_cast<T*>(p.a.gweight)[col] = from_f32<T>(sum);
     }
@@ -480,8 +481,8 @@ extern "C" int ovl_rms_norm_backward(const OvlRmsNorm* a, void* cuda_stream) {
     if (s != OVL_OK) return s;
     const uint32_t grid = (uint32_t)ovl::ceil_div(a->columns, 32);
     const int64_t parts = ovl::backward_blocks(a);
-    if (a->dtype == OVL_FLOAT32) ovl::norm_backward_weight<float><<<grid, 256, 0, stream>>>(p, parts);
-    else if (a->dtype == OVL_FLOAT16) ovl::norm_backward_weight<__half><<<grid, 256, 0, stream>>>(p, parts);
-    else ovl::norm_backward_weight<__nv_bfloat16><<<grid, 256, 0, stream>>>(p, parts);
+    if (a->dtype == OVL_FLOAT32) ovl::norm_backward_weight<float><<<grid, 32 * ovl::kPartWarps, 0, stream>>>(p, parts);
+    else if (a->dtype == OVL_FLOAT16) ovl::norm_backward_weight<__half><<<grid, 32 * ovl::kPartWarps, 0, stream>>>(p, parts);
+    else ovl::norm_backward_weight<__nv_bfloat16><<<grid, 32 * ovl::kPartWarps, 0, stream>>>(p, parts);
     return ovl::launch_status();
 }

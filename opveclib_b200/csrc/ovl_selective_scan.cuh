@@ -1044,8 +1044,8 @@ __global__ void scan_backward_params(const __grid_constant__ ScanParams p) {
 // ---------------------------------------------------------------------------------------------------------
 // one token
 
-// A thread has 4 states of a channel and walks over ROWS rows; what belongs
-// to the channel (A, D, the bias) is loaded once.  What bounds it: bytes, the states in and out.
+// A thread has 4 states of a channel for ROWS rows, all of whose loads are under way before the first is used; what
+// belongs to the channel (A, D, the bias) is loaded once.  What bounds it: bytes, the states in and out.
 constexpr int kStepRows = 4;           // rows of a block, if that leaves enough blocks
 
 // The slot of a row: -1 for padding, -2 for one that does not exist or that an earlier row has.  All threads of the block
@@ -1059,56 +1059,63 @@ __device__ __forceinline__ int64_t slot_of(const int32_t* slot_of_row, int64_t s
     return slot < 0 ? -1 : slot >= slots || taken ? -2 : slot;
 }
 
-template <typename T, int P>
-__global__ void __launch_bounds__(128) scan_step(const __grid_constant__ OvlSelectiveScanStep a, int tiles, int rows_of_block,
-                                                 int vec_states) {
+template <typename T, int P, int ROWS>
+__global__ void __launch_bounds__(128) scan_step(const __grid_constant__ OvlSelectiveScanStep a, int tiles, int vec_states, int vec_bc) {
     const int tile = blockIdx.x % tiles, tid = threadIdx.x, lane = tid % 32, j = lane % P, n0 = 4 * j;
-    const int64_t row0 = (int64_t)(blockIdx.x / tiles) * rows_of_block;
+    const int64_t row0 = (int64_t)(blockIdx.x / tiles) * ROWS;
     const int channel_at = tile * (128 / P) + tid / P, channels = (int)a.channels, states = (int)a.states;
     const bool live = channel_at < channels;
     const int channel = live ? channel_at : channels - 1;
     const int group = channel / (channels / (int)a.groups);
-    F2 A[2];
-    load_states(A, a.A + (int64_t)channel * states, n0, states, vec_states);
-#pragma unroll
-    for (int k = 0; k < 2; ++k) A[k] = mul2(A[k], same2(kLog2e));
-    const float skip = a.D ? a.D[channel] : 0.0f, bias = a.delta_bias ? a.delta_bias[channel] : 0.0f;
-    const T* const B = reinterpret_cast<const T*>(a.B) + group * a.B_group + n0;
-    const T* const C = reinterpret_cast<const T*>(a.C) + group * a.C_group + n0;
     const int left = states - n0;                                        // states of this thread (and behind it)
-    for (int64_t row = row0; row < row0 + rows_of_block && row < a.rows; ++row) {
-        T* const out = reinterpret_cast<T*>(a.out) + row * channels + channel;
-        const int64_t slot = slot_of(a.slot_of_row, a.slots, row);
-        if (slot < 0) {
-            if (live && j == 0) *out = from_f32<T>(slot == -1 ? 0.0f : __int_as_float(0x7fffffff));
-            continue;
-        }
-        float* const state = a.state + (slot * channels + channel) * states;
-        F2 h[2], b[2], c[2];
-        load_states(h, state, n0, states, vec_states);
-        const float u = to_f32(reinterpret_cast<const T*>(a.u)[row * a.u_row + channel]);
-        float dt = to_f32(reinterpret_cast<const T*>(a.delta)[row * a.delta_row + channel]) + bias;
-        const float z = a.z ? to_f32(reinterpret_cast<const T*>(a.z)[row * a.z_row + channel]) : 0.0f;
+    const bool wide = vec_bc && left >= 4;
+    int64_t slot[ROWS];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const T* const bk = B + row * a.B_row + 2 * k;
-            const T* const ck = C + row * a.C_row + 2 * k;
-            b[k] = pack2(2 * k < left ? to_f32(bk[0]) : 0.0f, 2 * k + 1 < left ? to_f32(bk[1]) : 0.0f);
-            c[k] = pack2(2 * k < left ? to_f32(ck[0]) : 0.0f, 2 * k + 1 < left ? to_f32(ck[1]) : 0.0f);
-        }
-        if (a.delta_softplus) dt = softplus(dt);
+    for (int r = 0; r < ROWS; ++r) slot[r] = row0 + r < a.rows ? slot_of(a.slot_of_row, a.slots, row0 + r) : -3;
+    if (a.slots > 0) {
+        F2 A[2], h[ROWS][2];
+        T u[ROWS], dt[ROWS], z[ROWS];
+        Pack<T, 4> b[ROWS], c[ROWS];
+        // (a row without a state reads the first one's, and leaves it alone)
 #pragma unroll
-        for (int k = 0; k < 2; ++k) h[k] = fma2(decay(A[k], same2(dt)), h[k], mul2(same2(dt * u), b[k]));
-        float y[1] = {dot(h, c)};
-        reduce_lanes<1, P, 1>(y, lane);
-        if (!live) continue;
-        store_states(state, h, n0, states, vec_states);
-        if (j == 0) {
-            float o = fmaf(skip, u, y[0]);
-            if (a.z) o *= silu(z);
-            *out = from_f32<T>(o);
+        for (int r = 0; r < ROWS; ++r) {
+            const int64_t from = slot[r] < 0 ? 0 : slot[r], row = row0 + r < a.rows ? row0 + r : a.rows - 1;
+            load_states(h[r], a.state + (from * channels + channel) * states, n0, states, vec_states);
+            u[r] = reinterpret_cast<const T*>(a.u)[row * a.u_row + channel];
+            dt[r] = reinterpret_cast<const T*>(a.delta)[row * a.delta_row + channel];
+            if (a.z) z[r] = reinterpret_cast<const T*>(a.z)[row * a.z_row + channel];
+            b[r] = load_pack<T, 4>(reinterpret_cast<const T*>(a.B) + row * a.B_row + group * a.B_group + n0, wide, left);
+            c[r] = load_pack<T, 4>(reinterpret_cast<const T*>(a.C) + row * a.C_row + group * a.C_group + n0, wide, left);
+        }
+        load_states(A, a.A + (int64_t)channel * states, n0, states, vec_states);
+        const float skip = a.D ? a.D[channel] : 0.0f, bias = a.delta_bias ? a.delta_bias[channel] : 0.0f;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) A[k] = mul2(A[k], same2(kLog2e));
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            const float x = to_f32(u[r]);
+            float step = to_f32(dt[r]) + bias;
+            if (a.delta_softplus) step = softplus(step);
+            const F2 bb[2] = {pack2(to_f32(b[r].v[0]), to_f32(b[r].v[1])), pack2(to_f32(b[r].v[2]), to_f32(b[r].v[3]))};
+            const F2 cc[2] = {pack2(to_f32(c[r].v[0]), to_f32(c[r].v[1])), pack2(to_f32(c[r].v[2]), to_f32(c[r].v[3]))};
+#pragma unroll
+            for (int k = 0; k < 2; ++k) h[r][k] = fma2(decay(A[k], same2(step)), h[r][k], mul2(same2(step * x), bb[k]));
+            float y[1] = {dot(h[r], cc)};
+            reduce_lanes<1, P, 1>(y, lane);
+            if (!live || slot[r] < 0) continue;
+            store_states(a.state + (slot[r] * channels + channel) * states, h[r], n0, states, vec_states);
+            if (j == 0) {
+                float o = fmaf(skip, x, y[0]);
+                if (a.z) o *= silu(to_f32(z[r]));
+                reinterpret_cast<T*>(a.out)[(row0 + r) * channels + channel] = from_f32<T>(o);
+            }
         }
     }
+    if (!live || j != 0) return;
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+        if (slot[r] == -1 || slot[r] == -2)
+            reinterpret_cast<T*>(a.out)[(row0 + r) * channels + channel] = from_f32<T>(slot[r] == -1 ? 0.0f : __int_as_float(0x7fffffff));
 }
 
 // ---------------------------------------------------------------------------------------------------------
@@ -1195,24 +1202,30 @@ int scan_dispatch(const ScanParams& p, const ScanShape& s, bool backward, cudaSt
     return OVL_ERR_INVALID;
 }
 
-template <typename T>
-int scan_step_dispatch(const OvlSelectiveScanStep& a, int lanes, cudaStream_t stream) {
-    const int64_t tiles = ceil_div(a.channels, 128 / lanes);
-    const int rows = tiles * ceil_div(a.rows, kStepRows) >= 8 * (int64_t)sequence_sm_count() ? kStepRows : 1;
-    const int64_t blocks = tiles * ceil_div(a.rows, rows);
+template <typename T, int P>
+int run_step(const OvlSelectiveScanStep& a, cudaStream_t stream) {
+    const int64_t tiles = ceil_div(a.channels, 128 / P);
+    const bool many = tiles * ceil_div(a.rows, kStepRows) >= 8 * (int64_t)sequence_sm_count();
+    const int64_t blocks = tiles * ceil_div(a.rows, many ? kStepRows : 1);
     if (blocks > 0x7fffffff || a.channels > 0x7fffffff) return OVL_ERR_TOO_LARGE;
     const int vec = a.states % 4 == 0 && aligned16(a.A) && aligned16(a.state);
-    const uint32_t grid = (uint32_t)blocks;
-    const int t = (int)tiles;
-    switch (lanes) {
-        case 1: scan_step<T, 1><<<grid, 128, 0, stream>>>(a, t, rows, vec); break;
-        case 2: scan_step<T, 2><<<grid, 128, 0, stream>>>(a, t, rows, vec); break;
-        case 4: scan_step<T, 4><<<grid, 128, 0, stream>>>(a, t, rows, vec); break;
-        case 8: scan_step<T, 8><<<grid, 128, 0, stream>>>(a, t, rows, vec); break;
-        case 16: scan_step<T, 16><<<grid, 128, 0, stream>>>(a, t, rows, vec); break;
-        default: scan_step<T, 32><<<grid, 128, 0, stream>>>(a, t, rows, vec); break;
-    }
+    const int vec_bc = a.states % 4 == 0 && aligned16(a.B) && aligned16(a.C) && a.B_row % 4 == 0 && a.C_row % 4 == 0 &&
+                       a.B_group % 4 == 0 && a.C_group % 4 == 0;
+    if (many) scan_step<T, P, kStepRows><<<(uint32_t)blocks, 128, 0, stream>>>(a, (int)tiles, vec, vec_bc);
+    else scan_step<T, P, 1><<<(uint32_t)blocks, 128, 0, stream>>>(a, (int)tiles, vec, vec_bc);
     return launch_status();
+}
+
+template <typename T>
+int scan_step_dispatch(const OvlSelectiveScanStep& a, int lanes, cudaStream_t stream) {
+    switch (lanes) {
+        case 1: return run_step<T, 1>(a, stream);
+        case 2: return run_step<T, 2>(a, stream);
+        case 4: return run_step<T, 4>(a, stream);
+        case 8: return run_step<T, 8>(a, stream);
+        case 16: return run_step<T, 16>(a, stream);
+        default: return run_step<T, 32>(a, stream);
+    }
 }
 
 }  // namespace

@@ -20,13 +20,18 @@ from . import launcher
 
 _torch_module = None
 _codes = None
+_raw_stream = None
 
 
 def _torch():
-    global _torch_module, _codes
+    global _torch_module, _codes, _raw_stream
     if _torch_module is None:
         import torch
         _codes = {torch.float16: 1, torch.float32: 2, torch.bfloat16: 12}
+        # the current stream's handle without the Stream object around it (2 us of a small call)
+        _raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)
+        if _raw_stream is None:
+            _raw_stream = lambda index: torch.cuda.current_stream(index).cuda_stream  # noqa: E731
         _torch_module = torch
     return _torch_module
 
@@ -44,19 +49,25 @@ def _ptr(x):
     return 0 if x is None else x.data_ptr()
 
 
-def _tensor(x, name, shape, dtype, what):
-    """Refuse anything but a tensor of this shape and type; a copy where the innermost axis is not contiguous."""
+def _refuse(x, name, shape, dtype, what):
     if not isinstance(x, _torch_module.Tensor):
         raise TypeError('%s: %s must be a torch tensor' % (what, name))
     if x.dtype is not dtype:
         raise TypeError('%s: %s must be %s, not %s' % (what, name, dtype, x.dtype))
-    if x.shape != shape:
-        raise ValueError('%s: %s must have the shape %s, not %s' % (what, name, tuple(shape), tuple(x.shape)))
+    raise ValueError('%s: %s must have the shape %s, not %s' % (what, name, tuple(shape), tuple(x.shape)))
+
+
+def _tensor(x, name, shape, dtype, what):
+    """Refuse anything but a tensor of this shape and type; a copy where the innermost axis is not contiguous."""
+    if not isinstance(x, _torch_module.Tensor) or x.dtype is not dtype or x.shape != shape:
+        _refuse(x, name, shape, dtype, what)
     return x if x.stride(-1) == 1 else x.contiguous()
 
 
 def _dense(x, name, shape, dtype, what):
-    return _tensor(x, name, shape, dtype, what).contiguous()
+    if not isinstance(x, _torch_module.Tensor) or x.dtype is not dtype or x.shape != shape:
+        _refuse(x, name, shape, dtype, what)
+    return x.contiguous()
 
 
 def _first(x, name, rank, what):
@@ -99,15 +110,16 @@ def _one_device(what, *tensors):
 
 
 def _launch(name, args, device):
+    """Enqueue on torch's current stream of the tensors' device, whichever device is the current one."""
     torch = _torch_module
     function = getattr(launcher.library(), name)
-    stream = torch.cuda.current_stream(device).cuda_stream
     if device.index == torch.cuda.current_device():
-        status = function(args, stream)
+        status = function(args, _raw_stream(device.index))
     else:
         with torch.cuda.device(device):
-            status = function(args, stream)
-    launcher.check(status, name)
+            status = function(args, _raw_stream(device.index))
+    if status:
+        launcher.check(status, name)
 
 
 def _workspace(size, device):
@@ -123,7 +135,16 @@ def _with_device(device, function, *args):
 
 
 def _differentiable(*tensors):
-    return _torch_module.is_grad_enabled() and any(x is not None and x.requires_grad for x in tensors)
+    if _torch_module.is_grad_enabled():
+        for x in tensors:
+            if x is not None and x.requires_grad:
+                return True
+    return False
+
+
+def _like(x):
+    """A dense tensor of the shape, type and device of x."""
+    return _torch_module.empty_like(x, memory_format=_torch_module.contiguous_format)
 
 
 def _no_gradient(what, *tensors):
@@ -296,7 +317,7 @@ def selective_scan_step(state, u, delta, A, B, C, D=None, z=None, delta_bias=Non
     slots = _index(slots, 'slots', rows, what)
     _no_gradient(what, state, u, delta, A, B, C, D, z, delta_bias)
     device = _one_device(what, u, state, delta, A, B, C, D, z, delta_bias, slots)
-    out = torch.empty((rows, channels), dtype=t, device=device)
+    out = _like(u)
     _launch('ovl_selective_scan_step', _SCAN_STEP.pack(
         _codes[t], rows, channels, states, groups, 1 if delta_softplus else 0, n_slots, u.data_ptr(), delta.data_ptr(),
         _ptr(z), B.data_ptr(), C.data_ptr(), A.data_ptr(), _ptr(D), _ptr(delta_bias), _ptr(slots), u.stride(0),
@@ -427,7 +448,7 @@ def causal_conv1d_step(state, x, weight, bias=None, activation=None, slots=None)
     slots = _index(slots, 'slots', rows, what)
     _no_gradient(what, state, x, weight, bias)
     device = _one_device(what, x, state, weight, bias, slots)
-    out = torch.empty((rows, channels), dtype=t, device=device)
+    out = _like(x)
     _launch('ovl_causal_conv_step', _CONV_STEP.pack(
         _codes[t], rows, channels, taps, silu, p is torch.float32, state.shape[0], x.data_ptr(), weight.data_ptr(),
         _ptr(bias), _ptr(slots), x.stride(0), state.data_ptr(), out.data_ptr()), device)
@@ -467,10 +488,9 @@ def _norm_check(x, weight, residual, eps, what):
 
 
 def _norm_forward(x, weight, residual, eps):
-    torch = _torch_module
     x, residual = _rows(x), None if residual is None else _rows(residual)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    residual_out = None if residual is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = _like(x)
+    residual_out = None if residual is None else _like(x)
     _launch('ovl_rms_norm', _norm_args(x, weight, eps, 0, residual, y, residual_out), x.device)
     return y, residual_out
 
@@ -483,7 +503,7 @@ def _norm_backward(x, weight, eps, gy, gres):
     gy = gy if gy.stride(-1) == 1 else gy.contiguous()
     if gres is not None and gres.stride(-1) != 1:
         gres = gres.contiguous()
-    gx = torch.empty(x.shape, dtype=x.dtype, device=device)
+    gx = _like(x)
     gweight = torch.empty(weight.shape, dtype=weight.dtype, device=device)
     size = _with_device(device, launcher.library().ovl_rms_norm_workspace_bytes, _norm_args(x, weight, eps))
     _launch('ovl_rms_norm_backward',
@@ -505,8 +525,9 @@ def rms_norm(x, weight, residual=None, eps=1e-6):
         y, residual_out = _autograd().norm.apply(x, weight, residual, eps)
     else:
         y, residual_out = _norm_forward(x, weight, residual, eps)
-        y = y.view(x.shape)
-        residual_out = None if residual_out is None else residual_out.view(x.shape)
+        if x.dim() != 2:
+            y = y.view(x.shape)
+            residual_out = None if residual_out is None else residual_out.view(x.shape)
     return y if residual is None else (y, residual_out)
 
 
@@ -526,12 +547,14 @@ def rms_norm_quantize(x, weight, residual=None, eps=1e-6, group=None):
         raise ValueError('%s: group must divide the %d columns, not %r' % (what, columns, group))
     _no_gradient(what, x, weight, residual)
     shape, x, residual = x.shape, _rows(x), None if residual is None else _rows(residual)
-    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=device)
+    q = torch.empty_like(x, dtype=torch.float8_e4m3fn, memory_format=torch.contiguous_format)
     scale = torch.empty((x.shape[0], columns // group), dtype=torch.float32, device=device)
-    residual_out = None if residual is None else torch.empty(x.shape, dtype=x.dtype, device=device)
+    residual_out = None if residual is None else _like(x)
     _launch('ovl_rms_norm', _norm_args(x, weight, eps, group, residual, None, residual_out, q, scale), device)
-    q, scale = q.view(shape), scale.view(shape[:-1] + (columns // group,))
-    return (q, scale) if residual is None else (q, scale, residual_out.view(shape))
+    if len(shape) != 2:
+        q, scale = q.view(shape), scale.view(shape[:-1] + (columns // group,))
+        residual_out = None if residual is None else residual_out.view(shape)
+    return (q, scale) if residual is None else (q, scale, residual_out)
 
 
 # ---------------------------------------------------------------------------------------------------------
