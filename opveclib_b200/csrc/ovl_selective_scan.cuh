@@ -1044,8 +1044,9 @@ __global__ void scan_backward_params(const __grid_constant__ ScanParams p) {
 // ---------------------------------------------------------------------------------------------------------
 // one token
 
-// A thread has 4 states of a channel for ROWS rows, all of whose loads are under way before the first is used; what
-// belongs to the channel (A, D, the bias) is loaded once.  What bounds it: bytes, the states in and out.
+// A thread has 4 states of a channel for ROWS rows, all of whose loads are under way before the first is used; A is loaded
+// once for all rows.  What is needed once per (row, channel) - softplus, the gate, the output - is shared out among the
+// channel's lanes, a row (or more) each.  What bounds it: bytes, the states in and out.
 constexpr int kStepRows = 4;           // rows of a block, if that leaves enough blocks
 
 // The slot of a row: -1 for padding, -2 for one that does not exist or that an earlier row has.  All threads of the block
@@ -1059,63 +1060,88 @@ __device__ __forceinline__ int64_t slot_of(const int32_t* slot_of_row, int64_t s
     return slot < 0 ? -1 : slot >= slots || taken ? -2 : slot;
 }
 
-template <typename T, int P, int ROWS>
-__global__ void __launch_bounds__(128) scan_step(const __grid_constant__ OvlSelectiveScanStep a, int tiles, int vec_states, int vec_bc) {
+// EXACT: 4 P states, rows of A, B, C and the states on boundaries of 4 elements: no load depends on a condition.
+template <typename T, int P, int ROWS, bool EXACT>
+__global__ void __launch_bounds__(128) scan_step(const __grid_constant__ OvlSelectiveScanStep a, int tiles) {
+    constexpr int OWN = reduced_count<ROWS, P>();                        // rows of a lane
     const int tile = blockIdx.x % tiles, tid = threadIdx.x, lane = tid % 32, j = lane % P, n0 = 4 * j;
     const int64_t row0 = (int64_t)(blockIdx.x / tiles) * ROWS;
-    const int channel_at = tile * (128 / P) + tid / P, channels = (int)a.channels, states = (int)a.states;
+    const int channel_at = tile * (128 / P) + tid / P, channels = (int)a.channels, states = EXACT ? 4 * P : (int)a.states;
     const bool live = channel_at < channels;
     const int channel = live ? channel_at : channels - 1;
     const int group = channel / (channels / (int)a.groups);
-    const int left = states - n0;                                        // states of this thread (and behind it)
-    const bool wide = vec_bc && left >= 4;
+    const int own = reduced_index<ROWS, P>(j);
     int64_t slot[ROWS];
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) slot[r] = row0 + r < a.rows ? slot_of(a.slot_of_row, a.slots, row0 + r) : -3;
+    float o[ROWS];
+    float x[OWN];
+    T z[OWN];
     if (a.slots > 0) {
         F2 A[2], h[ROWS][2];
-        T u[ROWS], dt[ROWS], z[ROWS];
         Pack<T, 4> b[ROWS], c[ROWS];
-        // (a row without a state reads the first one's, and leaves it alone)
+        // (a row without a state reads the first one's, and leaves it alone; behind the last row it is read again)
+        const int64_t last = a.rows - 1;
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
-            const int64_t from = slot[r] < 0 ? 0 : slot[r], row = row0 + r < a.rows ? row0 + r : a.rows - 1;
-            load_states(h[r], a.state + (from * channels + channel) * states, n0, states, vec_states);
-            u[r] = reinterpret_cast<const T*>(a.u)[row * a.u_row + channel];
-            dt[r] = reinterpret_cast<const T*>(a.delta)[row * a.delta_row + channel];
-            if (a.z) z[r] = reinterpret_cast<const T*>(a.z)[row * a.z_row + channel];
-            b[r] = load_pack<T, 4>(reinterpret_cast<const T*>(a.B) + row * a.B_row + group * a.B_group + n0, wide, left);
-            c[r] = load_pack<T, 4>(reinterpret_cast<const T*>(a.C) + row * a.C_row + group * a.C_group + n0, wide, left);
+            const int64_t from = slot[r] < 0 ? 0 : slot[r], row = row0 + r < last ? row0 + r : last;
+            load_states(h[r], a.state + (from * channels + channel) * states, n0, states, EXACT);
+            b[r] = load_pack<T, 4>(reinterpret_cast<const T*>(a.B) + row * a.B_row + group * a.B_group + n0, EXACT, states - n0);
+            c[r] = load_pack<T, 4>(reinterpret_cast<const T*>(a.C) + row * a.C_row + group * a.C_group + n0, EXACT, states - n0);
         }
-        load_states(A, a.A + (int64_t)channel * states, n0, states, vec_states);
-        const float skip = a.D ? a.D[channel] : 0.0f, bias = a.delta_bias ? a.delta_bias[channel] : 0.0f;
+        float dt[OWN], du[OWN];
+        T raw_u[OWN], raw_dt[OWN];
+#pragma unroll
+        for (int k = 0; k < OWN; ++k) {
+            const int64_t row = row0 + own + k < last ? row0 + own + k : last;
+            raw_u[k] = reinterpret_cast<const T*>(a.u)[row * a.u_row + channel];
+            raw_dt[k] = reinterpret_cast<const T*>(a.delta)[row * a.delta_row + channel];
+            if (a.z) z[k] = reinterpret_cast<const T*>(a.z)[row * a.z_row + channel];
+        }
+        load_states(A, a.A + (int64_t)channel * states, n0, states, EXACT);
+        const float bias = a.delta_bias ? a.delta_bias[channel] : 0.0f;
 #pragma unroll
         for (int k = 0; k < 2; ++k) A[k] = mul2(A[k], same2(kLog2e));
 #pragma unroll
+        for (int k = 0; k < OWN; ++k) {
+            x[k] = to_f32(raw_u[k]);
+            dt[k] = to_f32(raw_dt[k]) + bias;
+            if (a.delta_softplus) dt[k] = softplus(dt[k]);
+            du[k] = dt[k] * x[k];
+        }
+#pragma unroll
         for (int r = 0; r < ROWS; ++r) {
-            const float x = to_f32(u[r]);
-            float step = to_f32(dt[r]) + bias;
-            if (a.delta_softplus) step = softplus(step);
+            float step = dt[r % OWN], add = du[r % OWN];
+            if (ROWS > 1 && P > 1) {                                     // from the lane that has the row
+                const int source = (lane & ~(P - 1)) + (P >= ROWS ? r * (P / ROWS) : r / OWN);
+                step = __shfl_sync(0xffffffffu, step, source);
+                add = __shfl_sync(0xffffffffu, add, source);
+            }
             const F2 bb[2] = {pack2(to_f32(b[r].v[0]), to_f32(b[r].v[1])), pack2(to_f32(b[r].v[2]), to_f32(b[r].v[3]))};
             const F2 cc[2] = {pack2(to_f32(c[r].v[0]), to_f32(c[r].v[1])), pack2(to_f32(c[r].v[2]), to_f32(c[r].v[3]))};
 #pragma unroll
-            for (int k = 0; k < 2; ++k) h[r][k] = fma2(decay(A[k], same2(step)), h[r][k], mul2(same2(step * x), bb[k]));
-            float y[1] = {dot(h[r], cc)};
-            reduce_lanes<1, P, 1>(y, lane);
-            if (!live || slot[r] < 0) continue;
-            store_states(a.state + (slot[r] * channels + channel) * states, h[r], n0, states, vec_states);
-            if (j == 0) {
-                float o = fmaf(skip, x, y[0]);
-                if (a.z) o *= silu(to_f32(z[r]));
-                reinterpret_cast<T*>(a.out)[(row0 + r) * channels + channel] = from_f32<T>(o);
-            }
+            for (int k = 0; k < 2; ++k) h[r][k] = fma2(decay(A[k], same2(step)), h[r][k], mul2(same2(add), bb[k]));
+            o[r] = dot(h[r], cc);
+            if (live && slot[r] >= 0) store_states(a.state + (slot[r] * channels + channel) * states, h[r], n0, states, EXACT);
         }
+        reduce_lanes<ROWS, P, 1>(o, lane);
     }
-    if (!live || j != 0) return;
+    if (!live || !reduced_owner<ROWS, P>(j)) return;
+    const float skip = a.D ? a.D[channel] : 0.0f;
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r)
-        if (slot[r] == -1 || slot[r] == -2)
-            reinterpret_cast<T*>(a.out)[(row0 + r) * channels + channel] = from_f32<T>(slot[r] == -1 ? 0.0f : __int_as_float(0x7fffffff));
+    for (int k = 0; k < OWN; ++k) {
+        int64_t at = slot[k];                                            // of row own + k; slots are indexed by registers
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r)
+            if (r == own + k) at = slot[r];
+        if (at == -3) continue;
+        float y = at == -1 ? 0.0f : __int_as_float(0x7fffffff);
+        if (at >= 0) {
+            y = fmaf(skip, x[k], o[k]);
+            if (a.z) y *= silu(to_f32(z[k]));
+        }
+        reinterpret_cast<T*>(a.out)[(row0 + own + k) * channels + channel] = from_f32<T>(y);
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------------
@@ -1202,18 +1228,22 @@ int scan_dispatch(const ScanParams& p, const ScanShape& s, bool backward, cudaSt
     return OVL_ERR_INVALID;
 }
 
+template <typename T, int P, int ROWS>
+int run_step_rows(const OvlSelectiveScanStep& a, int64_t tiles, cudaStream_t stream) {
+    const int64_t blocks = tiles * ceil_div(a.rows, ROWS);
+    if (blocks > 0x7fffffff || a.channels > 0x7fffffff) return OVL_ERR_TOO_LARGE;
+    const bool exact = a.states == 4 * P && aligned16(a.A) && aligned16(a.state) && aligned16(a.B) && aligned16(a.C) &&
+                       a.B_row % 4 == 0 && a.C_row % 4 == 0 && a.B_group % 4 == 0 && a.C_group % 4 == 0;
+    if (exact) scan_step<T, P, ROWS, true><<<(uint32_t)blocks, 128, 0, stream>>>(a, (int)tiles);
+    else scan_step<T, P, ROWS, false><<<(uint32_t)blocks, 128, 0, stream>>>(a, (int)tiles);
+    return launch_status();
+}
+
 template <typename T, int P>
 int run_step(const OvlSelectiveScanStep& a, cudaStream_t stream) {
     const int64_t tiles = ceil_div(a.channels, 128 / P);
-    const bool many = tiles * ceil_div(a.rows, kStepRows) >= 8 * (int64_t)sequence_sm_count();
-    const int64_t blocks = tiles * ceil_div(a.rows, many ? kStepRows : 1);
-    if (blocks > 0x7fffffff || a.channels > 0x7fffffff) return OVL_ERR_TOO_LARGE;
-    const int vec = a.states % 4 == 0 && aligned16(a.A) && aligned16(a.state);
-    const int vec_bc = a.states % 4 == 0 && aligned16(a.B) && aligned16(a.C) && a.B_row % 4 == 0 && a.C_row % 4 == 0 &&
-                       a.B_group % 4 == 0 && a.C_group % 4 == 0;
-    if (many) scan_step<T, P, kStepRows><<<(uint32_t)blocks, 128, 0, stream>>>(a, (int)tiles, vec, vec_bc);
-    else scan_step<T, P, 1><<<(uint32_t)blocks, 128, 0, stream>>>(a, (int)tiles, vec, vec_bc);
-    return launch_status();
+    if (tiles * ceil_div(a.rows, kStepRows) >= 8 * (int64_t)sequence_sm_count()) return run_step_rows<T, P, kStepRows>(a, tiles, stream);
+    return run_step_rows<T, P, 1>(a, tiles, stream);
 }
 
 template <typename T>
