@@ -336,9 +336,9 @@ int ovl_causal_conv_step(const OvlCausalConvStep* args, void* cuda_stream);
  * With group > 0 the output is 8 bits wide instead: y is cut into groups of `group` columns (which divides columns),
  *     scale = max(max |y| / 448, 2^-126),  q = y / scale rounded to the nearest e4m3 value, ties to even
  * with q [rows, columns] bytes and scale [rows, columns / group] fp32.
- * The backward call takes s as residual_out of the forward call holds it (x itself without a residual) in `x`, and the
- * gradients of y and of residual_out (NULL: zero); gx is the gradient of x and of the residual alike.  Its workspace:
- * ovl_rms_norm_workspace_bytes(args) bytes; the forward call needs none. */
+ * The backward call takes the forward call's x and residual and the gradients of y and of residual_out (NULL: zero); gx
+ * is the gradient of x and of the residual alike.  Its workspace: ovl_rms_norm_workspace_bytes(args) bytes; the forward
+ * call needs none. */
 typedef struct OvlRmsNorm {
     int64_t dtype, rows, columns, params_f32, group;
     double eps;

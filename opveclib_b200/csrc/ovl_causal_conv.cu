@@ -484,7 +484,7 @@ template <typename F>
 int launch(F kernel, const ConvParams& p, size_t smem, cudaStream_t stream) {
     const int64_t blocks = p.column_tiles * p.strips * p.a.batch;
     if (blocks > 0x7fffffff) return OVL_ERR_TOO_LARGE;
-    if (smem > 32 * 1024) {
+    if (smem > 24 * 1024) {                                              // (the backward kernels have up to 18 KB beside it)
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return record_cuda_error(e);
     }

@@ -265,9 +265,11 @@ __global__ void __launch_bounds__(TeamShape<TEAM>::THREADS) norm_backward(const 
     }
     const int64_t first = (int64_t)blockIdx.x * S::TEAMS + team, step = (int64_t)gridDim.x * S::TEAMS;
     const bool more = a.gresidual_out != nullptr;
-    Pack<T, N> next_x[K], next_g[K], next_r[K];
+    const bool sum_of_two = a.residual != nullptr;
+    Pack<T, N> next_x[K], next_s[K], next_g[K], next_r[K];
     auto fetch = [&](int64_t row) {
         const T* const x = reinterpret_cast<const T*>(a.x) + row * a.x_row;
+        const T* const res = reinterpret_cast<const T*>(a.residual) + row * a.residual_row;
         const T* const gy = reinterpret_cast<const T*>(a.gy) + row * a.gy_row;
         const T* const gr = reinterpret_cast<const T*>(a.gresidual_out) + row * a.gresidual_out_row;
 #pragma unroll
@@ -279,16 +281,29 @@ __global__ void __launch_bounds__(TeamShape<TEAM>::THREADS) norm_backward(const 
 #pragma unroll
             for (int k = 0; k < K; ++k) next_r[k] = cols.load(gr, k);
         }
+        if (sum_of_two) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) next_s[k] = cols.load(res, k);
+        }
     };
     if (AHEAD && first < a.rows) fetch(first);
     for (int64_t row = first; row < a.rows; row += step) {
         if (!AHEAD) fetch(row);
-        Pack<T, N> rx[K], rg[K], rr[K];
+        // the sum in 32 bits, as the forward pass had it (its rounded copy would put another rounding on gweight)
+        float s[K][N];
+        Pack<T, N> rg[K], rr[K];
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            rx[k] = next_x[k];
+#pragma unroll
+            for (int i = 0; i < N; ++i) s[k][i] = to_f32(next_x[k].v[i]);
             rg[k] = next_g[k];
             if (more) rr[k] = next_r[k];
+        }
+        if (sum_of_two) {
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int i = 0; i < N; ++i) s[k][i] += to_f32(next_s[k].v[i]);
         }
         // (behind the last row the last one is read again, so that no load waits for a condition)
         if (AHEAD) fetch(row + step < a.rows ? row + step : a.rows - 1);
@@ -298,9 +313,8 @@ __global__ void __launch_bounds__(TeamShape<TEAM>::THREADS) norm_backward(const 
             if (VEC && !cols.in(k)) continue;
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const float s = to_f32(rx[k].v[i]);
-                sum[0] = fmaf(s, s, sum[0]);
-                sum[1] = fmaf(s * w[k][i], to_f32(rg[k].v[i]), sum[1]);
+                sum[0] = fmaf(s[k][i], s[k][i], sum[0]);
+                sum[1] = fmaf(s[k][i] * w[k][i], to_f32(rg[k].v[i]), sum[1]);
             }
         }
         team_sum<TEAM, 2>(sum, s_sum);
@@ -311,9 +325,9 @@ __global__ void __launch_bounds__(TeamShape<TEAM>::THREADS) norm_backward(const 
             float gx[N];
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const float s = to_f32(rx[k].v[i]), g = to_f32(rg[k].v[i]);
-                gx[i] = r * fmaf(-s, mean, g * w[k][i]);
-                gw[k][i] = fmaf(g, s * r, gw[k][i]);
+                const float g = to_f32(rg[k].v[i]);
+                gx[i] = r * fmaf(-s[k][i], mean, g * w[k][i]);
+                gw[k][i] = fmaf(g, s[k][i] * r, gw[k][i]);
             }
             if (more) {
 #pragma unroll
@@ -473,7 +487,8 @@ extern "C" int ovl_rms_norm_backward(const OvlRmsNorm* a, void* cuda_stream) {
     ovl::NormParams p{};
     p.a = *a;
     p.part = reinterpret_cast<float*>(a->workspace);
-    p.vec = a->columns % 8 == 0 && ovl::aligned16(a->x) && a->x_row % 8 == 0 && ovl::aligned16(a->gy) && a->gy_row % 8 == 0 &&
+    p.vec = a->columns % 8 == 0 && ovl::aligned16(a->x) && a->x_row % 8 == 0 && ovl::aligned16(a->residual) &&
+            (!a->residual || a->residual_row % 8 == 0) && ovl::aligned16(a->gy) && a->gy_row % 8 == 0 &&
             ovl::aligned16(a->gresidual_out) && (!a->gresidual_out || a->gresidual_out_row % 8 == 0) && ovl::aligned16(a->gx) &&
             ovl::aligned16(a->weight);
     const cudaStream_t stream = (cudaStream_t)cuda_stream;

@@ -495,7 +495,7 @@ def _norm_forward(x, weight, residual, eps):
     return y, residual_out
 
 
-def _norm_backward(x, weight, eps, gy, gres):
+def _norm_backward(x, weight, residual, eps, gy, gres):
     torch = _torch_module
     device = x.device
     if gy is None:
@@ -507,7 +507,8 @@ def _norm_backward(x, weight, eps, gy, gres):
     gweight = torch.empty(weight.shape, dtype=weight.dtype, device=device)
     size = _with_device(device, launcher.library().ovl_rms_norm_workspace_bytes, _norm_args(x, weight, eps))
     _launch('ovl_rms_norm_backward',
-            _norm_args(x, weight, eps, gy=gy, gres=gres, gx=gx, gweight=gweight, workspace=_workspace(size, device)), device)
+            _norm_args(x, weight, eps, residual=residual, gy=gy, gres=gres, gx=gx, gweight=gweight,
+                       workspace=_workspace(size, device)), device)
     return gx, gweight
 
 
@@ -518,8 +519,7 @@ def rms_norm(x, weight, residual=None, eps=1e-6):
 
     ``x``, ``residual``: [..., columns] of one type, 1 to 32768 columns; ``weight``: [columns], in that type or float32.
     Returns ``y``, with a ``residual`` the pair ``(y, s)``: ``s`` rounded to the type of ``x`` is the residual of the next
-    block (the norm itself uses the unrounded sum).  Differentiable with respect to all three; the backward pass starts
-    from ``s`` as it was rounded."""
+    block (the norm itself, and its gradient, use the unrounded sum).  Differentiable with respect to all three."""
     x, weight, residual, eps, _ = _norm_check(x, weight, residual, eps, 'rms_norm')
     if _differentiable(x, weight, residual):
         y, residual_out = _autograd().norm.apply(x, weight, residual, eps)
@@ -613,8 +613,7 @@ def _autograd():
             y = y.view(x.shape)
             residual_out = None if residual_out is None else residual_out.view(x.shape)
             ctx.eps = eps
-            # the backward pass starts from the sum; without a residual that is x itself
-            ctx.save_for_backward(x if residual_out is None else residual_out, weight)
+            ctx.save_for_backward(x, weight, residual)
             ctx.set_materialize_grads(False)
             return y, residual_out
 
@@ -623,10 +622,10 @@ def _autograd():
         def backward(ctx, gy, gres):
             if gy is None and gres is None:
                 return None, None, None, None
-            s, weight = ctx.saved_tensors
-            gx, gweight = _norm_backward(_rows(s), weight, ctx.eps, None if gy is None else _rows(gy),
-                                         None if gres is None else _rows(gres))
-            gx = gx.view(s.shape)
+            x, weight, residual = ctx.saved_tensors
+            gx, gweight = _norm_backward(_rows(x), weight, None if residual is None else _rows(residual), ctx.eps,
+                                         None if gy is None else _rows(gy), None if gres is None else _rows(gres))
+            gx = gx.view(x.shape)
             return gx, gweight, gx if ctx.needs_input_grad[2] else None, None
 
     _functions = types.SimpleNamespace(scan=SelectiveScan, conv=CausalConv, norm=RmsNorm)
