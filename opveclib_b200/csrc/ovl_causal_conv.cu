@@ -18,7 +18,7 @@ struct ConvParams {
     OvlCausalConv a;
     int64_t column_tiles, strips;      // tiles of 32 x (channels of a thread) channels, blocks of kWarps strips
     int64_t strip;                     // tokens of a thread
-    int32_t vec;
+    int32_t vec, width;                // wide loads and stores; else copies of `width` elements
     float* part;                       // backward: [batch * strips, taps + 1, channels]
 };
 
@@ -109,7 +109,7 @@ __device__ __forceinline__ void widen_slot(F2 (&x)[N / 2], const T* slot) {
 }
 
 // TAPS: the number of taps, or 8 for any number up to 8 (`taps` says which)
-template <typename T, int TAPS>
+template <typename T, int TAPS, bool FULL>
 __global__ void __launch_bounds__(32 * kWarps, TAPS == kMaxTaps ? 1 : 4) conv_forward(const __grid_constant__ ConvParams p) {
     constexpr int N = 8, CHUNK = kChunk;
     extern __shared__ __align__(16) char smem[];
@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(32 * kWarps, TAPS == kMaxTaps ? 1 : 4) conv_fo
     const int64_t channel = column * N;
     if (channel >= a.channels) return;
     const int valid = a.channels - channel < N ? (int)(a.channels - channel) : N;
-    const bool vec = p.vec && valid == N;
+    const bool vec = FULL;                                               // then valid is N or 0
     const int64_t used = used_length(a.lengths, batch, a.length);
     const int64_t t_begin = strip * p.strip, t_end = t_begin + p.strip < a.length ? t_begin + p.strip : a.length;
     const int64_t t_used = used < t_end ? used : t_end;
@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(32 * kWarps, TAPS == kMaxTaps ? 1 : 4) conv_fo
             const Pack<T, N> raw = load_token<T, N>(a, batch, t, used, channel, vec, valid);
 #pragma unroll
             for (int c = 0; c < N; ++c) x[c] = to_f32(raw.v[c]);
-            store_pack<T, N>(reinterpret_cast<T*>(a.final_state) + (batch * (taps - 1) + k) * a.channels + channel, x, vec, valid);
+            store_pack<T, N>(reinterpret_cast<T*>(a.final_state) + (batch * (taps - 1) + k) * a.channels + channel, x, vec, valid, p.width);
         }
     }
     if (t_begin >= t_end) return;
@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(32 * kWarps, TAPS == kMaxTaps ? 1 : 4) conv_fo
     auto fetch = [&](int64_t t0, int chunk) {
 #pragma unroll
         for (int s = 0; s < CHUNK; ++s)
-            if (t0 + s < t_used) fetch_pack<T, N>(ring.slot(chunk, s), x + (t0 + s) * a.x_token, vec, valid);
+            if (t0 + s < t_used) fetch_pack<T, N>(ring.slot(chunk, s), x + (t0 + s) * a.x_token, vec, valid, p.width);
         copy_commit();
     };
 #pragma unroll
@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(32 * kWarps, TAPS == kMaxTaps ? 1 : 4) conv_fo
 #pragma unroll
             for (int c = 0; c < N; ++c) y[c] = 0.0f;
         }
-        if (INSIDE || t < t_end) store_pack<T, N>(out + t * a.channels, y, vec, valid);
+        if (INSIDE || t < t_end) store_pack<T, N>(out + t * a.channels, y, vec, valid, p.width);
 #pragma unroll
         for (int k = 0; k < TAPS - 1; ++k)
 #pragma unroll
@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(32 * kWarps, TAPS == kMaxTaps ? 1 : 4) conv_fo
 // gx_t = sum_k w[k] gpre_{t + (taps - 1) - k} with gpre = gout act'(pre): the walk runs taps - 1 tokens past the strip
 // (gx of the strip needs them).  The first strip also has the gradient of the initial state, gx of the tokens
 // -(taps - 1) ... -1.
-template <typename T, int TAPS>
+template <typename T, int TAPS, bool FULL>
 __global__ void __launch_bounds__(32 * kWarps, TAPS == kMaxTaps ? 1 : 4) conv_backward(const __grid_constant__ ConvParams p) {
     constexpr int N = 4, CHUNK = kChunk;
     extern __shared__ __align__(16) char smem[];
@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(32 * kWarps, TAPS == kMaxTaps ? 1 : 4) conv_ba
     const int64_t channel = column * N;
     const bool live = channel < a.channels;
     const int valid = !live ? 0 : a.channels - channel < N ? (int)(a.channels - channel) : N;
-    const bool vec = p.vec && valid == N;
+    const bool vec = FULL;                                               // then valid is N or 0
     const int64_t used = used_length(a.lengths, batch, a.length);
     const int64_t t_begin = strip * p.strip, t_end = t_begin + p.strip < a.length ? t_begin + p.strip : a.length;
 
@@ -239,8 +239,8 @@ __global__ void __launch_bounds__(32 * kWarps, TAPS == kMaxTaps ? 1 : 4) conv_ba
             for (int s = 0; s < CHUNK; ++s) {
                 const int64_t t = t0 + s;
                 if (t < walk_used) {
-                    fetch_pack<T, N>(ring_x.slot(chunk, s), x + t * a.x_token, vec, valid);
-                    fetch_pack<T, N>(ring_g.slot(chunk, s), gout + t * a.gout_token, vec, valid);
+                    fetch_pack<T, N>(ring_x.slot(chunk, s), x + t * a.x_token, vec, valid, p.width);
+                    fetch_pack<T, N>(ring_g.slot(chunk, s), gout + t * a.gout_token, vec, valid, p.width);
                 }
             }
             copy_commit();
@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(32 * kWarps, TAPS == kMaxTaps ? 1 : 4) conv_ba
                 }
                 T* const dst = state ? reinterpret_cast<T*>(a.ginitial) + (batch * (taps - 1) + (taps - 1) + to) * a.channels
                                      : reinterpret_cast<T*>(a.gx) + (batch * a.length + to) * a.channels;
-                store_pack<T, N>(dst + channel, gx, vec, valid);
+                store_pack<T, N>(dst + channel, gx, vec, valid, p.width);
             }
 #pragma unroll
             for (int k = 0; k < TAPS - 1; ++k)
@@ -480,8 +480,10 @@ bool wide(const OvlCausalConv* a, int n, bool backward) {
            aligned16(a->gx) && aligned16(a->ginitial);
 }
 
+// `full`: whole packs of channels on 16-byte boundaries (the kernel has no other path then), else `any`
 template <typename F>
-int launch(F kernel, const ConvParams& p, size_t smem, cudaStream_t stream) {
+int launch(const ConvParams& p, size_t smem, cudaStream_t stream, F full, F any) {
+    F kernel = p.vec ? full : any;
     const int64_t blocks = p.column_tiles * p.strips * p.a.batch;
     if (blocks > 0x7fffffff) return OVL_ERR_TOO_LARGE;
     if (smem > 24 * 1024) {                                              // (the backward kernels have up to 18 KB beside it)
@@ -496,12 +498,13 @@ template <typename T>
 int run_forward(ConvParams p, cudaStream_t stream) {
     cut(&p.a, 8, &p);
     p.vec = wide(&p.a, 8, false);
+    p.width = copy_width<T>({p.a.x, p.a.out, p.a.initial_state, p.a.final_state}, {p.a.channels, p.a.x_batch, p.a.x_token});
     constexpr size_t smem = Ring<T, 8>::bytes;
     switch (p.a.taps) {
-        case 2: return launch(conv_forward<T, 2>, p, smem, stream);
-        case 3: return launch(conv_forward<T, 3>, p, smem, stream);
-        case 4: return launch(conv_forward<T, 4>, p, smem, stream);
-        default: return launch(conv_forward<T, kMaxTaps>, p, smem, stream);
+        case 2: return launch(p, smem, stream, conv_forward<T, 2, true>, conv_forward<T, 2, false>);
+        case 3: return launch(p, smem, stream, conv_forward<T, 3, true>, conv_forward<T, 3, false>);
+        case 4: return launch(p, smem, stream, conv_forward<T, 4, true>, conv_forward<T, 4, false>);
+        default: return launch(p, smem, stream, conv_forward<T, kMaxTaps, true>, conv_forward<T, kMaxTaps, false>);
     }
 }
 
@@ -509,14 +512,16 @@ template <typename T>
 int run_backward(ConvParams p, cudaStream_t stream) {
     cut(&p.a, 4, &p);
     p.vec = wide(&p.a, 4, true);
+    p.width = copy_width<T>({p.a.x, p.a.gout, p.a.gx, p.a.initial_state, p.a.gfinal, p.a.ginitial},
+                            {p.a.channels, p.a.x_batch, p.a.x_token, p.a.gout_batch, p.a.gout_token});
     p.part = reinterpret_cast<float*>(p.a.workspace);
     constexpr size_t smem = 2 * Ring<T, 4>::bytes;
     int st;
     switch (p.a.taps) {
-        case 2: st = launch(conv_backward<T, 2>, p, smem, stream); break;
-        case 3: st = launch(conv_backward<T, 3>, p, smem, stream); break;
-        case 4: st = launch(conv_backward<T, 4>, p, smem, stream); break;
-        default: st = launch(conv_backward<T, kMaxTaps>, p, smem, stream); break;
+        case 2: st = launch(p, smem, stream, conv_backward<T, 2, true>, conv_backward<T, 2, false>); break;
+        case 3: st = launch(p, smem, stream, conv_backward<T, 3, true>, conv_backward<T, 3, false>); break;
+        case 4: st = launch(p, smem, stream, conv_backward<T, 4, true>, conv_backward<T, 4, false>); break;
+        default: st = launch(p, smem, stream, conv_backward<T, kMaxTaps, true>, conv_backward<T, kMaxTaps, false>); break;
     }
     if (st != OVL_OK) return st;
     conv_backward_params<T><<<(uint32_t)ceil_div((p.a.taps + 1) * p.a.channels, 32), 256, 0, stream>>>(p);

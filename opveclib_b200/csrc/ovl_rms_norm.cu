@@ -244,14 +244,23 @@ __global__ void __launch_bounds__(TeamShape<TEAM>::THREADS) norm_forward(const _
 }
 
 // With g = gy w and xhat = s r: gx = r (g - xhat mean(g xhat)) + gresidual_out; gweight = sum over the rows of gy xhat.
-// Every team walks over rows with its sums for gweight in registers, the next row's elements on their way.
+// Every team walks over rows with its sums for gweight in registers; as long as shared memory lasts the next row is copied
+// there meanwhile, each thread what it will need itself.
+template <typename T, int TEAM, int K>
+struct BackRows {
+    static constexpr size_t stage = sizeof(T) * 4 * K * TeamShape<TEAM>::THREADS * 8;        // x, residual, gy, gresidual_out
+    static constexpr bool AHEAD = 2 * stage <= 128 * 1024;
+    static constexpr size_t bytes = AHEAD ? 2 * stage : 0;
+};
+
 template <typename T, int TEAM, int K, bool VEC>
 __global__ void __launch_bounds__(TeamShape<TEAM>::THREADS) norm_backward(const __grid_constant__ NormParams p) {
     using S = TeamShape<TEAM>;
     constexpr int N = 8;
-    constexpr bool AHEAD = K * sizeof(T) <= 8;                           // as long as the registers last
+    constexpr bool AHEAD = BackRows<T, TEAM, K>::AHEAD;
     __shared__ float s_sum[2][32];
     __shared__ float s_w[TEAM == 32 ? S::TEAMS : 1][TEAM == 32 ? TEAM * K * N : 1];
+    extern __shared__ __align__(16) char smem[];
     const OvlRmsNorm& a = p.a;
     const int team = threadIdx.x / TEAM, me = threadIdx.x % TEAM;
     const int columns = (int)a.columns;
@@ -264,77 +273,90 @@ __global__ void __launch_bounds__(TeamShape<TEAM>::THREADS) norm_backward(const 
         for (int i = 0; i < N; ++i) gw[k][i] = 0.0f;
     }
     const int64_t first = (int64_t)blockIdx.x * S::TEAMS + team, step = (int64_t)gridDim.x * S::TEAMS;
-    const bool more = a.gresidual_out != nullptr;
-    const bool sum_of_two = a.residual != nullptr;
-    Pack<T, N> next_x[K], next_s[K], next_g[K], next_r[K];
-    auto fetch = [&](int64_t row) {
-        const T* const x = reinterpret_cast<const T*>(a.x) + row * a.x_row;
-        const T* const res = reinterpret_cast<const T*>(a.residual) + row * a.residual_row;
-        const T* const gy = reinterpret_cast<const T*>(a.gy) + row * a.gy_row;
-        const T* const gr = reinterpret_cast<const T*>(a.gresidual_out) + row * a.gresidual_out_row;
+    const bool more = a.gresidual_out != nullptr, sum_of_two = a.residual != nullptr;
+    auto row_of = [&](int which, int64_t row) {
+        return which == 0   ? reinterpret_cast<const T*>(a.x) + row * a.x_row
+               : which == 1 ? reinterpret_cast<const T*>(a.residual) + row * a.residual_row
+               : which == 2 ? reinterpret_cast<const T*>(a.gy) + row * a.gy_row
+                            : reinterpret_cast<const T*>(a.gresidual_out) + row * a.gresidual_out_row;
+    };
+    auto slot_of = [&](int stage, int which, int k) {
+        return reinterpret_cast<T*>(smem) + (((stage * 4 + which) * K + k) * S::THREADS + threadIdx.x) * 8;
+    };
+    auto fetch = [&](int64_t row, int stage) {
+        if (row < a.rows) {
+#pragma unroll
+            for (int which = 0; which < 4; ++which) {
+                if ((which == 1 && !sum_of_two) || (which == 3 && !more)) continue;
+                const T* const from = row_of(which, row);
+#pragma unroll
+                for (int k = 0; k < K; ++k)
+                    if (cols.in(k)) fetch_pack<T, N>(slot_of(stage, which, k), from + cols.at(k), VEC, cols.valid(k), 0);
+            }
+        }
+        copy_commit();
+    };
+    auto read = [&](float (&x)[K][N], int which, int64_t row, int stage) {
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            next_x[k] = cols.load(x, k);
-            next_g[k] = cols.load(gy, k);
-        }
-        if (more) {
+            if (AHEAD) {
+                read_slot<T, N>(slot_of(stage, which, k), x[k]);
+            } else {
+                const Pack<T, N> raw = cols.load(row_of(which, row), k);
 #pragma unroll
-            for (int k = 0; k < K; ++k) next_r[k] = cols.load(gr, k);
-        }
-        if (sum_of_two) {
+                for (int i = 0; i < N; ++i) x[k][i] = to_f32(raw.v[i]);
+            }
+            if (!cols.in(k)) {
 #pragma unroll
-            for (int k = 0; k < K; ++k) next_s[k] = cols.load(res, k);
+                for (int i = 0; i < N; ++i) x[k][i] = 0.0f;
+            }
         }
     };
-    if (AHEAD && first < a.rows) fetch(first);
-    for (int64_t row = first; row < a.rows; row += step) {
-        if (!AHEAD) fetch(row);
-        // the sum in 32 bits, as the forward pass had it (its rounded copy would put another rounding on gweight)
-        float s[K][N];
-        Pack<T, N> rg[K], rr[K];
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) s[k][i] = to_f32(next_x[k].v[i]);
-            rg[k] = next_g[k];
-            if (more) rr[k] = next_r[k];
+    int stage = 0;
+    if (AHEAD) fetch(first, 0);
+    for (int64_t row = first; row < a.rows; row += step, stage ^= 1) {
+        if (AHEAD) {
+            fetch(row + step, stage ^ 1);
+            copy_wait<1>();
         }
+        // the sum in 32 bits, as the forward pass had it (its rounded copy would put another rounding on gweight)
+        float s[K][N], g[K][N];
+        read(s, 0, row, stage);
         if (sum_of_two) {
+            read(g, 1, row, stage);
 #pragma unroll
             for (int k = 0; k < K; ++k)
 #pragma unroll
-                for (int i = 0; i < N; ++i) s[k][i] += to_f32(next_s[k].v[i]);
+                for (int i = 0; i < N; ++i) s[k][i] += g[k][i];
         }
-        // (behind the last row the last one is read again, so that no load waits for a condition)
-        if (AHEAD) fetch(row + step < a.rows ? row + step : a.rows - 1);
+        read(g, 2, row, stage);
         float sum[2] = {0.0f, 0.0f};
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            if (VEC && !cols.in(k)) continue;
+        for (int k = 0; k < K; ++k)
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 sum[0] = fmaf(s[k][i], s[k][i], sum[0]);
-                sum[1] = fmaf(s[k][i] * w[k][i], to_f32(rg[k].v[i]), sum[1]);
+                sum[1] = fmaf(s[k][i] * w[k][i], g[k][i], sum[1]);
             }
-        }
         team_sum<TEAM, 2>(sum, s_sum);
         const float r = rsqrtf(sum[0] / (float)columns + (float)a.eps);
         const float mean = r * r * (sum[1] / (float)columns);            // xhat mean(g xhat) = s mean, apart from a factor r
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            float gx[N];
+        for (int k = 0; k < K; ++k)
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const float g = to_f32(rg[k].v[i]);
-                gx[i] = r * fmaf(-s[k][i], mean, g * w[k][i]);
-                gw[k][i] = fmaf(g, s[k][i] * r, gw[k][i]);
+                gw[k][i] = fmaf(g[k][i], s[k][i] * r, gw[k][i]);
+                s[k][i] = r * fmaf(-s[k][i], mean, g[k][i] * w[k][i]);
             }
-            if (more) {
+        if (more) {
+            read(g, 3, row, stage);
 #pragma unroll
-                for (int i = 0; i < N; ++i) gx[i] += to_f32(rr[k].v[i]);
-            }
-            cols.store(reinterpret_cast<T*>(a.gx) + row * a.columns, k, gx);
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int i = 0; i < N; ++i) s[k][i] += g[k][i];
         }
+#pragma unroll
+        for (int k = 0; k < K; ++k) cols.store(reinterpret_cast<T*>(a.gx) + row * a.columns, k, s[k]);
     }
     float* const part = p.part + (int64_t)blockIdx.x * columns;
     if constexpr (TEAM == 32) {
@@ -408,7 +430,13 @@ template <typename T, int TEAM, int K, bool VEC>
 int launch_as(const NormParams& p, bool backward, cudaStream_t stream) {
     using S = TeamShape<TEAM>;
     if (backward) {
-        norm_backward<T, TEAM, K, VEC><<<(uint32_t)backward_blocks(&p.a), S::THREADS, 0, stream>>>(p);
+        constexpr size_t smem = BackRows<T, TEAM, K>::bytes;
+        if (smem > 24 * 1024) {                                          // (up to 17 KB beside it)
+            const cudaError_t e =
+                cudaFuncSetAttribute(norm_backward<T, TEAM, K, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+            if (e != cudaSuccess) return record_cuda_error(e);
+        }
+        norm_backward<T, TEAM, K, VEC><<<(uint32_t)backward_blocks(&p.a), S::THREADS, smem, stream>>>(p);
         return launch_status();
     }
     const int64_t blocks = ceil_div(p.a.rows, S::TEAMS);

@@ -126,6 +126,14 @@ int run(const OvlSelectiveScan* a, bool backward, cudaStream_t stream) {
                  multiple_of(4, a->C_batch, a->C_token) && a->B_group % 4 == 0 && a->C_group % 4 == 0;
     p.d.vec_states = a->states % 4 == 0 && aligned16(a->A) && aligned16(a->initial_state) && aligned16(a->final_state) &&
                      aligned16(a->checkpoints) && aligned16(a->gfinal) && aligned16(a->ginitial);
+    auto width = [&](auto one) {
+        using T = decltype(one);
+        const bool b = backward;
+        return copy_width<T>({a->u, a->delta, a->z, b ? a->gout : nullptr, b ? a->gu : a->out, b ? a->gdelta : nullptr, b ? a->gz : nullptr},
+                             {p.d.group_channels, a->u_batch, a->u_token, a->delta_batch, a->delta_token, a->z ? a->z_batch : 0,
+                              a->z ? a->z_token : 0, b ? a->gout_batch : 0, b ? a->gout_token : 0});
+    };
+    p.d.width = a->dtype == OVL_FLOAT32 ? width(float()) : width(__half());
     if (a->dtype == OVL_FLOAT32) return scan_run_f32(p, shape, backward, stream);
     if (a->dtype == OVL_FLOAT16) return scan_run_f16(p, shape, backward, stream);
     return scan_run_bf16(p, shape, backward, stream);

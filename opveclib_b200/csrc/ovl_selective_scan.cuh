@@ -27,7 +27,7 @@ struct ScanDims {
     int64_t segments, segment_length;  // the length cut into segments (a multiple of 32) that run side by side
     int64_t first_segment, launch_segments;   // those of this launch
     int32_t ahead;                     // the first of two launches, see below
-    int32_t softplus, vec;             // vec: wide loads and stores of channel vectors
+    int32_t softplus, vec, width;      // vec: wide loads and stores of channel vectors; else copies of `width` elements
     int32_t vec_states, vec_bc;        // wide loads and stores of 4 states; of 4 elements of B and C
 };
 
@@ -298,7 +298,7 @@ __device__ __forceinline__ void scan_forward_scan(const ScanParams& p, const Pla
 
 // The helping threads, one tile ahead of the scan and one behind it: they fetch u, delta, z, B and C (AHEAD tiles ahead,
 // each thread what it will need itself), leave dt, dt u, B and C for the scan, and finish the outputs from its sums.
-template <typename T, int P, int M, bool LOCAL>
+template <typename T, int P, int M, bool LOCAL, bool FULL>
 __device__ __forceinline__ void scan_forward_help(const ScanParams& p, const Place& at, char* smem, int64_t t_begin, int64_t t_end,
                                                   int64_t t_used) {
     using S = ForwardShape<P, M>;
@@ -322,7 +322,7 @@ __device__ __forceinline__ void scan_forward_help(const ScanParams& p, const Pla
     constexpr int ITEM_STEP = S::HELP / (CH / 8);                        // tokens between two parts of a thread
     const bool has_item = tid < S::ITEMS;
     const int valid = !has_item || item_c >= at.n_channels ? 0 : at.n_channels - item_c < 8 ? (int)(at.n_channels - item_c) : 8;
-    const bool vec = d.vec && valid == 8;
+    const bool vec = FULL;                                               // then valid is 8 or 0
     float skip[8], bias[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -342,9 +342,9 @@ __device__ __forceinline__ void scan_forward_help(const ScanParams& p, const Pla
             for (int k = 0; k < IPT; ++k) {
                 const int64_t t = t0 + item_t + k * ITEM_STEP;
                 if (valid > 0 && t < t_used) {
-                    fetch_pack<T, 8>(slot_of(slot, 0, k), u + t * a.u_token + item_c, vec, valid);
-                    fetch_pack<T, 8>(slot_of(slot, 1, k), delta + t * a.delta_token + item_c, vec, valid);
-                    if (!LOCAL && z) fetch_pack<T, 8>(slot_of(slot, 2, k), z + t * a.z_token + item_c, vec, valid);
+                    fetch_pack<T, 8>(slot_of(slot, 0, k), u + t * a.u_token + item_c, vec, valid, d.width);
+                    fetch_pack<T, 8>(slot_of(slot, 1, k), delta + t * a.delta_token + item_c, vec, valid, d.width);
+                    if (!LOCAL && z) fetch_pack<T, 8>(slot_of(slot, 2, k), z + t * a.z_token + item_c, vec, valid, d.width);
                 }
             }
 #pragma unroll
@@ -352,9 +352,9 @@ __device__ __forceinline__ void scan_forward_help(const ScanParams& p, const Pla
                 const int e = tid + k * S::HELP, n = e % P * 4;
                 const int64_t t = t0 + e / P;
                 if (e < S::QUADS && t < t_used && n < states) {
-                    const bool wide = d.vec_bc && n + 4 <= states;
-                    fetch_pack<T, 4>(quad_of(bc_slot, 0, e), B + t * a.B_token + n, wide, states - n);
-                    if (!LOCAL) fetch_pack<T, 4>(quad_of(bc_slot, 1, e), C + t * a.C_token + n, wide, states - n);
+                    const bool wide = FULL || (d.vec_bc && n + 4 <= states);
+                    fetch_pack<T, 4>(quad_of(bc_slot, 0, e), B + t * a.B_token + n, wide, states - n, 0);
+                    if (!LOCAL) fetch_pack<T, 4>(quad_of(bc_slot, 1, e), C + t * a.C_token + n, wide, states - n, 0);
                 }
             }
         }
@@ -421,7 +421,7 @@ __device__ __forceinline__ void scan_forward_help(const ScanParams& p, const Pla
                     for (int i = 0; i < 8; ++i) o[i] *= silu(g[i]);
                 }
             }
-            store_pack<T, 8>(out + t * d.channels + item_c, o, vec, valid);
+            store_pack<T, 8>(out + t * d.channels + item_c, o, vec, valid, d.width);
         }
     };
 
@@ -453,14 +453,14 @@ __device__ __forceinline__ void scan_forward_help(const ScanParams& p, const Pla
         const float zero[8] = {};
         constexpr int TOKENS = S::ITEMS < S::HELP ? STEPS : ITEM_STEP;   // that the threads cover together
         for (int64_t t = covered + item_t; t < t_end; t += TOKENS)
-            store_pack<T, 8>(out + t * d.channels + item_c, zero, vec, valid);
+            store_pack<T, 8>(out + t * d.channels + item_c, zero, vec, valid, d.width);
     }
 }
 
 // A length that is cut into segments takes two launches: the first does the first segment and finds out what each of
 // those between the first and the last adds to the state (LOCAL: the end of a state that starts at zero, and the sum of
 // dt); the second does the other segments, seeded from the segments before.
-template <typename T, int P, int M, bool LOCAL>
+template <typename T, int P, int M, bool LOCAL, bool FULL>
 __device__ __forceinline__ void scan_forward_block(const ScanParams& p, const Place& at, char* smem) {
     const ScanDims& d = p.d;
     const int64_t used = used_length(p.a.lengths, at.batch, d.length);
@@ -468,15 +468,15 @@ __device__ __forceinline__ void scan_forward_block(const ScanParams& p, const Pl
     const int64_t t_end = t_begin + d.segment_length < d.length ? t_begin + d.segment_length : d.length;
     const int64_t t_used = used < t_end ? used : t_end;                  // tokens of the segment that count
     if (threadIdx.x < ForwardShape<P, M>::SCAN) scan_forward_scan<T, P, M, LOCAL>(p, at, smem, t_begin, t_used);
-    else scan_forward_help<T, P, M, LOCAL>(p, at, smem, t_begin, t_end, t_used);
+    else scan_forward_help<T, P, M, LOCAL, FULL>(p, at, smem, t_begin, t_end, t_used);
 }
 
-template <typename T, int P, int M>
+template <typename T, int P, int M, bool FULL>
 __global__ void __launch_bounds__(ForwardShape<P, M>::THREADS, 2) scan_forward(const __grid_constant__ ScanParams p) {
     extern __shared__ __align__(16) char smem[];
     const Place at = block_place(p.d, ForwardShape<P, M>::CH);
-    if (p.d.ahead && at.segment > 0) scan_forward_block<T, P, M, true>(p, at, smem);
-    else scan_forward_block<T, P, M, false>(p, at, smem);
+    if (p.d.ahead && at.segment > 0) scan_forward_block<T, P, M, true, FULL>(p, at, smem);
+    else scan_forward_block<T, P, M, false, FULL>(p, at, smem);
 }
 
 // ---------------------------------------------------------------------------------------------------------
@@ -745,7 +745,7 @@ __device__ __forceinline__ void scan_backward_scan(const ScanParams& p, const Pl
     }
 }
 
-template <typename T, int P, int K, int M, bool LOCAL>
+template <typename T, int P, int K, int M, bool LOCAL, bool FULL>
 __device__ __forceinline__ void scan_backward_help(const ScanParams& p, const Place& at, char* smem, int64_t t_begin, int64_t t_end,
                                                    int64_t t_used) {
     using S = BackShape<P, K, M>;
@@ -773,7 +773,7 @@ __device__ __forceinline__ void scan_backward_help(const ScanParams& p, const Pl
     const bool has_item = tid < ITEMS;
     const int item_t = tid / S::CHV, cc = tid % S::CHV * 4;
     const int valid = !has_item || cc >= at.n_channels ? 0 : at.n_channels - cc < 4 ? (int)(at.n_channels - cc) : 4;
-    const bool vec = d.vec && valid == 4;
+    const bool vec = FULL;                                               // then valid is 4 or 0
     float bias[4], skip[4], gD[4] = {}, gbias[4] = {};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -792,10 +792,10 @@ __device__ __forceinline__ void scan_backward_help(const ScanParams& p, const Pl
             for (int k = 0; k < IPT; ++k) {
                 const int64_t t = t0 + item_t + k * ITEM_STEP;
                 if (valid > 0 && t < t_used) {
-                    if (!LOCAL) fetch_pack<T, 4>(slot_of(slot, 0, k), u + t * a.u_token + cc, vec, valid);
-                    fetch_pack<T, 4>(slot_of(slot, 1, k), delta + t * a.delta_token + cc, vec, valid);
-                    if (z) fetch_pack<T, 4>(slot_of(slot, 2, k), z + t * a.z_token + cc, vec, valid);
-                    fetch_pack<T, 4>(slot_of(slot, 3, k), gout + t * a.gout_token + cc, vec, valid);
+                    if (!LOCAL) fetch_pack<T, 4>(slot_of(slot, 0, k), u + t * a.u_token + cc, vec, valid, d.width);
+                    fetch_pack<T, 4>(slot_of(slot, 1, k), delta + t * a.delta_token + cc, vec, valid, d.width);
+                    if (z) fetch_pack<T, 4>(slot_of(slot, 2, k), z + t * a.z_token + cc, vec, valid, d.width);
+                    fetch_pack<T, 4>(slot_of(slot, 3, k), gout + t * a.gout_token + cc, vec, valid, d.width);
                 }
             }
 #pragma unroll
@@ -803,9 +803,9 @@ __device__ __forceinline__ void scan_backward_help(const ScanParams& p, const Pl
                 const int e = tid + k * S::HELP, n = e % (NP / 4) * 4;
                 const int64_t t = t0 + e / (NP / 4);
                 if (e < S::QUADS && t < t_used && n < states) {
-                    const bool wide = d.vec_bc && n + 4 <= states;
-                    if (!LOCAL) fetch_pack<T, 4>(quad_of(bc_slot, 0, e), B + t * a.B_token + n, wide, states - n);
-                    fetch_pack<T, 4>(quad_of(bc_slot, 1, e), C + t * a.C_token + n, wide, states - n);
+                    const bool wide = FULL || (d.vec_bc && n + 4 <= states);
+                    if (!LOCAL) fetch_pack<T, 4>(quad_of(bc_slot, 0, e), B + t * a.B_token + n, wide, states - n, 0);
+                    fetch_pack<T, 4>(quad_of(bc_slot, 1, e), C + t * a.C_token + n, wide, states - n, 0);
                 }
             }
         }
@@ -908,9 +908,9 @@ __device__ __forceinline__ void scan_backward_help(const ScanParams& p, const Pl
                 }
             }
             const int64_t o = (at.batch * d.length + t) * d.channels + base_c + cc;
-            store_pack<T, 4>(reinterpret_cast<T*>(a.gu) + o, gu, vec, valid);
-            store_pack<T, 4>(reinterpret_cast<T*>(a.gdelta) + o, gd, vec, valid);
-            if (a.gz) store_pack<T, 4>(reinterpret_cast<T*>(a.gz) + o, gz, vec, valid);
+            store_pack<T, 4>(reinterpret_cast<T*>(a.gu) + o, gu, vec, valid, d.width);
+            store_pack<T, 4>(reinterpret_cast<T*>(a.gdelta) + o, gd, vec, valid, d.width);
+            if (a.gz) store_pack<T, 4>(reinterpret_cast<T*>(a.gz) + o, gz, vec, valid, d.width);
         }
         float4* const part = reinterpret_cast<float4*>(
             p.part_bc + (((at.batch * d.groups + at.group) * d.tiles + at.tile) * d.length + t0) * 2 * NP);
@@ -952,9 +952,9 @@ __device__ __forceinline__ void scan_backward_help(const ScanParams& p, const Pl
             const int64_t t = t0 + item_t + k * ITEM_STEP;
             if (valid > 0 && t < t_end) {
                 const int64_t o = (at.batch * d.length + t) * d.channels + base_c + cc;
-                store_pack<T, 4>(reinterpret_cast<T*>(a.gu) + o, zero, vec, valid);
-                store_pack<T, 4>(reinterpret_cast<T*>(a.gdelta) + o, zero, vec, valid);
-                if (a.gz) store_pack<T, 4>(reinterpret_cast<T*>(a.gz) + o, zero, vec, valid);
+                store_pack<T, 4>(reinterpret_cast<T*>(a.gu) + o, zero, vec, valid, d.width);
+                store_pack<T, 4>(reinterpret_cast<T*>(a.gdelta) + o, zero, vec, valid, d.width);
+                if (a.gz) store_pack<T, 4>(reinterpret_cast<T*>(a.gz) + o, zero, vec, valid, d.width);
             }
         }
     }
@@ -981,7 +981,7 @@ __device__ __forceinline__ void scan_backward_help(const ScanParams& p, const Pl
     }
 }
 
-template <typename T, int P, int K, int M, bool LOCAL>
+template <typename T, int P, int K, int M, bool LOCAL, bool FULL>
 __device__ __forceinline__ void scan_backward_block(const ScanParams& p, const Place& at, char* smem) {
     using S = BackShape<P, K, M>;
     const ScanDims& d = p.d;
@@ -994,41 +994,53 @@ __device__ __forceinline__ void scan_backward_block(const ScanParams& p, const P
         scan_backward_scan<T, P, K, M, LOCAL>(p, at, smem, t_begin, t_used);
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::HELP_REGISTERS));
-        scan_backward_help<T, P, K, M, LOCAL>(p, at, smem, t_begin, t_end, t_used);
+        scan_backward_help<T, P, K, M, LOCAL, FULL>(p, at, smem, t_begin, t_end, t_used);
     }
 }
 
 // the segments from last to first, in two launches like the forward ones
-template <typename T, int P, int K, int M>
+template <typename T, int P, int K, int M, bool FULL>
 __global__ void __launch_bounds__(BackShape<P, K, M>::THREADS, 2) scan_backward(const __grid_constant__ ScanParams p) {
     extern __shared__ __align__(16) char smem[];
     const Place at = block_place(p.d, BackShape<P, K, M>::CH);
-    if (p.d.ahead && at.segment < p.d.segments - 1) scan_backward_block<T, P, K, M, true>(p, at, smem);
-    else scan_backward_block<T, P, K, M, false>(p, at, smem);
+    if (p.d.ahead && at.segment < p.d.segments - 1) scan_backward_block<T, P, K, M, true, FULL>(p, at, smem);
+    else scan_backward_block<T, P, K, M, false, FULL>(p, at, smem);
 }
 
-// gB and gC: the channel tiles' parts added up in tile order; one thread per (batch, token, group, state)
-template <typename T>
-__global__ void scan_backward_bc(const __grid_constant__ ScanParams p, int np) {
+// gB and gC: the channel tiles' parts added up, 4 values per thread; a block's 4 slices of the tiles each in order, then the
+// slices.  The parts of a (batch, group) and tile are one piece of memory, [length][2][NP].
+template <typename T, int NP>
+__global__ void __launch_bounds__(256) scan_backward_bc(const __grid_constant__ ScanParams p) {
+    __shared__ float4 s_sum[3][64];
     const ScanDims& d = p.d;
-    const int64_t per = d.length * d.groups * d.states;
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < p.a.batch * per; i += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t b = i / per;
-        int64_t k = i % per;
-        const int n = (int)(k % d.states);
-        k /= d.states;
-        const int64_t g = k % d.groups, t = k / d.groups;
-        float c = 0.0f, bb = 0.0f;
-        if (t < used_length(p.a.lengths, b, d.length)) {
-            const float* src = p.part_bc + ((b * d.groups + g) * d.tiles * d.length + t) * 2 * np + n;
-            for (int64_t tile = 0; tile < d.tiles; ++tile) {
-                c += src[tile * d.length * 2 * np];
-                bb += src[tile * d.length * 2 * np + np];
-            }
+    const int lane = threadIdx.x % 64, slice = threadIdx.x / 64;
+    const int64_t quads = d.length * NP / 2, blocks = (quads + 63) / 64;
+    const int64_t bg = blockIdx.x / blocks, q = blockIdx.x % blocks * 64 + lane;
+    const int64_t t = q / (NP / 2), b = bg / d.groups, g = bg % d.groups;
+    const bool in = q < quads && t < used_length(p.a.lengths, b, d.length);
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (in) {
+        const float4* const src = reinterpret_cast<const float4*>(p.part_bc) + bg * d.tiles * quads + q;
+#pragma unroll 8
+        for (int64_t tile = slice; tile < d.tiles; tile += 4) {
+            const float4 v = src[tile * quads];
+            sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
         }
-        reinterpret_cast<T*>(p.a.gC)[i] = from_f32<T>(c);
-        reinterpret_cast<T*>(p.a.gB)[i] = from_f32<T>(bb);
     }
+    if (slice > 0) s_sum[slice - 1][lane] = sum;
+    __syncthreads();
+    if (slice > 0 || q >= quads) return;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        const float4 v = s_sum[k][lane];
+        sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+    }
+    const int part = (int)(q % (NP / 2)), n0 = part % (NP / 4) * 4;
+    T* const to = reinterpret_cast<T*>(part < NP / 4 ? p.a.gC : p.a.gB) + ((b * d.length + t) * d.groups + g) * d.states;
+    const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        if (n0 + k < d.states) to[n0 + k] = from_f32<T>(v[k]);
 }
 
 // gA, gD, gdelta_bias: the parts of batches and segments added up in order
@@ -1179,7 +1191,10 @@ int launch_segments(F kernel, ScanParams p, int threads, size_t smem, bool backw
 
 template <typename T, int P, int M>
 int run_forward(const ScanParams& p, cudaStream_t stream) {
-    return launch_segments(scan_forward<T, P, M>, p, ForwardShape<P, M>::THREADS, ForwardSmem<T, P, M>::bytes, false, stream);
+    constexpr int threads = ForwardShape<P, M>::THREADS;
+    constexpr size_t smem = ForwardSmem<T, P, M>::bytes;
+    if (p.d.vec && p.d.vec_bc) return launch_segments(scan_forward<T, P, M, true>, p, threads, smem, false, stream);
+    return launch_segments(scan_forward<T, P, M, false>, p, threads, smem, false, stream);
 }
 
 inline uint32_t grid_for(int64_t items) {
@@ -1187,18 +1202,30 @@ inline uint32_t grid_for(int64_t items) {
     return (uint32_t)(blocks < 1 ? 1 : blocks < most ? blocks : most);
 }
 
+// The scanning threads' registers come out of those that the block starts with: `registers` is what all threads hold then.
+template <typename F>
+int launch_backward(F kernel, const ScanParams& p, int threads, int registers, size_t smem, cudaStream_t stream) {
+    cudaFuncAttributes attributes;
+    const cudaError_t e = cudaFuncGetAttributes(&attributes, kernel);
+    if (e != cudaSuccess) return record_cuda_error(e);
+    if (attributes.numRegs * threads < registers) return OVL_ERR_INVALID;
+    return launch_segments(kernel, p, threads, smem, true, stream);
+}
+
 template <typename T, int P, int K, int M>
 int run_backward(const ScanParams& p, cudaStream_t stream) {
     using S = BackShape<P, K, M>;
-    // the scanning threads' registers come out of those that the block starts with
-    cudaFuncAttributes attributes;
-    const cudaError_t e = cudaFuncGetAttributes(&attributes, scan_backward<T, P, K, M>);
-    if (e != cudaSuccess) return record_cuda_error(e);
-    if (attributes.numRegs * S::THREADS < S::SCAN * S::SCAN_REGISTERS + S::HELP * S::HELP_REGISTERS) return OVL_ERR_INVALID;
-    int st = launch_segments(scan_backward<T, P, K, M>, p, S::THREADS, BackSmem<T, P, K, M>::bytes, true, stream);
+    constexpr int registers = S::SCAN * S::SCAN_REGISTERS + S::HELP * S::HELP_REGISTERS;
+    constexpr size_t smem = BackSmem<T, P, K, M>::bytes;
+    int st = p.d.vec && p.d.vec_bc ? launch_backward(scan_backward<T, P, K, M, true>, p, S::THREADS, registers, smem, stream)
+                                   : launch_backward(scan_backward<T, P, K, M, false>, p, S::THREADS, registers, smem, stream);
     if (st != OVL_OK) return st;
-    scan_backward_bc<T><<<grid_for(p.a.batch * p.d.length * p.d.groups * p.d.states), 256, 0, stream>>>(p, S::NP);
-    if ((st = launch_status()) != OVL_OK) return st;
+    const int64_t bc_blocks = ceil_div(p.d.length * S::NP / 2, 64) * p.a.batch * p.d.groups;
+    if (bc_blocks > 0x7fffffff) return OVL_ERR_TOO_LARGE;
+    if (bc_blocks > 0) {
+        scan_backward_bc<T, S::NP><<<(uint32_t)bc_blocks, 256, 0, stream>>>(p);
+        if ((st = launch_status()) != OVL_OK) return st;
+    }
     scan_backward_params<<<grid_for(p.d.channels * (p.d.states + 2)), 256, 0, stream>>>(p);
     return launch_status();
 }

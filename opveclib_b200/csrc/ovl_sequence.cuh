@@ -6,6 +6,7 @@
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+#include <initializer_list>
 
 #include "../../include/ovl_b200.h"
 
@@ -70,7 +71,7 @@ __device__ __forceinline__ Pack<T, N> load_pack(const T* __restrict__ p, bool ve
 }
 
 template <typename T, int N>
-__device__ __forceinline__ void store_pack(T* __restrict__ p, const float (&x)[N], bool vec, int valid) {
+__device__ __forceinline__ void store_pack(T* __restrict__ p, const float (&x)[N], bool vec, int valid, int width = 0) {
     if (vec) {
         constexpr int H = sizeof(T) * N <= 16 ? N : 16 / (int)sizeof(T);
 #pragma unroll
@@ -79,6 +80,14 @@ __device__ __forceinline__ void store_pack(T* __restrict__ p, const float (&x)[N
 #pragma unroll
             for (int k = 0; k < H; ++k) r.v[k] = from_f32<T>(x[i + k]);
             *reinterpret_cast<Pack<T, H>*>(p + i) = r;
+        }
+    } else if (width >= 2) {                                             // (then `valid` is even)
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            Pack<T, 2> r;
+            r.v[0] = from_f32<T>(x[i]);
+            r.v[1] = from_f32<T>(x[i + 1]);
+            if (i < valid) *reinterpret_cast<Pack<T, 2>*>(p + i) = r;
         }
     } else {
 #pragma unroll
@@ -194,17 +203,43 @@ __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_gr
 template <int LEFT>
 __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
 
-// N elements into a slot of shared memory that only this thread reads: in flight while it goes on (`vec`: aligned and
-// all there), otherwise element by element
+// The widest copy, in elements, that all rows allow: 16, 8 or 4 bytes; 0: single 16-bit elements.  `of`: base addresses,
+// `strides`: strides and sizes in elements.
+template <typename T>
+inline int copy_width(std::initializer_list<const void*> of, std::initializer_list<int64_t> strides) {
+    for (int bytes = 16; bytes >= 4; bytes /= 2) {
+        const int width = bytes / (int)sizeof(T);
+        bool fits = true;
+        for (const void* p : of) fits = fits && (uintptr_t)p % bytes == 0;
+        for (int64_t s : strides) fits = fits && s % width == 0;
+        if (fits) return width;
+    }
+    return 0;
+}
+
+// N elements into a slot of shared memory that only this thread reads: in flight while it goes on.  `vec`: all N are
+// there, on 16-byte boundaries (or the pack's size); otherwise `valid` of them in copies of `width` elements, or, with
+// width 0, one by one.
 template <typename T, int N>
-__device__ __forceinline__ void fetch_pack(T* slot, const T* __restrict__ p, bool vec, int valid) {
+__device__ __forceinline__ void fetch_pack(T* slot, const T* __restrict__ p, bool vec, int valid, int width) {
     if (vec) {
         constexpr int BYTES = sizeof(T) * N > 16 ? 16 : (int)sizeof(T) * N, H = BYTES / (int)sizeof(T);
 #pragma unroll
         for (int i = 0; i < N; i += H) copy_async<BYTES>(slot + i, p + i);
-    } else {
+    } else if (width > 0) {
+        constexpr int H = sizeof(T) == 2 ? 2 : 1;                        // 4 bytes: every width is a multiple
 #pragma unroll
-        for (int i = 0; i < N; ++i) slot[i] = i < valid ? p[i] : from_f32<T>(0.0f);
+        for (int i = 0; i < N; i += H) {
+            if (i < valid) copy_async<4>(slot + i, p + i);
+            else if (H == 1) slot[i] = from_f32<T>(0.0f);
+            else slot[i] = slot[i + 1] = from_f32<T>(0.0f);
+        }
+    } else {
+        T v[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = p[i < valid ? i : valid - 1];
+#pragma unroll
+        for (int i = 0; i < N; ++i) slot[i] = i < valid ? v[i] : from_f32<T>(0.0f);
     }
 }
 // the same slot, converted
