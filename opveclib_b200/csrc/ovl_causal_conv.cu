@@ -486,10 +486,8 @@ int launch(const ConvParams& p, size_t smem, cudaStream_t stream, F full, F any)
     F kernel = p.vec ? full : any;
     const int64_t blocks = p.column_tiles * p.strips * p.a.batch;
     if (blocks > 0x7fffffff) return OVL_ERR_TOO_LARGE;
-    if (smem > 24 * 1024) {                                              // (the backward kernels have up to 18 KB beside it)
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return record_cuda_error(e);
-    }
+    const int st = prepare_kernel((const void*)kernel, smem);
+    if (st != OVL_OK) return st;
     kernel<<<(uint32_t)blocks, 32 * kWarps, smem, stream>>>(p);
     return launch_status();
 }

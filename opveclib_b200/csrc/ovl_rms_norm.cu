@@ -431,11 +431,8 @@ int launch_as(const NormParams& p, bool backward, cudaStream_t stream) {
     using S = TeamShape<TEAM>;
     if (backward) {
         constexpr size_t smem = BackRows<T, TEAM, K>::bytes;
-        if (smem > 24 * 1024) {                                          // (up to 17 KB beside it)
-            const cudaError_t e =
-                cudaFuncSetAttribute(norm_backward<T, TEAM, K, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-            if (e != cudaSuccess) return record_cuda_error(e);
-        }
+        const int st = prepare_kernel((const void*)norm_backward<T, TEAM, K, VEC>, smem);
+        if (st != OVL_OK) return st;
         norm_backward<T, TEAM, K, VEC><<<(uint32_t)backward_blocks(&p.a), S::THREADS, smem, stream>>>(p);
         return launch_status();
     }
@@ -444,10 +441,9 @@ int launch_as(const NormParams& p, bool backward, cudaStream_t stream) {
     if (p.a.group > 0) {
         const size_t groups = p.a.columns / p.a.group;
         const size_t smem = p.group_lanes && groups > 1 ? 0 : S::TEAMS * groups * sizeof(unsigned int);
-        if (smem > 40 * 1024) {
-            const cudaError_t e =
-                cudaFuncSetAttribute(norm_forward<T, TEAM, K, true, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-            if (e != cudaSuccess) return record_cuda_error(e);
+        if (smem > 24 * 1024) {                                          // up to a scale for every column
+            const int st = prepare_kernel((const void*)norm_forward<T, TEAM, K, true, VEC>, sizeof(unsigned int) * S::TEAMS * TEAM * K * 8);
+            if (st != OVL_OK) return st;
         }
         norm_forward<T, TEAM, K, true, VEC><<<(uint32_t)blocks, S::THREADS, smem, stream>>>(p);
     } else {

@@ -2,9 +2,35 @@
 // ovl_selective_scan.cuh; interface: include/ovl_b200.h.
 #include <stdio.h>
 #include <stdlib.h>
+#include <mutex>
+#include <set>
+#include <utility>
 #include "ovl_selective_scan.cuh"
 
 namespace ovl {
+
+int prepare_kernel(const void* kernel, size_t smem, int threads, int registers) {
+    static std::mutex mutex;
+    static std::set<std::pair<const void*, int>> done;
+    if (smem <= 24 * 1024 && registers == 0) return OVL_OK;              // (with the 18 KB that some have beside it: 48 KB need no leave)
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return record_cuda_error(e);
+    const std::pair<const void*, int> key(kernel, device);
+    std::lock_guard<std::mutex> lock(mutex);
+    if (done.count(key)) return OVL_OK;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return record_cuda_error(e);
+    if (registers > 0) {
+        cudaFuncAttributes attributes;
+        e = cudaFuncGetAttributes(&attributes, kernel);
+        if (e != cudaSuccess) return record_cuda_error(e);
+        if (attributes.numRegs * threads < registers) return OVL_ERR_INVALID;
+    }
+    done.insert(key);
+    return OVL_OK;
+}
+
 namespace {
 
 bool multiple_of(int64_t n, int64_t a, int64_t b) { return a % n == 0 && b % n == 0; }

@@ -1164,19 +1164,10 @@ __global__ void __launch_bounds__(128) scan_step(const __grid_constant__ OvlSele
 // ---------------------------------------------------------------------------------------------------------
 // launches
 
-template <typename F>
-int allow_smem(F kernel, size_t bytes) {
-    if (bytes > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-        if (e != cudaSuccess) return record_cuda_error(e);
-    }
-    return OVL_OK;
-}
-
 // One launch, or the two of a length that is cut into segments.
 template <typename F>
-int launch_segments(F kernel, ScanParams p, int threads, size_t smem, bool backward, cudaStream_t stream) {
-    int st = allow_smem(kernel, smem);
+int launch_segments(F kernel, ScanParams p, int threads, size_t smem, bool backward, cudaStream_t stream, int registers = 0) {
+    int st = prepare_kernel((const void*)kernel, smem, threads, registers);
     if (st != OVL_OK) return st;
     const int64_t n = p.d.segments, blocks = p.a.batch * p.d.groups * p.d.tiles;
     for (int launch = n > 1 ? 0 : 1; launch < 2; ++launch) {
@@ -1202,23 +1193,14 @@ inline uint32_t grid_for(int64_t items) {
     return (uint32_t)(blocks < 1 ? 1 : blocks < most ? blocks : most);
 }
 
-// The scanning threads' registers come out of those that the block starts with: `registers` is what all threads hold then.
-template <typename F>
-int launch_backward(F kernel, const ScanParams& p, int threads, int registers, size_t smem, cudaStream_t stream) {
-    cudaFuncAttributes attributes;
-    const cudaError_t e = cudaFuncGetAttributes(&attributes, kernel);
-    if (e != cudaSuccess) return record_cuda_error(e);
-    if (attributes.numRegs * threads < registers) return OVL_ERR_INVALID;
-    return launch_segments(kernel, p, threads, smem, true, stream);
-}
-
 template <typename T, int P, int K, int M>
 int run_backward(const ScanParams& p, cudaStream_t stream) {
     using S = BackShape<P, K, M>;
+    // the scanning threads' registers come out of those that the block starts with: what all threads hold then
     constexpr int registers = S::SCAN * S::SCAN_REGISTERS + S::HELP * S::HELP_REGISTERS;
     constexpr size_t smem = BackSmem<T, P, K, M>::bytes;
-    int st = p.d.vec && p.d.vec_bc ? launch_backward(scan_backward<T, P, K, M, true>, p, S::THREADS, registers, smem, stream)
-                                   : launch_backward(scan_backward<T, P, K, M, false>, p, S::THREADS, registers, smem, stream);
+    int st = p.d.vec && p.d.vec_bc ? launch_segments(scan_backward<T, P, K, M, true>, p, S::THREADS, smem, true, stream, registers)
+                                   : launch_segments(scan_backward<T, P, K, M, false>, p, S::THREADS, smem, true, stream, registers);
     if (st != OVL_OK) return st;
     const int64_t bc_blocks = ceil_div(p.d.length * S::NP / 2, 64) * p.a.batch * p.d.groups;
     if (bc_blocks > 0x7fffffff) return OVL_ERR_TOO_LARGE;

@@ -27,6 +27,10 @@ constexpr float kLn2 = 0.6931471805599453f;
 
 __host__ __device__ inline bool aligned16(const void* p) { return ((uintptr_t)p % 16) == 0; }
 
+// Allows a kernel `smem` bytes of dynamic shared memory and, with `registers` > 0, makes sure that its blocks of `threads`
+// start with that many (OVL_ERR_INVALID if not); asked of the driver once per kernel and device.
+__attribute__((visibility("hidden"))) int prepare_kernel(const void* kernel, size_t smem, int threads = 0, int registers = 0);
+
 // SM count of the current device (148 on a B200), asked once per device.
 __attribute__((visibility("hidden"))) int sequence_sm_count();
 

@@ -36,6 +36,7 @@ def _torch():
     return _torch_module
 
 
+_TWO = struct.Struct('2q')
 _SCAN = struct.Struct('47q')
 _SCAN_STEP = struct.Struct('25q')
 _CONV = struct.Struct('26q')
@@ -122,8 +123,13 @@ def _launch(name, args, device):
         launcher.check(status, name)
 
 
-def _workspace(size, device):
-    return _torch_module.empty(size, dtype=_torch_module.uint8, device=device) if size else None
+def _with_workspace(args, at, size, device):
+    """The packed arguments with a workspace of ``size`` bytes in the fields ``at`` and ``at + 1``, and the workspace, which
+    the caller holds until the launch."""
+    if not size:
+        return args, None
+    workspace = _torch_module.empty(size, dtype=_torch_module.uint8, device=device)
+    return args[:8 * at] + _TWO.pack(workspace.data_ptr(), size) + args[8 * at + 16:], workspace
 
 
 def _with_device(device, function, *args):
@@ -159,7 +165,7 @@ def _strides(x, *axes):
 # ---------------------------------------------------------------------------------------------------------
 # selective scan
 
-def _scan_args(dims, x, out=(None, None, None), workspace=None, above=(None, None), grads=(None,) * 9):
+def _scan_args(dims, x, out=(None, None, None), above=(None, None), grads=(None,) * 9):
     u, delta, A, B, C, D, z, delta_bias, initial_state, lengths = x
     batch, length, channels, states, groups, softplus = dims
     gout, gfinal = above
@@ -168,7 +174,7 @@ def _scan_args(dims, x, out=(None, None, None), workspace=None, above=(None, Non
         _codes[u.dtype], batch, length, channels, states, groups, softplus, u.data_ptr(), delta.data_ptr(), _ptr(z),
         B.data_ptr(), C.data_ptr(), A.data_ptr(), _ptr(D), _ptr(delta_bias), _ptr(initial_state), _ptr(lengths),
         *u.stride()[:2], *delta.stride()[:2], *_strides(z, 0, 1), *B.stride()[:3], *C.stride()[:3],
-        _ptr(out[0]), _ptr(out[1]), _ptr(out[2]), _ptr(workspace), 0 if workspace is None else workspace.numel(),
+        _ptr(out[0]), _ptr(out[1]), _ptr(out[2]), 0, 0,
         _ptr(gout), *_strides(gout, 0, 1), _ptr(gfinal), _ptr(gu), _ptr(gdelta), _ptr(gz), _ptr(gB), _ptr(gC), _ptr(gA),
         _ptr(gD), _ptr(gbias), _ptr(ginitial))
 
@@ -178,12 +184,13 @@ def _scan_forward(x, dims, save):
     u, A = x[0], x[2]
     batch, length, channels, states, _, _ = dims
     device = u.device
-    out = torch.empty((batch, length, channels), dtype=u.dtype, device=device)
-    final = torch.empty((batch, channels, states), dtype=torch.float32, device=device)
-    saved = torch.empty((batch, (length + 15) // 16, channels, states), dtype=torch.float32, device=device) if save else None
-    size = _with_device(device, launcher.library().ovl_selective_scan_workspace_bytes, _scan_args(dims, x), 0)
-    workspace = _workspace(size, device)
-    _launch('ovl_selective_scan', _scan_args(dims, x, (out, final, saved), workspace), device)
+    out = _like(u)
+    final = A.new_empty((batch, channels, states)) if x[8] is None else torch.empty_like(x[8])
+    saved = A.new_empty((batch, (length + 15) // 16, channels, states)) if save else None
+    args = _scan_args(dims, x, (out, final, saved))
+    size = _with_device(device, launcher.library().ovl_selective_scan_workspace_bytes, args, 0)
+    args, workspace = _with_workspace(args, 32, size, device)
+    _launch('ovl_selective_scan', args, device)
     return out, final, saved
 
 
@@ -191,28 +198,21 @@ def _scan_backward(x, dims, saved, gout, gfinal):
     torch = _torch_module
     u, delta, A, B, C, D, z, delta_bias, initial_state, lengths = x
     batch, length, channels, states, groups, _ = dims
-    device, like = u.device, dict(dtype=u.dtype, device=u.device)
+    device = u.device
     if gout is None:                                         # only the final state is used further on
-        gout = torch.zeros(channels, **like).expand(batch, length, channels)
+        gout = u.new_zeros(channels).expand(batch, length, channels)
     gout = gout if gout.stride(-1) == 1 else gout.contiguous()
     gfinal = None if gfinal is None else gfinal.contiguous()
-    make = torch.zeros if batch == 0 else torch.empty
-    gu = torch.empty((batch, length, channels), **like)
-    gdelta = torch.empty((batch, length, channels), **like)
-    gz = None if z is None else torch.empty((batch, length, channels), **like)
-    gB = torch.empty((batch, length, groups, states), **like)
-    gC = torch.empty((batch, length, groups, states), **like)
-    gA = make(A.shape, dtype=torch.float32, device=device)
-    gD = None if D is None else make((channels,), dtype=torch.float32, device=device)
-    gbias = None if delta_bias is None else make((channels,), dtype=torch.float32, device=device)
-    ginitial = None
-    if initial_state is not None:
-        ginitial = torch.empty((batch, channels, states), dtype=torch.float32, device=device)
-    size = _with_device(device, launcher.library().ovl_selective_scan_workspace_bytes, _scan_args(dims, x), 1)
-    workspace = _workspace(size, device)
+    make = torch.zeros_like if batch == 0 else torch.empty_like
+    gu, gdelta, gz = _like(u), _like(delta), None if z is None else _like(z)
+    gB, gC = _like(B), _like(C)
+    gA, gD, gbias = make(A), None if D is None else make(D), None if delta_bias is None else make(delta_bias)
+    ginitial = None if initial_state is None else torch.empty_like(initial_state)
     grads = (gu, gdelta, gA, gB, gC, gD, gz, gbias, ginitial)
-    _launch('ovl_selective_scan_backward',
-            _scan_args(dims, x, (None, None, saved), workspace, (gout, gfinal), grads), device)
+    args = _scan_args(dims, x, (None, None, saved), (gout, gfinal), grads)
+    size = _with_device(device, launcher.library().ovl_selective_scan_workspace_bytes, args, 1)
+    args, workspace = _with_workspace(args, 32, size, device)
+    _launch('ovl_selective_scan_backward', args, device)
     return grads
 
 
@@ -343,23 +343,23 @@ def _param_type(weight, name, t, what):
     return weight.dtype
 
 
-def _conv_args(dims, x, out=(None, None), above=(None, None), grads=(None,) * 4, workspace=None):
+def _conv_args(dims, x, out=(None, None), above=(None, None), grads=(None,) * 4):
     x, weight, bias, initial_state, lengths = x
     batch, length, channels, taps, silu = dims
     gout, gfinal = above
     return _CONV.pack(
         _codes[x.dtype], batch, length, channels, taps, silu, weight.dtype is _torch_module.float32, x.data_ptr(),
         weight.data_ptr(), _ptr(bias), _ptr(initial_state), _ptr(lengths), *x.stride()[:2], _ptr(out[0]), _ptr(out[1]),
-        _ptr(gout), *_strides(gout, 0, 1), _ptr(gfinal), *map(_ptr, grads), _ptr(workspace),
-        0 if workspace is None else workspace.numel())
+        _ptr(gout), *_strides(gout, 0, 1), _ptr(gfinal), *map(_ptr, grads), 0, 0)
 
 
 def _conv_forward(x, dims, state):
     torch = _torch_module
     batch, length, channels, taps, _ = dims
-    like = dict(dtype=x[0].dtype, device=x[0].device)
-    out = torch.empty((batch, length, channels), **like)
-    final = torch.empty((batch, taps - 1, channels), **like) if state else None
+    out = _like(x[0])
+    final = None
+    if state:
+        final = out.new_empty((batch, taps - 1, channels)) if x[3] is None else torch.empty_like(x[3])
     _launch('ovl_causal_conv', _conv_args(dims, x, (out, final)), out.device)
     return out, final
 
@@ -368,19 +368,19 @@ def _conv_backward(x, dims, gout, gfinal):
     torch = _torch_module
     batch, length, channels, taps, _ = dims
     tokens, weight, bias, initial_state, _ = x
-    device, like = tokens.device, dict(dtype=tokens.dtype, device=tokens.device)
+    device = tokens.device
     if gout is None:
-        gout = torch.zeros(channels, **like).expand(batch, length, channels)
+        gout = tokens.new_zeros(channels).expand(batch, length, channels)
     gout = gout if gout.stride(-1) == 1 else gout.contiguous()
     gfinal = None if gfinal is None else gfinal.contiguous()
-    make = torch.zeros if batch == 0 else torch.empty
-    gx = torch.empty((batch, length, channels), **like)
-    gweight = make((channels, taps), dtype=weight.dtype, device=device)
-    gbias = None if bias is None else make((channels,), dtype=weight.dtype, device=device)
-    ginitial = None if initial_state is None else torch.empty((batch, taps - 1, channels), **like)
-    workspace = _workspace(launcher.library().ovl_causal_conv_workspace_bytes(_conv_args(dims, x)), device)
+    make = torch.zeros_like if batch == 0 else torch.empty_like
+    gx, gweight, gbias = _like(tokens), make(weight), None if bias is None else make(bias)
+    ginitial = None if initial_state is None else torch.empty_like(initial_state)
     grads = (gx, gweight, gbias, ginitial)
-    _launch('ovl_causal_conv_backward', _conv_args(dims, x, (None, None), (gout, gfinal), grads, workspace), device)
+    args = _conv_args(dims, x, (None, None), (gout, gfinal), grads)
+    size = _with_device(device, launcher.library().ovl_causal_conv_workspace_bytes, args)
+    args, workspace = _with_workspace(args, 24, size, device)
+    _launch('ovl_causal_conv_backward', args, device)
     return grads
 
 
@@ -464,13 +464,12 @@ def _rows(x):
 
 
 def _norm_args(x, weight, eps, group=0, residual=None, y=None, residual_out=None, q=None, scale=None, gy=None, gres=None,
-               gx=None, gweight=None, workspace=None):
+               gx=None, gweight=None):
     return _NORM.pack(
         _codes[x.dtype], x.shape[0], x.shape[1], weight.dtype is _torch_module.float32, group, eps, x.data_ptr(),
         _ptr(residual), weight.data_ptr(), x.stride(0), 0 if residual is None else residual.stride(0), _ptr(y),
         _ptr(residual_out), _ptr(q), _ptr(scale), _ptr(gy), _ptr(gres), 0 if gy is None else gy.stride(0),
-        0 if gres is None else gres.stride(0), _ptr(gx), _ptr(gweight), _ptr(workspace),
-        0 if workspace is None else workspace.numel())
+        0 if gres is None else gres.stride(0), _ptr(gx), _ptr(gweight), 0, 0)
 
 
 def _norm_check(x, weight, residual, eps, what):
@@ -499,16 +498,16 @@ def _norm_backward(x, weight, residual, eps, gy, gres):
     torch = _torch_module
     device = x.device
     if gy is None:
-        gy = torch.zeros(x.shape[1], dtype=x.dtype, device=device).expand(x.shape)
+        gy = x.new_zeros(x.shape[1]).expand(x.shape)
     gy = gy if gy.stride(-1) == 1 else gy.contiguous()
     if gres is not None and gres.stride(-1) != 1:
         gres = gres.contiguous()
     gx = _like(x)
-    gweight = torch.empty(weight.shape, dtype=weight.dtype, device=device)
-    size = _with_device(device, launcher.library().ovl_rms_norm_workspace_bytes, _norm_args(x, weight, eps))
-    _launch('ovl_rms_norm_backward',
-            _norm_args(x, weight, eps, residual=residual, gy=gy, gres=gres, gx=gx, gweight=gweight,
-                       workspace=_workspace(size, device)), device)
+    gweight = torch.empty_like(weight)
+    args = _norm_args(x, weight, eps, residual=residual, gy=gy, gres=gres, gx=gx, gweight=gweight)
+    size = _with_device(device, launcher.library().ovl_rms_norm_workspace_bytes, args)
+    args, workspace = _with_workspace(args, 21, size, device)
+    _launch('ovl_rms_norm_backward', args, device)
     return gx, gweight
 
 
@@ -548,7 +547,7 @@ def rms_norm_quantize(x, weight, residual=None, eps=1e-6, group=None):
     _no_gradient(what, x, weight, residual)
     shape, x, residual = x.shape, _rows(x), None if residual is None else _rows(residual)
     q = torch.empty_like(x, dtype=torch.float8_e4m3fn, memory_format=torch.contiguous_format)
-    scale = torch.empty((x.shape[0], columns // group), dtype=torch.float32, device=device)
+    scale = x.new_empty((x.shape[0], columns // group), dtype=torch.float32)
     residual_out = None if residual is None else _like(x)
     _launch('ovl_rms_norm', _norm_args(x, weight, eps, group, residual, None, residual_out, q, scale), device)
     if len(shape) != 2:
