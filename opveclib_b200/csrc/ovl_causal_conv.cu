@@ -143,10 +143,17 @@ __global__ void __launch_bounds__(32 * kWarps, TAPS == kMaxTaps ? 1 : 4) conv_fo
     const T* const x = reinterpret_cast<const T*>(a.x) + batch * a.x_batch + channel;
     T* const out = reinterpret_cast<T*>(a.out) + batch * a.length * a.channels + channel;
     const Ring<T, N> ring(smem);
+    const T* next = x + t_begin * a.x_token;                             // of the next chunk to be fetched
     auto fetch = [&](int64_t t0, int chunk) {
+        if (FULL && t0 + CHUNK <= t_used) {
 #pragma unroll
-        for (int s = 0; s < CHUNK; ++s)
-            if (t0 + s < t_used) fetch_pack<T, N>(ring.slot(chunk, s), x + (t0 + s) * a.x_token, vec, valid, p.width);
+            for (int s = 0; s < CHUNK; ++s) fetch_pack<T, N>(ring.slot(chunk, s), next + s * a.x_token, true, N, 0);
+        } else {
+#pragma unroll
+            for (int s = 0; s < CHUNK; ++s)
+                if (t0 + s < t_used) fetch_pack<T, N>(ring.slot(chunk, s), next + s * a.x_token, vec, valid, p.width);
+        }
+        next += CHUNK * a.x_token;
         copy_commit();
     };
 #pragma unroll
@@ -158,6 +165,7 @@ __global__ void __launch_bounds__(32 * kWarps, TAPS == kMaxTaps ? 1 : 4) conv_fo
         widen<T, N>(win[k], load_token<T, N>(a, batch, t_begin - (TAPS - 1) + k, used, channel, vec, valid));
     const bool gated = a.silu;
     int chunk = 0;
+    T* out_t = out + t_begin * a.channels;
     // one token; INSIDE: it belongs to the strip and the sequence
     auto token = [&](int64_t t, const T* slot, auto inside) {
         constexpr bool INSIDE = decltype(inside)::value;
@@ -179,7 +187,8 @@ __global__ void __launch_bounds__(32 * kWarps, TAPS == kMaxTaps ? 1 : 4) conv_fo
 #pragma unroll
             for (int c = 0; c < N; ++c) y[c] = 0.0f;
         }
-        if (INSIDE || t < t_end) store_pack<T, N>(out + t * a.channels, y, vec, valid, p.width);
+        if (INSIDE || t < t_end) store_pack<T, N>(out_t, y, vec, valid, p.width);
+        out_t += a.channels;
 #pragma unroll
         for (int k = 0; k < TAPS - 1; ++k)
 #pragma unroll
@@ -234,15 +243,26 @@ __global__ void __launch_bounds__(32 * kWarps, TAPS == kMaxTaps ? 1 : 4) conv_ba
         const T* const x = reinterpret_cast<const T*>(a.x) + batch * a.x_batch + channel;
         const T* const gout = reinterpret_cast<const T*>(a.gout) + batch * a.gout_batch + channel;
         const Ring<T, N> ring_x(smem), ring_g(smem + Ring<T, N>::bytes);
+        const T* next_x = x + t_begin * a.x_token;                       // of the next chunk to be fetched
+        const T* next_g = gout + t_begin * a.gout_token;
         auto fetch = [&](int64_t t0, int chunk) {
+            if (FULL && t0 + CHUNK <= walk_used) {
 #pragma unroll
-            for (int s = 0; s < CHUNK; ++s) {
-                const int64_t t = t0 + s;
-                if (t < walk_used) {
-                    fetch_pack<T, N>(ring_x.slot(chunk, s), x + t * a.x_token, vec, valid, p.width);
-                    fetch_pack<T, N>(ring_g.slot(chunk, s), gout + t * a.gout_token, vec, valid, p.width);
+                for (int s = 0; s < CHUNK; ++s) {
+                    fetch_pack<T, N>(ring_x.slot(chunk, s), next_x + s * a.x_token, true, N, 0);
+                    fetch_pack<T, N>(ring_g.slot(chunk, s), next_g + s * a.gout_token, true, N, 0);
+                }
+            } else {
+#pragma unroll
+                for (int s = 0; s < CHUNK; ++s) {
+                    if (t0 + s < walk_used) {
+                        fetch_pack<T, N>(ring_x.slot(chunk, s), next_x + s * a.x_token, vec, valid, p.width);
+                        fetch_pack<T, N>(ring_g.slot(chunk, s), next_g + s * a.gout_token, vec, valid, p.width);
+                    }
                 }
             }
+            next_x += CHUNK * a.x_token;
+            next_g += CHUNK * a.gout_token;
             copy_commit();
         };
 #pragma unroll
@@ -253,6 +273,7 @@ __global__ void __launch_bounds__(32 * kWarps, TAPS == kMaxTaps ? 1 : 4) conv_ba
             widen<T, N>(win[k], load_token<T, N>(a, batch, t_begin - (TAPS - 1) + k, used, channel, vec, valid));
         const bool gated = a.silu;
         int chunk = 0;
+        T* gx_t = reinterpret_cast<T*>(a.gx) + (batch * a.length + t_begin - (taps - 1)) * a.channels + channel;   // of token t - (taps - 1)
         // one token; INSIDE: it belongs to the strip and the sequence, and so does the one whose gx it completes
         auto token = [&](int64_t t, const T* slot_x, const T* slot_g, auto inside) {
             constexpr bool INSIDE = decltype(inside)::value;
@@ -320,10 +341,11 @@ __global__ void __launch_bounds__(32 * kWarps, TAPS == kMaxTaps ? 1 : 4) conv_ba
                         for (int c = 0; c < N; ++c) gx[c] += to_f32(gf.v[c]);
                     }
                 }
-                T* const dst = state ? reinterpret_cast<T*>(a.ginitial) + (batch * (taps - 1) + (taps - 1) + to) * a.channels
-                                     : reinterpret_cast<T*>(a.gx) + (batch * a.length + to) * a.channels;
-                store_pack<T, N>(dst + channel, gx, vec, valid, p.width);
+                T* dst = gx_t;
+                if (state) dst = reinterpret_cast<T*>(a.ginitial) + (batch * (taps - 1) + (taps - 1) + to) * a.channels + channel;
+                store_pack<T, N>(dst, gx, vec, valid, p.width);
             }
+            gx_t += a.channels;
 #pragma unroll
             for (int k = 0; k < TAPS - 1; ++k)
 #pragma unroll

@@ -1,7 +1,5 @@
 // Selective scan: what its entry points check, how a problem is cut, and where the work space lies.  The kernels are in
 // ovl_selective_scan.cuh; interface: include/ovl_b200.h.
-#include <stdio.h>
-#include <stdlib.h>
 #include <mutex>
 #include <set>
 #include <utility>
@@ -74,11 +72,12 @@ void make_dims(const OvlSelectiveScan* a, ScanDims* d, ScanShape* shape, bool ba
     d->softplus = a->delta_softplus != 0;
     *shape = backward ? backward_shape(a) : forward_shape(a);
     d->tiles = ceil_div(d->group_channels, shape->block_channels());
-    int tune_s = 0;
-    if (const char* e = getenv("OVL_TUNE")) sscanf(e, "%d", &tune_s);
+    // Segments that run side by side in two launches (one less than there are segments in each): as many as two blocks per
+    // SM hold, from four segments on - with S segments the two launches walk 2 / S of the length.  bf16, one sequence, 16
+    // states: 2048 tokens x 2048 channels (64 blocks) 82 us in one piece, 59 us in 5 segments; 16384 x 4096 (128 blocks)
+    // 625 us in one piece, 637 us in 3 segments, 723 us in 4.
     const int64_t blocks = a->batch * a->groups * d->tiles;
     int64_t s = blocks > 0 ? 1 + 2 * (int64_t)sequence_sm_count() / blocks : 1;
-    if (tune_s) s = tune_s;
     const int64_t most = ceil_div(a->length, 64);
     if (s > most) s = most;
     if (s > kMaxSegments) s = kMaxSegments;
