@@ -123,12 +123,12 @@ def _launch(name, args, device):
         launcher.check(status, name)
 
 
-def _with_workspace(args, at, size, device):
-    """The packed arguments with a workspace of ``size`` bytes in the fields ``at`` and ``at + 1``, and the workspace, which
-    the caller holds until the launch."""
+def _with_workspace(args, at, size, x):
+    """The packed arguments with a workspace of ``size`` bytes, on the device of ``x``, in the fields ``at`` and ``at + 1``,
+    and the workspace, which the caller holds until the launch."""
     if not size:
         return args, None
-    workspace = _torch_module.empty(size, dtype=_torch_module.uint8, device=device)
+    workspace = x.new_empty(-(-size // x.element_size()))
     return args[:8 * at] + _TWO.pack(workspace.data_ptr(), size) + args[8 * at + 16:], workspace
 
 
@@ -150,7 +150,9 @@ def _differentiable(*tensors):
 
 def _like(x):
     """A dense tensor of the shape, type and device of x."""
-    return _torch_module.empty_like(x, memory_format=_torch_module.contiguous_format)
+    if x.is_contiguous():
+        return _torch_module.empty_like(x)
+    return x.new_empty(x.shape)
 
 
 def _no_gradient(what, *tensors):
@@ -189,7 +191,7 @@ def _scan_forward(x, dims, save):
     saved = A.new_empty((batch, (length + 15) // 16, channels, states)) if save else None
     args = _scan_args(dims, x, (out, final, saved))
     size = _with_device(device, launcher.library().ovl_selective_scan_workspace_bytes, args, 0)
-    args, workspace = _with_workspace(args, 32, size, device)
+    args, workspace = _with_workspace(args, 32, size, u)
     _launch('ovl_selective_scan', args, device)
     return out, final, saved
 
@@ -211,7 +213,7 @@ def _scan_backward(x, dims, saved, gout, gfinal):
     grads = (gu, gdelta, gA, gB, gC, gD, gz, gbias, ginitial)
     args = _scan_args(dims, x, (None, None, saved), (gout, gfinal), grads)
     size = _with_device(device, launcher.library().ovl_selective_scan_workspace_bytes, args, 1)
-    args, workspace = _with_workspace(args, 32, size, device)
+    args, workspace = _with_workspace(args, 32, size, u)
     _launch('ovl_selective_scan_backward', args, device)
     return grads
 
@@ -379,7 +381,7 @@ def _conv_backward(x, dims, gout, gfinal):
     grads = (gx, gweight, gbias, ginitial)
     args = _conv_args(dims, x, (None, None), (gout, gfinal), grads)
     size = _with_device(device, launcher.library().ovl_causal_conv_workspace_bytes, args)
-    args, workspace = _with_workspace(args, 24, size, device)
+    args, workspace = _with_workspace(args, 24, size, tokens)
     _launch('ovl_causal_conv_backward', args, device)
     return grads
 
@@ -506,7 +508,7 @@ def _norm_backward(x, weight, residual, eps, gy, gres):
     gweight = torch.empty_like(weight)
     args = _norm_args(x, weight, eps, residual=residual, gy=gy, gres=gres, gx=gx, gweight=gweight)
     size = _with_device(device, launcher.library().ovl_rms_norm_workspace_bytes, args)
-    args, workspace = _with_workspace(args, 21, size, device)
+    args, workspace = _with_workspace(args, 21, size, x)
     _launch('ovl_rms_norm_backward', args, device)
     return gx, gweight
 
@@ -546,7 +548,7 @@ def rms_norm_quantize(x, weight, residual=None, eps=1e-6, group=None):
         raise ValueError('%s: group must divide the %d columns, not %r' % (what, columns, group))
     _no_gradient(what, x, weight, residual)
     shape, x, residual = x.shape, _rows(x), None if residual is None else _rows(residual)
-    q = torch.empty_like(x, dtype=torch.float8_e4m3fn, memory_format=torch.contiguous_format)
+    q = x.new_empty(x.shape, dtype=torch.float8_e4m3fn)
     scale = x.new_empty((x.shape[0], columns // group), dtype=torch.float32)
     residual_out = None if residual is None else _like(x)
     _launch('ovl_rms_norm', _norm_args(x, weight, eps, group, residual, None, residual_out, q, scale), device)
