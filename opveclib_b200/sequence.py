@@ -155,6 +155,12 @@ def _like(x):
     return x.new_empty(x.shape)
 
 
+def _changed(state):
+    """A state that a kernel wrote to: a backward pass that kept it finds out, as with any change in place."""
+    if not state.is_inference():
+        _torch_module.autograd.graph.increment_version(state)
+
+
 def _no_gradient(what, *tensors):
     if _differentiable(*tensors):
         raise RuntimeError('%s has no gradient: call it under torch.no_grad()' % what)
@@ -325,6 +331,7 @@ def selective_scan_step(state, u, delta, A, B, C, D=None, z=None, delta_bias=Non
         _ptr(z), B.data_ptr(), C.data_ptr(), A.data_ptr(), _ptr(D), _ptr(delta_bias), _ptr(slots), u.stride(0),
         delta.stride(0), 0 if z is None else z.stride(0), B.stride(0), B.stride(1), C.stride(0), C.stride(1),
         state.data_ptr(), out.data_ptr()), device)
+    _changed(state)
     return out
 
 
@@ -454,6 +461,7 @@ def causal_conv1d_step(state, x, weight, bias=None, activation=None, slots=None)
     _launch('ovl_causal_conv_step', _CONV_STEP.pack(
         _codes[t], rows, channels, taps, silu, p is torch.float32, state.shape[0], x.data_ptr(), weight.data_ptr(),
         _ptr(bias), _ptr(slots), x.stride(0), state.data_ptr(), out.data_ptr()), device)
+    _changed(state)
     return out
 
 

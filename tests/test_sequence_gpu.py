@@ -697,6 +697,21 @@ def test_other_streams_and_captured_graphs():
         assert torch.equal(step, s)
 
 
+def test_a_state_changed_in_place_is_noticed_by_the_backward_pass():
+    x, opts = _scan_case(F32, 2, 5, 16, 8)
+    state = x['initial_state']
+    x['u'] = x['u'].requires_grad_()
+    out = ovl.selective_scan(**x, **opts)
+    step = {k: v[:, 0].detach() if k in ('u', 'delta', 'B', 'C', 'z') else v for k, v in x.items() if k != 'initial_state'}
+    ovl.selective_scan_step(state, **step)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        out.sum().backward()
+    with torch.inference_mode():
+        inside = torch.zeros(2, 16, 8, device='cuda')
+        ovl.selective_scan_step(inside, **step)
+        assert bool(inside.any())
+
+
 def test_two_calls_at_once_on_two_streams():
     x, opts = _scan_case(BF16, 1, 600, 64, 16)                # cut into segments: both calls have workspaces
     want = ovl.selective_scan(**x, **opts, return_state=True)
