@@ -21,10 +21,12 @@ from . import launcher
 _torch_module = None
 _codes = None
 _raw_stream = None
+_current_device = None
+_entries = {}
 
 
 def _torch():
-    global _torch_module, _codes, _raw_stream
+    global _torch_module, _codes, _raw_stream, _current_device
     if _torch_module is None:
         import torch
         _codes = {torch.float16: 1, torch.float32: 2, torch.bfloat16: 12}
@@ -32,6 +34,8 @@ def _torch():
         _raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)
         if _raw_stream is None:
             _raw_stream = lambda index: torch.cuda.current_stream(index).cuda_stream  # noqa: E731
+        # (asked for only once tensors are known to be CUDA tensors: the runtime is up then)
+        _current_device = getattr(torch._C, '_cuda_getDevice', torch.cuda.current_device)
         _torch_module = torch
     return _torch_module
 
@@ -60,15 +64,23 @@ def _refuse(x, name, shape, dtype, what):
 
 def _tensor(x, name, shape, dtype, what):
     """Refuse anything but a tensor of this shape and type; a copy where the innermost axis is not contiguous."""
-    if not isinstance(x, _torch_module.Tensor) or x.dtype is not dtype or x.shape != shape:
+    try:
+        right = x.dtype is dtype and x.shape == shape
+    except AttributeError:
+        right = False
+    if not right:
         _refuse(x, name, shape, dtype, what)
-    return x if x.stride(-1) == 1 else x.contiguous()
+    return x if x.is_contiguous() or x.stride(-1) == 1 else x.contiguous()
 
 
 def _dense(x, name, shape, dtype, what):
-    if not isinstance(x, _torch_module.Tensor) or x.dtype is not dtype or x.shape != shape:
+    try:
+        right = x.dtype is dtype and x.shape == shape
+    except AttributeError:
+        right = False
+    if not right:
         _refuse(x, name, shape, dtype, what)
-    return x.contiguous()
+    return x if x.is_contiguous() else x.contiguous()
 
 
 def _first(x, name, rank, what):
@@ -112,13 +124,15 @@ def _one_device(what, *tensors):
 
 def _launch(name, args, device):
     """Enqueue on torch's current stream of the tensors' device, whichever device is the current one."""
-    torch = _torch_module
-    function = getattr(launcher.library(), name)
-    if device.index == torch.cuda.current_device():
-        status = function(args, _raw_stream(device.index))
+    function = _entries.get(name)
+    if function is None:
+        function = _entries[name] = getattr(launcher.library(), name)
+    index = device.index
+    if index == _current_device():
+        status = function(args, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
-            status = function(args, _raw_stream(device.index))
+        with _torch_module.cuda.device(device):
+            status = function(args, _raw_stream(index))
     if status:
         launcher.check(status, name)
 
@@ -134,7 +148,7 @@ def _with_workspace(args, at, size, x):
 
 def _with_device(device, function, *args):
     """A size query: the answer depends on the device's SM count."""
-    if device.index == _torch_module.cuda.current_device():
+    if device.index == _current_device():
         return function(*args)
     with _torch_module.cuda.device(device):
         return function(*args)
