@@ -177,11 +177,8 @@ __global__ void __launch_bounds__(32 * kWarps, TAPS == kMaxTaps ? 1 : 4) conv_fo
 #pragma unroll
             for (int k = 0; k < TAPS; ++k)
                 if (TAPS != kMaxTaps || k >= TAPS - taps) sum = fma2(w[k][c], win[k][c], sum);
+            if (gated) sum = silu2(sum);
             unpack2(sum, y[2 * c], y[2 * c + 1]);
-        }
-        if (gated) {
-#pragma unroll
-            for (int c = 0; c < N; ++c) y[c] = silu(y[c]);
         }
         if (!INSIDE && t >= used) {
 #pragma unroll
@@ -277,29 +274,25 @@ __global__ void __launch_bounds__(32 * kWarps, TAPS == kMaxTaps ? 1 : 4) conv_ba
         // one token; INSIDE: it belongs to the strip and the sequence, and so does the one whose gx it completes
         auto token = [&](int64_t t, const T* slot_x, const T* slot_g, auto inside) {
             constexpr bool INSIDE = decltype(inside)::value;
-            float g[N];
+            F2 g[N / 2];
             widen_slot<T, N>(win[TAPS - 1], slot_x);
-            read_slot<T, N>(slot_g, g);
+            widen_slot<T, N>(g, slot_g);
             if (gated) {
 #pragma unroll
                 for (int c = 0; c < N / 2; ++c) {
-                    F2 sum = bias[c];
+                    F2 pre = bias[c];
 #pragma unroll
                     for (int k = 0; k < TAPS; ++k)
-                        if (TAPS != kMaxTaps || k >= TAPS - taps) sum = fma2(w[k][c], win[k][c], sum);
-                    float pre[2];
-                    unpack2(sum, pre[0], pre[1]);
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const float sig = sigmoid(pre[e]);
-                        g[2 * c + e] *= sig * fmaf(pre[e], 1.0f - sig, 1.0f);
-                    }
+                        if (TAPS != kMaxTaps || k >= TAPS - taps) pre = fma2(w[k][c], win[k][c], pre);
+                    // the derivative of silu: sig + silu (1 - sig)
+                    const F2 sig = sigmoid2(pre);
+                    g[c] = mul2(g[c], fma2(mul2(pre, sig), fma2(sig, same2(-1.0f), same2(1.0f)), sig));
                 }
             }
             // outside the sequence nothing comes from above, whatever the inputs there
             const bool in = INSIDE || t < used;
 #pragma unroll
-            for (int c = 0; c < N / 2; ++c) gp[TAPS - 1][c] = in ? pack2(g[2 * c], g[2 * c + 1]) : same2(0.0f);
+            for (int c = 0; c < N / 2; ++c) gp[TAPS - 1][c] = in ? g[c] : same2(0.0f);
             if (INSIDE || (in && t < t_end)) {
 #pragma unroll
                 for (int c = 0; c < N / 2; ++c) {

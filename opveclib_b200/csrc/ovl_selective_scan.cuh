@@ -418,7 +418,8 @@ __device__ __forceinline__ void scan_forward_help(const ScanParams& p, const Pla
                 if (z) {
                     read_slot<T, 8>(slot_of(slot, 2, k), g);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) o[i] *= silu(g[i]);
+                    for (int i = 0; i < 8; i += 2)
+                        unpack2(mul2(pack2(o[i], o[i + 1]), silu2(pack2(g[i], g[i + 1]))), o[i], o[i + 1]);
                 }
             }
             store_pack<T, 8>(out + t * d.channels + item_c, o, vec, valid, d.width);
@@ -841,10 +842,10 @@ __device__ __forceinline__ void scan_backward_help(const ScanParams& p, const Pl
             if (z && in && valid > 0) {
                 read_slot<T, 4>(slot_of(slot, 2, k), zz);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float sig = sigmoid(zz[i]), gate = zz[i] * sig;
-                    gate_slope[i] = g[i] * fmaf(gate, 1.0f - sig, sig);
-                    g[i] *= gate;
+                for (int i = 0; i < 4; i += 2) {
+                    const F2 zi = pack2(zz[i], zz[i + 1]), gi = pack2(g[i], g[i + 1]), sig = sigmoid2(zi), gate = mul2(zi, sig);
+                    unpack2(mul2(gi, fma2(gate, fma2(sig, same2(-1.0f), same2(1.0f)), sig)), gate_slope[i], gate_slope[i + 1]);
+                    unpack2(mul2(gi, gate), g[i], g[i + 1]);
                 }
             }
             // padding: dt = 0 hands the gradient on as it is, gy = dt u = 0 adds nothing

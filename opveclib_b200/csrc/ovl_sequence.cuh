@@ -164,6 +164,14 @@ __device__ __forceinline__ float rcp_approx(float x) {
 // 1 / (1 + e^-x): two special-function instructions
 __device__ __forceinline__ float sigmoid(float x) { return rcp_approx(1.0f + exp2_approx(-kLog2e * x)); }
 __device__ __forceinline__ float silu(float x) { return x * sigmoid(x); }
+// the same for pairs: one instruction for two values but for the special functions
+__device__ __forceinline__ F2 sigmoid2(F2 x) {
+    const F2 d = add2(exp2_pair(mul2(x, same2(-kLog2e))), same2(1.0f));
+    float a, b;
+    unpack2(d, a, b);
+    return pack2(rcp_approx(a), rcp_approx(b));
+}
+__device__ __forceinline__ F2 silu2(F2 x) { return mul2(x, sigmoid2(x)); }
 
 // log(1 + e^x) = max(x, 0) + log1p(e^-|x|), relatively exact to 3e-7 also where it is small (a step size of 0.001 is
 // softplus(-6.9)): e = e^-|x| with the product by log2 e in two parts, then log1p(e) = e p(e) with p the polynomial of
