@@ -15,7 +15,7 @@ import subprocess
 import threading
 
 from . import cuda_emit
-from .local import cache_directory, nvcc_path, gpu_arch_flags, version, logger
+from .local import cache_directory, cuda_directory, cxx, nvcc_path, gpu_arch_flags, version, logger
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 TEMPLATE_DIR = os.path.join(_PKG, 'csrc', 'templates')
@@ -27,6 +27,9 @@ LAUNCHER_SRC = os.path.join(CSRC_DIR, 'ovl_launcher.cu')
 LIBRARY_SOURCES = [LAUNCHER_SRC] + [os.path.join(CSRC_DIR, fn) for fn in
                                     ('ovl_selective_scan.cu', 'ovl_selective_scan_f32.cu', 'ovl_selective_scan_f16.cu',
                                      'ovl_selective_scan_bf16.cu', 'ovl_causal_conv.cu', 'ovl_rms_norm.cu')]
+#: the short way from Python's arguments to a launch of the sequence operators (optional: without it sequence.py does it all)
+FRONT_SRC = os.path.join(CSRC_DIR, 'ovl_front.cpp')
+FRONT_PATH = os.path.join(LIB_DIR, 'ovl_front.so')
 NVCC_FLAGS = ['-O3', '--fmad=false', '-std=c++17', '-lineinfo', '-diag-suppress', '128,177,186,550']
 _lock = threading.Lock()
 
@@ -140,3 +143,40 @@ def build_launcher(force=False):
             f.write(stamp)
         os.replace(stamp_path + '.%d.tmp' % os.getpid(), stamp_path)
         return LIB_PATH
+
+
+def build_front(force=False):
+    """Compile csrc/ovl_front.cpp, a Python extension module over torch's C++ interface, into lib/ovl_front.so and return
+    its path.  Rebuilt when its source, torch or Python differ from what it was built from; without a host compiler the
+    module that is there is kept as it is if it fits, else None comes back."""
+    import shutil
+    import sys
+    import sysconfig
+    import torch
+    from torch.utils import cpp_extension
+    with _lock:
+        h = hashlib.sha224()
+        for path in (FRONT_SRC, os.path.join(_PKG, '..', 'include', 'ovl_b200.h')):
+            with open(path, 'rb') as f:
+                h.update(f.read())
+        h.update((torch.__version__ + sys.version).encode('utf-8'))
+        stamp, stamp_path = h.hexdigest(), FRONT_PATH + '.stamp'
+        if not force and os.path.exists(FRONT_PATH) and os.path.exists(stamp_path):
+            with open(stamp_path) as f:
+                if f.read().strip() == stamp:
+                    return FRONT_PATH
+        if not shutil.which(cxx):
+            return None
+        os.makedirs(LIB_DIR, exist_ok=True)
+        tmp = FRONT_PATH + '.%d.tmp' % os.getpid()
+        include = cpp_extension.include_paths() + [sysconfig.get_paths()['include'], os.path.join(cuda_directory, 'include')]
+        library = os.path.join(os.path.dirname(torch.__file__), 'lib')
+        _run([cxx, '-O2', '-std=c++17', '-fPIC', '-shared', '-fvisibility=hidden', '-w',
+              '-D_GLIBCXX_USE_CXX11_ABI=%d' % torch.compiled_with_cxx11_abi()] + ['-I' + d for d in include] +
+             ['-o', tmp, FRONT_SRC, '-L' + library, '-ltorch', '-ltorch_cpu', '-ltorch_python', '-lc10', '-lc10_cuda',
+              '-Wl,-rpath,' + library])
+        os.replace(tmp, FRONT_PATH)
+        with open(stamp_path + '.%d.tmp' % os.getpid(), 'w') as f:
+            f.write(stamp)
+        os.replace(stamp_path + '.%d.tmp' % os.getpid(), stamp_path)
+        return FRONT_PATH

@@ -782,3 +782,219 @@ def test_empty_batches():
         assert ovl.selective_scan_step(torch.zeros(0, 16, 8, device='cuda'), **step).shape == (0, 16)
     q, s = ovl.rms_norm_quantize(torch.zeros(0, 16, device='cuda'), torch.ones(16, device='cuda'))
     assert q.shape == (0, 16) and s.shape == (0, 1)
+
+
+# ---- the compiled way of the usual calls --------------------------------------------------------------
+
+from opveclib_b200 import sequence  # noqa: E402
+
+def front_calls(dtype=torch.bfloat16):
+    """name -> (call, the tensors it reads); every call draws the same inputs and returns a tuple."""
+    g = torch.Generator().manual_seed(3)
+    draw = lambda *shape: torch.randn(*shape, generator=g)  # noqa: E731
+    u, z, dt = (draw(2, 21, 24).to(dtype).cuda() for _ in range(3))
+    B, C = draw(2, 21, 2, 5).to(dtype).cuda(), draw(2, 21, 2, 5).to(dtype).cuda()
+    A, D, h = -draw(24, 5).abs().cuda(), draw(24).cuda(), draw(2, 24, 5).cuda()
+    w, bias, tail = draw(24, 4).cuda(), draw(24).cuda(), draw(2, 3, 24).to(dtype).cuda()
+    lengths = torch.tensor([21, 9], dtype=torch.int32, device='cuda')
+    slots = torch.tensor([1, 0], dtype=torch.int32, device='cuda')
+
+    def step():
+        state = h.clone()
+        y = ovl.selective_scan_step(state, u[:, 0], dt[:, 0], A, B[:, 0], C[:, 0], D, z[:, 0], D, True, slots)
+        return y, state
+
+    def conv_step():
+        state = tail.clone()
+        return ovl.causal_conv1d_step(state, u[:, 0], w, bias, 'silu', slots), state
+    return {
+        'scan': lambda: ovl.selective_scan(u, dt, A, B, C, D, z, D, True, h, lengths, True),
+        'scan, least': lambda: (ovl.selective_scan(u, dt, A, B[:, :, 0], C[:, :, 0]),),
+        'scan step': step,
+        'conv': lambda: ovl.causal_conv1d(u, w, bias, 'silu', tail, lengths, True),
+        'conv, least': lambda: (ovl.causal_conv1d(u, w.to(dtype)),),
+        'conv step': conv_step,
+        'norm': lambda: ovl.rms_norm(u, D, z),
+        'norm, rows': lambda: (ovl.rms_norm(u[:, 0], D.to(dtype)),),
+        'norm to 8 bits': lambda: ovl.rms_norm_quantize(u, D, z, 1e-5, 8),
+        'norm to 8 bits, row': lambda: ovl.rms_norm_quantize(u[0], D),
+    }
+
+
+def bits(x):
+    return x.view(torch.uint8) if x.dtype == torch.float8_e4m3fn else x
+
+
+@pytest.mark.parametrize('name', [
+    'scan', 'scan, least', 'scan step', 'conv', 'conv, least', 'conv step', 'norm', 'norm, rows', 'norm to 8 bits',
+    'norm to 8 bits, row'])
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+def test_the_compiled_way_is_taken_and_gives_the_same(name, dtype, monkeypatch):
+    call = front_calls(dtype)[name]
+    call()                                                   # (the first call loads it)
+    assert sequence._front is not None
+    taken = []
+    monkeypatch.setattr(sequence, '_launch', lambda *a: taken.append(a))
+    short = call()
+    assert not taken                                         # nothing went through the long way
+    monkeypatch.undo()
+    monkeypatch.setattr(sequence, '_front', None)
+    long = call()
+    assert len(short) == len(long)
+    for a, b in zip(short, long):
+        assert a.dtype == b.dtype and a.shape == b.shape and a.stride() == b.stride()
+        assert torch.equal(bits(a), bits(b))
+
+
+def test_the_compiled_way_leaves_alone_what_it_cannot_do():
+    for call in front_calls().values():
+        call()
+    f = sequence._front
+    x, w = torch.randn(4, 16, device='cuda'), torch.ones(16, device='cuda')
+    assert f.rms_norm(x, w, None, 1e-6) is not None
+    state, cx, cw = torch.zeros(4, 3, 16, device='cuda'), x, torch.ones(16, 4, device='cuda')
+    assert f.causal_conv1d_step(state, cx, cw, None, None, None) is not None
+    version = state._version
+    for call in (lambda: f.rms_norm(x, w), lambda: f.rms_norm(x, w, None, 1), lambda: f.rms_norm(x.cpu(), w, None, 1e-6),
+                 lambda: f.rms_norm(x, w.double(), None, 1e-6), lambda: f.rms_norm(x, w[:8], None, 1e-6),
+                 lambda: f.rms_norm(x, w, x[:2], 1e-6), lambda: f.rms_norm(x.t(), w[:4], None, 1e-6),
+                 lambda: f.rms_norm(x, w.clone().requires_grad_(), None, 1e-6, None),
+                 lambda: f.rms_norm(x, w, None, -1e-6),
+                 lambda: f.rms_norm(x, w, None, float('nan')), lambda: f.rms_norm(x, w, None, 1e-6, 3),
+                 lambda: f.rms_norm(x, w, None, 1e-6, -1), lambda: f.rms_norm(x, w, None, 1e-6, 0),
+                 lambda: f.rms_norm(x, w, None, 1e-6, True), lambda: f.rms_norm(x, w, None, 1e-6, 1 << 70),
+                 lambda: f.rms_norm(torch._neg_view(x), w, None, 1e-6), lambda: f.rms_norm(None, w, None, 1e-6),
+                 lambda: f.rms_norm(x.half(), w, x, 1e-6), lambda: f.rms_norm(x[0, 0], w, None, 1e-6),
+                 lambda: f.causal_conv1d_step(state, cx, cw, None, 'tanh', None),
+                 lambda: f.causal_conv1d_step(state[:2], cx, cw, None, None, None),
+                 lambda: f.causal_conv1d_step(state[:, :2], cx, cw, None, None, None),
+                 lambda: f.causal_conv1d_step(state, cx, cw, None, None, [0, 1, 2, 3])):
+        assert call() is None
+    assert state._version == version
+    for bad in (dict(group=-1), dict(group=0), dict(group=True), dict(eps=-1.0)):
+        with pytest.raises(ValueError):
+            ovl.rms_norm_quantize(x, w, **bad)
+
+
+def test_views_of_negated_values():
+    x, w = torch.randn(6, 32, device='cuda'), torch.ones(32, device='cuda')
+    assert torch.equal(ovl.rms_norm(torch._neg_view(x), w), ovl.rms_norm(-x, w))
+    taps = torch.randn(32, 4, device='cuda')
+    assert torch.equal(ovl.causal_conv1d(x[None], torch._neg_view(taps)), ovl.causal_conv1d(x[None], -taps))
+
+
+def test_forward_derivatives_are_refused():
+    import torch.autograd.forward_ad as forward_ad
+    x, w = torch.randn(6, 32, device='cuda'), torch.ones(32, device='cuda')
+    ovl.rms_norm(x, w)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            ovl.rms_norm(dual, w)
+        with pytest.raises(RuntimeError):
+            ovl.rms_norm_quantize(dual, w)
+
+
+def front_losses(dtype=torch.bfloat16):
+    """name -> (call, names of the leaves it differentiates, the leaves): outputs of a call whose gradients are looked at."""
+    g = torch.Generator().manual_seed(4)
+    draw = lambda *shape: torch.randn(*shape, generator=g)  # noqa: E731
+    seq = [draw(2, 37, 24).to(dtype) for _ in range(3)]
+    bc = [draw(2, 37, 2, 5).to(dtype) for _ in range(2)]
+    par = [-draw(24, 5).abs(), draw(24), draw(24), draw(2, 24, 5)]
+    conv = [draw(24, 4), draw(24), draw(2, 3, 24).to(dtype)]
+    lengths = torch.tensor([37, 18], dtype=torch.int32, device='cuda')
+    return {
+        'scan': (lambda u, dt, z, B, C, A, D, b, h: ovl.selective_scan(u, dt, A, B, C, D, z, b, True, h, lengths, True),
+                 seq + bc + par),
+        'scan, least': (lambda u, dt, B, C, A: (ovl.selective_scan(u, dt, A, B[:, :, 0], C[:, :, 1]),), seq[:2] + bc + par[:1]),
+        'conv': (lambda x, w, b, h: ovl.causal_conv1d(x, w, b, 'silu', h, lengths, True), seq[:1] + conv),
+        'conv, least': (lambda x, w: (ovl.causal_conv1d(x, w),), [seq[0], conv[0].to(dtype)]),
+        'norm': (lambda x, r, w: ovl.rms_norm(x, w, r), seq[:2] + par[1:2]),
+        'norm, rows': (lambda x, w: (ovl.rms_norm(x[:, 3], w),), [seq[0], par[1].to(dtype)]),
+    }
+
+
+@pytest.mark.parametrize('name', ['scan', 'scan, least', 'conv', 'conv, least', 'norm', 'norm, rows'])
+@pytest.mark.parametrize('above', ['dense', 'broadcast', 'first only', 'last only'])
+def test_gradients_of_the_compiled_way(name, above, monkeypatch):
+    call, values = front_losses()[name]
+
+    def gradients():
+        leaves = [v.cuda().requires_grad_() for v in values]
+        outs = list(call(*leaves))
+        way = type(outs[0].grad_fn).__name__
+        g = torch.Generator(device='cuda').manual_seed(5)
+        top = [torch.randn(o.shape, generator=g, device='cuda').to(o.dtype) for o in outs]
+        if above == 'broadcast':
+            top = [t.flatten()[0].expand(o.shape) for t, o in zip(top, outs)]
+        if above == 'first only':
+            outs, top = outs[:1], top[:1]
+        if above == 'last only':
+            outs, top = outs[-1:], top[-1:]
+        return way, torch.autograd.grad(outs, leaves, top)
+    gradients()
+    assert sequence._front is not None
+    way, short = gradients()
+    assert way not in ('SelectiveScanBackward', 'CausalConvBackward', 'RmsNormBackward')
+    monkeypatch.setattr(sequence, '_front', None)
+    way, long = gradients()
+    assert way in ('SelectiveScanBackward', 'CausalConvBackward', 'RmsNormBackward')
+    for a, b in zip(short, long):
+        assert a.dtype == b.dtype and a.shape == b.shape and torch.equal(a, b)
+
+
+@pytest.mark.parametrize('front', [True, False])
+@pytest.mark.parametrize('name', ['scan', 'conv', 'norm'])
+def test_a_second_derivative_is_refused(name, front, monkeypatch):
+    call, values = front_losses(torch.float32)[name]
+    call(*(v.cuda() for v in values))
+    if not front:
+        monkeypatch.setattr(sequence, '_front', None)
+    leaves = [v.cuda().requires_grad_() for v in values]
+    loss = sum(o.sum() for o in call(*leaves))
+    first = torch.autograd.grad(loss, leaves[0], create_graph=True)[0]      # the first derivative is there to be looked at
+    assert bool(first.isfinite().all())
+    with pytest.raises(RuntimeError, match='differentiable once'):
+        (first ** 2).sum().backward()
+
+
+def test_kept_tensors_changed_in_place_and_packed():
+    call, values = front_losses()['norm, rows']
+    call(*(v.cuda() for v in values))
+    leaves = [v.cuda().requires_grad_() for v in values]
+    x = leaves[0] * 2
+    y, = call(x, leaves[1])
+    x.mul_(2)
+    with pytest.raises(RuntimeError, match='in-?place'):
+        y.sum().backward()
+    packed = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: packed.append(t) or t.cpu(), lambda t: t.cuda()):
+        y, = call(*leaves)
+    y.sum().backward()
+    assert packed and leaves[0].grad is not None
+    y, = call(*leaves)
+    y.sum().backward()
+    with pytest.raises(RuntimeError, match='second time'):
+        y.sum().backward()
+
+
+@pytest.mark.parametrize('name', ['scan', 'conv', 'norm'])
+@pytest.mark.parametrize('front', [True, False])
+def test_checkpointed_calls(name, front, monkeypatch):
+    """Checkpointing ends the repeated forward pass by an exception from where tensors are kept."""
+    from torch.utils.checkpoint import checkpoint
+    call, values = front_losses()[name]
+    call(*(v.cuda() for v in values))
+    if not front:
+        monkeypatch.setattr(sequence, '_front', None)
+
+    def gradients(run):
+        leaves = [v.cuda().requires_grad_() for v in values]
+        run(leaves).backward()
+        return [v.grad for v in leaves]
+    loss = lambda *leaves: sum(o.float().sum() for o in call(*leaves))  # noqa: E731
+    want = gradients(lambda leaves: loss(*leaves))
+    for reentrant in (False, True):
+        got = gradients(lambda leaves: checkpoint(loss, *leaves, use_reentrant=reentrant))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
