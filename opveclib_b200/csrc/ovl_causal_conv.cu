@@ -12,13 +12,14 @@ namespace {
 constexpr int kMaxTaps = 8;
 constexpr int kMaxStrip = 64;          // tokens of a thread, if that leaves enough blocks
 constexpr int kMinStrip = 8;
+constexpr int kForward = 8, kBackward = 4;   // channels of a thread
 constexpr int kWarps = 4;              // warps of a block: strips that follow each other
 
 struct ConvParams {
     OvlCausalConv a;
     int64_t column_tiles, strips;      // tiles of 32 x (channels of a thread) channels, blocks of kWarps strips
     int64_t strip;                     // tokens of a thread
-    int32_t vec, width;                // wide loads and stores; else copies of `width` elements
+    int32_t vec, width;                // whole packs on their boundaries; else runs of `width` elements
     float* part;                       // backward: [batch * strips, taps + 1, channels]
 };
 
@@ -28,26 +29,88 @@ __device__ __forceinline__ int64_t used_length(const int32_t* lengths, int64_t b
     return n < 0 ? 0 : n > length ? length : n;
 }
 
+// Which N channels a thread has: in runs of W, those of a warp's lanes next to each other, run after run.  W = N: a pack
+// of its own, on its boundary.  Where rows of packs do not begin on boundaries, short runs keep what a warp touches with
+// one instruction together (fp32, 1 x 2290 x 1705, forward: 14.1 us against 30.1 with 8 channels in a row for each lane,
+// fetched one by one; bf16 5 x 312 x 5721: 26.7 against 36.6).
+template <int W>
+__device__ __forceinline__ constexpr int channel_of(int c) { return c / W * 32 * W + c % W; }
+template <int W>
+__device__ __forceinline__ int valid_channels(int64_t left, int n) {     // of the channels that are left from the thread's first
+    int valid = 0;
+    for (int c = 0; c < n; ++c) valid += channel_of<W>(c) < left;
+    return valid;
+}
+
+template <typename T, int N, int W>
+__device__ __forceinline__ Pack<T, N> load_channels(const T* __restrict__ p, int valid) {
+    if constexpr (W == N) {
+        return load_pack<T, N>(p, valid > 0, 0);
+    } else {
+        Pack<T, N> r;
+#pragma unroll
+        for (int c = 0; c < N; ++c) r.v[c] = c < valid ? p[channel_of<W>(c)] : from_f32<T>(0.0f);
+        return r;
+    }
+}
+template <typename T, int N, int W>
+__device__ __forceinline__ void store_channels(T* __restrict__ p, const float (&x)[N], int valid) {
+    if constexpr (W == N) {
+        store_pack<T, N>(p, x, true, N);
+    } else {
+#pragma unroll
+        for (int c = 0; c < N; c += W) {
+            Pack<T, W> r;
+#pragma unroll
+            for (int k = 0; k < W; ++k) r.v[k] = from_f32<T>(x[c + k]);
+            if (c < valid) *reinterpret_cast<Pack<T, W>*>(p + channel_of<W>(c)) = r;
+        }
+    }
+}
+// into a slot of the thread's own, in flight while it goes on (but for single elements of 16 bits, which no copy takes)
+template <typename T, int N, int W>
+__device__ __forceinline__ void fetch_channels(T* slot, const T* __restrict__ p, int valid) {
+    if constexpr (W == N) {
+        fetch_pack<T, N>(slot, p, true, N, 0);
+    } else if constexpr (sizeof(T) * W == 4) {
+#pragma unroll
+        for (int c = 0; c < N; c += W) {
+            if (c < valid) {
+                copy_async<4>(slot + c, p + channel_of<W>(c));
+            } else {
+#pragma unroll
+                for (int k = 0; k < W; ++k) slot[c + k] = from_f32<T>(0.0f);
+            }
+        }
+    } else {
+        static_assert(W == 1, "");
+        T v[N];
+#pragma unroll
+        for (int c = 0; c < N; ++c) v[c] = p[c < valid ? channel_of<1>(c) : 0];
+#pragma unroll
+        for (int c = 0; c < N; ++c) slot[c] = c < valid ? v[c] : from_f32<T>(0.0f);
+    }
+}
+
 // A token in front of the first one comes from the state; `t` counts from the first token, -(taps - 1) is the oldest.
-template <typename T, int N>
-__device__ __forceinline__ Pack<T, N> load_token(const OvlCausalConv& a, int64_t batch, int64_t t, int64_t used, int64_t channel,
-                                                 bool vec, int valid) {
+template <typename T, int N, int W>
+__device__ __forceinline__ Pack<T, N> load_token(const OvlCausalConv& a, int64_t batch, int64_t t, int64_t used, int64_t channel, int valid) {
     const T* x = reinterpret_cast<const T*>(a.x) + batch * a.x_batch + t * a.x_token + channel;
     bool in = t < used;
     if (t < 0) {
         x = reinterpret_cast<const T*>(a.initial_state) + (batch * (a.taps - 1) + (a.taps - 1) + t) * a.channels + channel;
         in = a.initial_state != nullptr && t >= 1 - a.taps;
     }
-    return load_pack<T, N>(x, vec && in, in ? valid : 0);
+    return load_channels<T, N, W>(x, in ? valid : 0);
 }
 
 // The weights of a thread's N channels as pairs of channels, the oldest tap first; with TAPS = 8 the unused ones in front
 // are zeros, which the sums leave out.
-template <typename T, int TAPS, int N>
+template <typename T, int TAPS, int N, int W>
 __device__ __forceinline__ void load_weights(F2 (&w)[TAPS][N / 2], F2 (&bias)[N / 2], const OvlCausalConv& a, int taps, int64_t channel,
                                              int valid) {
     float v[TAPS][N], b[N];
-    if (TAPS != kMaxTaps && !a.params_f32 && valid == N && aligned16(a.weight) && (N * TAPS * sizeof(T)) % 16 == 0 && channel % N == 0) {
+    if (W == N && TAPS != kMaxTaps && !a.params_f32 && valid == N && aligned16(a.weight) && (N * TAPS * sizeof(T)) % 16 == 0 && channel % N == 0) {
         const Pack<T, N * TAPS> raw = load_pack<T, N * TAPS>(reinterpret_cast<const T*>(a.weight) + channel * TAPS, true, 0);
 #pragma unroll
         for (int c = 0; c < N; ++c)
@@ -59,11 +122,11 @@ __device__ __forceinline__ void load_weights(F2 (&w)[TAPS][N / 2], F2 (&bias)[N 
 #pragma unroll
             for (int k = 0; k < TAPS; ++k) {
                 const int kk = k - (TAPS - taps);
-                v[k][c] = kk >= 0 && c < valid ? load_param<T>(a.weight, (channel + c) * taps + kk, a.params_f32) : 0.0f;
+                v[k][c] = kk >= 0 && c < valid ? load_param<T>(a.weight, (channel + channel_of<W>(c)) * taps + kk, a.params_f32) : 0.0f;
             }
     }
 #pragma unroll
-    for (int c = 0; c < N; ++c) b[c] = a.bias && c < valid ? load_param<T>(a.bias, channel + c, a.params_f32) : 0.0f;
+    for (int c = 0; c < N; ++c) b[c] = a.bias && c < valid ? load_param<T>(a.bias, channel + channel_of<W>(c), a.params_f32) : 0.0f;
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) {
         bias[i] = pack2(b[2 * i], b[2 * i + 1]);
@@ -108,21 +171,20 @@ __device__ __forceinline__ void widen_slot(F2 (&x)[N / 2], const T* slot) {
     for (int i = 0; i < N / 2; ++i) x[i] = pack2(v[2 * i], v[2 * i + 1]);
 }
 
-// TAPS: the number of taps, or 8 for any number up to 8 (`taps` says which)
-template <typename T, int TAPS, bool FULL>
+// TAPS: the number of taps, or 8 for any number up to 8 (`taps` says which); W: see channel_of
+template <typename T, int TAPS, int W>
 __global__ void __launch_bounds__(32 * kWarps, TAPS == kMaxTaps ? 1 : 4) conv_forward(const __grid_constant__ ConvParams p) {
-    constexpr int N = 8, CHUNK = kChunk;
+    constexpr int N = kForward, CHUNK = kChunk;
+    constexpr bool FULL = W == N;
     extern __shared__ __align__(16) char smem[];
     const OvlCausalConv& a = p.a;
     const int taps = TAPS == kMaxTaps ? (int)a.taps : TAPS;
     int64_t i = blockIdx.x;
-    const int64_t column = (i % p.column_tiles) * 32 + threadIdx.x % 32;
+    const int64_t channel = (i % p.column_tiles) * 32 * N + threadIdx.x % 32 * W;
     i /= p.column_tiles;
     const int64_t strip = (i % p.strips) * kWarps + threadIdx.x / 32, batch = i / p.strips;
-    const int64_t channel = column * N;
     if (channel >= a.channels) return;
-    const int valid = a.channels - channel < N ? (int)(a.channels - channel) : N;
-    const bool vec = FULL;                                               // then valid is N or 0
+    const int valid = FULL ? N : valid_channels<W>(a.channels - channel, N);
     const int64_t used = used_length(a.lengths, batch, a.length);
     const int64_t t_begin = strip * p.strip, t_end = t_begin + p.strip < a.length ? t_begin + p.strip : a.length;
     const int64_t t_used = used < t_end ? used : t_end;
@@ -132,10 +194,10 @@ __global__ void __launch_bounds__(32 * kWarps, TAPS == kMaxTaps ? 1 : 4) conv_fo
         for (int64_t k = 0; k < taps - 1; ++k) {
             const int64_t t = used - (taps - 1) + k;
             float x[N];
-            const Pack<T, N> raw = load_token<T, N>(a, batch, t, used, channel, vec, valid);
+            const Pack<T, N> raw = load_token<T, N, W>(a, batch, t, used, channel, valid);
 #pragma unroll
             for (int c = 0; c < N; ++c) x[c] = to_f32(raw.v[c]);
-            store_pack<T, N>(reinterpret_cast<T*>(a.final_state) + (batch * (taps - 1) + k) * a.channels + channel, x, vec, valid, p.width);
+            store_channels<T, N, W>(reinterpret_cast<T*>(a.final_state) + (batch * (taps - 1) + k) * a.channels + channel, x, valid);
         }
     }
     if (t_begin >= t_end) return;
@@ -147,11 +209,11 @@ __global__ void __launch_bounds__(32 * kWarps, TAPS == kMaxTaps ? 1 : 4) conv_fo
     auto fetch = [&](int64_t t0, int chunk) {
         if (FULL && t0 + CHUNK <= t_used) {
 #pragma unroll
-            for (int s = 0; s < CHUNK; ++s) fetch_pack<T, N>(ring.slot(chunk, s), next + s * a.x_token, true, N, 0);
+            for (int s = 0; s < CHUNK; ++s) fetch_channels<T, N, W>(ring.slot(chunk, s), next + s * a.x_token, N);
         } else {
 #pragma unroll
             for (int s = 0; s < CHUNK; ++s)
-                if (t0 + s < t_used) fetch_pack<T, N>(ring.slot(chunk, s), next + s * a.x_token, vec, valid, p.width);
+                if (t0 + s < t_used) fetch_channels<T, N, W>(ring.slot(chunk, s), next + s * a.x_token, valid);
         }
         next += CHUNK * a.x_token;
         copy_commit();
@@ -159,10 +221,10 @@ __global__ void __launch_bounds__(32 * kWarps, TAPS == kMaxTaps ? 1 : 4) conv_fo
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) fetch(t_begin + k * CHUNK, k);
     F2 w[TAPS][N / 2], bias[N / 2], win[TAPS][N / 2];
-    load_weights<T, TAPS, N>(w, bias, a, taps, channel, valid);
+    load_weights<T, TAPS, N, W>(w, bias, a, taps, channel, valid);
 #pragma unroll
     for (int k = 0; k < TAPS - 1; ++k)
-        widen<T, N>(win[k], load_token<T, N>(a, batch, t_begin - (TAPS - 1) + k, used, channel, vec, valid));
+        widen<T, N>(win[k], load_token<T, N, W>(a, batch, t_begin - (TAPS - 1) + k, used, channel, valid));
     const bool gated = a.silu;
     int chunk = 0;
     T* out_t = out + t_begin * a.channels;
@@ -184,7 +246,7 @@ __global__ void __launch_bounds__(32 * kWarps, TAPS == kMaxTaps ? 1 : 4) conv_fo
 #pragma unroll
             for (int c = 0; c < N; ++c) y[c] = 0.0f;
         }
-        if (INSIDE || t < t_end) store_pack<T, N>(out_t, y, vec, valid, p.width);
+        if (INSIDE || t < t_end) store_channels<T, N, W>(out_t, y, valid);
         out_t += a.channels;
 #pragma unroll
         for (int k = 0; k < TAPS - 1; ++k)
@@ -208,21 +270,19 @@ __global__ void __launch_bounds__(32 * kWarps, TAPS == kMaxTaps ? 1 : 4) conv_fo
 // gx_t = sum_k w[k] gpre_{t + (taps - 1) - k} with gpre = gout act'(pre): the walk runs taps - 1 tokens past the strip
 // (gx of the strip needs them).  The first strip also has the gradient of the initial state, gx of the tokens
 // -(taps - 1) ... -1.
-template <typename T, int TAPS, bool FULL>
+template <typename T, int TAPS, int W>
 __global__ void __launch_bounds__(32 * kWarps, TAPS == kMaxTaps ? 1 : 4) conv_backward(const __grid_constant__ ConvParams p) {
-    constexpr int N = 4, CHUNK = kChunk;
+    constexpr int N = kBackward, CHUNK = kChunk;
+    constexpr bool FULL = W == N;
     extern __shared__ __align__(16) char smem[];
     const OvlCausalConv& a = p.a;
     const int taps = TAPS == kMaxTaps ? (int)a.taps : TAPS;
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     int64_t i = blockIdx.x;
-    const int64_t column = (i % p.column_tiles) * 32 + lane;
+    const int64_t channel = (i % p.column_tiles) * 32 * N + lane * W;
     i /= p.column_tiles;
     const int64_t strip_block = i % p.strips, strip = strip_block * kWarps + warp, batch = i / p.strips;
-    const int64_t channel = column * N;
-    const bool live = channel < a.channels;
-    const int valid = !live ? 0 : a.channels - channel < N ? (int)(a.channels - channel) : N;
-    const bool vec = FULL;                                               // then valid is N or 0
+    const int valid = channel >= a.channels ? 0 : FULL ? N : valid_channels<W>(a.channels - channel, N);
     const int64_t used = used_length(a.lengths, batch, a.length);
     const int64_t t_begin = strip * p.strip, t_end = t_begin + p.strip < a.length ? t_begin + p.strip : a.length;
 
@@ -246,15 +306,15 @@ __global__ void __launch_bounds__(32 * kWarps, TAPS == kMaxTaps ? 1 : 4) conv_ba
             if (FULL && t0 + CHUNK <= walk_used) {
 #pragma unroll
                 for (int s = 0; s < CHUNK; ++s) {
-                    fetch_pack<T, N>(ring_x.slot(chunk, s), next_x + s * a.x_token, true, N, 0);
-                    fetch_pack<T, N>(ring_g.slot(chunk, s), next_g + s * a.gout_token, true, N, 0);
+                    fetch_channels<T, N, W>(ring_x.slot(chunk, s), next_x + s * a.x_token, N);
+                    fetch_channels<T, N, W>(ring_g.slot(chunk, s), next_g + s * a.gout_token, N);
                 }
             } else {
 #pragma unroll
                 for (int s = 0; s < CHUNK; ++s) {
                     if (t0 + s < walk_used) {
-                        fetch_pack<T, N>(ring_x.slot(chunk, s), next_x + s * a.x_token, vec, valid, p.width);
-                        fetch_pack<T, N>(ring_g.slot(chunk, s), next_g + s * a.gout_token, vec, valid, p.width);
+                        fetch_channels<T, N, W>(ring_x.slot(chunk, s), next_x + s * a.x_token, valid);
+                        fetch_channels<T, N, W>(ring_g.slot(chunk, s), next_g + s * a.gout_token, valid);
                     }
                 }
             }
@@ -264,10 +324,10 @@ __global__ void __launch_bounds__(32 * kWarps, TAPS == kMaxTaps ? 1 : 4) conv_ba
         };
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) fetch(t_begin + k * CHUNK, k);
-        load_weights<T, TAPS, N>(w, bias, a, taps, channel, valid);
+        load_weights<T, TAPS, N, W>(w, bias, a, taps, channel, valid);
 #pragma unroll
         for (int k = 0; k < TAPS - 1; ++k)
-            widen<T, N>(win[k], load_token<T, N>(a, batch, t_begin - (TAPS - 1) + k, used, channel, vec, valid));
+            widen<T, N>(win[k], load_token<T, N, W>(a, batch, t_begin - (TAPS - 1) + k, used, channel, valid));
         const bool gated = a.silu;
         int chunk = 0;
         T* gx_t = reinterpret_cast<T*>(a.gx) + (batch * a.length + t_begin - (taps - 1)) * a.channels + channel;   // of token t - (taps - 1)
@@ -328,15 +388,15 @@ __global__ void __launch_bounds__(32 * kWarps, TAPS == kMaxTaps ? 1 : 4) conv_ba
                     // the state after the sequence holds the inputs used - (taps - 1) ... used - 1
                     const int64_t k = to - (used - (taps - 1));
                     if (k >= 0 && k < taps - 1) {
-                        const Pack<T, N> gf = load_pack<T, N>(
-                            reinterpret_cast<const T*>(a.gfinal) + (batch * (taps - 1) + k) * a.channels + channel, vec, valid);
+                        const Pack<T, N> gf = load_channels<T, N, W>(
+                            reinterpret_cast<const T*>(a.gfinal) + (batch * (taps - 1) + k) * a.channels + channel, valid);
 #pragma unroll
                         for (int c = 0; c < N; ++c) gx[c] += to_f32(gf.v[c]);
                     }
                 }
                 T* dst = gx_t;
                 if (state) dst = reinterpret_cast<T*>(a.ginitial) + (batch * (taps - 1) + (taps - 1) + to) * a.channels + channel;
-                store_pack<T, N>(dst, gx, vec, valid, p.width);
+                store_channels<T, N, W>(dst, gx, valid);
             }
             gx_t += a.channels;
 #pragma unroll
@@ -384,29 +444,27 @@ __global__ void __launch_bounds__(32 * kWarps, TAPS == kMaxTaps ? 1 : 4) conv_ba
         if (k < 0 || ch >= a.channels) continue;
         float sum = 0.0f;
 #pragma unroll
-        for (int s = 0; s < kWarps; ++s) sum += s_part[s][(e / (N * 32)) * N + cc % N][cc / N];
+        for (int s = 0; s < kWarps; ++s) sum += s_part[s][(e / (N * 32)) * N + cc / (32 * W) * W + cc % W][cc / W % 32];
         p.part[(row * (taps + 1) + k) * a.channels + ch] = sum;
     }
 }
 
-// the strips' parts added up in order: the lanes of a warp are 32 sums, the 8 warps of a block slices of the parts
+// the strips' parts added up in order, by slices (see sum_slices) of one block
 template <typename T>
-__global__ void __launch_bounds__(256) conv_backward_params(const __grid_constant__ ConvParams p) {
-    __shared__ float s_part[8][32];
+__global__ void __launch_bounds__(kSumThreads) conv_backward_params(const __grid_constant__ ConvParams p, int slices) {
+    __shared__ float s_part[kSumThreads];
     const OvlCausalConv& a = p.a;
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    const int64_t total = (a.taps + 1) * a.channels, rows = a.batch * p.strips, i = (int64_t)blockIdx.x * 32 + lane;
+    const int values = kSumThreads / slices, v = threadIdx.x % values, slice = threadIdx.x / values;
+    const int64_t total = (a.taps + 1) * a.channels, rows = a.batch * p.strips, i = (int64_t)blockIdx.x * values + v;
     float sum = 0.0f;
     if (i < total) {
-#pragma unroll 4
-        for (int64_t r = warp; r < rows; r += 8) sum += p.part[r * total + i];
+#pragma unroll 8
+        for (int64_t r = slice; r < rows; r += slices) sum += p.part[r * total + i];
     }
-    s_part[warp][lane] = sum;
+    s_part[threadIdx.x] = sum;
     __syncthreads();
-    if (warp != 0 || i >= total) return;
-    sum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) sum += s_part[w][lane];
+    if (slice != 0 || i >= total) return;
+    for (int s = 1; s < slices; ++s) sum += s_part[s * values + v];
     const int64_t k = i / a.channels, ch = i % a.channels;
     void* const to = k < a.taps ? a.gweight : a.gbias;
     const int64_t at = k < a.taps ? ch * a.taps + k : ch;
@@ -478,7 +536,9 @@ int check(const OvlCausalConv* a) {
     return OVL_OK;
 }
 
-// Strips of 64 tokens, shorter ones where there would be fewer than four blocks for every SM.
+// Strips of 64 tokens, shorter ones where there would be fewer than four blocks for every SM (bf16 1 x 512 x 2048, forward
+// and backward: 4.2 and 9.7 us, with strips of 64 tokens 12.2 and 18.4; with sixteen blocks for every SM asked for,
+// 4 x 4096 x 4096 takes 69.9 us forward, not 52.2: every strip loads the taps - 1 tokens in front of it again).
 void cut(const OvlCausalConv* a, int channels_of_thread, ConvParams* p) {
     p->column_tiles = ceil_div(a->channels, 32 * channels_of_thread);
     p->strip = kMaxStrip;
@@ -495,10 +555,11 @@ bool wide(const OvlCausalConv* a, int n, bool backward) {
            aligned16(a->gx) && aligned16(a->ginitial);
 }
 
-// `full`: whole packs of channels on 16-byte boundaries (the kernel has no other path then), else `any`
+// `full`: whole packs of channels on 16-byte boundaries (the kernel has no other path then); `pairs`: two elements of 16
+// bits on 4-byte boundaries; `single`: what is left
 template <typename F>
-int launch(const ConvParams& p, size_t smem, cudaStream_t stream, F full, F any) {
-    F kernel = p.vec ? full : any;
+int launch(const ConvParams& p, size_t smem, cudaStream_t stream, F full, F pairs, F single) {
+    F kernel = p.vec ? full : p.width >= 2 ? pairs : single;
     const int64_t blocks = p.column_tiles * p.strips * p.a.batch;
     if (blocks > 0x7fffffff) return OVL_ERR_TOO_LARGE;
     const int st = prepare_kernel((const void*)kernel, smem);
@@ -508,36 +569,40 @@ int launch(const ConvParams& p, size_t smem, cudaStream_t stream, F full, F any)
 }
 
 template <typename T>
+constexpr int kPairs = sizeof(T) == 2 ? 2 : 1;
+
+template <typename T>
 int run_forward(ConvParams p, cudaStream_t stream) {
-    cut(&p.a, 8, &p);
-    p.vec = wide(&p.a, 8, false);
+    cut(&p.a, kForward, &p);
+    p.vec = wide(&p.a, kForward, false);
     p.width = copy_width<T>({p.a.x, p.a.out, p.a.initial_state, p.a.final_state}, {p.a.channels, p.a.x_batch, p.a.x_token});
-    constexpr size_t smem = Ring<T, 8>::bytes;
+    constexpr size_t smem = Ring<T, kForward>::bytes;
     switch (p.a.taps) {
-        case 2: return launch(p, smem, stream, conv_forward<T, 2, true>, conv_forward<T, 2, false>);
-        case 3: return launch(p, smem, stream, conv_forward<T, 3, true>, conv_forward<T, 3, false>);
-        case 4: return launch(p, smem, stream, conv_forward<T, 4, true>, conv_forward<T, 4, false>);
-        default: return launch(p, smem, stream, conv_forward<T, kMaxTaps, true>, conv_forward<T, kMaxTaps, false>);
+        case 2: return launch(p, smem, stream, conv_forward<T, 2, kForward>, conv_forward<T, 2, kPairs<T>>, conv_forward<T, 2, 1>);
+        case 3: return launch(p, smem, stream, conv_forward<T, 3, kForward>, conv_forward<T, 3, kPairs<T>>, conv_forward<T, 3, 1>);
+        case 4: return launch(p, smem, stream, conv_forward<T, 4, kForward>, conv_forward<T, 4, kPairs<T>>, conv_forward<T, 4, 1>);
+        default: return launch(p, smem, stream, conv_forward<T, kMaxTaps, kForward>, conv_forward<T, kMaxTaps, kPairs<T>>, conv_forward<T, kMaxTaps, 1>);
     }
 }
 
 template <typename T>
 int run_backward(ConvParams p, cudaStream_t stream) {
-    cut(&p.a, 4, &p);
-    p.vec = wide(&p.a, 4, true);
+    cut(&p.a, kBackward, &p);
+    p.vec = wide(&p.a, kBackward, true);
     p.width = copy_width<T>({p.a.x, p.a.gout, p.a.gx, p.a.initial_state, p.a.gfinal, p.a.ginitial},
                             {p.a.channels, p.a.x_batch, p.a.x_token, p.a.gout_batch, p.a.gout_token});
     p.part = reinterpret_cast<float*>(p.a.workspace);
-    constexpr size_t smem = 2 * Ring<T, 4>::bytes;
+    constexpr size_t smem = 2 * Ring<T, kBackward>::bytes;
     int st;
     switch (p.a.taps) {
-        case 2: st = launch(p, smem, stream, conv_backward<T, 2, true>, conv_backward<T, 2, false>); break;
-        case 3: st = launch(p, smem, stream, conv_backward<T, 3, true>, conv_backward<T, 3, false>); break;
-        case 4: st = launch(p, smem, stream, conv_backward<T, 4, true>, conv_backward<T, 4, false>); break;
-        default: st = launch(p, smem, stream, conv_backward<T, kMaxTaps, true>, conv_backward<T, kMaxTaps, false>); break;
+        case 2: st = launch(p, smem, stream, conv_backward<T, 2, kBackward>, conv_backward<T, 2, kPairs<T>>, conv_backward<T, 2, 1>); break;
+        case 3: st = launch(p, smem, stream, conv_backward<T, 3, kBackward>, conv_backward<T, 3, kPairs<T>>, conv_backward<T, 3, 1>); break;
+        case 4: st = launch(p, smem, stream, conv_backward<T, 4, kBackward>, conv_backward<T, 4, kPairs<T>>, conv_backward<T, 4, 1>); break;
+        default: st = launch(p, smem, stream, conv_backward<T, kMaxTaps, kBackward>, conv_backward<T, kMaxTaps, kPairs<T>>, conv_backward<T, kMaxTaps, 1>); break;
     }
     if (st != OVL_OK) return st;
-    conv_backward_params<T><<<(uint32_t)ceil_div((p.a.taps + 1) * p.a.channels, 32), 256, 0, stream>>>(p);
+    const int slices = sum_slices(p.a.batch * p.strips);
+    conv_backward_params<T><<<(uint32_t)ceil_div((p.a.taps + 1) * p.a.channels, kSumThreads / slices), kSumThreads, 0, stream>>>(p, slices);
     return launch_status();
 }
 
@@ -562,7 +627,7 @@ int run_step(const OvlCausalConvStep& a, cudaStream_t stream) {
 extern "C" uint64_t ovl_causal_conv_workspace_bytes(const OvlCausalConv* a) {
     if (ovl::check(a) != OVL_OK) return 0;
     ovl::ConvParams p{};
-    ovl::cut(a, 4, &p);
+    ovl::cut(a, ovl::kBackward, &p);
     return (uint64_t)a->batch * p.strips * (a->taps + 1) * a->channels * sizeof(float);
 }
 

@@ -1044,19 +1044,27 @@ __global__ void __launch_bounds__(256) scan_backward_bc(const __grid_constant__ 
         if (n0 + k < d.states) to[n0 + k] = from_f32<T>(v[k]);
 }
 
-// gA, gD, gdelta_bias: the parts of batches and segments added up in order
-__global__ void scan_backward_params(const __grid_constant__ ScanParams p) {
+// gA, gD, gdelta_bias: the parts of batches and segments added up in order, by slices (see sum_slices) of one block
+__global__ void __launch_bounds__(kSumThreads) scan_backward_params(const __grid_constant__ ScanParams p, int slices) {
+    __shared__ double s_part[kSumThreads];
     const ScanDims& d = p.d;
+    const int values = kSumThreads / slices, v = threadIdx.x % values, slice = threadIdx.x / values;
     const int64_t rows = p.a.batch * d.segments, n_A = d.channels * d.states, total = n_A + 2 * d.channels;
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-        const bool in_A = i < n_A;
-        const int64_t k = in_A ? i : i - n_A, stride = in_A ? n_A : 2 * d.channels;
-        const float* src = (in_A ? p.part_A : p.part_D) + k;
-        double sum = 0.0;
-        for (int64_t r = 0; r < rows; ++r) sum += src[r * stride];
-        float* const to = in_A ? p.a.gA : k < d.channels ? p.a.gD : p.a.gdelta_bias;
-        if (to) to[in_A || k < d.channels ? k : k - d.channels] = (float)sum;
+    const int64_t i = (int64_t)blockIdx.x * values + v;
+    const bool in_A = i < n_A;
+    const int64_t k = in_A ? i : i - n_A, stride = in_A ? n_A : 2 * d.channels;
+    double sum = 0.0;
+    if (i < total) {
+        const float* const src = (in_A ? p.part_A : p.part_D) + k;
+#pragma unroll 8
+        for (int64_t r = slice; r < rows; r += slices) sum += src[r * stride];
     }
+    s_part[threadIdx.x] = sum;
+    __syncthreads();
+    if (slice != 0 || i >= total) return;
+    for (int s = 1; s < slices; ++s) sum += s_part[s * values + v];
+    float* const to = in_A ? p.a.gA : k < d.channels ? p.a.gD : p.a.gdelta_bias;
+    if (to) to[in_A || k < d.channels ? k : k - d.channels] = (float)sum;
 }
 
 // ---------------------------------------------------------------------------------------------------------
@@ -1065,7 +1073,9 @@ __global__ void scan_backward_params(const __grid_constant__ ScanParams p) {
 // A thread has 4 states of a channel for ROWS rows, all of whose loads are under way before the first is used; A is loaded
 // once for all rows.  What is needed once per (row, channel) - softplus, the gate, the output - is shared out among the
 // channel's lanes, a row (or more) each.  What bounds it: bytes, the states in and out.
-constexpr int kStepRows = 4;           // rows of a block, if that leaves enough blocks
+// rows of a block, if that leaves enough blocks (256 rows x 4096 channels x 16 states: 31 us, 50 with a row for each block,
+// which loads A 256 times)
+constexpr int kStepRows = 4;
 
 // The slot of a row: -1 for padding, -2 for one that does not exist or that an earlier row has.  All threads of the block
 // call it.
@@ -1189,11 +1199,6 @@ int run_forward(const ScanParams& p, cudaStream_t stream) {
     return launch_segments(scan_forward<T, P, M, false>, p, threads, smem, false, stream);
 }
 
-inline uint32_t grid_for(int64_t items) {
-    const int64_t blocks = ceil_div(items, 256), most = 16 * 8 * (int64_t)sequence_sm_count();
-    return (uint32_t)(blocks < 1 ? 1 : blocks < most ? blocks : most);
-}
-
 template <typename T, int P, int K, int M>
 int run_backward(const ScanParams& p, cudaStream_t stream) {
     using S = BackShape<P, K, M>;
@@ -1209,7 +1214,10 @@ int run_backward(const ScanParams& p, cudaStream_t stream) {
         scan_backward_bc<T, S::NP><<<(uint32_t)bc_blocks, 256, 0, stream>>>(p);
         if ((st = launch_status()) != OVL_OK) return st;
     }
-    scan_backward_params<<<grid_for(p.d.channels * (p.d.states + 2)), 256, 0, stream>>>(p);
+    const int slices = sum_slices(p.a.batch * p.d.segments);
+    const int64_t sums = ceil_div(p.d.channels * (p.d.states + 2), kSumThreads / slices);
+    if (sums > 0x7fffffff) return OVL_ERR_TOO_LARGE;
+    scan_backward_params<<<(uint32_t)sums, kSumThreads, 0, stream>>>(p, slices);
     return launch_status();
 }
 
