@@ -174,6 +174,7 @@ def build_front(force=False):
         _run([cxx, '-O2', '-std=c++17', '-fPIC', '-shared', '-fvisibility=hidden', '-w',
               '-D_GLIBCXX_USE_CXX11_ABI=%d' % torch.compiled_with_cxx11_abi()] + ['-I' + d for d in include] +
              ['-o', tmp, FRONT_SRC, '-L' + library, '-ltorch', '-ltorch_cpu', '-ltorch_python', '-lc10', '-lc10_cuda',
+              '-ltorch_cuda',
               '-Wl,-rpath,' + library])
         os.replace(tmp, FRONT_PATH)
         with open(stamp_path + '.%d.tmp' % os.getpid(), 'w') as f:
