@@ -10,8 +10,7 @@ namespace ovl {
 namespace {
 
 constexpr int kMaxTaps = 8;
-constexpr int kMaxStrip = 64;          // tokens of a thread, if that leaves enough blocks
-constexpr int kMinStrip = 8;
+constexpr int kMinStrip = 8, kMaxStrip = 128;   // tokens of a thread
 constexpr int kForward = 8, kBackward = 4;   // channels of a thread
 constexpr int kWarps = 4;              // warps of a block: strips that follow each other
 
@@ -536,15 +535,26 @@ int check(const OvlCausalConv* a) {
     return OVL_OK;
 }
 
-// Strips of 64 tokens, shorter ones where there would be fewer than four blocks for every SM (bf16 1 x 512 x 2048, forward
-// and backward: 4.2 and 9.7 us, with strips of 64 tokens 12.2 and 18.4; with sixteen blocks for every SM asked for,
-// 4 x 4096 x 4096 takes 69.9 us forward, not 52.2: every strip loads the taps - 1 tokens in front of it again).
+// The strips' length: a block of k on one SM costs its tokens (and what it does before the first, as much as 12 tokens)
+// times k + 3/4, which fits the times of strips of 8 to 256 tokens over the sizes below to a tenth, so the length of least
+// cost is taken.  Measured (us; forward, backward) against other lengths, bf16:
+//   4 x 4096 x 4096    64 tokens: 52.3, 103.7   128: 57.6, 97.5    48: 55.3, 112.5   16: 70.3, 160.1
+//   1 x 2048 x 4096    20 tokens: 13.1, 23.5     40: 14.9, 19.8     8: 14.3, 32.6    64: 16.6, 20.9
+//   1 x 512 x 2048      8 tokens:  5.9,  7.9     16:  8.1,  8.7    64: 15.6, 16.3
 void cut(const OvlCausalConv* a, int channels_of_thread, ConvParams* p) {
     p->column_tiles = ceil_div(a->channels, 32 * channels_of_thread);
-    p->strip = kMaxStrip;
-    while (p->strip > kMinStrip && a->batch * p->column_tiles * ceil_div(a->length, p->strip * kWarps) < 4 * (int64_t)sequence_sm_count())
-        p->strip /= 2;
-    p->strips = ceil_div(a->length, p->strip * kWarps);
+    const int64_t columns = a->batch * p->column_tiles, sms = sequence_sm_count();
+    double least = 0;
+    for (int64_t strip = kMinStrip; strip <= kMaxStrip; strip += kChunk) {
+        const int64_t strips = ceil_div(a->length, strip * kWarps);
+        const double cost = (double)(strip + 12) * (ceil_div(columns * strips, sms) + 0.75);
+        if (strip == kMinStrip || cost < least) {
+            least = cost;
+            p->strip = strip;
+            p->strips = strips;
+        }
+        if (strips <= 1) break;
+    }
     if (p->strips < 1) p->strips = 1;                                    // states without tokens are passed on too
 }
 
