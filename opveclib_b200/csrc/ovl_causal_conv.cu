@@ -6,6 +6,8 @@
 // taps - 1 inputs in registers, so an input is loaded once but for the taps - 1 tokens in front of the strip.
 #include "ovl_sequence.cuh"
 
+#include <type_traits>
+
 namespace ovl {
 namespace {
 
@@ -31,7 +33,7 @@ __device__ __forceinline__ int64_t used_length(const int32_t* lengths, int64_t b
 // Which N channels a thread has: in runs of W, those of a warp's lanes next to each other, run after run.  W = N: a pack
 // of its own, on its boundary.  Where rows of packs do not begin on boundaries, short runs keep what a warp touches with
 // one instruction together (fp32, 1 x 2290 x 1705, forward: 14.1 us against 30.1 with 8 channels in a row for each lane,
-// fetched one by one; bf16 5 x 312 x 5721: 26.7 against 36.6).
+// fetched one by one).
 template <int W>
 __device__ __forceinline__ constexpr int channel_of(int c) { return c / W * 32 * W + c % W; }
 template <int W>
@@ -66,31 +68,6 @@ __device__ __forceinline__ void store_channels(T* __restrict__ p, const float (&
         }
     }
 }
-// into a slot of the thread's own, in flight while it goes on (but for single elements of 16 bits, which no copy takes)
-template <typename T, int N, int W>
-__device__ __forceinline__ void fetch_channels(T* slot, const T* __restrict__ p, int valid) {
-    if constexpr (W == N) {
-        fetch_pack<T, N>(slot, p, true, N, 0);
-    } else if constexpr (sizeof(T) * W == 4) {
-#pragma unroll
-        for (int c = 0; c < N; c += W) {
-            if (c < valid) {
-                copy_async<4>(slot + c, p + channel_of<W>(c));
-            } else {
-#pragma unroll
-                for (int k = 0; k < W; ++k) slot[c + k] = from_f32<T>(0.0f);
-            }
-        }
-    } else {
-        static_assert(W == 1, "");
-        T v[N];
-#pragma unroll
-        for (int c = 0; c < N; ++c) v[c] = p[c < valid ? channel_of<1>(c) : 0];
-#pragma unroll
-        for (int c = 0; c < N; ++c) slot[c] = c < valid ? v[c] : from_f32<T>(0.0f);
-    }
-}
-
 // A token in front of the first one comes from the state; `t` counts from the first token, -(taps - 1) is the oldest.
 template <typename T, int N, int W>
 __device__ __forceinline__ Pack<T, N> load_token(const OvlCausalConv& a, int64_t batch, int64_t t, int64_t used, int64_t channel, int valid) {
@@ -140,6 +117,13 @@ __device__ __forceinline__ void widen(F2 (&x)[N / 2], const Pack<T, N>& raw) {
     for (int i = 0; i < N / 2; ++i) x[i] = pack2(to_f32(raw.v[2 * i]), to_f32(raw.v[2 * i + 1]));
 }
 
+__device__ __forceinline__ float half_of(uint32_t word, uint32_t upper, __half) {
+    return __half2float(__ushort_as_half((unsigned short)(word >> 16 * upper)));
+}
+__device__ __forceinline__ float half_of(uint32_t word, uint32_t upper, __nv_bfloat16) {
+    return __bfloat162float(__ushort_as_bfloat16((unsigned short)(word >> 16 * upper)));
+}
+
 // Tokens on their way while earlier ones are worked on: every thread copies what it will need itself into slots of its
 // own, so nothing waits but the thread that needs a token (a register that a load may or may not fill is waited for at
 // once: 197 us for the forward pass of bf16 4 x 4096 x 4096 with the next tokens in registers).
@@ -154,21 +138,52 @@ struct False {
     static constexpr bool value = false;
 };
 
-template <typename T, int N>
+// Packs stand in the slots as they are.  Runs are copied by words of 4 bytes, a thread's words a block's width apart (next
+// to each other they would meet in the same banks): pairs of 16-bit elements, or, for single ones, which no asynchronous
+// copy takes, the aligned word with the element in one of its halves.  A word with an element in it is memory of the
+// tensor's allocation, whose boundaries are far coarser.  bf16 8 x 2048 x 4095, forward and backward: 97 and 170 us; with
+// a thread's words next to each other 138 and 223; with loads into registers that go to the slot at once 142 and 277.
+template <typename T, int N, int W>
 struct Ring {
-    T* base;                           // [kRing][kChunk][threads][N]
-    __device__ __forceinline__ explicit Ring(void* smem) : base(reinterpret_cast<T*>(smem) + threadIdx.x * N) {}
-    __device__ __forceinline__ T* slot(int chunk, int s) const { return base + (chunk * kChunk + s) * (32 * kWarps * N); }
-    static constexpr size_t bytes = sizeof(T) * kRing * kChunk * 32 * kWarps * N;
-};
+    static constexpr bool kPacks = W == N;
+    using Slot = std::conditional_t<kPacks, T, uint32_t>;
+    static constexpr int kOfWord = sizeof(T) * W == 4 ? W : 1;           // channels of a word
+    static constexpr int kSize = kPacks ? N : N / kOfWord, kStep = 32 * kWarps;
+    static constexpr size_t bytes = sizeof(Slot) * kRing * kChunk * 32 * kWarps * kSize;
+    Slot* base;                        // [kRing][kChunk] of: packs [threads][N], or words [kSize][threads]
+    __device__ __forceinline__ explicit Ring(void* smem) : base(reinterpret_cast<Slot*>(smem) + threadIdx.x * (kPacks ? N : 1)) {}
+    __device__ __forceinline__ Slot* slot(int chunk, int s) const { return base + (chunk * kChunk + s) * (32 * kWarps * kSize); }
 
-template <typename T, int N>
-__device__ __forceinline__ void widen_slot(F2 (&x)[N / 2], const T* slot) {
-    float v[N];
-    read_slot<T, N>(slot, v);
+    // into a slot of the thread's own, in flight while it goes on
+    static __device__ __forceinline__ void fetch(Slot* slot, const T* __restrict__ p, int valid) {
+        if constexpr (kPacks) {
+            fetch_pack<T, N>(slot, p, true, N, 0);
+        } else {
 #pragma unroll
-    for (int i = 0; i < N / 2; ++i) x[i] = pack2(v[2 * i], v[2 * i + 1]);
-}
+            for (int k = 0; k < kSize; ++k) {
+                const T* const from = p + channel_of<W>(k * kOfWord);
+                if (k * kOfWord < valid) copy_async<4>(slot + k * kStep, reinterpret_cast<const void*>((uintptr_t)from & ~(uintptr_t)3));
+                else slot[k * kStep] = 0;
+            }
+        }
+    }
+    // `upper`: which half of its word a single element of 16 bits is in
+    static __device__ __forceinline__ void widen(F2 (&x)[N / 2], const Slot* slot, uint32_t upper) {
+        float v[N];
+        if constexpr (kPacks) {
+            read_slot<T, N>(slot, v);
+        } else {
+#pragma unroll
+            for (int c = 0; c < N; ++c) {
+                const uint32_t word = slot[c / kOfWord * kStep];
+                if constexpr (sizeof(T) == 4) v[c] = __uint_as_float(word);
+                else v[c] = half_of(word, kOfWord == 2 ? c % 2 : upper, T{});
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) x[i] = pack2(v[2 * i], v[2 * i + 1]);
+    }
+};
 
 // TAPS: the number of taps, or 8 for any number up to 8 (`taps` says which); W: see channel_of
 template <typename T, int TAPS, int W>
@@ -203,16 +218,19 @@ __global__ void __launch_bounds__(32 * kWarps, TAPS == kMaxTaps ? 1 : 4) conv_fo
 
     const T* const x = reinterpret_cast<const T*>(a.x) + batch * a.x_batch + channel;
     T* const out = reinterpret_cast<T*>(a.out) + batch * a.length * a.channels + channel;
-    const Ring<T, N> ring(smem);
+    using Tokens = Ring<T, N, W>;
+    using Slot = typename Tokens::Slot;
+    const Tokens ring(smem);
+    const uint32_t x_at = (uint32_t)((uintptr_t)x / sizeof(T));        // which halves of words the thread's elements are in
     const T* next = x + t_begin * a.x_token;                             // of the next chunk to be fetched
     auto fetch = [&](int64_t t0, int chunk) {
         if (FULL && t0 + CHUNK <= t_used) {
 #pragma unroll
-            for (int s = 0; s < CHUNK; ++s) fetch_channels<T, N, W>(ring.slot(chunk, s), next + s * a.x_token, N);
+            for (int s = 0; s < CHUNK; ++s) Tokens::fetch(ring.slot(chunk, s), next + s * a.x_token, N);
         } else {
 #pragma unroll
             for (int s = 0; s < CHUNK; ++s)
-                if (t0 + s < t_used) fetch_channels<T, N, W>(ring.slot(chunk, s), next + s * a.x_token, valid);
+                if (t0 + s < t_used) Tokens::fetch(ring.slot(chunk, s), next + s * a.x_token, valid);
         }
         next += CHUNK * a.x_token;
         copy_commit();
@@ -228,9 +246,9 @@ __global__ void __launch_bounds__(32 * kWarps, TAPS == kMaxTaps ? 1 : 4) conv_fo
     int chunk = 0;
     T* out_t = out + t_begin * a.channels;
     // one token; INSIDE: it belongs to the strip and the sequence
-    auto token = [&](int64_t t, const T* slot, auto inside) {
+    auto token = [&](int64_t t, const Slot* slot, auto inside) {
         constexpr bool INSIDE = decltype(inside)::value;
-        widen_slot<T, N>(win[TAPS - 1], slot);                           // (behind the sequence: anything, and not used)
+        Tokens::widen(win[TAPS - 1], slot, (x_at + (uint32_t)t * (uint32_t)a.x_token) & 1);   // (behind the sequence: anything, and not used)
         float y[N];
 #pragma unroll
         for (int c = 0; c < N / 2; ++c) {
@@ -298,22 +316,25 @@ __global__ void __launch_bounds__(32 * kWarps, TAPS == kMaxTaps ? 1 : 4) conv_ba
         const int64_t walk_used = used < walk_end ? used : walk_end;
         const T* const x = reinterpret_cast<const T*>(a.x) + batch * a.x_batch + channel;
         const T* const gout = reinterpret_cast<const T*>(a.gout) + batch * a.gout_batch + channel;
-        const Ring<T, N> ring_x(smem), ring_g(smem + Ring<T, N>::bytes);
+        using Tokens = Ring<T, N, W>;
+        using Slot = typename Tokens::Slot;
+        const Tokens ring_x(smem), ring_g(smem + Tokens::bytes);
+        const uint32_t x_at = (uint32_t)((uintptr_t)x / sizeof(T)), g_at = (uint32_t)((uintptr_t)gout / sizeof(T));
         const T* next_x = x + t_begin * a.x_token;                       // of the next chunk to be fetched
         const T* next_g = gout + t_begin * a.gout_token;
         auto fetch = [&](int64_t t0, int chunk) {
             if (FULL && t0 + CHUNK <= walk_used) {
 #pragma unroll
                 for (int s = 0; s < CHUNK; ++s) {
-                    fetch_channels<T, N, W>(ring_x.slot(chunk, s), next_x + s * a.x_token, N);
-                    fetch_channels<T, N, W>(ring_g.slot(chunk, s), next_g + s * a.gout_token, N);
+                    Tokens::fetch(ring_x.slot(chunk, s), next_x + s * a.x_token, N);
+                    Tokens::fetch(ring_g.slot(chunk, s), next_g + s * a.gout_token, N);
                 }
             } else {
 #pragma unroll
                 for (int s = 0; s < CHUNK; ++s) {
                     if (t0 + s < walk_used) {
-                        fetch_channels<T, N, W>(ring_x.slot(chunk, s), next_x + s * a.x_token, valid);
-                        fetch_channels<T, N, W>(ring_g.slot(chunk, s), next_g + s * a.gout_token, valid);
+                        Tokens::fetch(ring_x.slot(chunk, s), next_x + s * a.x_token, valid);
+                        Tokens::fetch(ring_g.slot(chunk, s), next_g + s * a.gout_token, valid);
                     }
                 }
             }
@@ -331,11 +352,11 @@ __global__ void __launch_bounds__(32 * kWarps, TAPS == kMaxTaps ? 1 : 4) conv_ba
         int chunk = 0;
         T* gx_t = reinterpret_cast<T*>(a.gx) + (batch * a.length + t_begin - (taps - 1)) * a.channels + channel;   // of token t - (taps - 1)
         // one token; INSIDE: it belongs to the strip and the sequence, and so does the one whose gx it completes
-        auto token = [&](int64_t t, const T* slot_x, const T* slot_g, auto inside) {
+        auto token = [&](int64_t t, const Slot* slot_x, const Slot* slot_g, auto inside) {
             constexpr bool INSIDE = decltype(inside)::value;
             F2 g[N / 2];
-            widen_slot<T, N>(win[TAPS - 1], slot_x);
-            widen_slot<T, N>(g, slot_g);
+            Tokens::widen(win[TAPS - 1], slot_x, (x_at + (uint32_t)t * (uint32_t)a.x_token) & 1);
+            Tokens::widen(g, slot_g, (g_at + (uint32_t)t * (uint32_t)a.gout_token) & 1);
             if (gated) {
 #pragma unroll
                 for (int c = 0; c < N / 2; ++c) {
@@ -586,7 +607,7 @@ int run_forward(ConvParams p, cudaStream_t stream) {
     cut(&p.a, kForward, &p);
     p.vec = wide(&p.a, kForward, false);
     p.width = copy_width<T>({p.a.x, p.a.out, p.a.initial_state, p.a.final_state}, {p.a.channels, p.a.x_batch, p.a.x_token});
-    constexpr size_t smem = Ring<T, kForward>::bytes;
+    const size_t smem = p.vec || p.width >= 1 ? Ring<T, kForward, kForward>::bytes : Ring<T, kForward, 1>::bytes;
     switch (p.a.taps) {
         case 2: return launch(p, smem, stream, conv_forward<T, 2, kForward>, conv_forward<T, 2, kPairs<T>>, conv_forward<T, 2, 1>);
         case 3: return launch(p, smem, stream, conv_forward<T, 3, kForward>, conv_forward<T, 3, kPairs<T>>, conv_forward<T, 3, 1>);
@@ -602,7 +623,7 @@ int run_backward(ConvParams p, cudaStream_t stream) {
     p.width = copy_width<T>({p.a.x, p.a.gout, p.a.gx, p.a.initial_state, p.a.gfinal, p.a.ginitial},
                             {p.a.channels, p.a.x_batch, p.a.x_token, p.a.gout_batch, p.a.gout_token});
     p.part = reinterpret_cast<float*>(p.a.workspace);
-    constexpr size_t smem = 2 * Ring<T, kBackward>::bytes;
+    const size_t smem = 2 * (p.vec || p.width >= 1 ? Ring<T, kBackward, kBackward>::bytes : Ring<T, kBackward, 1>::bytes);
     int st;
     switch (p.a.taps) {
         case 2: st = launch(p, smem, stream, conv_backward<T, 2, kBackward>, conv_backward<T, 2, kPairs<T>>, conv_backward<T, 2, 1>); break;

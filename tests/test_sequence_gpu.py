@@ -998,3 +998,30 @@ def test_checkpointed_calls(name, front, monkeypatch):
     for reentrant in (False, True):
         got = gradients(lambda leaves: checkpoint(loss, *leaves, use_reentrant=reentrant))
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize('dtype', [F16, BF16])
+@pytest.mark.parametrize('batch, length, channels, taps', [(2, 77, 1, 4), (3, 130, 31, 2), (1, 65, 257, 3), (2, 200, 519, 5)])
+@pytest.mark.parametrize('skip', [0, 1])
+def test_conv_rows_of_single_elements(dtype, batch, length, channels, taps, skip):
+    """An odd number of 16-bit elements in a row, a first element in either half of a word: neighbours of other rows, and
+    what stands in front of the tensor and behind it, are NaN."""
+    gen = _generator(channels + skip)
+    n = batch * length * channels
+    memory = torch.full((n + 2 + skip,), float('nan'), device='cuda', dtype=dtype)
+    x = memory[1 + skip:1 + skip + n].view(batch, length, channels)
+    x.copy_(_normal(gen, batch, length, channels, dtype=dtype))
+    w, b = _normal(gen, channels, taps, dtype=dtype), _normal(gen, channels, dtype=dtype)
+    gout = _normal(gen, batch, length, channels + skip, dtype=dtype)[..., skip:]
+    every = []
+    for t in (x, x.float()):                                 # (rows of whole words: the other kernels)
+        ts = [v.to(t.dtype).detach().requires_grad_() for v in (t, w, b)]
+        if t is x:
+            ts[0] = x.detach().requires_grad_()
+        y = ovl.causal_conv1d(*ts, 'silu')
+        every.append([y.detach(), *torch.autograd.grad(y, ts, gout.to(t.dtype))])
+    for got, want in zip(*every):
+        # one rounding of the same 32-bit sums (parameters' gradients: sums over tokens in another order, 2^-24 for each of
+        # the terms, whose magnitudes are below 2^5)
+        bound = torch.finfo(dtype).eps / 2 * want.abs() + batch * length * 2.0 ** -19 + torch.finfo(dtype).tiny
+        assert bool(((got.float() - want).abs() <= bound).all())
