@@ -71,8 +71,9 @@ def _run(cmd):
     try:
         return subprocess.check_output(cmd, stderr=subprocess.STDOUT, universal_newlines=True)
     except subprocess.CalledProcessError as exc:
-        logger.error('nvcc error: ' + exc.output)
-        raise RuntimeError('nvcc failed:\n' + exc.output)
+        name = os.path.basename(cmd[0])
+        logger.error(name + ' error: ' + exc.output)
+        raise RuntimeError(name + ' failed:\n' + exc.output)
 
 
 def compile_kernel(kernel, math='exact'):

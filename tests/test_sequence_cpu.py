@@ -165,3 +165,38 @@ def test_the_reference_statements_themselves():
     out, state = ref.conv(torch.arange(1.0, 4.0).view(1, 3, 1), torch.tensor([[10.0, 1.0]]))
     assert out.flatten().tolist() == [1.0, 12.0, 23.0] and state.item() == 3.0
     assert ref.e4m3(torch.tensor([17.0, 18.0, 19.0, 0.001, 449.0]).double()).tolist()[:3] == [16.0, 18.0, 20.0]
+
+
+# ---- the compiled way of the usual calls --------------------------------------------------------------
+
+def test_the_compiled_way_hands_back_what_is_not_its_own():
+    """Without a device every call is one that sequence.py has to refuse; nothing is launched, nothing raised."""
+    import importlib.util
+    from opveclib_b200 import compiler
+    path = compiler.build_front()
+    if path is None:
+        pytest.skip('no C++ compiler')
+    spec = importlib.util.spec_from_file_location('ovl_front', path)
+    front = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(front)
+    x, w = torch.randn(4, 16), torch.ones(16)
+    for call, args in ((front.rms_norm, (x, w, None, 1e-6)), (front.rms_norm, ()), (front.rms_norm, (x, w, None, 1e-6, 8, 8)),
+                       (front.rms_norm, (torch.nn.Parameter(x), w, None, 1e-6, None)), (front.selective_scan, (1, 2)),
+                       (front.selective_scan, (None,) * 11), (front.selective_scan_step, (x,) * 11),
+                       (front.causal_conv1d, (x,) * 7), (front.causal_conv1d_step, (x,) * 6), (front.causal_conv1d_step, ())):
+        assert call(*args) is None
+    for bad in ((), (torch.nn.Parameter,), (torch.nn.Parameter,) + (0,) * 11, (torch.nn.Parameter,) + ('x',) * 11):
+        with pytest.raises((TypeError, ValueError)):
+            front.bind(*bad)
+
+
+def test_a_module_that_cannot_be_built_is_done_without(monkeypatch, caplog):
+    from opveclib_b200 import compiler, sequence
+
+    def fails(force=False):
+        raise RuntimeError('no headers')
+    monkeypatch.setattr(compiler, 'build_front', fails)
+    monkeypatch.setattr(sequence, '_front', None)
+    monkeypatch.setattr(sequence, '_front_tried', False)
+    sequence._load_front()
+    assert sequence._front is None and sequence._front_tried
