@@ -335,7 +335,9 @@ int ovl_causal_conv_step(const OvlCausalConvStep* args, void* cuda_stream);
  *   weight, gweight [columns]: dtype, or fp32 when params_f32 is set.
  * With group > 0 the output is 8 bits wide instead: y is cut into groups of `group` columns (which divides columns),
  *     scale = max(max |y| / 448, 2^-126),  q = y / scale rounded to the nearest e4m3 value, ties to even
- * with q [rows, columns] bytes and scale [rows, columns / group] fp32.
+ * with q [rows, columns] bytes and scale [rows, columns / group] fp32.  Both quotients are rounded to 32 bits as a division
+ * does.  A NaN in y makes its group NaN as a whole; an infinite y (by an infinite weight) makes the scale infinite, itself
+ * NaN and the group's finite values zeros.
  * The backward call takes the forward call's x and residual and the gradients of y and of residual_out (NULL: zero); gx
  * is the gradient of x and of the residual alike.  Its workspace: ovl_rms_norm_workspace_bytes(args) bytes; the forward
  * call needs none. */

@@ -630,7 +630,9 @@ def rms_norm_quantize(x, weight, residual=None, eps=1e-6, group=None):
         scale = max(max |y| / 448, 2^-126);  q = y / scale, rounded to the nearest e4m3 value
 
     Returns ``(q, scale)``, with a ``residual`` ``(q, scale, s)``: ``q`` float8_e4m3fn in the shape of ``x``, ``scale``
-    float32 [..., columns / group].  A group with a NaN or an infinity is NaN as a whole.  No gradient."""
+    float32 [..., columns / group].  Both quotients are rounded to 32 bits as a division does.  A group whose ``y`` has a NaN
+    is NaN as a whole (an infinity of ``x`` or ``residual`` makes one); an infinite weight makes its group's scale infinite,
+    the infinite value NaN and the others zeros.  No gradient."""
     if _front is not None:
         y = _front.rms_norm(x, weight, residual, eps, group)
         if y is not None:
