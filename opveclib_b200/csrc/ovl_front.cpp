@@ -138,11 +138,16 @@ Tensor workspace(A& args, uint64_t size, const Tensor& like) {
     return w;
 }
 
-// The gradient above an output that nothing used is zeros; a kernel reads any strides but the innermost axis's.
+// A gradient from above may be a view of negated values, as an input (see Tensors::get): kernels read memory, so what they
+// get goes through one of these two.  The gradient above an output that nothing used is zeros; a kernel reads any strides
+// but the innermost axis's.
 Tensor above(const Tensor& grad, const Tensor& like, int64_t columns) {
     if (!grad.defined()) return at::zeros({columns}, like.options()).expand(like.sizes());
-    return grad.is_contiguous() || grad.stride(-1) == 1 ? grad : grad.contiguous();
+    const Tensor g = grad.resolve_neg();
+    return g.is_contiguous() || g.stride(-1) == 1 ? g : g.contiguous();
 }
+// the same of an output whose kernels read dense memory, or none for zeros
+Tensor dense_above(const Tensor& grad) { return grad.defined() ? grad.resolve_neg().contiguous() : grad; }
 
 // Gradients that are differentiated again (create_graph) say so instead of counting as constants.
 variable_list once(variable_list grads, const char* what) {
@@ -300,7 +305,7 @@ struct ScanFunction : torch::autograd::Function<ScanFunction> {
             const c10::AutoGradMode off(false);
             OvlSelectiveScan s = scan_args(u, delta, A, B, C, behind(x[5]), behind(x[6]), behind(x[7]), behind(x[8]), behind(x[9]),
                                            ctx->saved_data["softplus"].toInt());
-            const Tensor gout = above(grads[0], u, s.channels), gfinal = grads[1].defined() ? grads[1].contiguous() : Tensor();
+            const Tensor gout = above(grads[0], u, s.channels), gfinal = dense_above(grads[1]);
             for (int i = 0; i < 9; ++i)
                 if (x[i].defined()) g[i + 1] = fresh(x[i].sizes(), x[i].scalar_type(), x[i]);
             s.checkpoints = data<float>(&x[10]);
@@ -388,7 +393,7 @@ struct ConvFunction : torch::autograd::Function<ConvFunction> {
         {
             const c10::AutoGradMode off(false);
             OvlCausalConv s = conv_args(x[0], x[1], behind(x[2]), behind(x[3]), behind(x[4]), ctx->saved_data["silu"].toInt());
-            const Tensor gout = above(grads[0], x[0], s.channels), gfinal = last.defined() ? last.contiguous() : Tensor();
+            const Tensor gout = above(grads[0], x[0], s.channels), gfinal = dense_above(last);
             for (int i = 0; i < 4; ++i)
                 if (x[i].defined()) g[i + 2] = fresh(x[i].sizes(), x[i].scalar_type(), x[i]);
             s.gout = gout.data_ptr(), s.gout_batch = gout.stride(0), s.gout_token = gout.stride(1);
@@ -464,8 +469,8 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
             OvlRmsNorm s = norm_args(x, weight, behind(v[2]), ctx->saved_data["eps"].toDouble());
             // (rows that follow each other, where there are other than two axes)
             const Tensor gy = x.dim() == 2 || !grads[0].defined() ? above(grads[0], x.dim() == 2 ? x : x.view({s.rows, s.columns}), s.columns)
-                                                                  : grads[0].contiguous();
-            const Tensor gres = !last.defined() ? last : x.dim() == 2 ? above(last, x, s.columns) : last.contiguous();
+                                                                  : dense_above(grads[0]);
+            const Tensor gres = last.defined() && x.dim() == 2 ? above(last, x, s.columns) : dense_above(last);
             gx = fresh(x.sizes(), x.scalar_type(), x), gweight = fresh(weight.sizes(), weight.scalar_type(), weight);
             s.gy = gy.data_ptr(), s.gy_row = row_stride(gy);
             s.gresidual_out = data(behind(gres)), s.gresidual_out_row = gres.defined() ? row_stride(gres) : 0;

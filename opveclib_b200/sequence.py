@@ -218,6 +218,20 @@ def _like(x):
     return x.new_empty(x.shape)
 
 
+def _above(grad):
+    """A gradient from above as the kernels read it: memory of its own values (it may be a view of negated ones) whose
+    innermost axis is contiguous."""
+    if grad is None:
+        return None
+    if grad.is_neg():
+        grad = grad.resolve_neg()
+    return grad if grad.stride(-1) == 1 else grad.contiguous()
+
+
+def _dense_above(grad):
+    return None if grad is None else _above(grad).contiguous()
+
+
 def _changed(state):
     """A state that a kernel wrote to: a backward pass that kept it finds out, as with any change in place."""
     if not state.is_inference():
@@ -272,8 +286,7 @@ def _scan_backward(x, dims, saved, gout, gfinal):
     device = u.device
     if gout is None:                                         # only the final state is used further on
         gout = u.new_zeros(channels).expand(batch, length, channels)
-    gout = gout if gout.stride(-1) == 1 else gout.contiguous()
-    gfinal = None if gfinal is None else gfinal.contiguous()
+    gout, gfinal = _above(gout), _dense_above(gfinal)
     make = torch.zeros_like if batch == 0 else torch.empty_like
     gu, gdelta, gz = _like(u), _like(delta), None if z is None else _like(z)
     gB, gC = _like(B), _like(C)
@@ -451,8 +464,7 @@ def _conv_backward(x, dims, gout, gfinal):
     device = tokens.device
     if gout is None:
         gout = tokens.new_zeros(channels).expand(batch, length, channels)
-    gout = gout if gout.stride(-1) == 1 else gout.contiguous()
-    gfinal = None if gfinal is None else gfinal.contiguous()
+    gout, gfinal = _above(gout), _dense_above(gfinal)
     make = torch.zeros_like if batch == 0 else torch.empty_like
     gx, gweight, gbias = _like(tokens), make(weight), None if bias is None else make(bias)
     ginitial = None if initial_state is None else torch.empty_like(initial_state)
@@ -588,9 +600,7 @@ def _norm_backward(x, weight, residual, eps, gy, gres):
     device = x.device
     if gy is None:
         gy = x.new_zeros(x.shape[1]).expand(x.shape)
-    gy = gy if gy.stride(-1) == 1 else gy.contiguous()
-    if gres is not None and gres.stride(-1) != 1:
-        gres = gres.contiguous()
+    gy, gres = _above(gy), _above(gres)
     gx = _like(x)
     gweight = torch.empty_like(weight)
     args = _norm_args(x, weight, eps, residual=residual, gy=gy, gres=gres, gx=gx, gweight=gweight)

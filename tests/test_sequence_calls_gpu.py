@@ -58,3 +58,67 @@ def test_norm_to_8_bits_of_an_infinite_weight():
         mine = q[:, at * inside:(at + 1) * inside].float()
         assert int(mine.isnan().sum()) == 2 and not bool(torch.nan_to_num(mine).any())
         assert bool((q[:, (at + 1) * inside:].float() == 448).all())
+
+
+# ---- gradients from above that are views of negated values -------------------------------------------------------
+
+def losses(t=F32):
+    """name -> (call that returns all outputs, its leaves)"""
+    gen = torch.Generator().manual_seed(11)
+    draw = lambda *shape: torch.randn(*shape, generator=gen)  # noqa: E731
+    seq, bc = [draw(2, 9, 8).to(t) for _ in range(3)], [draw(2, 9, 2, 4).to(t) for _ in range(2)]
+    par, conv = [-draw(8, 4).abs(), draw(8), draw(8), draw(2, 8, 4)], [draw(8, 4), draw(8), draw(2, 3, 8).to(t)]
+    return {
+        'scan': (lambda u, dt, z, B, C, A, D, b, h: ovl.selective_scan(u, dt, A, B, C, D, z, b, True, h, None, True), seq + bc + par),
+        'conv': (lambda x, w, b, h: ovl.causal_conv1d(x, w, b, 'silu', h, None, True), seq[:1] + conv),
+        'norm': (lambda x, r, w: ovl.rms_norm(x, w, r), seq[:2] + par[1:2]),
+        'norm, rows': (lambda x, r, w: ovl.rms_norm(x[:, 0], w, r[:, 0]), seq[:2] + par[1:2]),
+    }
+
+
+@pytest.mark.parametrize('front', [True, False])
+@pytest.mark.parametrize('which', [(0,), (1,), (0, 1)])
+@pytest.mark.parametrize('name', ['scan', 'conv', 'norm', 'norm, rows'])
+@pytest.mark.parametrize('t', [F32, BF16])
+def test_gradients_from_above_that_are_negated_views(t, name, which, front, monkeypatch):
+    call, values = losses(t)[name]
+    call(*(v.cuda() for v in values))                         # (the first call loads the compiled way)
+    if front:
+        assert sequence._front is not None
+    else:
+        monkeypatch.setattr(sequence, '_front', None)
+    leaves = [v.cuda().requires_grad_() for v in values]
+    outs = call(*leaves)
+    gen = torch.Generator(device='cuda').manual_seed(12)
+    above = [torch.randn(o.shape, generator=gen, device='cuda').to(o.dtype) for o in outs]
+
+    def grads(views):
+        pick = [outs[i] for i in which]
+        top = [torch._neg_view(-above[i]) if views else above[i] for i in which]
+        assert all(g.is_neg() == views for g in top)
+        return torch.autograd.grad(pick, leaves, top, retain_graph=True, allow_unused=True)
+    for got, want in zip(grads(True), grads(False)):
+        assert (got is None) == (want is None)
+        assert got is None or torch.equal(got, want)
+
+
+@pytest.mark.parametrize('front', [True, False])
+def test_a_gradient_through_a_conjugated_complex_number(front, monkeypatch):
+    """One channel, and an output that becomes the imaginary part of a number whose conjugate is used further on: the
+    gradient comes back as a view of negated values with the stride 1 at its end."""
+    gen = torch.Generator(device='cuda').manual_seed(13)
+    draw = lambda *shape: torch.randn(*shape, generator=gen, device='cuda')  # noqa: E731
+    w, a, factor = draw(1, 3), draw(2, 5), torch.complex(draw(2, 5), draw(2, 5))
+    x = draw(2, 5, 1)
+    ovl.causal_conv1d(x, w)
+    if not front:
+        monkeypatch.setattr(sequence, '_front', None)
+
+    def gradient(conv, x, a, factor):
+        x = x.detach().requires_grad_()
+        (torch.complex(a, conv(x).squeeze(-1)).conj() * factor).real.sum().backward()
+        return x.grad
+    got = gradient(lambda v: ovl.causal_conv1d(v, w, activation='silu'), x, a, factor)
+    want = gradient(lambda v: ref.conv(v, w.double(), activation='silu')[0], x.double(), a.double(), factor.to(torch.complex128))
+    # sums of three products with silu's derivative (at most 1.1), 32 bits throughout: 16 roundings of at most 2^-24
+    assert bool(((got.double() - want).abs() <= 2.0 ** -20 * 1.1 * 3 * w.abs().max() * factor.abs().max()).all())
