@@ -8,6 +8,7 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/GradMode.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -16,6 +17,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <memory>
 #include <optional>
@@ -75,9 +77,11 @@ template <typename T = void>
 T* data(const at::Tensor* t) { return t ? reinterpret_cast<T*>(t->data_ptr()) : nullptr; }
 int64_t stride(const at::Tensor* t, int axis) { return t ? t->stride(axis) : 0; }
 
-// The current device is the tensors', and nothing looks on or changes the calls.
+// The current device is the tensors', and nothing looks on or changes the calls: neither a dispatch mode nor a tracer,
+// before dispatch either (sequence.py refuses those that would keep this call's answer).
 bool plain(const Tensors& all) {
-    return all.device.index() == c10::cuda::current_device() && !c10::impl::TorchDispatchModeTLS::any_modes_set();
+    return all.device.index() == c10::cuda::current_device() && !c10::impl::TorchDispatchModeTLS::any_modes_set() &&
+           !torch::jit::tracer::isTracing() && !c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch);
 }
 
 Maybe maybe(const at::Tensor* t) { return t ? Maybe(*t) : Maybe(); }

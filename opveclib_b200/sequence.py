@@ -12,7 +12,8 @@ All take torch CUDA tensors of one type (float32, float16 or bfloat16), compute 
 on torch's current stream of the tensors' device through the C-ABI library (``include/ovl_b200.h``); workspaces come from
 torch's allocator on that stream, so calls can be captured into CUDA graphs.  The first three are differentiable (once).
 A tensor whose innermost axis is not contiguous is copied first, any other strides are taken as they are.  Wrong types
-raise ``TypeError``, wrong shapes and values ``ValueError``, before anything is launched.
+raise ``TypeError``, wrong shapes and values ``ValueError``, before anything is launched; tracers (``torch.jit.trace``,
+``torch.export``) and the transforms of ``torch.func`` are refused with a ``RuntimeError``.
 """
 import struct
 
@@ -94,8 +95,19 @@ def _dense(x, name, shape, dtype, what):
     return x if x.is_contiguous() else x.contiguous()
 
 
+def _refuse_tracers(what):
+    """The kernels are launched past torch's dispatcher: a tracer would keep this call's answer, or memory that nothing
+    fills, and miss the states changed in place.  (torch.jit.trace; torch.fx's tracer of real tensors, before or behind
+    dispatch; torch.export on top of it.)"""
+    torch = _torch_module
+    if torch.jit.is_tracing() or torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None \
+            or torch._ops._len_torch_dispatch_stack_pre_dispatch() > 0:
+        raise RuntimeError('%s cannot be traced: call it outside of the trace' % what)
+
+
 def _first(x, name, rank, what):
     torch = _torch()
+    _refuse_tracers(what)
     if not isinstance(x, torch.Tensor):
         raise TypeError('%s: %s must be a torch tensor' % (what, name))
     if x.dtype not in _codes:

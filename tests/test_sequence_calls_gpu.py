@@ -122,3 +122,42 @@ def test_a_gradient_through_a_conjugated_complex_number(front, monkeypatch):
     want = gradient(lambda v: ref.conv(v, w.double(), activation='silu')[0], x.double(), a.double(), factor.to(torch.complex128))
     # sums of three products with silu's derivative (at most 1.1), 32 bits throughout: 16 roundings of at most 2^-24
     assert bool(((got.double() - want).abs() <= 2.0 ** -20 * 1.1 * 3 * w.abs().max() * factor.abs().max()).all())
+
+
+# ---- tracers ------------------------------------------------------------------------------------------------------
+
+def plain_calls():
+    """name -> (call of one tensor, the tensor)"""
+    gen = torch.Generator().manual_seed(14)
+    draw = lambda *shape: torch.randn(*shape, generator=gen).cuda()  # noqa: E731
+    x, w, taps, A, B = draw(2, 6, 8), draw(8), draw(8, 4), -draw(8, 4).abs(), draw(2, 6, 4)
+    state, tail = draw(2, 8, 4), draw(2, 3, 8)
+    return {
+        'scan': (lambda v: ovl.selective_scan(v, v, A, B, B, delta_softplus=True), x),
+        'conv': (lambda v: ovl.causal_conv1d(v, taps), x),
+        'norm': (lambda v: ovl.rms_norm(v, w), x),
+        'norm to 8 bits': (lambda v: ovl.rms_norm_quantize(v, w)[1], x),
+        'scan step': (lambda v: ovl.selective_scan_step(state, v, v, A, B[:, 0], B[:, 0], delta_softplus=True), x[:, 0]),
+        'conv step': (lambda v: ovl.causal_conv1d_step(tail, v, taps), x[:, 0]),
+    }
+
+
+NAMES = ['scan', 'conv', 'norm', 'norm to 8 bits', 'scan step', 'conv step']
+
+
+@pytest.mark.parametrize('front', [True, False])
+@pytest.mark.parametrize('name', NAMES)
+@pytest.mark.parametrize('tracer', ['jit', 'fx', 'fx before dispatch'])
+def test_tracing_is_refused(tracer, name, front, monkeypatch):
+    """A trace would keep the example's answer."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    call, x = plain_calls()[name]
+    call(x)
+    if not front:
+        monkeypatch.setattr(sequence, '_front', None)
+    with torch.no_grad(), pytest.raises(RuntimeError, match='cannot be traced'):
+        if tracer == 'jit':
+            torch.jit.trace(lambda v: call(v * 2), (x,), check_trace=False)
+        else:
+            make_fx(lambda v: call(v * 2), pre_dispatch=tracer != 'fx')(x)
+    call(x)                                                   # and is over with the tracer

@@ -200,3 +200,30 @@ def test_a_module_that_cannot_be_built_is_done_without(monkeypatch, caplog):
     monkeypatch.setattr(sequence, '_front_tried', False)
     sequence._load_front()
     assert sequence._front is None and sequence._front_tried
+
+
+@pytest.mark.parametrize('tracer', ['jit', 'fx', 'fx before dispatch', 'export'])
+def test_tracing_is_refused_before_the_arguments_are_looked_at(tracer):
+    """A tracer would keep the example's answer (tests/test_sequence_calls_gpu.py has the calls on a device)."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    w, taps, state = torch.ones(8), torch.ones(8, 4), torch.zeros(2, 8, 4)
+    A, B = -torch.ones(8, 4), torch.ones(2, 5, 4)
+
+    def by(call, x):
+        if tracer == 'jit':
+            torch.jit.trace(call, (x,), check_trace=False)
+        elif tracer == 'export':
+            module = torch.nn.Module()
+            module.forward = call
+            torch.export.export(module, (x,), strict=False)
+        else:
+            make_fx(call, pre_dispatch=tracer != 'fx')(x)
+    x = torch.zeros(2, 5, 8)
+    for call, arg in ((lambda v: ovl.rms_norm(v * 2, w), x), (lambda v: ovl.rms_norm_quantize(v * 2, w)[1], x),
+                      (lambda v: ovl.causal_conv1d(v * 2, taps), x), (lambda v: ovl.selective_scan(v, v * 2, A, B, B), x),
+                      (lambda v: ovl.causal_conv1d_step(torch.zeros(2, 3, 8), v * 2, taps), x[:, 0]),
+                      (lambda v: ovl.selective_scan_step(state, v, v * 2, A, B[:, 0], B[:, 0]), x[:, 0])):
+        with pytest.raises(RuntimeError, match='cannot be traced'):
+            by(call, arg)
+    with pytest.raises(RuntimeError, match='needs CUDA tensors'):           # and is over with the tracer
+        ovl.rms_norm(x, w)
