@@ -57,6 +57,7 @@ struct Tensors {
         if (device.is_cpu()) device = t.device();
         else if (t.device() != device) return nullptr;
         if (t.is_neg() || t._fw_grad(0).defined()) return nullptr;
+        if (!t.const_data_ptr() && t.numel() > 0) return nullptr;        // (a null address would count as left out)
         differentiated |= grad && t.requires_grad();
         return &t;
     }

@@ -59,7 +59,14 @@ MAX_STATES, MAX_TAPS, MAX_COLUMNS = 128, 8, 32768
 
 
 def _ptr(x):
-    return 0 if x is None else x.data_ptr()
+    """The address of what may be left out (0): a tensor has one unless it is empty (those of torch.func.functionalize and of
+    other wrappers do not, and would count as left out)."""
+    if x is None:
+        return 0
+    address = x.data_ptr()
+    if not address and x.numel():
+        raise RuntimeError('opveclib_b200 needs tensors with memory of their own, not %s' % type(x).__name__)
+    return address
 
 
 def _refuse(x, name, shape, dtype, what):

@@ -161,3 +161,19 @@ def test_tracing_is_refused(tracer, name, front, monkeypatch):
         else:
             make_fx(lambda v: call(v * 2), pre_dispatch=tracer != 'fx')(x)
     call(x)                                                   # and is over with the tracer
+
+
+# ---- tensors without memory of their own --------------------------------------------------------------------------
+
+@pytest.mark.parametrize('front', [True, False])
+def test_a_tensor_without_memory_does_not_count_as_left_out(front, monkeypatch):
+    """torch.func.functionalize hands over tensors whose address is null; where a tensor may be left out, null means that."""
+    x, r, w = torch.randn(4, 16, device='cuda'), torch.randn(4, 16, device='cuda'), torch.ones(16, device='cuda')
+    taps, b = torch.randn(16, 4, device='cuda'), torch.randn(16, device='cuda')
+    ovl.rms_norm(x, w, r)
+    if not front:
+        monkeypatch.setattr(sequence, '_front', None)
+    for call, v in ((lambda v: ovl.rms_norm(x, w, v)[0], r), (lambda v: ovl.causal_conv1d(x[None], taps, v), b),
+                    (lambda v: ovl.rms_norm(v, w), x), (lambda v: ovl.rms_norm_quantize(x, w, v)[1], r)):
+        with pytest.raises(RuntimeError):
+            torch.func.functionalize(call)(v)
