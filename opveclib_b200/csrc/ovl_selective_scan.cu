@@ -63,6 +63,12 @@ ScanShape backward_shape(const OvlSelectiveScan* a) {
     return ScanShape{lanes_for(a->states, 2, 4), 1, 2};
 }
 
+constexpr int64_t kMostParts = (int64_t)1 << 30;
+// bytes of one channel tile's parts of gB and gC, over all batches and groups
+int64_t part_bytes(const OvlSelectiveScan* a, const ScanShape& shape) {
+    return a->batch * a->groups * a->length * 2 * shape.padded_states() * (int64_t)sizeof(float);
+}
+
 void make_dims(const OvlSelectiveScan* a, ScanDims* d, ScanShape* shape, bool backward) {
     d->length = a->length;
     d->channels = a->channels;
@@ -71,7 +77,8 @@ void make_dims(const OvlSelectiveScan* a, ScanDims* d, ScanShape* shape, bool ba
     d->group_channels = a->channels / a->groups;
     d->softplus = a->delta_softplus != 0;
     *shape = backward ? backward_shape(a) : forward_shape(a);
-    d->tiles = ceil_div(d->group_channels, shape->block_channels());
+    d->all_tiles = d->tiles = ceil_div(d->group_channels, shape->block_channels());
+    d->first_tile = 0;
     // Segments that run side by side in two launches (one less than there are segments in each): as many as two blocks per
     // SM hold, from four segments on - with S segments the two launches walk 2 / S of the length.  bf16, one sequence, 16
     // states: 2048 tokens x 2048 channels (64 blocks) 82 us in one piece, 59 us in 5 segments; 16384 x 4096 (128 blocks)
@@ -84,12 +91,24 @@ void make_dims(const OvlSelectiveScan* a, ScanDims* d, ScanShape* shape, bool ba
     if (s < 4) s = 1;
     d->segment_length = ceil_div(ceil_div(a->length > 0 ? a->length : 1, s), 32) * 32;
     d->segments = ceil_div(a->length > 0 ? a->length : 1, d->segment_length);
+    if (!backward || a->batch == 0) return;
+    // The parts of gB and gC are 8 bytes per token, padded state and tile, and tiles have fewer channels the more states there
+    // are (32 with 16 states, 8 with 64, 4 with 128): 4, 64 and 256 bytes per token and channel, 34 GB for 8 x 4096 x 4096 x
+    // 128.  What is more than kMostParts goes through the same memory in several launches, each with as many blocks as
+    // the SMs hold at a time (two each, one above 64 states: shared memory), or a multiple of them.  The backward pass of
+    // bf16 4 x 2048 x 4096 x 128: 10.7 ms with 1.2 GB allocated, 10.4 ms with 8.9 GB in one piece.
+    const int64_t bytes = part_bytes(a, *shape), at_a_time = (a->states > 64 ? 1 : 2) * (int64_t)sequence_sm_count();
+    if (d->all_tiles <= 1 || bytes * d->all_tiles <= kMostParts) return;
+    const int64_t wave = ceil_div(at_a_time, a->batch * a->groups * (d->segments > 1 ? d->segments - 1 : 1));
+    const int64_t waves = kMostParts / (bytes * wave);
+    d->tiles = wave * (waves > 1 ? waves : 1);
+    if (d->tiles > d->all_tiles) d->tiles = d->all_tiles;
 }
 
 uint64_t round16(uint64_t n) { return (n + 15) / 16 * 16; }
 
 struct Workspace {
-    uint64_t state, dt, bc, A, D, total;
+    uint64_t state, dt, bc, sum, A, D, total;
 };
 Workspace layout(const OvlSelectiveScan* a, const ScanDims& d, const ScanShape& shape, bool backward) {
     Workspace w{};
@@ -104,7 +123,8 @@ Workspace layout(const OvlSelectiveScan* a, const ScanDims& d, const ScanShape& 
         w.dt = take((uint64_t)a->batch * d.segments * d.channels);
     }
     if (backward) {
-        w.bc = take((uint64_t)a->batch * d.groups * d.tiles * d.length * 2 * shape.padded_states());
+        w.bc = take(part_bytes(a, shape) / sizeof(float) * d.tiles);
+        if (d.tiles < d.all_tiles) w.sum = take(part_bytes(a, shape) / sizeof(float));
         w.A = take((uint64_t)a->batch * d.segments * d.channels * d.states);
         w.D = take((uint64_t)a->batch * d.segments * 2 * d.channels);
     }
@@ -136,6 +156,7 @@ int run(const OvlSelectiveScan* a, bool backward, cudaStream_t stream) {
     p.seg_state = reinterpret_cast<float*>(ws + w.state);
     p.seg_dt = reinterpret_cast<float*>(ws + w.dt);
     p.part_bc = reinterpret_cast<float*>(ws + w.bc);
+    p.sum_bc = reinterpret_cast<float*>(ws + w.sum);
     p.part_A = reinterpret_cast<float*>(ws + w.A);
     p.part_D = reinterpret_cast<float*>(ws + w.D);
     // wide accesses: 8 elements at a time start on 16 bytes

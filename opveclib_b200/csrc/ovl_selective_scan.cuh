@@ -23,7 +23,8 @@ constexpr int kMaxSegments = 32;
 
 struct ScanDims {
     int64_t length, channels, states, groups;
-    int64_t group_channels, tiles;     // channels of a group, channel tiles of a group
+    int64_t group_channels;            // channels of a group
+    int64_t all_tiles, first_tile, tiles;      // channel tiles of a group; those of this launch
     int64_t segments, segment_length;  // the length cut into segments (a multiple of 32) that run side by side
     int64_t first_segment, launch_segments;   // those of this launch
     int32_t ahead;                     // the first of two launches, see below
@@ -36,7 +37,8 @@ struct ScanParams {
     OvlSelectiveScan a;
     float* seg_state;                  // [batch, segments, channels, states]: what a segment adds to the state
     float* seg_dt;                     // [batch, segments, channels]: sum of dt over the segment
-    float* part_bc;                    // [batch, groups, tiles, length, 2, 4P]: gC and gB of a channel tile
+    float* part_bc;                    // [batch, groups, tiles, length, 2, padded states]: gC and gB of a channel tile
+    float* sum_bc;                     // [batch, groups, length, 2, padded states]: their sum over the launches before
     float* part_A;                     // [batch * segments, channels, states]
     float* part_D;                     // [batch * segments, 2, channels]: gD, gdelta_bias
 };
@@ -119,9 +121,10 @@ __device__ __forceinline__ int64_t used_length(const int32_t* lengths, int64_t b
     return n < 0 ? 0 : n > length ? length : n;
 }
 
-// which piece of the problem a block works on (a launch covers the segments from first_segment on)
+// which piece of the problem a block works on (a launch covers the segments from first_segment and the tiles from
+// first_tile on)
 struct Place {
-    int64_t batch, segment, group, tile, channel0, n_channels;   // channels channel0 ... channel0 + n_channels - 1
+    int64_t batch, segment, group, tile, channel0, n_channels;   // tile: of the launch's; channels from channel0 on
 };
 __device__ __forceinline__ Place block_place(const ScanDims& d, int ch) {
     Place p;
@@ -132,8 +135,8 @@ __device__ __forceinline__ Place block_place(const ScanDims& d, int ch) {
     i /= d.groups;
     p.segment = d.first_segment + i % d.launch_segments;
     p.batch = i / d.launch_segments;
-    p.channel0 = p.group * d.group_channels + p.tile * ch;
-    const int64_t left = d.group_channels - p.tile * ch;
+    const int64_t skip = (d.first_tile + p.tile) * ch, left = d.group_channels - skip;
+    p.channel0 = p.group * d.group_channels + skip;
     p.n_channels = left < ch ? left : ch;
     return p;
 }
@@ -1009,7 +1012,8 @@ __global__ void __launch_bounds__(BackShape<P, K, M>::THREADS, 2) scan_backward(
 }
 
 // gB and gC: the channel tiles' parts added up, 4 values per thread; a block's 4 slices of the tiles each in order, then the
-// slices.  The parts of a (batch, group) and tile are one piece of memory, [length][2][NP].
+// slices, then the sum over the tiles of the launches before.  The parts of a (batch, group) and tile are one piece of
+// memory, [length][2][NP].
 template <typename T, int NP>
 __global__ void __launch_bounds__(256) scan_backward_bc(const __grid_constant__ ScanParams p) {
     __shared__ float4 s_sum[3][64];
@@ -1036,6 +1040,15 @@ __global__ void __launch_bounds__(256) scan_backward_bc(const __grid_constant__ 
         const float4 v = s_sum[k][lane];
         sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
     }
+    if (d.tiles < d.all_tiles && in) {
+        float4* const before = reinterpret_cast<float4*>(p.sum_bc) + bg * quads + q;
+        if (d.first_tile > 0) {
+            const float4 v = *before;
+            sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+        }
+        *before = sum;
+    }
+    if (d.first_tile + d.tiles < d.all_tiles) return;
     const int part = (int)(q % (NP / 2)), n0 = part % (NP / 4) * 4;
     T* const to = reinterpret_cast<T*>(part < NP / 4 ? p.a.gC : p.a.gB) + ((b * d.length + t) * d.groups + g) * d.states;
     const float v[4] = {sum.x, sum.y, sum.z, sum.w};
@@ -1200,17 +1213,20 @@ int run_forward(const ScanParams& p, cudaStream_t stream) {
 }
 
 template <typename T, int P, int K, int M>
-int run_backward(const ScanParams& p, cudaStream_t stream) {
+int run_backward(ScanParams p, cudaStream_t stream) {
     using S = BackShape<P, K, M>;
     // the scanning threads' registers come out of those that the block starts with: what all threads hold then
     constexpr int registers = S::SCAN * S::SCAN_REGISTERS + S::HELP * S::HELP_REGISTERS;
     constexpr size_t smem = BackSmem<T, P, K, M>::bytes;
-    int st = p.d.vec && p.d.vec_bc ? launch_segments(scan_backward<T, P, K, M, true>, p, S::THREADS, smem, true, stream, registers)
-                                   : launch_segments(scan_backward<T, P, K, M, false>, p, S::THREADS, smem, true, stream, registers);
-    if (st != OVL_OK) return st;
     const int64_t bc_blocks = ceil_div(p.d.length * S::NP / 2, 64) * p.a.batch * p.d.groups;
     if (bc_blocks > 0x7fffffff) return OVL_ERR_TOO_LARGE;
-    if (bc_blocks > 0) {
+    const int64_t most = p.d.tiles;                                      // of one launch: what the work space has room for
+    for (int64_t& first = p.d.first_tile; first < p.d.all_tiles; first += most) {
+        p.d.tiles = p.d.all_tiles - first < most ? p.d.all_tiles - first : most;
+        int st = p.d.vec && p.d.vec_bc ? launch_segments(scan_backward<T, P, K, M, true>, p, S::THREADS, smem, true, stream, registers)
+                                       : launch_segments(scan_backward<T, P, K, M, false>, p, S::THREADS, smem, true, stream, registers);
+        if (st != OVL_OK) return st;
+        if (bc_blocks == 0) continue;
         scan_backward_bc<T, S::NP><<<(uint32_t)bc_blocks, 256, 0, stream>>>(p);
         if ((st = launch_status()) != OVL_OK) return st;
     }

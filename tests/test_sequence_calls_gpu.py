@@ -177,3 +177,32 @@ def test_a_tensor_without_memory_does_not_count_as_left_out(front, monkeypatch):
                     (lambda v: ovl.rms_norm(v, w), x), (lambda v: ovl.rms_norm_quantize(x, w, v)[1], r)):
         with pytest.raises(RuntimeError):
             torch.func.functionalize(call)(v)
+
+
+# ---- many states ---------------------------------------------------------------------------------------------------
+
+def test_scan_gradients_with_the_parts_of_gB_and_gC_in_several_pieces():
+    """4096 channels of 128 states: the channel tiles' parts of gB and gC do not fit the work space at once.  Quarters of the
+    channels are calls without pieces.  Gradients that a channel has for itself are the same bits; gB and gC are the
+    quarters' sum, and as all terms are positive here, two sums of the same 1024 tiles' parts in different orders differ by
+    at most 2 x 1024 roundings of 2^-24."""
+    gen = torch.Generator(device='cuda').manual_seed(15)
+    batch, length, channels, states = 1, 2048, 4096, 128
+    draw = lambda *shape: torch.rand(*shape, generator=gen, device='cuda') + 0.1  # noqa: E731
+    u, delta, gout = draw(batch, length, channels), draw(batch, length, channels) - 3, draw(batch, length, channels)
+    B, C, A = draw(batch, length, states), draw(batch, length, states), -4 * draw(channels, states)
+    lengths = torch.tensor([length - 37], dtype=torch.int32, device='cuda')
+
+    def grads(part):
+        leaves = [v.clone().requires_grad_() for v in (u[..., part], delta[..., part], A[part], B, C)]
+        out = ovl.selective_scan(*leaves, delta_softplus=True, lengths=lengths)
+        return torch.autograd.grad(out, leaves, gout[..., part])
+    every, again = grads(slice(0, channels)), grads(slice(0, channels))
+    assert all(torch.equal(a, b) for a, b in zip(every, again))
+    quarters = [grads(slice(k * channels // 4, (k + 1) * channels // 4)) for k in range(4)]
+    for i, axis in ((0, -1), (1, -1), (2, 0)):
+        assert torch.equal(every[i], torch.cat([q[i] for q in quarters], axis))
+    for i in (3, 4):
+        want = sum(q[i].double() for q in quarters)
+        assert bool((want[:, :length - 37] > 0).all()) and not bool(every[i][:, length - 37:].any())
+        assert bool(((every[i].double() - want).abs() <= 2.0 ** -13 * want).all())

@@ -227,3 +227,17 @@ def test_tracing_is_refused_before_the_arguments_are_looked_at(tracer):
             by(call, arg)
     with pytest.raises(RuntimeError, match='needs CUDA tensors'):           # and is over with the tracer
         ovl.rms_norm(x, w)
+
+
+@pytest.mark.parametrize('batch, length, channels, states, groups', [(8, 4096, 4096, 128, 1), (4, 2048, 4096, 128, 1), (1, 16384, 8192, 64, 1),
+                                                                     (2, 4096, 8192, 100, 2), (64, 2048, 2048, 65, 1), (1, 8192, 16384, 33, 4)])
+def test_the_work_space_of_many_states_is_bounded(batch, length, channels, states, groups):
+    """The parts of gB and gC once took 8 bytes per token, padded state and tile of 4 to 8 channels: 34 GB for the first
+    case.  Now 1 GB, or what the blocks that run at a time leave (at most 2 on each of 148 SMs, and up to twice that by
+    rounding up), beside their sum and the parameters' parts."""
+    lib = launcher.library()
+    args = _scan_bytes(batch=batch, length=length, channels=channels, states=states, groups=groups)
+    padded = 64 if states <= 64 else 128
+    at_a_time = (148 + batch * groups) * (2 if states <= 64 else 1) * length * 2 * padded * 4
+    others = batch * groups * length * 2 * padded * 4 + 8 * batch * channels * (states + 2) * 4
+    assert 0 < lib.ovl_selective_scan_workspace_bytes(args, 1) <= max(1 << 30, at_a_time) + others
