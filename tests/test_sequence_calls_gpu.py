@@ -179,6 +179,63 @@ def test_a_tensor_without_memory_does_not_count_as_left_out(front, monkeypatch):
             torch.func.functionalize(call)(v)
 
 
+# ---- what the documents say of transforms and compilers -----------------------------------------------------------
+
+@pytest.mark.parametrize('front', [True, False])
+@pytest.mark.parametrize('name', NAMES)
+def test_transforms_are_refused(name, front, monkeypatch):
+    call, x = plain_calls()[name]
+    call(x)
+    if not front:
+        monkeypatch.setattr(sequence, '_front', None)
+    total = lambda v: call(v).float().sum()  # noqa: E731
+    for transform in (lambda: torch.func.grad(total)(x), lambda: torch.func.vmap(call)(x[None].expand(2, *x.shape)),
+                      lambda: torch.func.jvp(call, (x,), (x,)), lambda: torch.func.jacrev(call)(x),
+                      lambda: torch.func.functionalize(call)(x)):
+        with pytest.raises(RuntimeError):
+            transform()
+
+
+@pytest.mark.parametrize('front', [True, False])
+@pytest.mark.parametrize('name', ['scan', 'conv', 'norm'])
+def test_batched_gradients_are_refused(name, front, monkeypatch):
+    call, x = plain_calls()[name]
+    call(x)
+    if not front:
+        monkeypatch.setattr(sequence, '_front', None)
+    leaf = x.clone().requires_grad_()
+    out = call(leaf)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(out, leaf, torch.ones(3, *out.shape, device='cuda'), is_grads_batched=True)
+
+
+@pytest.mark.parametrize('front', [True, False])
+@pytest.mark.parametrize('name', NAMES)
+@pytest.mark.parametrize('backend', ['eager', 'aot_eager'])
+def test_a_compiler_runs_the_operators_between_its_graphs(backend, name, front, monkeypatch):
+    call, x = plain_calls()[name]
+    call(x)
+    if not front:
+        monkeypatch.setattr(sequence, '_front', None)
+    torch._dynamo.reset()
+    compiled = torch.compile(lambda v: call(v * 2) + 1, backend=backend)
+    for k in range(3):
+        call, x = plain_calls()[name]                         # (steps change their state: the same one for both)
+        with torch.no_grad():
+            want = call((x + k) * 2) + 1
+        call, x = plain_calls()[name]
+        with torch.no_grad():
+            assert torch.equal(compiled(x + k), want)
+    if 'step' in name or name == 'norm to 8 bits':
+        return
+    leaf, other = x.clone().requires_grad_(), x.clone().requires_grad_()
+    torch.autograd.backward((call(leaf * 2) + 1).sum())
+    torch.autograd.backward(torch.compile(lambda v: call(v * 2) + 1, backend=backend)(other).sum())
+    assert torch.equal(leaf.grad, other.grad)
+    with pytest.raises(Exception):                            # (whatever the compiler raises)
+        torch.compile(lambda v: call(v * 2) + 1, backend=backend, fullgraph=True)(x)
+
+
 # ---- many states ---------------------------------------------------------------------------------------------------
 
 def test_scan_gradients_with_the_parts_of_gB_and_gC_in_several_pieces():
