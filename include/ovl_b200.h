@@ -233,7 +233,7 @@ int ovl_scan_f32_static_status(void* cuda_stream, int32_t* out_status);
  *  - take inputs whose innermost axis is contiguous, the other strides in elements (they may be 0), and write dense
  *    outputs; 16-byte aligned pointers, strides and sizes select wide loads, anything else works too;
  *  - run asynchronously on `cuda_stream`, allocate nothing, keep nothing between calls, and give the same bits for the
- *    same inputs (no atomics);
+ *    same inputs (no atomics but the largest magnitude of a group in shared memory, whose order changes nothing);
  *  - return OVL_OK without a launch when batch (or rows) is 0 - the gradients of the parameters are then not written
  *    either, except by ovl_rms_norm_backward - and OVL_ERR_NULL / _INVALID / _DTYPE / _SCRATCH /
  *    _TOO_LARGE for arguments they do not take.

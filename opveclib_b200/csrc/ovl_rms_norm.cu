@@ -504,8 +504,12 @@ int launch(const NormParams& p, bool backward, cudaStream_t stream) {
     return backward ? launch_backward<T, TEAM, K>(p, stream) : launch_forward<T, TEAM, K>(p, stream);
 }
 
-// Forwards 32 columns a thread from 1024 on: what a thread does once per row (the sum over the team, the roots and scales)
-// weighs less (bf16 16384 x 4096 to 8 bits: 89 us with 256 threads of 16 columns).  Backwards 16: registers.
+// Columns of a thread: 8, 16 and 32 for a warp's rows (up to 1024), then forwards 16 up to 2048 and 32 up to 16384 - what a
+// thread does once per row (the sum over the team, the roots and scales) weighs less than with 16 (bf16 16384 x 4096 to 8
+// bits, before its quotients were corrected: 85 us, 89 with 256 threads of 16 columns).  Backwards 8 up to 2048, 16 up to
+// 4096 and 32 up to 16384, and 64 above that both ways: from 8193 columns on the backward kernel spills (164 to 332 bytes of
+// loads with 32 columns, 1.4 KB in 16 bits and 4.4 KB in fp32 with 64; bf16 4096 x 16384: 149 us, 2.7 TB/s, 2048 x 32768: 329
+// us, 1.2 TB/s).
 template <typename T>
 int dispatch(const NormParams& p, bool backward, cudaStream_t stream) {
     const int64_t c = p.a.columns;

@@ -7,11 +7,13 @@
 // out of the way of the exponentials: it runs serially over the tokens in registers (no scan over lanes, which would
 // multiply the arithmetic), and everything that is needed once per (token, channel) is computed once, in shared memory.
 //
-// Layout.  A channel is P lanes of a warp with 4 states each (P = 1 ... 32: up to 128 states); a block is 128 threads
-// (256 for P = 32) = CH channels of one group of one batch.  Tokens come in tiles of STEPS: while a tile is scanned the
-// next one's elements are in flight to shared memory, each to the thread that will convert, mask and combine them
-// (softplus, dt * u) into what all lanes of a channel read; double-buffered, with one barrier per tile.  The sums over the states of P steps are formed together
-// (reduce_lanes: less than one exchange per step), and the same threads that loaded u and z finish the outputs.
+// Layout.  Prompts, forwards: a lane has 4 states of M channels (1 or 2), a channel P lanes of a warp (P = 1 ... 32: up to
+// 128 states, rounded up to a power of two).  A block is 128 scanning threads = CH channels of one group of one batch, and
+// 128 helping ones.  Tokens come in tiles of STEPS: while a tile is scanned the helping threads have the next ones'
+// elements in flight to shared memory, each those that it will convert, mask and combine itself (softplus, dt * u) into
+// what all lanes of a channel read, and finish the outputs of the tile before; double-buffered, with one barrier per tile.
+// The sums over the states of V steps are formed together (reduce_lanes: less than one exchange per step).  Backwards alike,
+// with 2 states (4 above 64) of 2 channels (1 above 64) a lane.
 #pragma once
 #include "ovl_sequence.cuh"
 

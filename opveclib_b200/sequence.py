@@ -10,7 +10,8 @@
 
 All take torch CUDA tensors of one type (float32, float16 or bfloat16), compute in 32 bits and round once.  Kernels run
 on torch's current stream of the tensors' device through the C-ABI library (``include/ovl_b200.h``); workspaces come from
-torch's allocator on that stream, so calls can be captured into CUDA graphs.  The first three are differentiable (once).
+torch's allocator on that stream, so calls can be captured into CUDA graphs.  The first three are differentiable (once;
+every gradient is computed, also those of inputs that need none).
 A tensor whose innermost axis is not contiguous is copied first, any other strides are taken as they are.  Wrong types
 raise ``TypeError``, wrong shapes and values ``ValueError``, before anything is launched; tracers (``torch.jit.trace``,
 ``torch.export``) and the transforms of ``torch.func`` are refused with a ``RuntimeError``.
